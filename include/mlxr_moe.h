@@ -27,7 +27,11 @@
  *
  * dtypes: MLXR_MOE_FLOAT32, MLXR_MOE_BFLOAT16 (bf16 as raw uint16 bits).
  * Quantisation: mode "affine" (or NULL), group_size 64 (32 and 128 also for
- * quantize/dequantize), bits 4 or 8 (2 also for quantize/dequantize).
+ * quantize/dequantize), bits 4 or 8 (2 also for quantize/dequantize); or mode
+ * "mxfp4", group_size 32 and bits 4 (their defaults there): microscaled 4-bit
+ * floating point, codes of sign, two exponent bits and a mantissa bit (0, 0.5,
+ * 1, 1.5, 2, 3, 4, 6) packed as the affine ones, one scale byte b per group
+ * standing for 2^(b - 127) (255: NaN), no biases.
  */
 #ifndef MLXR_MOE_H
 #define MLXR_MOE_H
@@ -42,6 +46,9 @@ extern "C" {
 typedef void* mlxr_moe_stream; /* hipStream_t */
 
 enum { MLXR_MOE_FLOAT32 = 0, MLXR_MOE_BFLOAT16 = 1 };
+
+/* The scales of mode "mxfp4" (one byte per group), as a scales dtype. */
+enum { MLXR_MOE_UINT8 = 2 };
 
 /* mlx_optional_int (crates/mlxr/src/ops/quantization.rs:16-21) */
 typedef struct {
@@ -61,7 +68,11 @@ int mlxr_moe_version(void);
  * cols*bits/32] and scales/biases [rows, cols/group_size] in w's dtype.
  * Replaces mlx_quantize as called by quantize_device
  * (crates/mlxr/src/ops/quantization.rs:47-70); defaults g64 / 4-bit
- * (quantization.rs:11-13). */
+ * (quantization.rs:11-13).  Mode "mxfp4": scales uint8 [rows, cols/32],
+ * biases NULL; a group's scale is 2^(floor(log2 max|w|) - 2), at least 2^-127,
+ * its codes the nearest ones to w / scale (ties to the even code, magnitudes
+ * above 6 to 6); a group holding an infinity or a NaN gets scale byte 255 (NaN)
+ * and codes 0. */
 int mlxr_moe_quantize(const void* w, int w_dtype, int64_t rows, int64_t cols,
                       mlxr_moe_optional_int group_size,
                       mlxr_moe_optional_int bits, const char* mode,
@@ -71,7 +82,9 @@ int mlxr_moe_quantize(const void* w, int w_dtype, int64_t rows, int64_t cols,
 /* out [rows, cols] (out_dtype) = code * scale + bias, evaluated as one fused
  * multiply-add rounded once.  Replaces mlx_dequantize as called by
  * dequantize_device (crates/mlxr/src/ops/quantization.rs:118-146).
- * biases are required for mode "affine". */
+ * biases are required for mode "affine".  Mode "mxfp4": code * scale, exact
+ * (past the output type's range an infinity); sb_dtype MLXR_MOE_UINT8, biases
+ * NULL. */
 int mlxr_moe_dequantize(const uint32_t* wq, const void* scales,
                         const void* biases, int sb_dtype, int64_t rows,
                         int64_t cols, mlxr_moe_optional_int group_size,
@@ -88,7 +101,10 @@ int mlxr_moe_dequantize(const uint32_t* wq, const void* scales,
  * Replaces mlx_gather_qmm as called by gather_qmm_device
  * (crates/mlxr/src/ops/quantization.rs:171-221).  `sorted_indices` is the
  * reference's locality hint; rows are always grouped by expert here.
- * Requires N % 64 == 0, K % 64 == 0, group 64, bits 4 or 8. */
+ * Requires N % 64 == 0, K % 64 == 0, group 64, bits 4 or 8.
+ * Mode "mxfp4" (group 32): w [E, N, K/8], scales uint8 [E, N, K/32] (sb_dtype
+ * MLXR_MOE_UINT8), biases NULL; every weight is an exact bf16 value (scale
+ * bytes below 253) and every sum is in f32, whatever the number of rows. */
 size_t mlxr_moe_gather_qmm_workspace_size(int64_t B, int64_t M,
                                           int64_t num_experts);
 int mlxr_moe_gather_qmm(const void* x, int x_dtype, int64_t x_batch,
@@ -204,7 +220,12 @@ int mlxr_moe_combine(const void* y, const float* w, int64_t T, int64_t K,
  * (crates/mlxr/src/quantization.rs:6-147): a dense SwitchLinear
  * (switch.rs:49-94, applied with gather_mm) or Linear, weight bf16
  * [E, output_dims, input_dims], scales and biases NULL, group_size
- * ignored.  The projections of one module share their bits. */
+ * ignored.  bits = MLXR_MOE_BITS_MXFP4 describes mode "mxfp4": weight u32 [E,
+ * output_dims, input_dims/8], scales uint8 [E, output_dims, input_dims/32],
+ * biases NULL, group_size 32 (expert and shared-expert projections; routers
+ * and gates take the other forms).  The projections of one module share their
+ * bits. */
+enum { MLXR_MOE_BITS_MXFP4 = 0x104 };
 typedef struct {
   const uint32_t* weight;
   const void* scales;

@@ -16,6 +16,8 @@ LIB_PATH = Path(os.environ.get("MLXR_MOE_LIB", Path(__file__).resolve().parent /
 
 FLOAT32 = 0
 BFLOAT16 = 1
+UINT8 = 2
+BITS_MXFP4 = 0x104
 
 
 class MlxrMoeError(RuntimeError):

@@ -25,6 +25,9 @@ ARCH = "gfx950"
 
 SOURCES = [
     "quant.hip",
+    "mx_quant.hip",
+    "mx_stream.hip",
+    "mx_tile.hip",
     "router.hip",
     "dispatch.hip",
     "qgemm.hip",

@@ -38,6 +38,19 @@ hipStream_t as_stream(mlxr_moe_stream s) {
 
 bool dtype_ok(int dt) { return dt == MLXR_MOE_FLOAT32 || dt == MLXR_MOE_BFLOAT16; }
 
+static_assert(MLXR_MOE_BITS_MXFP4 == kBitsMxfp4, "one code for both");
+
+bool is_mxfp4(const char* mode) { return mode && std::strcmp(mode, "mxfp4") == 0; }
+
+// group_size and bits of mode "mxfp4": 32 and 4, given or not
+Status resolve_mxfp4(mlxr_moe_optional_int gs, mlxr_moe_optional_int bits) {
+  const int g = gs.has_value ? gs.value : 32, b = bits.has_value ? bits.value : 4;
+  if (g != 32 || b != 4)
+    return Status::error("mode mxfp4 takes group_size 32 and bits 4, got " +
+                         std::to_string(g) + " and " + std::to_string(b));
+  return Status{};
+}
+
 // mode, group_size and bits as mlx-c resolves them (defaults from
 // crates/mlxr/src/ops/quantization.rs:11-13).
 Status resolve_quant(const char* mode, mlxr_moe_optional_int gs,
@@ -45,7 +58,7 @@ Status resolve_quant(const char* mode, mlxr_moe_optional_int gs,
                      int* b_out) {
   if (mode && std::strcmp(mode, "affine") != 0)
     return Status::error(std::string("unsupported quantization mode '") +
-                         mode + "' (only 'affine')");
+                         mode + "' (only 'affine' and 'mxfp4')");
   const int g = gs.has_value ? gs.value : 64;
   const int b = bits.has_value ? bits.value : 4;
   if (kernel_path) {
@@ -116,7 +129,7 @@ int run_gather(const char* op, const void* x, int64_t x_batch, int64_t M,
   if (B * M > INT32_MAX / 2) return fail(o + ": too many rows");
   if (bits == 16 && x_batch * M * K * 2 >= ((int64_t)1 << 31))
     return fail(o + ": x must be under 2 GB");  // the M-tiled kernel's buffer
-  if (N * K * bits / 8 >= ((int64_t)1 << 31))
+  if (N * K * weight_bits(bits) / 8 >= ((int64_t)1 << 31))
     return fail(o + ": one expert's weights must be under 2 GB");
   if (B > 0 && (!x || !w || !out)) return fail(o + ": null array");
   if (!aligned(x, 16) || !aligned(w, 16))
@@ -188,14 +201,26 @@ int mlxr_moe_quantize(const void* w, int w_dtype, int64_t rows, int64_t cols,
                       mlxr_moe_optional_int bits, const char* mode,
                       uint32_t* wq, void* scales, void* biases,
                       mlxr_moe_stream stream) {
-  int g, b;
-  Status st = resolve_quant(mode, group_size, bits, false, &g, &b);
+  int g = 32, b = 4;
+  const bool mx = is_mxfp4(mode);
+  Status st = mx ? resolve_mxfp4(group_size, bits)
+                 : resolve_quant(mode, group_size, bits, false, &g, &b);
   if (!st.ok) return finish(st);
   if (!dtype_ok(w_dtype)) return fail("quantize: w dtype must be f32 or bf16");
   if (rows < 0 || cols <= 0) return fail("quantize: bad shape");
   if (cols % g)
     return fail("quantize: last dim " + std::to_string(cols) +
                 " is not a multiple of group_size " + std::to_string(g));
+  if (mx) {
+    if (biases) return fail("quantize: mode mxfp4 has no biases");
+    if (rows && (!w || !wq || !scales)) return fail("quantize: null array");
+    if (!aligned(w, w_dtype == MLXR_MOE_BFLOAT16 ? 2 : 4) || !aligned(wq, 4))
+      return fail("quantize: w must be aligned to its elements, wq to 4 bytes");
+    return finish(from_hip(launch_mx_quantize(w, w_dtype == MLXR_MOE_BFLOAT16, rows * cols, wq,
+                                              static_cast<uint8_t*>(scales),
+                                              as_stream(stream)),
+                           "quantize"));
+  }
   if (rows && (!w || !wq || !scales || !biases))
     return fail("quantize: null array");
   return finish(from_hip(launch_quantize(w, w_dtype == MLXR_MOE_BFLOAT16, rows,
@@ -209,6 +234,21 @@ int mlxr_moe_dequantize(const uint32_t* wq, const void* scales,
                         int64_t cols, mlxr_moe_optional_int group_size,
                         mlxr_moe_optional_int bits, const char* mode,
                         void* out, int out_dtype, mlxr_moe_stream stream) {
+  if (is_mxfp4(mode)) {
+    const Status st = resolve_mxfp4(group_size, bits);
+    if (!st.ok) return finish(st);
+    if (sb_dtype != MLXR_MOE_UINT8 || !dtype_ok(out_dtype))
+      return fail("dequantize: mode mxfp4 takes uint8 scales and a f32 or bf16 out");
+    if (rows < 0 || cols <= 0 || cols % 32) return fail("dequantize: bad shape");
+    if (biases) return fail("dequantize: mode mxfp4 has no biases");
+    if (rows && (!wq || !scales || !out)) return fail("dequantize: null array");
+    if (!aligned(out, out_dtype == MLXR_MOE_BFLOAT16 ? 2 : 4) || !aligned(wq, 4))
+      return fail("dequantize: out must be aligned to its elements, wq to 4 bytes");
+    return finish(from_hip(
+        launch_mx_dequantize(wq, static_cast<const uint8_t*>(scales), rows * cols, out,
+                             out_dtype == MLXR_MOE_BFLOAT16, as_stream(stream)),
+        "dequantize"));
+  }
   int g, b;
   Status st = resolve_quant(mode, group_size, bits, false, &g, &b);
   if (!st.ok) return finish(st);
@@ -242,12 +282,24 @@ int mlxr_moe_gather_qmm(const void* x, int x_dtype, int64_t x_batch,
                         void* workspace, size_t workspace_size,
                         mlxr_moe_stream stream) {
   (void)sorted_indices;
-  int g, b;
-  Status st = resolve_quant(mode, group_size, bits, true, &g, &b);
+  int g = 32, b = 4;
+  const bool mx = is_mxfp4(mode);
+  Status st = mx ? resolve_mxfp4(group_size, bits)
+                 : resolve_quant(mode, group_size, bits, true, &g, &b);
   if (!st.ok) return finish(st);
   if (!transpose)
     return fail("gather_qmm: only transpose=true (the [E, N, K] layout of "
                 "QuantizedSwitchLinear) is supported");
+  if (mx) {
+    if (x_dtype != MLXR_MOE_BFLOAT16 || sb_dtype != MLXR_MOE_UINT8 ||
+        out_dtype != MLXR_MOE_BFLOAT16)
+      return fail("gather_qmm: mode mxfp4 takes bf16 x and out and uint8 scales");
+    if (biases) return fail("gather_qmm: mode mxfp4 has no biases");
+    if (!scales) return fail("gather_qmm: null array");
+    return run_gather("gather_qmm", x, x_batch, M, K, w, scales, nullptr, kBitsMxfp4, E, N,
+                      lhs_indices, rhs_indices, B, out, workspace, workspace_size,
+                      as_stream(stream));
+  }
   if (x_dtype != MLXR_MOE_BFLOAT16 || sb_dtype != MLXR_MOE_BFLOAT16 ||
       out_dtype != MLXR_MOE_BFLOAT16)
     return fail("gather_qmm: x, scales/biases and out must be bf16");

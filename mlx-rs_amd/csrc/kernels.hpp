@@ -41,6 +41,13 @@ hipError_t launch_dequantize(const uint32_t* wq, const void* scales,
                              int64_t cols, int group_size, int bits, void* out,
                              bool out_bf16, hipStream_t s);
 
+// ------------------------------------------------------------- mx_quant.hip
+// Mode "mxfp4" of the same (mx.hpp), over n flat values, whole groups of 32.
+hipError_t launch_mx_quantize(const void* w, bool w_bf16, int64_t n, uint32_t* wq,
+                              uint8_t* scales, hipStream_t s);
+hipError_t launch_mx_dequantize(const uint32_t* wq, const uint8_t* scales, int64_t n, void* out,
+                                bool out_bf16, hipStream_t s);
+
 // --------------------------------------------------------------- router.hip
 // Router weights: an f32 Linear [E, d] (bits == 0), a bf16 Linear (bits ==
 // 16), or a QuantizedLinear (bits 4 or 8, group 64): packed codes
@@ -193,7 +200,12 @@ hipError_t launch_dispatch_identity(int64_t n, int tile_rows,
 
 // ---------------------------------------------------------------- qgemm.hip
 // bits 4/8: packed codes plus scales and biases; bits 16: dense bf16
-// weights [E, N, K] (gather_mm), no scales or biases.
+// weights [E, N, K] (gather_mm), no scales or biases; kBitsMxfp4: e2m1 codes
+// [E, N, K/8], scales one byte per 32 [E, N, K/32] (behind the uint16_t pointer),
+// no biases.
+constexpr int kBitsMxfp4 = 0x104;
+// bits a weight takes
+__host__ __device__ constexpr int weight_bits(int bits) { return bits & 0xff; }
 struct QWeights {
   const uint32_t* w;       // [E, N, K*bits/32]
   const uint16_t* scales;  // [E, N, K/64] bf16
@@ -356,6 +368,15 @@ hipError_t launch_qgemm_prefill_reg(const QGemmArgs& a, int64_t x_rows, int64_t 
 hipError_t launch_qgemm_prefill_tall(const QGemmArgs& a, int64_t x_rows, int64_t max_tiles,
                                      hipStream_t s, const char* profile,
                                      const QGemmArgs* shared, int64_t shared_rows);
+
+// ------------------------------------------- mx_stream.hip, mx_tile.hip
+// launch_qgemm's kernels for kBitsMxfp4: work items (few rows per expert), and
+// M-tiles of tile_rows (64 or 128) rows.
+hipError_t launch_mx_stream(const QGemmArgs& a, int64_t max_items, const QGemmArgs* shared,
+                            int64_t shared_rows, const char* profile, hipStream_t s);
+hipError_t launch_mx_tile(const QGemmArgs& a, int64_t x_rows, int tile_rows, int64_t max_tiles,
+                          const QGemmArgs* shared, int64_t shared_rows, const char* profile,
+                          hipStream_t s);
 
 // -------------------------------------------------------------- combine.hip
 // out f32 [T, d], or bf16 when bf16 (the routing weights are then bf16

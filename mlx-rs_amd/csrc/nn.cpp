@@ -25,17 +25,22 @@ Status check_qlinear(const mlxr_moe_qlinear& q, int64_t experts, int64_t out,
   // bits 16: a dense bf16 SwitchLinear / Linear (weight [E, out, in] bf16,
   // no scales or biases; group_size unused)
   const bool dense = q.bits == 16;
+  // kBitsMxfp4: e2m1 codes, a scale byte per 32, no biases
+  const bool mx = q.bits == MLXR_MOE_BITS_MXFP4;
+  if (mx && (!q.weight || !q.scales || q.biases))
+    return Status::error(n + ": mode mxfp4 takes weight and scales, no biases");
   if (dense && (!q.weight || q.scales || q.biases))
     return Status::error(n + ": a dense (bits 16) weight takes no scales or "
                              "biases");
-  if (!dense && (!q.weight || !q.scales || !q.biases))
+  if (!dense && !mx && (!q.weight || !q.scales || !q.biases))
     return Status::error(n + ": weight, scales and biases are required "
                              "(affine mode)");
-  if (q.bits != 4 && q.bits != 8 && !dense)
+  if (q.bits != 4 && q.bits != 8 && !dense && !mx)
     return Status::error(n + ": bits must be 4 or 8 (16 for dense bf16 "
                              "weights), got " + std::to_string(q.bits));
-  if (!dense && q.group_size != 64)
-    return Status::error(n + ": group_size must be 64, got " +
+  const int group = mx ? 32 : 64;
+  if (!dense && q.group_size != group)
+    return Status::error(n + ": group_size must be " + std::to_string(group) + ", got " +
                          std::to_string(q.group_size));
   if (q.num_experts != experts || q.output_dims != out || q.input_dims != in)
     return Status::error(
@@ -50,7 +55,7 @@ Status check_qlinear(const mlxr_moe_qlinear& q, int64_t experts, int64_t out,
     return Status::error(n + ": input dims above " +
                          std::to_string(kMaxInputDims) + " are not supported");
   if ((reinterpret_cast<uintptr_t>(q.weight) & 15) ||
-      (reinterpret_cast<uintptr_t>(q.scales) & 1) ||
+      (!mx && (reinterpret_cast<uintptr_t>(q.scales) & 1)) ||
       (reinterpret_cast<uintptr_t>(q.biases) & 1))
     return Status::error(n + ": weight must be 16-byte aligned");
   if (dense && (int64_t)out * in * 2 >= ((int64_t)1 << 31))
@@ -256,9 +261,12 @@ PackedSwitchFfn::PackedSwitchFfn(const mlxr_moe_packed_switch_glu& w) : w_(w) {
   sw_.gate = qw(gu);
   sw_.up = sw_.gate;
   if (gu.weight && gu.bits > 0) {
-    const int64_t words = sw_.f * sw_.d * gu.bits / 32;
+    const int64_t words = sw_.f * sw_.d * weight_bits(gu.bits) / 32;
     sw_.up.w = gu.weight + words;
-    if (gu.bits != 16 && gu.scales && gu.biases) {
+    if (gu.bits == kBitsMxfp4 && gu.scales)  // one byte per 32
+      sw_.up.scales = reinterpret_cast<const uint16_t*>(
+          static_cast<const uint8_t*>(gu.scales) + sw_.f * (sw_.d / 32));
+    else if (gu.bits != 16 && gu.scales && gu.biases) {
       const int64_t g = sw_.d / (gu.group_size > 0 ? gu.group_size : 64);
       sw_.up.scales = sw_.gate.scales + sw_.f * g;
       sw_.up.biases = sw_.gate.biases + sw_.f * g;

@@ -72,16 +72,18 @@ bool prefill_supported(const QGemmArgs& a, int64_t x_rows) {
   // buffer offsets are 32-bit: x, and one expert's weights, under 2 GB
   // outputs leave as 16-byte runs of a row
   const bool out16 = (reinterpret_cast<uintptr_t>(a.out) & 15) == 0 && a.out_ld % 8 == 0;
-  return (a.bits == 4 || a.bits == 8 || a.bits == 16) && a.K % 64 == 0 && a.N % 64 == 0 &&
+  return (a.bits == 4 || a.bits == 8 || a.bits == 16 || a.bits == kBitsMxfp4) && a.K % 64 == 0 && a.N % 64 == 0 &&
          a.sorted != nullptr && out16 && a.row_div >= 1 && a.row_div <= 65536 &&
          x_rows * a.x_ld * 2 < ((int64_t)1 << 31) &&
-         (int64_t)a.N * a.K * a.bits / 8 < ((int64_t)1 << 31);
+         (int64_t)a.N * a.K * weight_bits(a.bits) / 8 < ((int64_t)1 << 31);
 }
 
 hipError_t launch_qgemm_prefill(const QGemmArgs& a, int64_t x_rows,
                                 int tile_rows, int64_t max_tiles,
                                 hipStream_t s, const char* profile,
                                 const QGemmArgs* shared, int64_t shared_rows) {
+  if (a.bits == kBitsMxfp4)
+    return launch_mx_tile(a, x_rows, tile_rows, max_tiles, shared, shared_rows, profile, s);
   if (tile_rows == kPrefillMinTileRows)
     return launch_qgemm_prefill_reg(a, x_rows, max_tiles, s, profile, shared, shared_rows);
   if (a.bits != 16)

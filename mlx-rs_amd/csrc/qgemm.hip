@@ -533,6 +533,11 @@ int work_rows_for(int64_t n, int64_t E, std::initializer_list<const QGemmArgs*> 
   if (!wide_items_possible(n, E)) return kWorkRows;
   const int64_t items = dispatch_max_work(n, E, kWorkRowsWide);
   for (const QGemmArgs* g : gemms) {
+    if (g->bits == kBitsMxfp4) {
+      // (16 rows of x in LDS leave room for two workgroups a CU up to here)
+      if (g->K > 2048) return kWorkRows;
+      continue;
+    }
     if (g->bits == 16 || !(g->K <= kWideWhole || g->K % kWideSlice == 0) ||
         items * (g->N / 16) < kStreamMinBlocks)
       return kWorkRows;
@@ -566,6 +571,8 @@ hipError_t launch_qgemm(const QGemmArgs& a, int64_t total_rows,
                                 dispatch_max_tiles(total_rows, a.E, tile_rows), s, profile,
                                 shared, shared_rows);
   }
+  if (a.bits == kBitsMxfp4)
+    return launch_mx_stream(a, max_items, shared, shared_rows, profile, s);
   const int groups = a.K / 64;
   // Many (expert, block) items: the streaming kernel (one block per wave,
   // x in LDS, a ring of weight loads).  Few: the split-K kernel below, which

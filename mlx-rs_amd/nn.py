@@ -24,6 +24,13 @@ from . import ops
 from ._capi import MlxrMoeError
 
 
+def _group_size(group_size, mode):
+    """The given group size, or the mode's own."""
+    if group_size is not None:
+        return group_size
+    return ops.MXFP4_GROUP_SIZE if mode == "mxfp4" else ops.DEFAULT_GROUP_SIZE
+
+
 class SwitchLinear:
     """Expert-stacked dense linear (the unquantised MaybeQuantized slot):
     weight bf16 [E, out, in], applied with gather_mm (switch.rs:84-93).  No
@@ -54,9 +61,9 @@ class SwitchLinear:
         """SwitchLinear::apply (switch.rs:84-93)."""
         return ops.gather_mm(x, self.weight, None, indices, sorted)
 
-    def try_into_quantized(self, group_size=64, bits=4):
+    def try_into_quantized(self, group_size=None, bits=4, mode="affine"):
         """Quantizable::try_into_quantized (switch.rs:96-113)."""
-        return QuantizedSwitchLinear.try_from_switch_linear(self.weight, group_size, bits)
+        return QuantizedSwitchLinear.try_from_switch_linear(self.weight, group_size, bits, mode)
 
     def descriptor(self) -> C.QLinear:
         return C.QLinear(self.weight.data_ptr(), None, None, self.num_experts,
@@ -70,8 +77,8 @@ class Linear(SwitchLinear):
     def __init__(self, weight):
         super().__init__(weight.reshape((1,) + tuple(weight.shape)))
 
-    def try_into_quantized(self, group_size=64, bits=4):
-        return QuantizedLinear.try_from_linear(self.weight[0], group_size, bits)
+    def try_into_quantized(self, group_size=None, bits=4, mode="affine"):
+        return QuantizedLinear.try_from_linear(self.weight[0], group_size, bits, mode)
 
     def forward(self, x):
         """x @ weight^T in bf16 (layers/linear.rs:91-95)."""
@@ -84,22 +91,32 @@ class Linear(SwitchLinear):
 
 class QuantizedSwitchLinear:
     """Expert-stacked quantised linear: weight [E, out, in*bits/32] (int32
-    storage of uint32 words), scales/biases bf16 [E, out, in/group]."""
+    storage of uint32 words), scales/biases bf16 [E, out, in/group].  Mode
+    "mxfp4" (group_size 32, bits 4): scales uint8 [E, out, in/32], biases
+    None."""
 
-    def __init__(self, weight, scales, biases, group_size=64, bits=4):
+    def __init__(self, weight, scales, biases=None, group_size=None, bits=4, mode="affine"):
         if weight.ndim != 3:
             raise MlxrMoeError("QuantizedSwitchLinear weight must be [E, out, packed_in]")
+        if ops._check_mode(mode):
+            ops._check_mxfp4("QuantizedSwitchLinear", weight, scales, biases)
+            if group_size not in (None, ops.MXFP4_GROUP_SIZE) or bits != 4:
+                raise MlxrMoeError("QuantizedSwitchLinear: mode mxfp4 takes group_size 32 and "
+                                   f"bits 4, got {group_size} and {bits}")
+        elif biases is None:
+            raise MlxrMoeError("QuantizedSwitchLinear: biases are required (affine mode)")
         self.weight = weight.contiguous()
         self.scales = scales.contiguous()
-        self.biases = biases.contiguous()
-        self.group_size = group_size
+        self.biases = None if biases is None else biases.contiguous()
+        self.mode = mode
+        self.group_size = _group_size(group_size, mode)
         self.bits = bits
 
     @classmethod
-    def try_from_switch_linear(cls, weight, group_size=64, bits=4):
+    def try_from_switch_linear(cls, weight, group_size=None, bits=4, mode="affine"):
         """QuantizedSwitchLinear::try_from_switch_linear (switch.rs:129-145)."""
-        wq, s, b = ops.quantize(weight, group_size, bits)
-        return cls(wq, s, b, group_size, bits)
+        wq, s, b = ops.quantize(weight, _group_size(group_size, mode), bits, mode)
+        return cls(wq, s, b, group_size, bits, mode)
 
     @property
     def num_experts(self):
@@ -116,28 +133,29 @@ class QuantizedSwitchLinear:
     def apply(self, x, indices, sorted=False):
         """QuantizedSwitchLinear::apply (switch.rs:148-167)."""
         return ops.gather_qmm(x, self.weight, self.scales, self.biases, None, indices, True,
-                              self.group_size, self.bits, sorted)
+                              self.group_size, self.bits, sorted, self.mode)
 
     def descriptor(self) -> C.QLinear:
-        return C.QLinear(self.weight.data_ptr(), self.scales.data_ptr(), self.biases.data_ptr(),
+        return C.QLinear(self.weight.data_ptr(), self.scales.data_ptr(), _ptr(self.biases),
                          self.num_experts, self.output_dims, self.input_dims,
-                         self.group_size, self.bits)
+                         self.group_size, C.BITS_MXFP4 if self.mode == "mxfp4" else self.bits)
 
 
 class QuantizedLinear(QuantizedSwitchLinear):
     """A single quantised linear (weight [out, in*bits/32]) seen as one
     expert."""
 
-    def __init__(self, weight, scales, biases, group_size=64, bits=4):
+    def __init__(self, weight, scales, biases=None, group_size=None, bits=4, mode="affine"):
         super().__init__(weight.reshape((1,) + tuple(weight.shape)),
                          scales.reshape((1,) + tuple(scales.shape)),
-                         biases.reshape((1,) + tuple(biases.shape)), group_size, bits)
+                         None if biases is None else biases.reshape((1,) + tuple(biases.shape)),
+                         group_size, bits, mode)
 
     @classmethod
-    def try_from_linear(cls, weight, group_size=64, bits=4):
+    def try_from_linear(cls, weight, group_size=None, bits=4, mode="affine"):
         """QuantizedLinear::try_from_linear (layers/quantized.rs:249-273)."""
-        wq, s, b = ops.quantize(weight, group_size, bits)
-        return cls(wq, s, b, group_size, bits)
+        wq, s, b = ops.quantize(weight, _group_size(group_size, mode), bits, mode)
+        return cls(wq, s, b, group_size, bits, mode)
 
     def forward(self, x):
         """quantized_matmul(x, w, transpose=true) (layers/quantized.rs:356-373)."""
@@ -145,7 +163,7 @@ class QuantizedLinear(QuantizedSwitchLinear):
         x2 = x.reshape(-1, 1, x.shape[-1])
         idx = torch.zeros(x2.shape[0], dtype=torch.int32, device=x.device)
         y = ops.gather_qmm(x2, self.weight, self.scales, self.biases, None, idx, True,
-                           self.group_size, self.bits)
+                           self.group_size, self.bits, mode=self.mode)
         return y.reshape(lead + (self.output_dims,))
 
 
@@ -189,12 +207,12 @@ class SplitSwitchFfn:
                                  down_proj.descriptor())
 
     @classmethod
-    def from_dense(cls, gate_w, up_w, down_w, group_size=64, bits=4):
+    def from_dense(cls, gate_w, up_w, down_w, group_size=None, bits=4, mode="affine"):
         """Quantise dense expert weights, as try_into_quantized does
         (switch.rs:478-491)."""
         q = QuantizedSwitchLinear.try_from_switch_linear
-        return cls(q(gate_w, group_size, bits), q(up_w, group_size, bits),
-                   q(down_w, group_size, bits))
+        return cls(q(gate_w, group_size, bits, mode), q(up_w, group_size, bits, mode),
+                   q(down_w, group_size, bits, mode))
 
     def descriptor(self) -> C.SwitchGlu:
         return self._desc
@@ -260,10 +278,12 @@ class PackedSwitchFfn:
                                        C.ACT_GEGLU if activation == "geglu" else C.ACT_SWIGLU)
 
     @classmethod
-    def from_dense(cls, gate_up_w, down_w, group_size=64, bits=4, activation="geglu"):
+    def from_dense(cls, gate_up_w, down_w, group_size=None, bits=4, activation="geglu",
+                   mode="affine"):
         """Quantise dense expert weights (try_into_quantized, switch.rs:323-335)."""
         q = QuantizedSwitchLinear.try_from_switch_linear
-        return cls(q(gate_up_w, group_size, bits), q(down_w, group_size, bits), activation)
+        return cls(q(gate_up_w, group_size, bits, mode), q(down_w, group_size, bits, mode),
+                   activation)
 
     def descriptor(self) -> C.PackedSwitchGlu:
         return self._desc

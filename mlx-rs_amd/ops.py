@@ -23,6 +23,16 @@ from ._capi import MlxrMoeError
 
 DEFAULT_GROUP_SIZE = 64
 DEFAULT_BITS = 4
+# mode "mxfp4": e2m1 codes, a power-of-two scale byte per 32
+MXFP4_GROUP_SIZE = 32
+MODES = ("affine", "mxfp4")
+
+
+def _check_mode(mode: str) -> bool:
+    """True for mode "mxfp4"."""
+    if mode not in MODES:
+        raise MlxrMoeError(f"unsupported quantization mode {mode!r} (only {MODES})")
+    return mode == "mxfp4"
 
 
 def _p(t):
@@ -31,6 +41,22 @@ def _p(t):
 
 def _stream(t: torch.Tensor):
     return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+
+
+class _on:
+    """The tensor's device as the current one (kernels are launched there)."""
+
+    def __init__(self, t: torch.Tensor):
+        self.want = t.device.index
+
+    def __enter__(self):
+        self.was = torch.cuda.current_device()
+        if self.was != self.want:
+            torch.cuda.set_device(self.want)
+
+    def __exit__(self, *exc):
+        if self.was != self.want:
+            torch.cuda.set_device(self.was)
 
 
 def _code(t: torch.Tensor) -> int:
@@ -89,9 +115,13 @@ def _check_x_batch(name: str, x_batch_shape, idx_shape):
             f"{tuple(idx_shape)} followed by singletons (or pass lhs_indices)")
 
 
-def quantize(w: torch.Tensor, group_size=None, bits=None):
+def quantize(w: torch.Tensor, group_size=None, bits=None, mode="affine"):
     """(w_q, scales, biases) of MLX affine quantisation along the last axis.
-    w_q is int32 storage of mlx's uint32 words."""
+    w_q is int32 storage of mlx's uint32 words.  Mode "mxfp4" (group_size 32,
+    4 bits): e2m1 codes, scales uint8 (the exponent of a power of two plus
+    127; 255 is NaN), biases None."""
+    if _check_mode(mode):
+        return _quantize_mxfp4(w, group_size, bits)
     _dev(w)
     w = w.contiguous()
     gs = DEFAULT_GROUP_SIZE if group_size is None else group_size
@@ -111,10 +141,59 @@ def quantize(w: torch.Tensor, group_size=None, bits=None):
     return wq, sc, bi
 
 
+def _quantize_mxfp4(w, group_size, bits):
+    _dev(w)
+    w = w.contiguous()
+    cols = w.shape[-1] if w.ndim else 0
+    rows = w.numel() // cols if cols else 0
+    lead = tuple(w.shape[:-1])
+    ok = cols > 0 and cols % MXFP4_GROUP_SIZE == 0  # (else the library says what is wrong)
+    wq = torch.empty(lead + (cols // 8,) if ok else 1, dtype=torch.int32, device=w.device)
+    sc = torch.empty(lead + (cols // MXFP4_GROUP_SIZE,) if ok else 1, dtype=torch.uint8,
+                     device=w.device)
+    with _on(w):
+        C.check(C.lib().mlxr_moe_quantize(
+            _p(w), _code(w), rows, cols, C.OptionalInt.of(group_size), C.OptionalInt.of(bits),
+            b"mxfp4", _p(wq), _p(sc), None, _stream(w)))
+    return wq, sc, None
+
+
+def _check_mxfp4(name, w, scales, biases):
+    """w [.., K/8] words and scales [.., K/32] bytes of the same rows: the C
+    ABI reads that much of both."""
+    if biases is not None:
+        raise MlxrMoeError(f"{name}: mode mxfp4 has no biases")
+    if w.dtype not in (torch.int32, torch.uint32) or scales.dtype != torch.uint8:
+        raise MlxrMoeError(f"{name}: mode mxfp4 takes 32-bit words and uint8 scales, got "
+                           f"{w.dtype} and {scales.dtype}")
+    if (w.ndim < 1 or w.ndim != scales.ndim or w.shape[:-1] != scales.shape[:-1]
+            or w.shape[-1] * 8 != scales.shape[-1] * MXFP4_GROUP_SIZE):
+        raise MlxrMoeError(f"{name}: scales {tuple(scales.shape)} must hold one byte for each "
+                           f"four words of w {tuple(w.shape)}")
+
+
+def _dequantize_mxfp4(w, scales, biases, group_size, bits, out_dtype):
+    _dev(w, scales)
+    _check_mxfp4("dequantize", w, scales, biases)
+    w, scales = w.contiguous(), scales.contiguous()
+    cols = w.shape[-1] * 8
+    rows = w.numel() // w.shape[-1] if cols else 0
+    out = torch.empty(tuple(w.shape[:-1]) + (cols,), dtype=out_dtype or torch.bfloat16,
+                      device=w.device)
+    with _on(w):
+        C.check(C.lib().mlxr_moe_dequantize(
+            _p(w), _p(scales), None, C.UINT8, rows, cols, C.OptionalInt.of(group_size),
+            C.OptionalInt.of(bits), b"mxfp4", _p(out), _code(out), _stream(w)))
+    return out
+
+
 def dequantize(w: torch.Tensor, scales: torch.Tensor, biases=None, group_size=None,
-               bits=None, out_dtype=None):
+               bits=None, out_dtype=None, mode="affine"):
     """code * scale + bias (one fused multiply-add, rounded once) in scales'
-    dtype unless out_dtype is given."""
+    dtype unless out_dtype is given.  Mode "mxfp4": code * scale, exact, in
+    bf16 unless out_dtype is given."""
+    if _check_mode(mode):
+        return _dequantize_mxfp4(w, scales, biases, group_size, bits, out_dtype)
     _dev(w, scales, biases)
     b = DEFAULT_BITS if bits is None else bits
     cols = w.shape[-1] * 32 // b
@@ -130,12 +209,15 @@ def dequantize(w: torch.Tensor, scales: torch.Tensor, biases=None, group_size=No
 
 
 def gather_qmm(x, w, scales, biases=None, lhs_indices=None, rhs_indices=None,
-               transpose=True, group_size=None, bits=None, sorted_indices=False):
+               transpose=True, group_size=None, bits=None, sorted_indices=False,
+               mode="affine"):
     """out[b] = x[xb(b)] @ dequant(w[rhs_indices[b]])^T.
 
     x [..., M, K] bf16; w [E, N, K*bits/32]; output rhs_indices.shape +
     [M, N].  Without lhs_indices, x's batch broadcasts over the trailing
-    index axis (x [.., T, 1, 1, K] against indices [.., T, top_k])."""
+    index axis (x [.., T, 1, 1, K] against indices [.., T, top_k]).  Mode
+    "mxfp4": scales uint8 [E, N, K/32], no biases."""
+    mx = _check_mode(mode)
     if rhs_indices is None:
         raise MlxrMoeError("gather_qmm: rhs_indices are required")
     if lhs_indices is None and rhs_indices.numel():
@@ -146,6 +228,10 @@ def gather_qmm(x, w, scales, biases=None, lhs_indices=None, rhs_indices=None,
     M, K = x.shape[-2], x.shape[-1]
     x_batch = math.prod(x.shape[:-2])
     E, N = w.shape[0], w.shape[1]
+    if mx:
+        _check_mxfp4("gather_qmm", w, scales, biases)
+        if w.ndim != 3:
+            raise MlxrMoeError("gather_qmm: w must be [E, N, K/8]")
     if w.shape[-1] * 32 != K * b and transpose:
         raise MlxrMoeError(
             f"gather_qmm: w last dim {w.shape[-1]} does not match K={K} at {b} bits")
@@ -158,12 +244,14 @@ def gather_qmm(x, w, scales, biases=None, lhs_indices=None, rhs_indices=None,
     lib = C.lib()
     nbytes = lib.mlxr_moe_gather_qmm_workspace_size(B, M, E)
     ws = workspace(nbytes, x.device)
-    C.check(lib.mlxr_moe_gather_qmm(
-        _p(x), _code(x), x_batch, M, K, _p(w.contiguous()), _p(scales.contiguous()),
-        _p(None if biases is None else biases.contiguous()), _code(scales), E, N,
-        _p(lhs), _p(rhs), B, int(bool(transpose)), C.OptionalInt.of(group_size),
-        C.OptionalInt.of(bits), b"affine", int(bool(sorted_indices)), _p(out), C.BFLOAT16,
-        _p(ws), ws.numel(), _stream(x)))
+    with _on(x):
+        C.check(lib.mlxr_moe_gather_qmm(
+            _p(x), _code(x), x_batch, M, K, _p(w.contiguous()), _p(scales.contiguous()),
+            _p(None if biases is None else biases.contiguous()),
+            C.UINT8 if mx else _code(scales), E, N,
+            _p(lhs), _p(rhs), B, int(bool(transpose)), C.OptionalInt.of(group_size),
+            C.OptionalInt.of(bits), mode.encode(), int(bool(sorted_indices)), _p(out),
+            C.BFLOAT16, _p(ws), ws.numel(), _stream(x)))
     out._mlxr_workspace = ws  # keep the status word alive with the result
     return out
 

@@ -1,0 +1,570 @@
+"""Mode "mxfp4" (microscaled 4-bit weights): quantise, dequantise, gather_qmm
+and the expert modules, against plain 64-bit restatements of their formulas.
+
+Tolerances: a bf16 result is off by half a step of its value at most, 2^-8 of
+it; a sum of K products in f32 by K * 2^-23 of the sum of their magnitudes at
+most (each of K additions by a step of what has been added so far).  Quantised
+and dequantised values are exact.
+"""
+import ctypes
+
+import pytest
+import torch
+
+E2M1 = [0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0]
+gpu = pytest.mark.gpu
+
+
+# ------------------------------------------------------------ 64-bit formulas
+def values64(wq, sc):
+    """The weights of packed words [.., K/8] and scale bytes [.., K/32]."""
+    table = torch.tensor(E2M1 + [-v for v in E2M1], dtype=torch.float64)
+    words = wq.cpu().long() & 0xFFFFFFFF
+    code = torch.stack([(words >> (4 * i)) & 15 for i in range(8)], -1).flatten(-2)
+    b = sc.cpu().long()
+    scale = ((b + 896) << 52).view(torch.float64)  # 2^(b - 127)
+    scale = torch.where(b == 255, torch.full_like(scale, float("nan")), scale)
+    return table[code] * scale.repeat_interleave(32, -1)
+
+
+def quantise64(w):
+    """(values, scale bytes) of the nearest representable weights, by search
+    over the eight magnitudes."""
+    v = w.cpu().double().unflatten(-1, (-1, 32))
+    big = v.abs().amax(-1)
+    bad = ~torch.isfinite(v).all(-1)
+    ok = torch.where(bad, torch.ones_like(big), big)
+    # floor(log2 big) from the f64's exponent field (big is a normal f64 or 0)
+    ex = ((ok.view(torch.int64) >> 52) & 0x7FF) - 1023
+    byte = (ex - 2 + 127).clamp_min(0)
+    unit = ((byte + 896) << 52).view(torch.float64)
+    a = v.abs() / unit[..., None]
+    mags = torch.tensor(E2M1, dtype=torch.float64)
+    d = (a[..., None] - mags).abs()
+    best = d.amin(-1, keepdim=True)
+    # ties: the even code
+    odd = torch.arange(8) % 2
+    code = torch.where(d == best, odd, 2).argmin(-1)
+    out = torch.copysign(mags[code], v) * unit[..., None]
+    out = torch.where(bad[..., None], torch.full_like(out, float("nan")), out)
+    return out.flatten(-2), torch.where(bad, torch.full_like(byte, 255), byte)
+
+
+def bank(g, shape, std=0.02):
+    """Random codes and scales around std: [E, N, K/8] int32, [E, N, K/32]."""
+    E, N, K = shape
+    wq = torch.randint(-2 ** 31, 2 ** 31 - 1, (E, N, K // 8), generator=g, dtype=torch.int64)
+    base = 127 + int(torch.tensor(std / 3.0).log2().floor())
+    sc = torch.randint(base - 2, base + 3, (E, N, K // 32), generator=g)
+    return wq.to(torch.int32), sc.to(torch.uint8)
+
+
+def check_sum(y, x64, w64, K):
+    """y [.., N] against x64 [.., K] @ w64 [N, K]^T, one bf16 rounding of an
+    f32 sum."""
+    want = x64 @ w64.t()
+    mass = x64.abs() @ w64.abs().t()
+    err = (y.double() - want).abs()
+    slack = K * 2.0 ** -23 * mass
+    bound = 2.0 ** -8 * (want.abs() + slack) + slack
+    worst = float((err - bound).max()) if err.numel() else -1.0
+    assert worst <= 0, f"error {float(err.max()):.3e} past its bound by {worst:.3e}"
+
+
+# ------------------------------------------------------------------ refusals
+def test_quantize_and_dequantize_refuse(pkg):
+    lib, C = pkg._capi.lib(), pkg._capi
+    OI = C.OptionalInt
+
+    def q(gs=None, bits=None, cols=64, dt=C.BFLOAT16, biases=None, w=16, wq=16):
+        return lib.mlxr_moe_quantize(w, dt, 4, cols, OI.of(gs), OI.of(bits), b"mxfp4", wq, 16,
+                                     biases, None)
+
+    assert q(gs=64) == -1 and "group_size 32" in C.last_error()
+    assert q(bits=8) == -1 and "bits 4" in C.last_error()
+    assert q(cols=48) == -1 and "multiple of group_size 32" in C.last_error()
+    assert q(dt=C.UINT8) == -1 and "dtype" in C.last_error()
+    assert q(biases=16) == -1 and "no biases" in C.last_error()
+    assert q(w=None) == -1 and "null array" in C.last_error()
+    assert q(w=17) == -1 and "aligned" in C.last_error()
+    assert q(wq=18) == -1 and "aligned" in C.last_error()
+
+    def dq(dt=C.UINT8, biases=None, cols=64, out=16, odt=C.FLOAT32, bits=None):
+        return lib.mlxr_moe_dequantize(16, 16, biases, dt, 4, cols, OI.of(32), OI.of(bits),
+                                       b"mxfp4", out, odt, None)
+
+    assert dq(dt=C.BFLOAT16) == -1 and "uint8 scales" in C.last_error()
+    assert dq(biases=16) == -1 and "no biases" in C.last_error()
+    assert dq(cols=40) == -1 and "bad shape" in C.last_error()
+    assert dq(bits=8) == -1 and "bits 4" in C.last_error()
+    assert dq(out=None) == -1 and "null array" in C.last_error()
+    assert dq(out=18) == -1 and "aligned" in C.last_error()
+    assert dq(odt=C.UINT8) == -1 and "out" in C.last_error()
+    # an empty array needs no memory
+    assert lib.mlxr_moe_quantize(None, C.BFLOAT16, 0, 64, OI.of(None), OI.of(None), b"mxfp4",
+                                 None, None, None, None) == 0
+    assert lib.mlxr_moe_quantize(16, C.BFLOAT16, 4, 64, OI.of(None), OI.of(None), b"nvfp4", 16,
+                                 16, None, None) == -1
+    assert "mode" in C.last_error()
+
+
+def test_gather_qmm_refuses(pkg):
+    lib, C = pkg._capi.lib(), pkg._capi
+    OI = C.OptionalInt
+
+    def call(K=128, N=64, sdt=C.UINT8, biases=None, scales=16, x=16, w=16, gs=None, bits=None,
+             transpose=1, rhs=16, E=4):
+        return lib.mlxr_moe_gather_qmm(x, C.BFLOAT16, 1, 1, K, w, scales, biases, sdt, E, N,
+                                       None, rhs, 1, transpose, OI.of(gs), OI.of(bits), b"mxfp4",
+                                       0, 16, C.BFLOAT16, None, 0, None)
+
+    assert call(sdt=C.BFLOAT16) == -1 and "uint8 scales" in C.last_error()
+    assert call(biases=16) == -1 and "no biases" in C.last_error()
+    assert call(scales=None) == -1 and "null array" in C.last_error()
+    assert call(gs=64) == -1 and "group_size 32" in C.last_error()
+    assert call(bits=8) == -1 and "bits 4" in C.last_error()
+    assert call(transpose=0) == -1 and "transpose" in C.last_error()
+    assert call(K=96) == -1 and "multiples of 64" in C.last_error()
+    assert call(N=96) == -1 and "multiples of 64" in C.last_error()
+    assert call(K=4160) == -1 and "K above" in C.last_error()
+    assert call(E=1025) == -1 and "num_experts" in C.last_error()
+    assert call(x=8) == -1 and "aligned" in C.last_error()
+    assert call(w=None) == -1 and "null array" in C.last_error()
+    assert call() == -1 and "workspace" in C.last_error()
+
+
+def test_descriptors_refuse(pkg):
+    C = pkg._capi
+    lib = C.lib()
+    M = C.BITS_MXFP4
+    gate = C.QLinear(16, 16, None, 8, 256, 512, 32, M)
+    down = C.QLinear(16, 16, None, 8, 512, 256, 32, M)
+
+    def glu(g, u, d):
+        ffn = C.SwitchGlu(g, u, d)
+        return lib.mlxr_moe_switch_glu_forward(ctypes.byref(ffn), None, 1, None, None, 2, None,
+                                               None, 0, None)
+
+    assert glu(gate, gate, down) == -1 and "null array" in C.last_error()
+    assert glu(C.QLinear(16, 16, 16, 8, 256, 512, 32, M), gate, down) == -1
+    assert "no biases" in C.last_error()
+    assert glu(C.QLinear(16, None, None, 8, 256, 512, 32, M), gate, down) == -1
+    assert "weight and scales" in C.last_error()
+    assert glu(C.QLinear(16, 16, None, 8, 256, 512, 64, M), gate, down) == -1
+    assert "group_size must be 32" in C.last_error()
+    assert glu(gate, gate, C.QLinear(16, 16, 16, 8, 512, 256, 64, 4)) == -1
+    assert "share bits" in C.last_error()
+    # routers and gates stay affine, dense or f32
+    g = C.QLinear(16, 16, None, 1, 128, 2048, 32, M)
+    assert lib.mlxr_moe_router_topk_quantized(None, 1, ctypes.byref(g), 8, None, None, None, 0,
+                                              None) == -1
+    assert "bits must be 4 or 8" in C.last_error()
+
+
+def test_python_refuses(pkg):
+    ops, nn, Err = pkg.ops, pkg.nn, pkg.MlxrMoeError
+    wq = torch.zeros((4, 64, 16), dtype=torch.int32)
+    sc = torch.zeros((4, 64, 4), dtype=torch.uint8)
+    with pytest.raises(Err, match="mode"):
+        ops.quantize(torch.zeros(2, 64), mode="nvfp4")
+    with pytest.raises(Err, match="ROCm device"):
+        ops.quantize(torch.zeros(2, 64), mode="mxfp4")
+    with pytest.raises(Err, match="no biases"):
+        nn.QuantizedSwitchLinear(wq, sc, sc, mode="mxfp4")
+    with pytest.raises(Err, match="uint8"):
+        nn.QuantizedSwitchLinear(wq, sc.bfloat16(), mode="mxfp4")
+    with pytest.raises(Err, match="one byte"):
+        nn.QuantizedSwitchLinear(wq, sc[:, :, :3], mode="mxfp4")
+    with pytest.raises(Err, match="one byte"):
+        nn.QuantizedSwitchLinear(wq, sc[:2], mode="mxfp4")
+    with pytest.raises(Err, match="group_size 32"):
+        nn.QuantizedSwitchLinear(wq, sc, None, 64, 4, "mxfp4")
+    with pytest.raises(Err, match="biases are required"):
+        nn.QuantizedSwitchLinear(wq, sc.bfloat16())
+    m = nn.QuantizedSwitchLinear(wq, sc, mode="mxfp4")
+    d = m.descriptor()
+    assert (d.bits, d.group_size, d.biases, d.input_dims) == (0x104, 32, None, 128)
+
+
+# ------------------------------------------------------ quantise, dequantise
+@gpu
+def test_every_code_and_scale(pkg, dev):
+    """All 16 codes under all 256 scale bytes, to f32 and bf16."""
+    code = torch.arange(32) % 16
+    words = sum(code.view(4, 8)[:, i] << (4 * i) for i in range(8))
+    words = torch.where(words >= 2 ** 31, words - 2 ** 32, words).to(torch.int32)
+    wq = words.repeat(256, 1).contiguous()
+    sc = torch.arange(256).to(torch.uint8)[:, None]
+    want = values64(wq, sc)
+    for dt in (torch.float32, torch.bfloat16):
+        got = pkg.ops.dequantize(wq.to(dev), sc.to(dev), mode="mxfp4", out_dtype=dt).cpu()
+        ref = want.to(dt)  # exact, or an infinity past the type's range
+        assert torch.equal(torch.isnan(got), torch.isnan(ref))
+        ok = ~torch.isnan(ref)
+        assert torch.equal(got[ok], ref[ok])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("shape", [(1, 32), (3, 64), (2, 5, 96), (7, 2048), (1, 509, 2080)])
+def test_quantise_is_nearest(pkg, dev, dtype, shape):
+    g = torch.Generator().manual_seed(sum(shape))
+    w = (torch.randn(shape, generator=g) * 0.02).to(dtype)
+    w.view(-1)[:32] = 0.0  # a group of zeros
+    wq, sc, bi = pkg.ops.quantize(w.to(dev), mode="mxfp4")
+    assert bi is None and wq.shape == shape[:-1] + (shape[-1] // 8,)
+    want, byte = quantise64(w)
+    assert torch.equal(sc.cpu().long(), byte)
+    assert torch.equal(values64(wq, sc), want)
+    back = pkg.ops.dequantize(wq, sc, mode="mxfp4", out_dtype=dtype)
+    assert torch.equal(back.cpu().double(), want)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_quantise_borders_and_extremes(pkg, dev, dtype):
+    """Midpoints between neighbours, magnitudes past 6, subnormal groups,
+    groups with one large value, infinities and NaN."""
+    rows = []
+    for scale in (1.0, 2.0 ** -20, 2.0 ** 100, 2.0 ** -118):
+        mid = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0, 7.0, 7.9375])
+        near = torch.cat([mid, mid * (1 + 2 ** -7), mid * (1 - 2 ** -7)])
+        rows.append(torch.cat([near * scale, torch.tensor([4.0, -6.0]) * scale]))
+    tiny = torch.arange(32) * 2.0 ** -130
+    rows += [tiny, -tiny, torch.arange(32) * 2.0 ** -127, torch.full((32,), 2.0 ** -126)]
+    one = torch.zeros(32)
+    one[17] = 3.0e38
+    rows.append(one)
+    for bad in (float("inf"), float("-inf"), float("nan")):
+        r = torch.ones(32)
+        r[5] = bad
+        rows.append(r)
+    w = torch.stack(rows).to(dtype)
+    wq, sc, _ = pkg.ops.quantize(w.to(dev), mode="mxfp4")
+    want, byte = quantise64(w)
+    assert torch.equal(sc.cpu().long(), byte)
+    got = values64(wq, sc)
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    ok = ~torch.isnan(want)
+    assert torch.equal(got[ok], want[ok])
+    assert bool((wq.cpu()[-3:] == 0).all())  # a bad group's codes
+
+
+@gpu
+def test_quantise_strided_and_unaligned(pkg, dev):
+    w = torch.randn(6, 128, device=dev)
+    q = pkg.ops.quantize
+    a = q(w[::2, 64:], mode="mxfp4")
+    b = q(w[::2, 64:].contiguous(), mode="mxfp4")
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    for dt in (torch.float32, torch.bfloat16):
+        flat = torch.randn(1 + 64 * 3, device=dev).to(dt)
+        v = flat[1:].view(3, 64)  # not 16-byte aligned
+        a, b = q(v, mode="mxfp4"), q(v.clone(), mode="mxfp4")
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+# ------------------------------------------------------------------- product
+def gather_case(pkg, dev, E, N, K, idx, x, seed=0, lhs=None, wq_sc=None):
+    g = torch.Generator().manual_seed(seed)
+    wq, sc = wq_sc if wq_sc is not None else bank(g, (E, N, K))
+    kw = {"lhs_indices": lhs.to(dev)} if lhs is not None else {}
+    y = pkg.ops.gather_qmm(x.to(dev), wq.to(dev), sc.to(dev), rhs_indices=idx.to(dev),
+                           mode="mxfp4", **kw).cpu()
+    return y, wq, sc
+
+
+@gpu
+@pytest.mark.parametrize("K", [64, 128, 192, 320, 768, 2048, 4096])
+@pytest.mark.parametrize("T,topk", [(1, 1), (1, 8), (3, 2), (9, 8), (40, 4)])
+def test_gather_few_rows(pkg, dev, K, T, topk):
+    """Work items: one row, a few, more than one item per expert; input dims
+    that end inside a step; one 64-channel tile and several."""
+    E, N = 11, 64 if K % 128 else 192
+    g = torch.Generator().manual_seed(K + T)
+    x = torch.randn((T, 1, 1, K), generator=g).bfloat16()
+    idx = torch.randint(0, E, (T, topk), generator=g, dtype=torch.int32)
+    idx[T // 2:] = idx[T // 2, 0]  # crowd one expert, the same one several times a row
+    y, wq, sc = gather_case(pkg, dev, E, N, K, idx, x, K)
+    w64 = values64(wq, sc)
+    for e in idx.unique().tolist():
+        t, k = (idx == e).nonzero(as_tuple=True)
+        check_sum(y[t, k, 0], x[t, 0, 0].double(), w64[e], K)
+
+
+@gpu
+@pytest.mark.parametrize("E,N,K,T,topk,skew", [
+    (4, 64, 64, 300, 2, 0),        # one N-tile, one x stage
+    (8, 192, 192, 200, 4, 0),      # part of a line, part of an N-tile
+    (8, 320, 768, 150, 4, 1),      # skewed: one expert takes most rows
+    (16, 768, 2048, 130, 4, 0),    # 64-row tiles
+    (3, 256, 512, 333, 2, 0),      # 128-row tiles, a ragged last one
+    (5, 448, 4096, 70, 8, 0),      # the largest input dim
+    (2, 64, 320, 777, 1, 1),
+])
+def test_gather_many_rows(pkg, dev, E, N, K, T, topk, skew):
+    g = torch.Generator().manual_seed(E * N + K)
+    x = torch.randn((T, 1, 1, K), generator=g).bfloat16()
+    idx = torch.randint(0, E, (T, topk), generator=g, dtype=torch.int32)
+    if skew:
+        idx[: T * 3 // 4] = 1
+    assert pkg.ops.gather_qmm_tiled(T * topk, E)  # past the rule for tiles
+    y, wq, sc = gather_case(pkg, dev, E, N, K, idx, x, K)
+    w64 = values64(wq, sc)
+    for e in idx.unique().tolist():
+        t, k = (idx == e).nonzero(as_tuple=True)
+        check_sum(y[t, k, 0], x[t, 0, 0].double(), w64[e], K)
+
+
+@gpu
+@pytest.mark.parametrize("T", [5, 400])
+def test_gather_lhs_M_and_bad_indices(pkg, dev, T):
+    """lhs indices, several rows per batch, and indices out of range: their
+    rows are zero, the status word says so, the others are as without them."""
+    E, N, K, M = 6, 128, 256, 2
+    g = torch.Generator().manual_seed(T)
+    x = torch.randn((7, M, K), generator=g).bfloat16()
+    rhs = torch.randint(0, E, (T,), generator=g, dtype=torch.int32)
+    lhs = torch.randint(0, 7, (T,), generator=g, dtype=torch.int32)
+    rhs[2], lhs[4] = E, 7
+    rhs[3] = -1
+    wq, sc = bank(g, (E, N, K))
+    out = pkg.ops.gather_qmm(x.to(dev), wq.to(dev), sc.to(dev), lhs_indices=lhs.to(dev),
+                             rhs_indices=rhs.to(dev), mode="mxfp4")
+    assert pkg.ops.workspace_status(out._mlxr_workspace) == 1
+    y = out.cpu()
+    assert bool((y[2:5] == 0).all())
+    w64 = values64(wq, sc)
+    for b in range(T):
+        if b not in (2, 3, 4):
+            check_sum(y[b], x[lhs[b]].double(), w64[rhs[b]], K)
+
+
+@gpu
+@pytest.mark.parametrize("T", [2, 600])
+def test_gather_extreme_scales(pkg, dev, T):
+    """Scale bytes at both ends of the range, NaN scales, infinities in x."""
+    E, N, K = 2, 64, 128
+    g = torch.Generator().manual_seed(T)
+    wq, sc = bank(g, (E, N, K))
+    sc[0, :, 0] = 0        # 2^-127: subnormal weights
+    sc[0, 5, 1] = 255      # a NaN group: channel 5 of expert 0
+    sc[1, :, :] = 120
+    x = torch.randn((T, 1, 1, K), generator=g).bfloat16()
+    idx = (torch.arange(T, dtype=torch.int32) % 2)[:, None]
+    y, _, _ = gather_case(pkg, dev, E, N, K, idx, x, wq_sc=(wq, sc))
+    w64 = values64(wq, sc)
+    keep = torch.arange(N) != 5
+    assert bool(torch.isnan(y[0::2, 0, 0, 5]).all())
+    check_sum(y[0::2, 0, 0][:, keep], x[0::2, 0, 0].double(), w64[0][keep], K)
+    check_sum(y[1::2, 0, 0], x[1::2, 0, 0].double(), w64[1], K)
+    # the largest scales that stay finite in the sums
+    sc[1, :, :] = 250
+    y, _, _ = gather_case(pkg, dev, E, N, K, idx, x * 2.0 ** -60, wq_sc=(wq, sc))
+    check_sum(y[1::2, 0, 0], (x * 2.0 ** -60)[1::2, 0, 0].double(), w64_of(wq, sc)[1], K)
+    # an infinity in one row leaves the others as they are
+    x2 = x.clone()
+    x2[1, 0, 0, 3] = float("inf")
+    sc[1, :, :] = 120
+    a, _, _ = gather_case(pkg, dev, E, N, K, idx, x, wq_sc=(wq, sc))
+    b, _, _ = gather_case(pkg, dev, E, N, K, idx, x2, wq_sc=(wq, sc))
+    rest = torch.arange(T) != 1
+    same = (a[rest] == b[rest]) | (torch.isnan(a[rest]) & torch.isnan(b[rest]))
+    assert bool(same.all())
+    code3 = (wq[1, :, 0].long() >> 12) & 7  # input 3's codes: inf * 0 is NaN
+    assert bool((torch.isnan(b[1, 0, 0]) == (code3 == 0)).all())
+
+
+def w64_of(wq, sc):
+    return values64(wq, sc)
+
+
+@gpu
+def test_gather_empty(pkg, dev):
+    wq, sc = bank(torch.Generator().manual_seed(0), (2, 64, 64))
+    y = pkg.ops.gather_qmm(torch.zeros((1, 1, 64), dtype=torch.bfloat16, device=dev), wq.to(dev),
+                           sc.to(dev), rhs_indices=torch.zeros(0, dtype=torch.int32, device=dev),
+                           mode="mxfp4")
+    assert y.shape == (0, 1, 64)
+
+
+@gpu
+@pytest.mark.parametrize("T", [6, 700])
+def test_gather_scales_at_any_address(pkg, dev, T):
+    """Scales need no alignment: a view one byte into its storage."""
+    E, N, K = 3, 128, 320
+    g = torch.Generator().manual_seed(T)
+    wq, sc = bank(g, (E, N, K))
+    x = torch.randn((T, 1, 1, K), generator=g).bfloat16()
+    idx = torch.randint(0, E, (T, 1), generator=g, dtype=torch.int32)
+    a, _, _ = gather_case(pkg, dev, E, N, K, idx, x, wq_sc=(wq, sc))
+    store = torch.zeros(sc.numel() + 1, dtype=torch.uint8, device=dev)
+    store[1:] = sc.flatten().to(dev)
+    b = pkg.ops.gather_qmm(x.to(dev), wq.to(dev), store[1:].view(sc.shape),
+                           rhs_indices=idx.to(dev), mode="mxfp4").cpu()
+    assert torch.equal(a, b)
+
+
+# ------------------------------------------------------------------- modules
+def glu64(x, w, idx, act):
+    """Expert outputs with bf16 rounding where the modules round (every op of
+    the activation, the projections' outputs), sums in 64 bits; and the bound
+    of each output's distance from it: a bf16 step more or less of any
+    intermediate moves h by 2^-7 of it per rounding."""
+    rb = lambda v: v.to(torch.bfloat16).double()  # noqa: E731
+    T, K = idx.shape
+    d = w[2].shape[1]
+    y = torch.zeros((T, K, d), dtype=torch.float64)
+    bound = torch.zeros_like(y)
+    for e in idx.unique().tolist():
+        t, k = (idx == e).nonzero(as_tuple=True)
+        g, u = rb(x[t] @ w[0][e].t()), rb(x[t] @ w[1][e].t())
+        if act == "swiglu":
+            h = rb(rb(g * rb(torch.sigmoid(g))) * u)
+        else:
+            c, s = 0.044677734375, 0.796875
+            inner = rb(g + rb(c * rb(rb(g * g) * g)))
+            h = rb(rb(rb(0.5 * g) * rb(1.0 + rb(torch.tanh(rb(s * inner))))) * u)
+        y[t, k] = h @ w[2][e].t()
+        # five roundings each a step off at most, and g's and u's sums; where
+        # GeGLU's 1 + tanh cancels, a step is one of 1, times g u / 2
+        floor = (g * u).abs()
+        slack = 5 * 2.0 ** -7 * (h.abs() + (floor if act == "geglu" else 0.2 * floor))
+        bound[t, k] = slack @ w[2][e].abs().t() + 2.0 ** -8 * y[t, k].abs()
+    return y, bound
+
+
+def ffn_inputs(seed, E, d, f, T, K):
+    g = torch.Generator().manual_seed(seed)
+    w = [bank(g, s) for s in ((E, f, d), (E, f, d), (E, d, f))]
+    x = torch.randn((T, d), generator=g).bfloat16()
+    idx = torch.rand((T, E), generator=g).topk(K, dim=1).indices.to(torch.int32)
+    return w, x, idx
+
+
+def ffn(pkg, dev, w):
+    nn = pkg.nn
+    return nn.SplitSwitchFfn(*[
+        nn.QuantizedSwitchLinear(q.to(dev), s.to(dev), mode="mxfp4") for q, s in w])
+
+
+@gpu
+@pytest.mark.parametrize("E,d,f,T,K", [(16, 256, 128, 1, 4), (16, 256, 192, 7, 4),
+                                       (32, 512, 256, 30, 8), (8, 2048, 320, 33, 2),
+                                       (16, 256, 128, 300, 4), (8, 512, 192, 600, 2)])
+def test_split_ffn(pkg, dev, E, d, f, T, K):
+    """One token to M-tiles: forward, forward_with_combine, and the same
+    results from the three projections one by one."""
+    w, x, idx = ffn_inputs(T + d, E, d, f, T, K)
+    m = ffn(pkg, dev, w)
+    y = m.forward(x.to(dev), idx.to(dev))
+    want, bound = glu64(x.double(), [values64(*b) for b in w], idx, "swiglu")
+    err = (y.cpu().double() - want).abs()
+    assert bool((err <= bound).all())
+    # independent roundings: their root sum is what is seen on the whole
+    assert float(err.norm() / want.norm()) < 8e-3
+    wts = torch.rand((T, K), generator=torch.Generator().manual_seed(1)).to(dev)
+    out = m.forward_with_combine(x.to(dev), idx.to(dev), wts)
+    ref = (y.double() * wts.double()[:, :, None]).sum(1)
+    mass = (y.double() * wts.double()[:, :, None]).abs().sum(1)
+    assert bool(((out.double() - ref).abs() <= 2 * K * 2.0 ** -24 * mass).all())
+    g = m.gate_proj.apply(x.to(dev)[:, None, None, :], idx.to(dev))[:, :, 0]
+    gw = values64(*w[0])
+    for e in idx.unique().tolist():
+        t, k = (idx == e).nonzero(as_tuple=True)
+        check_sum(g.cpu()[t, k], x[t].double(), gw[e], d)
+
+
+@gpu
+@pytest.mark.parametrize("T", [1, 9, 260])
+@pytest.mark.parametrize("act", ["geglu", "swiglu"])
+def test_packed_ffn(pkg, dev, T, act):
+    E, d, f, K = 8, 256, 128, 4
+    w, x, idx = ffn_inputs(T, E, d, f, T, K)
+    gu = (torch.cat([w[0][0], w[1][0]], 1), torch.cat([w[0][1], w[1][1]], 1))
+    nn = pkg.nn
+    lin = lambda b: nn.QuantizedSwitchLinear(b[0].to(dev), b[1].to(dev), mode="mxfp4")  # noqa: E731
+    m = nn.PackedSwitchFfn(lin(gu), lin(w[2]), act)
+    y = m.forward(x.to(dev), idx.to(dev)).cpu().double()
+    want, bound = glu64(x.double(), [values64(*b) for b in w], idx, act)
+    assert bool(((y - want).abs() <= bound).all())
+    if act == "swiglu":  # the packed tensor is the split ones, row for row
+        assert torch.equal(y, ffn(pkg, dev, w).forward(x.to(dev), idx.to(dev)).cpu().double())
+
+
+@gpu
+@pytest.mark.parametrize("T", [1, 5, 90, 300])
+@pytest.mark.parametrize("shared_mx", [True, False])
+def test_block(pkg, dev, T, shared_mx):
+    """The block over mxfp4 experts, its shared expert in the same form (in
+    the same launches) or affine: routing, shared branch and combine as with
+    the expert outputs of the modules alone; and the residual form."""
+    E, d, f, K = 16, 256, 128, 4
+    nn, ops = pkg.nn, pkg.ops
+    w, x, _ = ffn_inputs(T, E, d, f, T, K)
+    g = torch.Generator().manual_seed(7)
+    gate_w = torch.randn((E, d), generator=g).to(dev) * 0.1
+    sg = torch.randn((1, d), generator=g).to(dev) * 0.1
+    dense = [(torch.randn(s, generator=g) * 0.05).bfloat16().to(dev)
+             for s in ((f, d), (f, d), (d, f))]
+    mode = "mxfp4" if shared_mx else "affine"
+    shared = nn.SwigluMlp(*[nn.QuantizedLinear.try_from_linear(v, mode=mode) for v in dense])
+    m = ffn(pkg, dev, w)
+    blk = nn.Qwen35MoeBlock(gate_w, m, K, shared, sg)
+    xd = x.to(dev)
+    out = blk.forward(xd)
+    idx, wts = ops.router_topk(xd, gate_w, K)
+    y = m.forward(xd, idx)
+    sy = shared.forward(xd)
+    logit = xd.float() @ sg[0]
+    assert torch.equal(blk.last_indices, idx)
+    ref = (y.double() * wts.double()[:, :, None]).sum(1)
+    sgate = torch.sigmoid(logit.double())[:, None]
+    ref = ref + sy.double() * sgate
+    mass = (y.double() * wts.double()[:, :, None]).abs().sum(1) + (sy.double() * sgate).abs()
+    # the folded rows may be summed in another slicing of the input dim: a bf16
+    # step of any y; the shared gate's logit an f32 sum of d terms
+    lerr = d * 2.0 ** -22 * (xd.double().abs() @ sg[0].double().abs())[:, None]
+    tol = mass * (2.0 ** -6 + lerr)
+    assert bool(((out.double() - ref).abs() <= tol).all())
+    if T <= 5:
+        n = nn.RmsNorm(torch.ones(d).to(dev))
+        h = blk.forward_residual(xd, n)
+        assert bool(torch.isfinite(h).all())
+        assert torch.allclose(h, xd.float() + blk.forward(n.forward(xd)), rtol=1e-5, atol=1e-5)
+
+
+@gpu
+@pytest.mark.parametrize("T", [3, 400])
+def test_graph_and_streams(pkg, dev, T):
+    """A captured pass replayed with eager work between, and the same pass on
+    a side stream: the eager results, bit for bit."""
+    w, x, idx = ffn_inputs(3, 8, 256, 128, T, 4)
+    m = ffn(pkg, dev, w)
+    xs, ids = x.to(dev), idx.to(dev)
+    wq, sc = m.gate_proj.weight, m.gate_proj.scales
+
+    def step():
+        y = m.forward(xs, ids)
+        g = pkg.ops.gather_qmm(xs[:, None, None, :], wq, sc, rhs_indices=ids, mode="mxfp4")
+        q = pkg.ops.quantize(y, mode="mxfp4")
+        return [y, g, pkg.ops.dequantize(q[0], q[1], mode="mxfp4")]
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in range(4):
+        xs.copy_((x + i).bfloat16())
+        graph.replay()
+        eager = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, eager))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(other, eager))
