@@ -193,6 +193,46 @@ int mlxr_moe_router_topk(const void* x, int64_t T, int64_t d,
                          int32_t* topk_idx, float* topk_w, void* workspace,
                          size_t workspace_size, mlxr_moe_stream stream);
 
+/* The router's load-balance loss (no counterpart in the reference, which only
+ * runs trained routers).  logits [T, E] f32 or bf16, rows `ld` elements apart
+ * (ld >= E); indices int32 [T, K], each token's chosen experts; mask uint8 [T]
+ * or NULL: a token counts while its byte is not 0 (N tokens count).  With p =
+ * softmax of a row,
+ *   counts int32 [E]: choices of counted tokens that fell on each expert
+ *   probs f32 [E]: mean of p over the counted tokens
+ *   tokens int32 [1]: N
+ *   loss f32 [1] = E * sum_e counts_e / (N K) * probs_e
+ * all 0 when N is 0.  A row whose logits are all -inf adds no probability; an
+ * index outside [0, E) is not counted and sets the workspace's status word
+ * (mlxr_moe_workspace_status).  Sums are in f32 within 16 rows or more of a
+ * workgroup and in f64 across them, in a fixed order: equal inputs give equal
+ * bits.  E <= 1024, K <= 64. */
+size_t mlxr_moe_router_balance_workspace_size(int64_t T, int64_t E);
+int mlxr_moe_router_balance(const void* logits, int logits_dtype, int64_t ld,
+                            int64_t T, int64_t E, const int32_t* indices,
+                            int64_t K, const uint8_t* mask, float* loss,
+                            int32_t* counts, float* probs, int32_t* tokens,
+                            void* workspace, size_t workspace_size,
+                            mlxr_moe_stream stream);
+/* Its gradient: dlogits [T, E] (dense rows, the logits' dtype) =
+ *   dloss * E / N * p * (f - sum_j p_j f_j),  f = counts / (N K)
+ * (counts and tokens as the forward call left them, constants of the loss),
+ * plus, with dweights f32 [T, K], the gradient of router_topk's renormalised
+ * weights w = softmax of the chosen logits:
+ *   dlogits[t, indices[t, k]] += w_k (dweights_k - sum_j w_j dweights_j)
+ * (an expert named twice in a row gets both terms, an index out of range
+ * none).  dloss f32 [1] on the device; dloss NULL: no balance term (counts and
+ * tokens are then not read); dweights NULL: no weights' term; one of them is
+ * required.  Rows whose mask is 0, and terms of a row without a finite
+ * maximum, get 0.  dlogits must not overlap the inputs. */
+int mlxr_moe_router_balance_vjp(const void* logits, int logits_dtype,
+                                int64_t ld, int64_t T, int64_t E,
+                                const int32_t* indices, int64_t K,
+                                const uint8_t* mask, const int32_t* counts,
+                                const int32_t* tokens, const float* dloss,
+                                const float* dweights, void* dlogits,
+                                mlxr_moe_stream stream);
+
 /* Stable sort of flat expert ids [n] by expert: the permutation of
  * gather_sort (crates/mlxr-lm/src/nn/switch.rs:499-512), order =
  * argsort(ids) into `sorted`, inv = argsort(order) into `inv`, plus
@@ -451,7 +491,8 @@ int mlxr_moe_workspace_status(const void* workspace, size_t workspace_size,
  * `kernel` is armed, each launch of that kernel is bracketed by HIP events
  * on the stream it is launched on.  Names: "router_logits", "router_topk",
  * "dispatch", "qgemm_gated", "qgemm_down", "combine", the shared
- * expert's GEMMs "shared_gated", "shared_down", "rms_norm", and
+ * expert's GEMMs "shared_gated", "shared_down", "rms_norm",
+ * "router_balance", "router_balance_vjp", and
  * "read_probe" (mlxr_moe_profile_read).  NULL disarms.  Not for use while
  * the stream is being captured into a graph. */
 int mlxr_moe_profile_start(const char* kernel);

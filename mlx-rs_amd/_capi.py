@@ -115,6 +115,13 @@ SIGNATURES = {
     "mlxr_moe_router_topk": (c_int, [P, c_int64, c_int64, P, c_int64, c_int64, P, P, P, c_size_t, P]),
     "mlxr_moe_router_topk_quantized": (
         c_int, [P, c_int64, POINTER(QLinear), c_int64, P, P, P, c_size_t, P]),
+    "mlxr_moe_router_balance_workspace_size": (c_size_t, [c_int64, c_int64]),
+    "mlxr_moe_router_balance": (
+        c_int,
+        [P, c_int, c_int64, c_int64, c_int64, P, c_int64, P, P, P, P, P, P, c_size_t, P]),
+    "mlxr_moe_router_balance_vjp": (
+        c_int,
+        [P, c_int, c_int64, c_int64, c_int64, P, c_int64, P, P, P, P, P, P, P]),
     "mlxr_moe_dispatch_workspace_size": (c_size_t, [c_int64, c_int64]),
     "mlxr_moe_dispatch": (c_int, [P, c_int64, c_int64, P, P, P, P, P, c_size_t, P]),
     "mlxr_moe_combine": (c_int, [P, P, c_int64, c_int64, c_int64, P, P, P, P]),

@@ -36,6 +36,7 @@ SOURCES = [
     "prefill_reg.hip",
     "prefill_tall.hip",
     "combine.hip",
+    "balance.hip",
     "nn.cpp",
     "profile.cpp",
     "capi.cpp",

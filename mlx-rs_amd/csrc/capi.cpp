@@ -93,6 +93,23 @@ Status check_workspace(const Carve& plan, void* ws, size_t ws_size) {
   return Status{};
 }
 
+// What router_balance and its gradient share.
+Status check_balance(const char* op, const void* logits, int dtype, int64_t ld, int64_t T,
+                     int64_t E, const int32_t* indices, int64_t K) {
+  const std::string o(op);
+  if (!dtype_ok(dtype)) return Status::error(o + ": logits must be f32 or bf16");
+  if (T < 0 || E <= 0 || ld < E) return Status::error(o + ": bad shape");
+  if (E > kMaxExperts)
+    return Status::error(o + ": at most " + std::to_string(kMaxExperts) + " experts");
+  if (K < 1 || K > 64)
+    return Status::error(o + ": k must be in [1, 64], got " + std::to_string(K));
+  if (T > INT32_MAX / 64) return Status::error(o + ": too many tokens");
+  if (T && (!logits || !indices)) return Status::error(o + ": null array");
+  if (!aligned(logits, dtype == MLXR_MOE_BFLOAT16 ? 2 : 4) || !aligned(indices, 4))
+    return Status::error(o + ": logits and indices must be aligned to their elements");
+  return Status{};
+}
+
 // Workspace plans (the same carving the entry points run).
 void plan_gather(Carve& c, int64_t B, int64_t M, int64_t E) {
   const int64_t R = B * M;
@@ -468,6 +485,55 @@ int mlxr_moe_router_topk_quantized(const void* x, int64_t T,
                                      topk_w, nullptr, s),
                   "router top-k");
   return finish(st);
+}
+
+size_t mlxr_moe_router_balance_workspace_size(int64_t T, int64_t E) {
+  Carve c(nullptr);
+  if (T >= 0 && E > 0) plan_router_balance(c, T, E);
+  return c.off;
+}
+
+int mlxr_moe_router_balance(const void* logits, int logits_dtype, int64_t ld,
+                            int64_t T, int64_t E, const int32_t* indices,
+                            int64_t K, const uint8_t* mask, float* loss,
+                            int32_t* counts, float* probs, int32_t* tokens,
+                            void* workspace, size_t workspace_size,
+                            mlxr_moe_stream stream) {
+  Status st = check_balance("router_balance", logits, logits_dtype, ld, T, E, indices, K);
+  if (!st.ok) return finish(st);
+  if (!loss || !counts || !probs || !tokens) return fail("router_balance: null array");
+  Carve plan(nullptr);
+  plan_router_balance(plan, T, E);
+  st = check_workspace(plan, workspace, workspace_size);
+  if (!st.ok) return finish(st);
+  return finish(from_hip(
+      launch_router_balance(logits, logits_dtype == MLXR_MOE_BFLOAT16, ld, T, E, indices, K, mask,
+                            loss, counts, probs, tokens, Carve(workspace), as_stream(stream)),
+      "router_balance"));
+}
+
+int mlxr_moe_router_balance_vjp(const void* logits, int logits_dtype,
+                                int64_t ld, int64_t T, int64_t E,
+                                const int32_t* indices, int64_t K,
+                                const uint8_t* mask, const int32_t* counts,
+                                const int32_t* tokens, const float* dloss,
+                                const float* dweights, void* dlogits,
+                                mlxr_moe_stream stream) {
+  const Status st =
+      check_balance("router_balance_vjp", logits, logits_dtype, ld, T, E, indices, K);
+  if (!st.ok) return finish(st);
+  if (!dloss && !dweights)
+    return fail("router_balance_vjp: dloss, dweights or both are required");
+  if (dloss && (!counts || !tokens))
+    return fail("router_balance_vjp: dloss takes the forward's counts and tokens");
+  if (T && !dlogits) return fail("router_balance_vjp: null array");
+  if (!aligned(dlogits, logits_dtype == MLXR_MOE_BFLOAT16 ? 2 : 4))
+    return fail("router_balance_vjp: dlogits must be aligned to its elements");
+  return finish(from_hip(
+      launch_router_balance_vjp(logits, logits_dtype == MLXR_MOE_BFLOAT16, ld, T, E, indices, K,
+                                mask, counts, tokens, dloss, dweights, dlogits,
+                                as_stream(stream)),
+      "router_balance_vjp"));
 }
 
 size_t mlxr_moe_dispatch_workspace_size(int64_t n, int64_t E) {

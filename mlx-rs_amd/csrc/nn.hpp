@@ -52,6 +52,23 @@ Status from_hip(hipError_t e, const char* where);
 DispatchBuffers carve_dispatch(Carve& c, int64_t n, int64_t E,
                                int32_t* status);
 
+// ------------------------------------------------------------- balance.hip
+// The balance loss over logits z [T, E] (rows ld apart, f32 or bf16) and
+// choices idx [T, K]; ws as plan_router_balance carves it, its first word the
+// status (1: an index out of range).
+void plan_router_balance(Carve& c, int64_t T, int64_t E);
+hipError_t launch_router_balance(const void* z, bool bf16, int64_t ld, int64_t T, int64_t E,
+                                 const int32_t* idx, int64_t K, const uint8_t* mask, float* loss,
+                                 int32_t* counts, float* probs, int32_t* tokens, Carve ws,
+                                 hipStream_t s);
+// Its gradient in the logits (dloss null: none), plus the renormalised top-k
+// weights' (dweights null: none).
+hipError_t launch_router_balance_vjp(const void* z, bool bf16, int64_t ld, int64_t T, int64_t E,
+                                     const int32_t* idx, int64_t K, const uint8_t* mask,
+                                     const int32_t* counts, const int32_t* tokens,
+                                     const float* dloss, const float* dweights, void* dlogits,
+                                     hipStream_t s);
+
 namespace nn {
 
 // Rows per expert above which the MFMA tile kernel with LDS-dequantised

@@ -340,9 +340,10 @@ def softmax_axis(a: torch.Tensor, axis: int, precise=None):
     return out.movedim(-1, ax)
 
 
-def router_topk(x: torch.Tensor, gate_w: torch.Tensor, k: int):
+def router_topk(x: torch.Tensor, gate_w: torch.Tensor, k: int, return_logits=False):
     """softmax(x @ gate_w^T) -> top-k -> renormalise (moe.rs:122-138).
-    Returns (indices int32 [T, k], weights f32 [T, k])."""
+    Returns (indices int32 [T, k], weights f32 [T, k]), and with
+    return_logits the f32 logits [T, E] too (what router_balance takes)."""
     _dev(x, gate_w)
     x2 = x.reshape(-1, x.shape[-1]).contiguous()
     T, d = x2.shape
@@ -353,16 +354,24 @@ def router_topk(x: torch.Tensor, gate_w: torch.Tensor, k: int):
     ws = workspace(lib.mlxr_moe_router_workspace_size(T, E), x.device)
     C.check(lib.mlxr_moe_router_topk(_p(x2), T, d, _p(gate_w.contiguous()), E, k, _p(idx),
                                      _p(wts), _p(ws), ws.numel(), _stream(x)))
+    return _routing(x, k, E, idx, wts, ws, return_logits)
+
+
+def _routing(x, k, E, idx, wts, ws, return_logits):
     lead = tuple(x.shape[:-1])
-    return idx.reshape(lead + (k,)), wts.reshape(lead + (k,))
+    out = idx.reshape(lead + (k,)), wts.reshape(lead + (k,))
+    if not return_logits:
+        return out
+    T = idx.shape[0]  # the call's workspace is its logits [T, E] f32
+    return out + (ws[:4 * T * E].view(torch.float32).reshape(lead + (E,)),)
 
 
-def router_topk_quantized(x: torch.Tensor, gate, k: int):
+def router_topk_quantized(x: torch.Tensor, gate, k: int, return_logits=False):
     """router_topk with the router as a QuantizedLinear (nn.QuantizedLinear,
     4 or 8 bits, group 64; layers/quantized.rs:356-373) or a bf16 Linear
     (nn.Linear): bf16 logits and probabilities, top-k on the probabilities.
     Returns (indices int32 [T, k], weights [T, k] -- bf16 values held in
-    f32)."""
+    f32), and with return_logits the logits [T, E] (bf16 values in f32)."""
     _dev(x, gate.weight)
     x2 = x.reshape(-1, x.shape[-1]).contiguous()
     T = x2.shape[0]
@@ -373,8 +382,86 @@ def router_topk_quantized(x: torch.Tensor, gate, k: int):
     desc = gate.descriptor()
     C.check(lib.mlxr_moe_router_topk_quantized(_p(x2), T, ctypes.byref(desc), k, _p(idx),
                                                _p(wts), _p(ws), ws.numel(), _stream(x)))
-    lead = tuple(x.shape[:-1])
-    return idx.reshape(lead + (k,)), wts.reshape(lead + (k,))
+    return _routing(x, k, gate.output_dims, idx, wts, ws, return_logits)
+
+
+def _balance_inputs(name, logits, indices, mask):
+    """(logits rows, their stride, indices int32 [T, K], mask uint8 [T] or
+    None) of router_balance and its gradient."""
+    _dev(logits, indices, mask)
+    E = logits.shape[-1] if logits.ndim else 0
+    if logits.ndim < 1 or E < 1:
+        raise MlxrMoeError(f"{name}: logits must be [.., T, E], got {tuple(logits.shape)}")
+    if indices.ndim != logits.ndim or indices.shape[:-1] != logits.shape[:-1]:
+        raise MlxrMoeError(f"{name}: indices {tuple(indices.shape)} must be [.., T, K] over "
+                           f"logits {tuple(logits.shape)}")
+    z = logits.reshape(-1, E)
+    if z.stride(1) != 1 or z.stride(0) < E:
+        z = z.contiguous()
+    if mask is not None:
+        if mask.dtype not in (torch.bool, torch.uint8):
+            raise MlxrMoeError(f"{name}: mask must be bool or uint8, got {mask.dtype}")
+        if mask.shape != logits.shape[:-1]:
+            raise MlxrMoeError(f"{name}: mask {tuple(mask.shape)} must be one value per token "
+                               f"of logits {tuple(logits.shape)}")
+        mask = mask.reshape(-1).contiguous()
+    return z, max(z.stride(0), E), _as_u32(indices).reshape(-1, indices.shape[-1]), mask
+
+
+def router_balance(logits: torch.Tensor, indices: torch.Tensor, mask=None):
+    """The load-balance loss of a router over its logits [.., T, E] (f32 or
+    bf16) and its choices [.., T, K]: E * sum_e f_e P_e, f_e the share of the
+    choices that fell on expert e and P_e its mean probability, over the
+    tokens whose mask (bool or uint8, None: all) is not zero.  Returns (loss
+    f32 [], counts int32 [E], probs f32 [E], tokens int32 []).  An index out
+    of range is not counted and sets the workspace's status word."""
+    z, ld, idx, mask = _balance_inputs("router_balance", logits, indices, mask)
+    (T, E), K = z.shape, idx.shape[1]
+    dev = z.device
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    probs = torch.empty(E, dtype=torch.float32, device=dev)
+    counts = torch.empty(E, dtype=torch.int32, device=dev)
+    tokens = torch.empty((), dtype=torch.int32, device=dev)
+    lib = C.lib()
+    ws = workspace(lib.mlxr_moe_router_balance_workspace_size(T, E), dev)
+    with _on(z):
+        C.check(lib.mlxr_moe_router_balance(
+            _p(z), _code(z), ld, T, E, _p(idx), K, _p(mask), _p(loss), _p(counts), _p(probs),
+            _p(tokens), _p(ws), ws.numel(), _stream(z)))
+    loss._mlxr_workspace = ws  # keep the status word alive with the result
+    return loss, counts, probs, tokens
+
+
+def router_balance_vjp(logits: torch.Tensor, indices: torch.Tensor, counts=None, tokens=None,
+                       dloss=None, mask=None, dweights=None):
+    """The gradient of router_balance's loss in the logits (their shape and
+    dtype), for dloss f32 [] on the device, with counts and tokens as the
+    forward call returned them; and, with dweights [.., T, K], plus that of
+    router_topk's renormalised weights.  Masked tokens get zeros."""
+    z, ld, idx, mask = _balance_inputs("router_balance_vjp", logits, indices, mask)
+    (T, E), K = z.shape, idx.shape[1]
+    _dev(z, counts, tokens, dloss, dweights)
+    if dloss is not None:
+        if dloss.dtype != torch.float32 or dloss.numel() != 1:
+            raise MlxrMoeError("router_balance_vjp: dloss must be one float32")
+        if counts is None or tokens is None:
+            raise MlxrMoeError("router_balance_vjp: dloss takes the forward's counts and tokens")
+        if (counts.dtype != torch.int32 or counts.shape != (E,)
+                or tokens.dtype != torch.int32 or tokens.numel() != 1):
+            raise MlxrMoeError(f"router_balance_vjp: counts must be int32 [{E}] and tokens one "
+                               "int32")
+        counts = counts.contiguous()
+    if dweights is not None:
+        if dweights.shape != indices.shape:
+            raise MlxrMoeError(f"router_balance_vjp: dweights {tuple(dweights.shape)} must match "
+                               f"indices {tuple(indices.shape)}")
+        dweights = dweights.to(torch.float32).contiguous()
+    dz = torch.empty((T, E), dtype=z.dtype, device=z.device)
+    with _on(z):
+        C.check(C.lib().mlxr_moe_router_balance_vjp(
+            _p(z), _code(z), ld, T, E, _p(idx), K, _p(mask), _p(counts), _p(tokens), _p(dloss),
+            _p(dweights), _p(dz), _stream(z)))
+    return dz.reshape(logits.shape)
 
 
 def dispatch(ids: torch.Tensor, num_experts: int):
