@@ -103,8 +103,8 @@ int mlxr_moe_dequantize(const uint32_t* wq, const void* scales,
  * reference's locality hint; rows are always grouped by expert here.
  * Requires N % 64 == 0, K % 64 == 0, group 64, bits 4 or 8.
  * Mode "mxfp4" (group 32): w [E, N, K/8], scales uint8 [E, N, K/32] (sb_dtype
- * MLXR_MOE_UINT8), biases NULL; every weight is an exact bf16 value (scale
- * bytes below 253) and every sum is in f32, whatever the number of rows. */
+ * MLXR_MOE_UINT8, 4-byte aligned), biases NULL; every weight is an exact bf16
+ * value (scale bytes below 253) and every sum is in f32, whatever the number of rows. */
 size_t mlxr_moe_gather_qmm_workspace_size(int64_t B, int64_t M,
                                           int64_t num_experts);
 int mlxr_moe_gather_qmm(const void* x, int x_dtype, int64_t x_batch,
@@ -261,8 +261,8 @@ int mlxr_moe_combine(const void* y, const float* w, int64_t T, int64_t K,
  * (switch.rs:49-94, applied with gather_mm) or Linear, weight bf16
  * [E, output_dims, input_dims], scales and biases NULL, group_size
  * ignored.  bits = MLXR_MOE_BITS_MXFP4 describes mode "mxfp4": weight u32 [E,
- * output_dims, input_dims/8], scales uint8 [E, output_dims, input_dims/32],
- * biases NULL, group_size 32 (expert and shared-expert projections; routers
+ * output_dims, input_dims/8], scales uint8 [E, output_dims, input_dims/32]
+ * (4-byte aligned), biases NULL, group_size 32 (expert and shared-expert projections; routers
  * and gates take the other forms).  The projections of one module share their
  * bits. */
 enum { MLXR_MOE_BITS_MXFP4 = 0x104 };

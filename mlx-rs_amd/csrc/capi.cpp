@@ -313,6 +313,7 @@ int mlxr_moe_gather_qmm(const void* x, int x_dtype, int64_t x_batch,
       return fail("gather_qmm: mode mxfp4 takes bf16 x and out and uint8 scales");
     if (biases) return fail("gather_qmm: mode mxfp4 has no biases");
     if (!scales) return fail("gather_qmm: null array");
+    if (!aligned(scales, 4)) return fail("gather_qmm: scales must be 4-byte aligned");
     return run_gather("gather_qmm", x, x_batch, M, K, w, scales, nullptr, kBitsMxfp4, E, N,
                       lhs_indices, rhs_indices, B, out, workspace, workspace_size,
                       as_stream(stream));

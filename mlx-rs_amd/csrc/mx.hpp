@@ -36,4 +36,25 @@ __device__ __forceinline__ bf16x8_t mx_weights(uint32_t w, float scale) {
   return as_bf16x8(r);
 }
 
+// The gated products' activation in f32, rounded to bf16 once, where the second
+// product takes it up (the affine modules round after every op, as the
+// reference's bf16 chain does, and lose a bit more: y of a c2 bank is off by 2.3
+// parts in a thousand here and by 4.2 so, its own rounding 1.7 of them).
+//   swiglu: g sigmoid(g) u
+//   geglu:  0.5 g (1 + tanh(y)) u = g sigmoid(2 y) u,  y = c (g + k g^3), with the
+//           constants as the reference's bf16 chain holds them
+// The sigmoid from the hardware exp2 and reciprocal, about an ulp each.
+__device__ __forceinline__ float mx_act(int act, float g, float u) {
+  float y = g;
+  if (act == kActGeglu) {
+    const float k = 0.044677734375f, c = 0.796875f;
+    y = 2.0f * c * g * __builtin_fmaf(k * g, g, 1.0f);
+  }
+  const float e = __builtin_amdgcn_exp2f(-1.4426950408889634f * y);
+  return g * __builtin_amdgcn_rcpf(1.0f + e) * u;
+}
+__device__ __forceinline__ uint16_t mx_bf16(float v) {
+  return __builtin_bit_cast(uint16_t, (__bf16)v);
+}
+
 }  // namespace mlxr_moe

@@ -170,12 +170,11 @@ __global__ __launch_bounds__(64 * kWaves) void mx_stream_kernel(QGemmArgs a, QGe
     if (t < nt) {
       const int slot = row0 + t;
       if constexpr (GATED) {
-        r.out[(int64_t)slot * r.out_ld + ch] =
-            gated_act_bf16(r.act, bf16_round(acc[0][i]), bf16_round(acc[1][i]));
+        r.out[(int64_t)slot * r.out_ld + ch] = mx_bf16(mx_act(r.act, acc[0][i], acc[1][i]));
       } else {
         const int64_t orow =
             !r.out_by_flat ? slot : TT == 8 ? u.rec[4 + t] : r.sorted[slot];
-        r.out[orow * r.out_ld + ch] = f32_to_bf16(acc[0][i]);
+        r.out[orow * r.out_ld + ch] = mx_bf16(acc[0][i]);
       }
     }
   }

@@ -6,12 +6,17 @@
 // owns 32 gate and the same 32 up channels, or 64 down channels, for all rows of
 // the tile.
 //
-// Weights: lane (c, h) = (l % 32, l / 32) loads group 2 j + h of channel c in
-// load j of a 128-byte line (8 groups): 16 bytes, the operands of four
-// v_mfma_f32_32x32x16_bf16 whose K halves are 8 inputs of group 2 j and 8 of
-// group 2 j + 1.  One conversion instruction gives two weights, scale included,
-// so the conversion is a sixth of the MFMAs' time and nothing of the weights
-// passes through LDS.  x is staged 64 inputs (two groups) at a time.
+// Weights: 128-byte lines (8 groups) of the wave's 64 rows come straight to its own
+// 8 KB of LDS, consecutive lanes on consecutive 16 bytes (loads of 32 bytes from
+// each of 32 rows cost the address path four times the cycles: gate/up of c4
+// T=2048 212 us so, 153 with whole lines), and are then read to registers: lane
+// (c, h) = (l % 32, l / 32) takes group 2 j + h of channel c in stage j, the
+// operands of four v_mfma_f32_32x32x16_bf16 whose K halves are 8 inputs of group
+// 2 j and 8 of group 2 j + 1.  One conversion instruction gives two weights, scale
+// included: as many as there are MFMAs at 128 rows.  x is staged 64 inputs (two
+// groups) at a time, three stages, straight to LDS too.
+// c2 T=4096: gate/up 203 us, 1.0 PFLOP/s; of it about 155 are the MFMAs (all loads
+// taken out).
 #include <algorithm>
 
 #include "mx.hpp"
@@ -21,87 +26,127 @@ namespace mlxr_moe {
 namespace {
 
 constexpr int kWaves = 4, kNT = 64 * kWaves;
-constexpr int kScratch = 4096;  // per wave: the epilogue's 32 rows x 64 channels
+typedef __attribute__((address_space(3))) void* lds_ptr;
+constexpr int kXStages = 3;      // x stages of 64 inputs in LDS
+constexpr int kWLine = 32 * 128; // a wave's line of one side: 128 bytes of 32 rows
 template <int ROWS>
-constexpr int kTileLds = 2 * ROWS * 128 + kWaves * kScratch;
+constexpr int kTileLds = kXStages * ROWS * 128 + kWaves * 2 * kWLine;
+static_assert(2 * kTileLds<128> <= 160 * 1024, "two workgroups per CU");
 
-// A line of both sides: 4 loads each, and the 8 scale bytes of the line.
-struct MxLine {
-  u32x4_t w[2][4];
-  u32x2_t sc[2];
-};
+template <int N>
+__device__ __forceinline__ void wait_loads() {  // at most N loads not back
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
 
-// The rows [slot0, slot0 + rows) of expert e against N-tiles [nt0, nt1).
+// The workgroup's barrier, when at most N of this wave's loads are not back and its
+// reads of LDS are.  (__syncthreads would wait for every load to LDS.)
+template <int N>
+__device__ __forceinline__ void stage_barrier() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+// The rows [slot0, slot0 + rows) of expert e against N-tile nt.
 // NMB: 32-row blocks that hold rows.
 template <bool GATED, int ROWS, int NMB>
 __device__ __forceinline__ void mx_unit(const RegArgs& a, int N, int K, int e, int slot0,
-                                        int rows, int nt0, int nt1, char* smem) {
+                                        int rows, int nt, char* smem) {
   constexpr int TC = GATED ? 32 * kWaves : 64 * kWaves;  // channels per N-tile
   constexpr int WC = TC / kWaves;                        // ... per wave
   constexpr int kXBytes = ROWS * 128;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 31, h = lane >> 5;
-  const int G = K / kMxGroup, T = K >> 6;  // groups, x stages per tile
-  const int L = (T + 3) / 4;               // lines per tile
+  const int G = K / kMxGroup, T = K >> 6;  // groups, x stages with inputs
+  const int L = (T + 3) / 4;               // lines (of four stages)
   char* xl = smem;
-  char* scratch = smem + 2 * kXBytes + wave * kScratch;
+  char* wl = smem + kXStages * kXBytes + wave * 2 * kWLine;
 
-  // ---- weights and scales: the expert's rows
-  const int row_bytes = K / 2;
+  // ---- weights: lines straight to the wave's own LDS.  Instruction i of a side
+  // fills rows 8 i .. 8 i + 7, lane l the 16 bytes at position l % 8 of row l / 8;
+  // chunk (group) cc of row r sits at cc ^ (r & 7).  Rows past N and chunks past
+  // the row are out of range: zeros.
+  const uint32_t row_bytes = (uint32_t)K / 2;
   const __amdgpu_buffer_rsrc_t wr0 = __builtin_amdgcn_make_buffer_rsrc(
       const_cast<uint32_t*>(a.w0.w) + (int64_t)e * a.e_rows * (row_bytes / 4), 0,
-      (int)((int64_t)N * row_bytes), kBufFlags);
+      (int)(N * row_bytes), kBufFlags);
   const __amdgpu_buffer_rsrc_t wr1 = __builtin_amdgcn_make_buffer_rsrc(
       const_cast<uint32_t*>(GATED ? a.w1.w : a.w0.w) +
           (int64_t)e * a.e_rows * (row_bytes / 4),
-      0, (int)((int64_t)N * row_bytes), kBufFlags);
-  const gptr<const uint8_t> sp0 =
-      as_global<const uint8_t>(a.w0.scales) + (int64_t)e * a.e_rows * G;
-  const gptr<const uint8_t> sp1 =
-      as_global<const uint8_t>(GATED ? a.w1.scales : a.w0.scales) + (int64_t)e * a.e_rows * G;
-  auto channel0 = [&](int nt, int side) {
-    return nt * TC + wave * WC + (GATED ? 0 : 32 * side);
-  };
-  int pt = nt0, pl = 0;  // the next line to load: tile, line within it
-  // Every line issues the same loads; those past the row, of channels past N and
-  // of lines past the unit's are out of range (zeros, no memory round trip).
-  auto load_w = [&](MxLine& W) {
-    const bool on = pt < nt1;
+      0, (int)(N * row_bytes), kBufFlags);
+  const int och0 = nt * TC + wave * WC;  // the wave's first channel
+  const int wrow = lane >> 3, wch = (lane & 7) ^ wrow;
+  auto load_w = [&](int l) {
+    const bool ok = 8 * l + wch < G;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      const int ch = channel0(pt, s) + c;
-      const uint32_t off = (uint32_t)ch * (uint32_t)row_bytes + 128u * pl + 16u * h;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const bool ok = on && ch < N && 4 * pl + j < T;
-        W.w[s][j] = __builtin_amdgcn_raw_buffer_load_b128(s ? wr1 : wr0,
-                                                          ok ? off + 32u * j : kPastEnd, 0, 0);
+      for (int i = 0; i < 4; ++i) {
+        const int ch = och0 + (GATED ? 0 : 32 * s) + 8 * i + wrow;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            s ? wr1 : wr0, (lds_ptr)(wl + s * kWLine + 1024 * i), 16,
+            ok && ch < N ? (uint32_t)ch * row_bytes + 16u * wch : kPastEnd, 128 * l, 0, 0);
       }
-      // 8 scale bytes from group 8 pl on, in one load that ends within the
-      // expert's rows (shifted where that moved it); zeros past the row
-      typedef uint64_t u64_a1 __attribute__((aligned(1)));
-      const uint32_t so = (uint32_t)min(ch, N - 1) * (uint32_t)G + 8u * (on ? pl : 0);
-      const uint32_t at = min(so, (uint32_t)N * (uint32_t)G - 8u);
-      const int left = G - 8 * (on ? pl : 0);
-      uint64_t v = *(gptr<const u64_a1>)((s ? sp1 : sp0) + at) >> (8 * (so - at));
-      if (left < 8) v &= (1ull << (8 * left)) - 1;
-      W.sc[s] = u32x2_t{(uint32_t)v, (uint32_t)(v >> 32)};
-    }
-    if (++pl == L) {
-      pl = 0;
-      ++pt;
     }
   };
-  MxLine W, Wn;
-  load_w(W);
-  __builtin_amdgcn_sched_barrier(0);
+  constexpr int kWLoads = 8;
+  u32x4_t w[2][4];  // [side][stage of the line]: the group 2 stage + h of channel c
+  auto take_w = [&]() {
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        w[s][j] = *reinterpret_cast<const u32x4_t*>(wl + s * kWLine + c * 128 +
+                                                    16 * ((2 * j + h) ^ (c & 7)));
+  };
+  // ---- scales: 16 bytes of channel c (two lines) at a time, by aligned words; a
+  // row of an odd number of pairs starts in the middle of one
+  const __amdgpu_buffer_rsrc_t sr0 = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<uint16_t*>(a.w0.scales) + (int64_t)e * a.e_rows * (G / 2), 0, N * G, kBufFlags);
+  const __amdgpu_buffer_rsrc_t sr1 = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<uint16_t*>(GATED ? a.w1.scales : a.w0.scales) + (int64_t)e * a.e_rows * (G / 2),
+      0, N * G, kBufFlags);
+  struct Scales {
+    u32x4_t v;
+    uint32_t past;
+  };
+  Scales sn[2];  // of the two lines after the current ones
+  auto load_sc = [&](int l) {  // lines l, l + 1 (l even)
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int ch = och0 + (GATED ? 0 : 32 * s) + c;
+      const uint32_t off = (uint32_t)ch * (uint32_t)G & ~3u;
+      const bool ok = ch < N && 8 * l < G;
+      sn[s].v = __builtin_amdgcn_raw_buffer_load_b128(s ? sr1 : sr0, ok ? off : kPastEnd, 8 * l, 0);
+      sn[s].past = __builtin_amdgcn_raw_buffer_load_b32(
+          s ? sr1 : sr0, ok && (G & 2) ? off + 16 : kPastEnd, 8 * l, 0);
+    }
+  };
+  uint32_t sc4[2][4];  // the two lines' scale bytes, moved so that this lane's are 0 and 2
+  auto take_sc = [&](int l) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int ch = och0 + (GATED ? 0 : 32 * s) + c;
+      // bytes (2 i + h) of the row from group 8 l on, in words of two such
+      const uint32_t sh = 8 * (((uint32_t)ch * (uint32_t)G) & 3u) + 8 * h;
+      const uint32_t u[5] = {sn[s].v.x, sn[s].v.y, sn[s].v.z, sn[s].v.w, sn[s].past};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t v = __builtin_amdgcn_alignbit(u[i + 1], u[i], sh);
+        const int left = G - 8 * l - 4 * i;  // zeros past the row
+        sc4[s][i] = left >= 4 ? v : left > 0 ? v & 0xffffu : 0u;
+      }
+    }
+  };
 
-  // ---- x: thread -> 16-byte chunk tid % 8 of the 64 inputs of rows tid / 8 +
-  // 32 j; chunk cc of row r sits at cc ^ ((r >> 1) & 7)
+  // ---- x: straight to LDS, 64 inputs of every row a stage.  A wave's instruction j
+  // fills rows 32 j + 8 wave .. + 7, lane l the 16 bytes at position l % 8 of row
+  // l / 8 of them; chunk cc of row r sits at cc ^ ((r >> 1) & 7)
   const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc(
       const_cast<uint16_t*>(a.x), 0, (int)a.x_bytes, kBufFlags);
-  const int xrow0 = tid >> 3, xc = tid & 7;
+  const int xrow0 = tid >> 3, xc = (tid & 7) ^ swz(xrow0);
+  load_w(0);
+  load_sc(0);
+  __builtin_amdgcn_sched_barrier(0);
   uint32_t aoff[NMB];
   {
     int xrow[NMB];
@@ -124,156 +169,154 @@ __device__ __forceinline__ void mx_unit(const RegArgs& a, int N, int K, int e, i
       aoff[j] = xrow0 + 32 * j < rows ? (uint32_t)((int64_t)xrow[j] * a.x_ld * 2 + 16 * xc)
                                       : kPastEnd;
   }
-  const int aw = xrow0 * 128 + 16 * (xc ^ swz(xrow0));
-  u32x4_t xv[NMB];
-  int px = 0, left_x = T * (nt1 - nt0);
-  auto load_x = [&]() {
-    const bool on = left_x > 0;
+  // x stage g (zeros past K) into the LDS stage at byte `at`
+  auto load_x = [&](int g, int at) {
+    const bool on = g < T;
 #pragma unroll
     for (int j = 0; j < NMB; ++j)
-      xv[j] = __builtin_amdgcn_raw_buffer_load_b128(xr, on ? aoff[j] : kPastEnd,
-                                                    on ? 128 * px : 0, 0);
-    px = px + 1 < T ? px + 1 : 0;
-    --left_x;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          xr, (lds_ptr)(xl + at + 4096 * j + 1024 * wave), 16, on ? aoff[j] : kPastEnd,
+          on ? 128 * g : 0, 0, 0);
   };
-  auto store_x = [&](int st) {
 #pragma unroll
-    for (int j = 0; j < NMB; ++j)
-      *reinterpret_cast<u32x4_t*>(xl + st * kXBytes + aw + 4096 * j) = xv[j];
-  };
+  for (int g = 0; g < kXStages; ++g) load_x(g, g * kXBytes);
   // the output rows of tile rows lane and lane + 64 (the down projection)
   int orow[2] = {slot0 + min(lane, rows - 1), slot0 + min(lane + 64, rows - 1)};
   if (!GATED && a.out_by_flat) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) orow[i] = as_global<const int32_t>(a.sorted)[orow[i]];
   }
-  load_x();
-  store_x(0);
-  __syncthreads();
 
   f32x16_t acc[NMB][2];
-  auto clear = [&]() {
 #pragma unroll
-    for (int i = 0; i < NMB; ++i)
+  for (int i = 0; i < NMB; ++i)
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
-  };
-  clear();
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+
   const int aswz = swz(c);
-  auto read_a = [&](bf16x8_t (&af)[NMB], int st, int i) {
-    const char* A = xl + st * kXBytes + c * 128;
+  // chunk i (16 inputs) of the x stage at byte `at`: 8 of group h of its two
+  auto read_a = [&](bf16x8_t (&af)[NMB], int at, int i) {
+    const char* A = xl + at + c * 128 + 16 * ((4 * h + i) ^ aswz);
 #pragma unroll
     for (int mb = 0; mb < NMB; ++mb)
-      af[mb] = as_bf16x8(
-          *reinterpret_cast<const u32x4_t*>(A + 4096 * mb + 16 * ((4 * h + i) ^ aswz)));
+      af[mb] = as_bf16x8(*reinterpret_cast<const u32x4_t*>(A + 4096 * mb));
   };
+  bf16x8_t af[2][NMB], bf[2];
+  // side s of chunk i of stage j of the line of parity `odd`
+  auto weights = [&](int j, int i, int s, bool odd) {
+    const uint32_t v = odd ? sc4[s][2 + (j >> 1)] : sc4[s][j >> 1];
+    bf[s] = mx_weights(w[s][j][i], mx_scale((v >> (16 * (j & 1))) & 0xffu));
+  };
+  stage_barrier<0>();
+  take_w();
+  take_sc(0);
+  read_a(af[0], 0, 0);
+  weights(0, 0, 0, false);
+  weights(0, 0, 1, false);
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+  load_w(1);
+  load_sc(2);
+  __builtin_amdgcn_sched_barrier(0);
 
-  // ---- a finished tile: through the wave's scratch, 32 rows at a time, so that
-  // every store is 16 bytes of a row
-  uint16_t* O = reinterpret_cast<uint16_t*>(scratch);
-  auto epilogue = [&](int nt) {
-    const int och0 = nt * TC + wave * WC;
+  // ---- the lines, four x stages each, four chunks of 16 inputs a stage.  The
+  // operands of a chunk are read and converted during the one before it, so the
+  // matrix instructions wait for neither; that is why a stage's barrier stands
+  // before its last chunk, when its x has been read for good.  The x stage three
+  // ahead then takes its place, and after a line's last barrier the line after the
+  // next one the place of the next, which is in registers by then.
+  // Loads are back in the order of their issue: at stage j's barrier the next
+  // stage's x (two barriers old) is, when no more are out than the x stage issued
+  // since, and, in a line's first two stages, the weight line issued between.
+  int at = 0;
+#pragma nounroll
+  for (int l = 0; l < L; ++l) {
+    const bool odd = l & 1;
 #pragma unroll
-    for (int mb = 0; mb < NMB; ++mb) {
+    for (int j = 0; j < 4; ++j) {
+      const int next = at + kXBytes < kXStages * kXBytes ? at + kXBytes : 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (i == 3) {
+          if (j < 2)
+            stage_barrier<NMB + kWLoads>();
+          else
+            stage_barrier<NMB>();
+          load_x(4 * l + j + kXStages, at);
+          read_a(af[0], next, 0);
+          if (j == 3) take_w();
+        } else {
+          read_a(af[(i + 1) & 1], at, i + 1);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (i == 3 && j == 3 && odd) take_sc(l + 1);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+#pragma unroll
+          for (int mb = 0; mb < NMB; ++mb)
+            acc[mb][s] = mfma32x32x16(af[i & 1][mb], bf[s], acc[mb][s]);
+          if (i < 3)
+            weights(j, i + 1, s, odd);
+          else if (j < 3)
+            weights(j + 1, 0, s, odd);
+          else
+            weights(0, 0, s, !odd);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (i == 3 && j == 3) {
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+          load_w(l + 2);
+          if (odd) load_sc(l + 3);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      at = next;
+    }
+  }
+  // nothing may be on its way to LDS when its place is used again
+  wait_loads<0>();
+
+  // ---- through the wave's own LDS, 32 rows at a time, so that every store is 16
+  // bytes of a row
+  uint16_t* O = reinterpret_cast<uint16_t*>(wl);
+#pragma unroll
+  for (int mb = 0; mb < NMB; ++mb) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int row = 8 * (r >> 2) + 4 * h + (r & 3);
       if constexpr (GATED) {
-        auto rows_of = [&](auto geglu) {
-#pragma unroll
-          for (int r = 0; r < 16; r += 2) {
-            const int row = 8 * (r >> 2) + 4 * h + (r & 3);
-            uint32_t v;
-            if constexpr (decltype(geglu)::value)
-              v = (uint32_t)geglu_bf16(bf16_round(acc[mb][0][r]), bf16_round(acc[mb][1][r])) |
-                  ((uint32_t)geglu_bf16(bf16_round(acc[mb][0][r + 1]),
-                                        bf16_round(acc[mb][1][r + 1]))
-                   << 16);
-            else
-              v = swiglu_fast2(acc[mb][0][r], acc[mb][1][r], acc[mb][0][r + 1],
-                               acc[mb][1][r + 1]);
-            O[row * WC + c] = (uint16_t)v;
-            O[(row + 1) * WC + c] = (uint16_t)(v >> 16);
-          }
-        };
-        if (a.act == kActGeglu)
-          rows_of(PfFlag<true>{});
-        else
-          rows_of(PfFlag<false>{});
+        O[row * WC + c] = mx_bf16(mx_act(a.act, acc[mb][0][r], acc[mb][1][r]));
       } else {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int row = 8 * (r >> 2) + 4 * h + (r & 3);
-#pragma unroll
-          for (int s = 0; s < 2; ++s)
-            O[row * WC + 32 * s + c] = __builtin_bit_cast(uint16_t, (__bf16)acc[mb][s][r]);
-        }
+        for (int s = 0; s < 2; ++s) O[row * WC + 32 * s + c] = mx_bf16(acc[mb][s][r]);
       }
-      wave_sync();
-      constexpr int CPR = WC / 8;  // 16-byte runs per row
-#pragma unroll
-      for (int i = 0; i < 32 * CPR / 64; ++i) {
-        const int id = lane + 64 * i, row = id / CPR, cc = id % CPR;
-        const int trow = 32 * mb + row;
-        const int64_t orw = GATED ? slot0 + trow : __shfl(orow[mb >> 1], trow & 63, 64);
-        const u32x4_t v = *reinterpret_cast<const u32x4_t*>(O + row * WC + 8 * cc);
-        if (trow < rows && och0 + 8 * cc < N)
-          *(gptr<u32x4_t>)(as_global<uint16_t>(a.out) + orw * a.out_ld + och0 + 8 * cc) = v;
-      }
-      wave_sync();
     }
-  };
-
-  int xst = 0;
-#pragma nounroll
-  for (int nt = nt0; nt < nt1; ++nt) {
-#pragma nounroll
-    for (int l = 0; l < L; ++l) {
-      load_w(Wn);
+    wave_sync();
+    constexpr int CPR = WC / 8;  // 16-byte runs per row
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (4 * l + j < T) {
-          load_x();
-          __builtin_amdgcn_sched_barrier(0);
-          float sc[2];
-#pragma unroll
-          for (int s = 0; s < 2; ++s) {
-            const uint32_t pair = W.sc[s][j >> 1] >> (16 * (j & 1));
-            sc[s] = mx_scale((h ? pair >> 8 : pair) & 0xffu);
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            bf16x8_t af[NMB];
-            read_a(af, xst, i);
-            bf16x8_t bf[2];
-#pragma unroll
-            for (int s = 0; s < 2; ++s) bf[s] = mx_weights(W.w[s][j][i], sc[s]);
-#pragma unroll
-            for (int mb = 0; mb < NMB; ++mb)
-#pragma unroll
-              for (int s = 0; s < 2; ++s) acc[mb][s] = mfma32x32x16(af[mb], bf[s], acc[mb][s]);
-          }
-          __builtin_amdgcn_sched_barrier(0);
-          store_x(xst ^ 1);
-          __syncthreads();
-          xst ^= 1;
-        }
-      }
-      W = Wn;
+    for (int i = 0; i < 32 * CPR / 64; ++i) {
+      const int id = lane + 64 * i, row = id / CPR, cc = id % CPR;
+      const int trow = 32 * mb + row;
+      const int64_t orw = GATED ? slot0 + trow : __shfl(orow[mb >> 1], trow & 63, 64);
+      const u32x4_t v = *reinterpret_cast<const u32x4_t*>(O + row * WC + 8 * cc);
+      if (trow < rows && och0 + 8 * cc < N)
+        *(gptr<u32x4_t>)(as_global<uint16_t>(a.out) + orw * a.out_ld + och0 + 8 * cc) = v;
     }
-    epilogue(nt);
-    clear();
+    wave_sync();
   }
 }
 
 template <bool GATED, int ROWS>
-__global__ __launch_bounds__(kNT, ROWS == 128 ? 2 : 3) void mx_tile_kernel(RegLaunch L) {
+__global__ __launch_bounds__(kNT, 2) void mx_tile_kernel(RegLaunch L) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   RegUnit<ROWS> u;
   if (!u.place(L, blockIdx.x)) return;
   u.find_rows(L);
   const RegArgs r = pick_reg(u.second, L.a2, L.x_bytes2, L.a, L.x_bytes);
 #define MLXR_MXU(NMB_) \
-  mx_unit<GATED, ROWS, NMB_>(r, L.a.N, L.a.K, u.e, u.slot0, u.rows, u.nt0, u.nt1, smem)
+  mx_unit<GATED, ROWS, NMB_>(r, L.a.N, L.a.K, u.e, u.slot0, u.rows, u.nt0, smem)
   if constexpr (ROWS == 128) {
     if (u.rows > 96)
       MLXR_MXU(4);

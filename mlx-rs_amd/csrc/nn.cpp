@@ -29,6 +29,8 @@ Status check_qlinear(const mlxr_moe_qlinear& q, int64_t experts, int64_t out,
   const bool mx = q.bits == MLXR_MOE_BITS_MXFP4;
   if (mx && (!q.weight || !q.scales || q.biases))
     return Status::error(n + ": mode mxfp4 takes weight and scales, no biases");
+  if (mx && (reinterpret_cast<uintptr_t>(q.scales) & 3))
+    return Status::error(n + ": scales must be 4-byte aligned");
   if (dense && (!q.weight || q.scales || q.biases))
     return Status::error(n + ": a dense (bits 16) weight takes no scales or "
                              "biases");

@@ -107,6 +107,8 @@ class QuantizedSwitchLinear:
             raise MlxrMoeError("QuantizedSwitchLinear: biases are required (affine mode)")
         self.weight = weight.contiguous()
         self.scales = scales.contiguous()
+        if mode == "mxfp4":
+            self.scales = ops._aligned(self.scales, 4)
         self.biases = None if biases is None else biases.contiguous()
         self.mode = mode
         self.group_size = _group_size(group_size, mode)

@@ -158,6 +158,11 @@ def _quantize_mxfp4(w, group_size, bits):
     return wq, sc, None
 
 
+def _aligned(t, nbytes):
+    """t, or a copy of it where its address is not a multiple of nbytes."""
+    return t if t.data_ptr() % nbytes == 0 else t.clone()
+
+
 def _check_mxfp4(name, w, scales, biases):
     """w [.., K/8] words and scales [.., K/32] bytes of the same rows: the C
     ABI reads that much of both."""
@@ -232,6 +237,7 @@ def gather_qmm(x, w, scales, biases=None, lhs_indices=None, rhs_indices=None,
         _check_mxfp4("gather_qmm", w, scales, biases)
         if w.ndim != 3:
             raise MlxrMoeError("gather_qmm: w must be [E, N, K/8]")
+        scales = _aligned(scales.contiguous(), 4)
     if w.shape[-1] * 32 != K * b and transpose:
         raise MlxrMoeError(
             f"gather_qmm: w last dim {w.shape[-1]} does not match K={K} at {b} bits")

@@ -130,6 +130,7 @@ def test_gather_qmm_refuses(pkg):
     assert call(E=1025) == -1 and "num_experts" in C.last_error()
     assert call(x=8) == -1 and "aligned" in C.last_error()
     assert call(w=None) == -1 and "null array" in C.last_error()
+    assert call(scales=18) == -1 and "4-byte aligned" in C.last_error()
     assert call() == -1 and "workspace" in C.last_error()
 
 
@@ -150,6 +151,8 @@ def test_descriptors_refuse(pkg):
     assert "no biases" in C.last_error()
     assert glu(C.QLinear(16, None, None, 8, 256, 512, 32, M), gate, down) == -1
     assert "weight and scales" in C.last_error()
+    assert glu(C.QLinear(16, 18, None, 8, 256, 512, 32, M), gate, down) == -1
+    assert "4-byte aligned" in C.last_error()
     assert glu(C.QLinear(16, 16, None, 8, 256, 512, 64, M), gate, down) == -1
     assert "group_size must be 32" in C.last_error()
     assert glu(gate, gate, C.QLinear(16, 16, 16, 8, 512, 256, 64, 4)) == -1
@@ -391,7 +394,8 @@ def test_gather_empty(pkg, dev):
 @gpu
 @pytest.mark.parametrize("T", [6, 700])
 def test_gather_scales_at_any_address(pkg, dev, T):
-    """Scales need no alignment: a view one byte into its storage."""
+    """Scales at an address that the kernels do not take (a view one byte into
+    its storage) are copied."""
     E, N, K = 3, 128, 320
     g = torch.Generator().manual_seed(T)
     wq, sc = bank(g, (E, N, K))
