@@ -5,6 +5,7 @@
 // thread-local message.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cstring>
 #include <string>
 
@@ -164,9 +165,13 @@ int run_gather(const char* op, const void* x, int64_t x_batch, int64_t M,
   int32_t* xrow = c.take<int32_t>(R);
   DispatchBuffers db = carve_dispatch(c, R, E, status);
   uint16_t* ob = static_cast<uint16_t*>(out);
-  st = from_hip(launch_gather_prep(lhs_indices, rhs_indices, B, M, x_batch, E,
-                                   N, ids, xrow, ob, status, s),
-                (o + " prep").c_str());
+  // mxfp4, few rows: one launch, which groups the indices itself
+  const bool direct =
+      bits == kBitsMxfp4 && R <= kMxIdsRows && !nn::use_prefill_path(R, E, bits);
+  if (!direct)
+    st = from_hip(launch_gather_prep(lhs_indices, rhs_indices, B, M, x_batch, E,
+                                     N, ids, xrow, ob, status, s),
+                  (o + " prep").c_str());
   QGemmArgs a{};
   a.x = static_cast<const uint16_t*>(x);
   a.x_ld = K;
@@ -194,6 +199,21 @@ int run_gather(const char* op, const void* x, int64_t x_batch, int64_t M,
   a.out_ld = N;
   a.out_by_flat = true;
   a.gated = false;
+  if (direct) {
+    a.work_rows = kWorkRows;
+    MxIds d{};
+    d.ids = reinterpret_cast<const int32_t*>(rhs_indices);
+    d.lhs = lhs_indices;
+    d.status = status;
+    d.n = (int32_t)R;
+    d.M = (int32_t)M;
+    d.div = lhs_indices ? 1 : (int32_t)(B / x_batch);
+    d.E = (int32_t)E;
+    d.x_batch = (int32_t)std::min<int64_t>(x_batch, INT32_MAX);
+    d.zero_bad = true;
+    return finish(from_hip(
+        launch_mx_stream(a, dispatch_max_work(R, E), nullptr, 0, "qgemm_down", s, &d), op));
+  }
   db.work_rows = work_rows_for(R, E, {&a});
   a.work_rows = (uint8_t)db.work_rows;
   if (st.ok)

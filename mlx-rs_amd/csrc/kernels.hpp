@@ -371,9 +371,23 @@ hipError_t launch_qgemm_prefill_tall(const QGemmArgs& a, int64_t x_rows, int64_t
 
 // ------------------------------------------- mx_stream.hip, mx_tile.hip
 // launch_qgemm's kernels for kBitsMxfp4: work items (few rows per expert), and
-// M-tiles of tile_rows (64 or 128) rows.
+// M-tiles of tile_rows (64 or 128) rows.  With ids the work items of n <= 64 rows
+// are found in the kernel, from no dispatch: flat row f of batch b = f / M has
+// expert ids[b] and x row (lhs ? lhs[b] : b / div) * M + f % M, and its output row
+// is f.
+constexpr int kMxIdsRows = 64;
+struct MxIds {
+  const int32_t* ids;   // [n / M]
+  const uint32_t* lhs;  // [n / M] or null
+  int32_t* status;      // set to 1 by an index out of range, else to 0; may be null
+  int32_t n, M, div, E;
+  int32_t x_batch;      // bound on lhs
+  bool skip_minus1;     // an id of -1 is no error
+  bool zero_bad;        // rows of indices out of range are cleared
+};
 hipError_t launch_mx_stream(const QGemmArgs& a, int64_t max_items, const QGemmArgs* shared,
-                            int64_t shared_rows, const char* profile, hipStream_t s);
+                            int64_t shared_rows, const char* profile, hipStream_t s,
+                            const MxIds* ids = nullptr);
 hipError_t launch_mx_tile(const QGemmArgs& a, int64_t x_rows, int tile_rows, int64_t max_tiles,
                           const QGemmArgs* shared, int64_t shared_rows, const char* profile,
                           hipStream_t s);

@@ -3,19 +3,26 @@
 //
 //   out[p, n] = sum_k x[row(p), k] * w[e, n, k]
 //
-// over the work items of the dispatch (at most 8 or 16 rows of one expert), f32
-// sums of exact bf16 products.  HBM-bound: 4.25 bits a weight, each read once per
-// item.
+// over work items (at most 8 or 16 rows of one expert), f32 sums of exact bf16
+// products.  HBM-bound: 4.25 bits a weight, each read once per item.
 //
-// A workgroup is four waves: one item x 64 / KS channels.  A wave owns 16
-// channels (gated: of gate and of up) over one of KS slices of the input dim;
-// the slices' sums meet in LDS, added in slice order.  Per step of four groups
-// (128 inputs) lane (n, q) = (l % 16, l / 16) loads the 16 bytes of channel n's
-// group 4 s + q, one scale byte with it, and makes four MFMA operands of it: in
-// operand i, quarter q holds inputs 8 i .. 8 i + 7 of its group, so x is read
-// from LDS in the same order, and one v_mfma_f32_16x16x32_bf16 sums 8 inputs of
-// four groups at once.  A lane converts 32 weights with 16 instructions and one
-// scale.  D steps of loads are in flight per wave.
+// A workgroup is four waves: one item x (64 / KS) nb channels.  A wave owns nb
+// blocks of 16 channels (gated: of gate and of up) over one of KS slices of the
+// input dim; the slices' sums meet in LDS, added in slice order.  Per step of four
+// groups (128 inputs) lane (n, q) = (l % 16, l / 16) loads the 16 bytes of channel
+// n's group 4 s + q and makes four MFMA operands of them: in operand i, quarter q
+// holds inputs 8 i .. 8 i + 7 of its group, so x is read from LDS in the same
+// order, and one v_mfma_f32_16x16x32_bf16 sums 8 inputs of four groups at once.  A
+// lane converts its 32 weights with 16 instructions and one scale.  D steps of
+// loads are in flight per wave, across its blocks.  The scale bytes of the wave's
+// channels are contiguous in memory and come to LDS whole at the start: a byte
+// load per step from each of 16 rows takes the address path as long as the 1 KB of
+// weights beside it.
+//
+// The items come from a dispatch's records, or, with up to 64 rows, are found by
+// every workgroup for itself from the expert ids (MxIds): ten ballots group a
+// wave's ids, which takes less than waiting for a record and saves the dispatch's
+// launch.
 #include <algorithm>
 
 #include "mx.hpp"
@@ -25,61 +32,164 @@
 namespace mlxr_moe {
 namespace {
 
+// timing builds: steps in flight (gated, not), waves to slice for, blocks per wave
+// and workgroups to keep
+#ifndef MLXR_MX_DG
+#define MLXR_MX_DG 4
+#endif
+#ifndef MLXR_MX_D
+#define MLXR_MX_D 6
+#endif
+#ifndef MLXR_MX_KS_WAVES
+#define MLXR_MX_KS_WAVES 2048
+#endif
+#ifndef MLXR_MX_NB
+#define MLXR_MX_NB 4
+#endif
+#ifndef MLXR_MX_NB_UNITS
+#define MLXR_MX_NB_UNITS 768
+#endif
 constexpr int kWaves = 4;
+typedef __attribute__((address_space(3))) void* lds_ptr;
 
 struct MxShape {
   int tiles_n;  // channel tiles per item
+  int nb;       // 16-channel blocks per wave
   int units1, items1, rows2;
+  int sc_bytes;  // LDS of a wave's scales, one side (whole KB)
 };
 
-template <bool GATED, int TT, int KS, int D>
-__global__ __launch_bounds__(64 * kWaves) void mx_stream_kernel(QGemmArgs a, QGemmArgs a2,
-                                                                MxShape sh) {
+// An item: rows [0, nt) of expert e; flat rows in fl, or slots from row0 on.
+template <int TT>
+struct Item {
+  int e, nt, row0;
+  int fl[TT];
+};
+
+// The item of this workgroup from the ids, each wave for itself: equal ids form
+// an expert's rows, every TT-th of them starts an item; items are in the order of
+// those.  False without one.  Ids outside [0, E) are no one's: workgroup 0 sets the
+// status word, and with zero_bad every first item's workgroup clears their rows of
+// its channels [ch0, ch0 + chs).
+template <int TT>
+__device__ __forceinline__ bool find_item(const MxIds& d, int ai, bool status, int ch0, int chs,
+                                          uint16_t* out, int64_t out_ld, Item<TT>& it) {
+  const int lane = threadIdx.x & 63;
+  const bool row = lane < d.n;
+  const int batch = lane / d.M;
+  const int id = row ? d.ids[batch] : -1;
+  bool ok = row && (uint32_t)id < (uint32_t)d.E;
+  if (d.lhs && row) ok = ok && d.lhs[batch] < (uint32_t)d.x_batch;
+  uint64_t peers = __ballot(ok);
+#pragma unroll
+  for (int b = 0; b < 10; ++b) {
+    const uint64_t m = __ballot((id >> b) & 1);
+    peers &= (id >> b) & 1 ? m : ~m;
+  }
+  const uint64_t below = (1ull << lane) - 1;
+  const int rank = __popcll(peers & below);
+  const uint64_t starts = __ballot(ok && rank % TT == 0);
+  if (ai == 0) {
+    const uint64_t bad = __ballot(row && !ok && !(d.skip_minus1 && id == -1));
+    if (status && d.status && threadIdx.x == 0) *d.status = bad != 0;
+    if (d.zero_bad && bad) {
+      const uint64_t all = __ballot(row && !ok);
+      for (int r = 0; r < d.n; ++r)
+        if ((all >> r) & 1)
+          for (int i = threadIdx.x; i < chs; i += 64 * kWaves) out[r * out_ld + ch0 + i] = 0;
+    }
+  }
+  if (ai >= __popcll(starts)) return false;
+  // the lane that starts item ai
+  const uint64_t mine = __ballot(((starts >> lane) & 1) && __popcll(starts & below) == ai);
+  const int s = __ffsll((unsigned long long)mine) - 1;
+  const uint64_t rows = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(peers >> 32), s) << 32) |
+                        (uint32_t)__builtin_amdgcn_readlane((int)peers, s);
+  const int base = __builtin_amdgcn_readlane(rank, s);
+  it.e = __builtin_amdgcn_readlane(id, s);
+  it.nt = min(__popcll(rows) - base, TT);
+  it.row0 = 0;
+  const bool in = (rows >> lane) & 1;
+#pragma unroll
+  for (int t = 0; t < TT; ++t) {
+    const uint64_t m = __ballot(in && rank == base + min(t, it.nt - 1));
+    it.fl[t] = __ffsll((unsigned long long)m) - 1;
+  }
+  return true;
+}
+
+template <bool GATED, int TT, int KS, int D, bool IDS>
+__global__ __launch_bounds__(64 * kWaves, TT == 8 ? 4 : 2) void mx_stream_kernel(
+    QGemmArgs a, QGemmArgs a2, MxShape sh, MxIds ids) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   constexpr int NM = GATED ? 2 : 1;
-  Unit u;
-  if (!decode_unit<TT>(a, sh.tiles_n, sh.units1, sh.items1, sh.rows2, u)) return;
-  const RegArgs r = pick_reg(u.shared, a2, 0, a, 0);
-  const int K = a.K, G = K / kMxGroup, S = (G + 3) / 4;
-  const int e = u.wk.x, row0 = u.wk.y, nt = min(u.wk.z, TT);
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int cw = wave / KS, kq = wave % KS;
   const int n = lane & 15, q = lane >> 4;
-  const int ch = (u.tile * (kWaves / KS) + cw) * 16 + n;
-  const int64_t wrow = (int64_t)e * r.e_rows + ch;
+  Item<TT> it;
+  int tile;
+  bool second = false;
+  if constexpr (IDS) {
+    const int ai = blockIdx.x / sh.tiles_n;
+    tile = blockIdx.x - ai * sh.tiles_n;
+    const int chs = kWaves / KS * sh.nb * 16;
+    if (!find_item<TT>(ids, ai, blockIdx.x == 0, tile * chs, chs, a.out, a.out_ld, it)) return;
+  } else {
+    Unit u;
+    if (!decode_unit<TT>(a, sh.tiles_n, sh.units1, sh.items1, sh.rows2, u)) return;
+    second = u.shared;
+    tile = u.tile;
+    it.e = u.wk.x, it.row0 = u.wk.y, it.nt = min(u.wk.z, TT);
+    const int fl[8] = {u.fr0.x, u.fr0.y, u.fr0.z, u.fr0.w, u.fr1.x, u.fr1.y, u.fr1.z, u.fr1.w};
+#pragma unroll
+    for (int t = 0; t < TT; ++t) it.fl[t] = TT == 8 ? (t < it.nt ? fl[t & 7] : fl[0]) : 0;
+  }
+  const RegArgs r = pick_reg(second, a2, 0, a, 0);
+  const int K = a.K, G = K / kMxGroup, S = (G + 3) / 4;
+  const int nt = it.nt;
   const int SS = (S + KS - 1) / KS, s0 = kq * SS;
-  const int cnt = max(min(S - s0, SS), 0);  // this wave's steps
-
+  const int cnt = max(min(S - s0, SS), 0);  // this wave's steps of a block
+  const int nb = KS > 1 ? 1 : sh.nb;
+  const int total = nb * cnt;
+  const int ch0 = (tile * (kWaves / KS) + cw) * nb * 16;  // the wave's channels
+  const int64_t wrow0 = (int64_t)it.e * r.e_rows + ch0;
   const u32x4_t* wp[NM];
-  const uint8_t* sp[NM];
 #pragma unroll
   for (int m = 0; m < NM; ++m) {
     const QWeights& W = m == 0 ? r.w0 : r.w1;
-    wp[m] = reinterpret_cast<const u32x4_t*>(W.w) + wrow * G;
-    sp[m] = reinterpret_cast<const uint8_t*>(W.scales) + wrow * G;
+    wp[m] = reinterpret_cast<const u32x4_t*>(W.w) + (wrow0 + n) * G;
   }
+  const __amdgpu_buffer_rsrc_t sr0 = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<uint16_t*>(r.w0.scales) + wrow0 * (G / 2), 0, nb * 16 * G, kBufFlags);
+  const __amdgpu_buffer_rsrc_t sr1 = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<uint16_t*>(GATED ? r.w1.scales : r.w0.scales) + wrow0 * (G / 2), 0, nb * 16 * G,
+      kBufFlags);
+  // LDS: x [TT][xs], the waves' scales, and with slices their sums
+  const int xs = 128 * S + 8;  // 16 bytes more a row, so that rows start on other banks
+  uint16_t* xl = reinterpret_cast<uint16_t*>(smem);
+  const int x_bytes = (TT * xs * 2 + 15) & ~15;
+  char* scl = smem + x_bytes + wave * NM * sh.sc_bytes;
+#pragma unroll
+  for (int m = 0; m < NM; ++m)
+    for (int o = 0; o < sh.sc_bytes; o += 1024)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(m ? sr1 : sr0,
+                                               (lds_ptr)(scl + m * sh.sc_bytes + o), 16,
+                                               o + 16 * lane, 0, 0, 0);
   // x rows: thread k8 holds inputs 8 k8 .. 8 k8 + 7 of every row of the item
   int64_t xr[TT];
-  {
-    const int fl[8] = {u.fr0.x, u.fr0.y, u.fr0.z, u.fr0.w, u.fr1.x, u.fr1.y, u.fr1.z, u.fr1.w};
 #pragma unroll
-    for (int t = 0; t < TT; ++t) {
-      const int tt = min(t, nt - 1);
-      if (r.x_by_slot) {
-        xr[t] = row0 + tt;
-      } else {
-        int f;
-        if constexpr (TT == 8)
-          f = t < nt ? fl[t] : fl[0];
-        else
-          f = r.sorted[row0 + tt];
-        xr[t] = r.row_map ? r.row_map[f] : f / r.row_div;
-      }
+  for (int t = 0; t < TT; ++t) {
+    if constexpr (IDS) {
+      const int f = it.fl[t], b = f / ids.M;
+      xr[t] = (int64_t)(ids.lhs ? (int)ids.lhs[b] : b / ids.div) * ids.M + (f - b * ids.M);
+    } else if (r.x_by_slot) {
+      xr[t] = it.row0 + min(t, nt - 1);
+    } else {
+      const int f = TT == 8 ? it.fl[t] : r.sorted[it.row0 + min(t, nt - 1)];
+      xr[t] = r.row_map ? r.row_map[f] : f / r.row_div;
     }
   }
-  const int xs = 128 * S + 8;  // LDS row: 16 bytes more, so that rows start on other banks
-  uint16_t* xl = reinterpret_cast<uint16_t*>(smem);
   const u32x4_t zq = {0u, 0u, 0u, 0u};
   const int per_row = 16 * S, in_row = K >> 3;
   auto load_x = [&](int k8, u32x4_t (&v)[TT]) {
@@ -94,27 +204,28 @@ __global__ __launch_bounds__(64 * kWaves) void mx_stream_kernel(QGemmArgs a, QGe
     if (k8 < per_row) {
 #pragma unroll
       for (int t = 0; t < TT; ++t)
-        if (t < nt) *reinterpret_cast<u32x4_t*>(xl + (size_t)t * xs + 8 * k8) = v[t];
+        if (t < nt) *reinterpret_cast<u32x4_t*>(xl + t * xs + 8 * k8) = v[t];
     }
   };
   u32x4_t xv[TT];
   load_x(tid, xv);
+  asm volatile("" ::: "memory");
   __builtin_amdgcn_sched_barrier(0);
 
   u32x4_t w[D][NM];
-  uint32_t sc[D][NM];
-  auto load_w = [&](int j, int i) {  // step i of this wave into slot j
-    const int g = min(4 * (s0 + min(i, cnt - 1)) + q, G - 1);
+  int pb = 0, ps = 0;  // the next load: block, step within it (the last one again past the end)
+  auto load_w = [&](int j) {
+    const int64_t at = (int64_t)pb * 16 * G + min(4 * min(s0 + ps, S - 1) + q, G - 1);
 #pragma unroll
-    for (int m = 0; m < NM; ++m) {
-      w[j][m] = wp[m][g];
-      sc[j][m] = sp[m][g];
-    }
+    for (int m = 0; m < NM; ++m) w[j][m] = wp[m][at];
+    if (ps + 1 < cnt)
+      ++ps;
+    else if (pb + 1 < nb)
+      ps = 0, ++pb;
   };
-  if (cnt > 0) {
 #pragma unroll
-    for (int j = 0; j < D; ++j) load_w(j, j);
-  }
+  for (int j = 0; j < D; ++j) load_w(j);
+  asm volatile("" ::: "memory");
   __builtin_amdgcn_sched_barrier(0);
   store_x(tid, xv);
   for (int k8 = tid + 64 * kWaves; k8 < per_row; k8 += 64 * kWaves) {
@@ -122,39 +233,84 @@ __global__ __launch_bounds__(64 * kWaves) void mx_stream_kernel(QGemmArgs a, QGe
     load_x(k8, v);
     store_x(k8, v);
   }
+  // (the scales were issued before the D * NM weight loads)
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(D * NM) : "memory");
   __syncthreads();
 
   f32x4_t acc[NM];
 #pragma unroll
   for (int m = 0; m < NM; ++m) acc[m] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   // (rows past the item's read its first row: their sums go nowhere)
-  const uint16_t* xa = xl + (size_t)(n < nt ? n : 0) * xs + 32 * q;
-  for (int i0 = 0; i0 < cnt; i0 += D) {
+  const uint16_t* xa = xl + (n < nt ? n : 0) * xs + 32 * q;
+  const bool ragged = G & 3;  // the last step has groups past the row
+  auto finish = [&](int b) {  // block b's sums are whole
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int t = 4 * q + i;
+      if (t < nt) {
+        const int ch = ch0 + 16 * b + n;
+        int64_t orow = it.row0 + t;
+        if (IDS) {
+          int f = it.fl[0];
+#pragma unroll
+          for (int k = 1; k < TT; ++k) f = t == k ? it.fl[k] : f;
+          orow = f;
+        } else if (!GATED && r.out_by_flat) {
+          orow = r.sorted[it.row0 + t];
+        }
+        r.out[orow * r.out_ld + ch] =
+            GATED ? mx_bf16(mx_act(r.act, acc[0][i], acc[NM - 1][i])) : mx_bf16(acc[0][i]);
+      }
+    }
+  };
+  int cb = 0, cs = 0;  // block and step of the next sum
+  for (int g0 = 0; g0 < total; g0 += D) {
 #pragma unroll
     for (int j = 0; j < D; ++j) {
-      const int i = i0 + j;
-      if (i < cnt) {
-        const int s = s0 + i;
+      if (g0 + j < total) {
+        const int s = s0 + cs;
         bf16x8_t xf[4];
 #pragma unroll
         for (int f = 0; f < 4; ++f)
           xf[f] = as_bf16x8(*reinterpret_cast<const u32x4_t*>(xa + 128 * s + 8 * f));
-        const bool in = 4 * s + q < G;  // groups past the row: zeros (x is zero there too)
+        const int g = min(4 * s + q, G - 1);
+        uint32_t b[NM];
+#pragma unroll
+        for (int m = 0; m < NM; ++m)
+          b[m] = *reinterpret_cast<const uint8_t*>(scl + m * sh.sc_bytes + (16 * cb + n) * G + g);
+        if (ragged) {  // (x is zero there)
+          const bool in = 4 * s + q < G;
+#pragma unroll
+          for (int m = 0; m < NM; ++m) {
+            b[m] = in ? b[m] : 0u;
+#pragma unroll
+            for (int f = 0; f < 4; ++f) w[j][m][f] = in ? w[j][m][f] : 0u;
+          }
+        }
 #pragma unroll
         for (int m = 0; m < NM; ++m) {
-          const float scale = mx_scale(in ? sc[j][m] : 0u);
+          const float scale = mx_scale(b[m]);
 #pragma unroll
           for (int f = 0; f < 4; ++f)
-            acc[m] = mfma16x16x32(xf[f], mx_weights(in ? w[j][m][f] : 0u, scale), acc[m]);
+            acc[m] = mfma16x16x32(xf[f], mx_weights(w[j][m][f], scale), acc[m]);
+        }
+        if (++cs == cnt) {
+          if constexpr (KS == 1) {
+            finish(cb);
+#pragma unroll
+            for (int m = 0; m < NM; ++m) acc[m] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+          }
+          cs = 0;
+          ++cb;
         }
       }
-      load_w(j, i + D);
+      load_w(j);
     }
   }
 
   if constexpr (KS > 1) {
     // the slices' sums, in slice order, on the first slice's wave
-    f32x4_t* red = reinterpret_cast<f32x4_t*>(smem + (((size_t)TT * xs * 2 + 15) & ~size_t(15)));
+    f32x4_t* red = reinterpret_cast<f32x4_t*>(smem + x_bytes + kWaves * NM * sh.sc_bytes);
 #pragma unroll
     for (int m = 0; m < NM; ++m) red[(wave * NM + m) * 64 + lane] = acc[m];
     __syncthreads();
@@ -163,63 +319,64 @@ __global__ __launch_bounds__(64 * kWaves) void mx_stream_kernel(QGemmArgs a, QGe
     for (int k = 1; k < KS; ++k)
 #pragma unroll
       for (int m = 0; m < NM; ++m) acc[m] += red[((wave + k) * NM + m) * 64 + lane];
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int t = 4 * q + i;
-    if (t < nt) {
-      const int slot = row0 + t;
-      if constexpr (GATED) {
-        r.out[(int64_t)slot * r.out_ld + ch] = mx_bf16(mx_act(r.act, acc[0][i], acc[1][i]));
-      } else {
-        const int64_t orow =
-            !r.out_by_flat ? slot : TT == 8 ? u.rec[4 + t] : r.sorted[slot];
-        r.out[orow * r.out_ld + ch] = mx_bf16(acc[0][i]);
-      }
-    }
+    finish(0);
   }
 }
 
 }  // namespace
 
 hipError_t launch_mx_stream(const QGemmArgs& a, int64_t max_items, const QGemmArgs* shared,
-                            int64_t shared_rows, const char* profile, hipStream_t s) {
+                            int64_t shared_rows, const char* profile, hipStream_t s,
+                            const MxIds* ids) {
   const QGemmArgs& b = shared ? *shared : a;
   const int64_t items2 = shared ? (shared_rows + a.work_rows - 1) / a.work_rows : 0;
   const int64_t items = max_items + items2;
-  const int S = (a.K / kMxGroup + 3) / 4;
+  const int G = a.K / kMxGroup, S = (G + 3) / 4;
   // slices: until there are 2048 waves (two per SIMD), two steps each at least
   int ks = 1;
-  while (ks < kWaves && items * (a.N / 16) * ks < 2048 && S >= 4 * ks) ks *= 2;
-  const int tiles_n = a.N / (16 * (kWaves / ks));
+  while (ks < kWaves && items * (a.N / 16) * ks < MLXR_MX_KS_WAVES && S >= 4 * ks) ks *= 2;
+  int nb = 1;
+  if (ks == 1)
+    while (nb < MLXR_MX_NB && a.N % (64 * 2 * nb) == 0 &&
+           items * (a.N / (64 * 2 * nb)) >= MLXR_MX_NB_UNITS)
+      nb *= 2;
+  const int tiles_n = a.N / (16 * (kWaves / ks) * nb);
   const int nm = a.gated ? 2 : 1;
+  const int sc_bytes = (nb * 16 * G + 1023) / 1024 * 1024;
   const size_t x_lds = ((size_t)a.work_rows * (128 * S + 8) * 2 + 15) & ~size_t(15);
-  const size_t lds = x_lds + (ks > 1 ? (size_t)kWaves * nm * 64 * sizeof(f32x4_t) : 0);
-  const MxShape sh{tiles_n, (int)(max_items * tiles_n), (int)max_items, (int)shared_rows};
+  const size_t lds = x_lds + (size_t)kWaves * nm * sc_bytes +
+                     (ks > 1 ? (size_t)kWaves * nm * 64 * sizeof(f32x4_t) : 0);
+  const MxShape sh{tiles_n, nb, (int)(max_items * tiles_n), (int)max_items, (int)shared_rows,
+                   sc_bytes};
   const dim3 grid((unsigned)(items * tiles_n));
+  const MxIds none{};
   ProfileScope prof(profile, s);
-#define MLXR_MX(G_, TT_, KS_)                                                              \
-  mx_stream_kernel<G_, TT_, KS_, (G_) ? 4 : 4><<<grid, 64 * kWaves, lds, s>>>(a, b, sh)
-#define MLXR_MX_K(G_, TT_)   \
-  do {                       \
-    if (ks == 4)             \
-      MLXR_MX(G_, TT_, 4);   \
-    else if (ks == 2)        \
-      MLXR_MX(G_, TT_, 2);   \
-    else                     \
-      MLXR_MX(G_, TT_, 1);   \
+#define MLXR_MX(G_, TT_, KS_, IDS_)                                                       \
+  mx_stream_kernel<G_, TT_, KS_, (G_) ? MLXR_MX_DG : MLXR_MX_D, IDS_>                     \
+      <<<grid, 64 * kWaves, lds, s>>>(a, b, sh, IDS_ ? *ids : none)
+#define MLXR_MX_K(G_, TT_, IDS_)   \
+  do {                             \
+    if (ks == 4)                   \
+      MLXR_MX(G_, TT_, 4, IDS_);   \
+    else if (ks == 2)              \
+      MLXR_MX(G_, TT_, 2, IDS_);   \
+    else                           \
+      MLXR_MX(G_, TT_, 1, IDS_);   \
   } while (0)
-  if (a.work_rows == kWorkRowsWide) {
-    if (a.gated)
-      MLXR_MX_K(true, 16);
-    else
-      MLXR_MX_K(false, 16);
-  } else {
-    if (a.gated)
-      MLXR_MX_K(true, 8);
-    else
-      MLXR_MX_K(false, 8);
-  }
+#define MLXR_MX_G(TT_, IDS_)       \
+  do {                             \
+    if (a.gated)                   \
+      MLXR_MX_K(true, TT_, IDS_);  \
+    else                           \
+      MLXR_MX_K(false, TT_, IDS_); \
+  } while (0)
+  if (ids)
+    MLXR_MX_G(8, true);
+  else if (a.work_rows == kWorkRowsWide)
+    MLXR_MX_G(16, false);
+  else
+    MLXR_MX_G(8, false);
+#undef MLXR_MX_G
 #undef MLXR_MX_K
 #undef MLXR_MX
   return hipGetLastError();

@@ -315,6 +315,8 @@ Status SwitchFfn::forward(const uint16_t* x, int64_t T, const int32_t* indices,
   const int64_t E = sw_.E;
   const int64_t n = T * K;
   DispatchBuffers db = carve_dispatch(ws, n, E, status);
+  if (sw_.bits == kBitsMxfp4 && n <= kMxIdsRows && !use_prefill_path(n, E, sw_.bits))
+    return experts_direct(x, T, K, indices, y, ws, status, s);
   db.work_rows = work_rows(n, nullptr);
   // (the dispatch clears *status first: no launch of its own for that)
   Status st = from_hip(
@@ -322,6 +324,45 @@ Status SwitchFfn::forward(const uint16_t* x, int64_t T, const int32_t* indices,
       "switch_mlp dispatch");
   if (!st.ok) return st;
   return experts(x, T, K, db, y, ws, s, nullptr, dc, combined);
+}
+
+Status SwitchFfn::experts_direct(const uint16_t* x, int64_t T, int64_t K,
+                                 const int32_t* indices, uint16_t* y, Carve& ws,
+                                 int32_t* status, hipStream_t s) const {
+  const int64_t n = T * K, items = dispatch_max_work(n, sw_.E);
+  uint16_t* act = ws.take<uint16_t>(n * sw_.f);
+  QGemmArgs g = gemm_shape(sw_.gate, sw_.up, true, sw_.f, sw_.d, sw_.bits);
+  g.x = x;
+  g.x_ld = sw_.d;
+  g.work_rows = kWorkRows;
+  g.E = (int32_t)sw_.E;
+  g.e_rows = sw_.gate_rows;
+  g.act = sw_.act;
+  g.out = act;
+  g.out_ld = sw_.f;
+  MxIds ids{};
+  ids.ids = indices;
+  ids.status = status;
+  ids.n = (int32_t)n;
+  ids.M = 1;
+  ids.div = (int32_t)K;
+  ids.E = (int32_t)sw_.E;
+  ids.skip_minus1 = true;
+  Status st = from_hip(launch_mx_stream(g, items, nullptr, 0, "qgemm_gated", s, &ids),
+                       "switch_mlp gate/up");
+  if (!st.ok) return st;
+  QGemmArgs h = gemm_shape(sw_.down, QWeights{}, false, sw_.d, sw_.f, sw_.bits);
+  h.x = act;  // rows by flat index
+  h.x_ld = sw_.f;
+  h.work_rows = kWorkRows;
+  h.E = g.E;
+  h.e_rows = (int32_t)sw_.d;
+  h.out = y;
+  h.out_ld = sw_.d;
+  ids.status = nullptr;
+  ids.div = 1;
+  return from_hip(launch_mx_stream(h, items, nullptr, 0, "qgemm_down", s, &ids),
+                  "switch_mlp down");
 }
 
 int SwitchFfn::work_rows(int64_t n, const SharedFold* fold) const {

@@ -146,6 +146,10 @@ class SwitchFfn {
                  const DispatchBuffers& db, uint16_t* y, Carve& ws,
                  hipStream_t s, const SharedFold* fold = nullptr,
                  const DownCombine* dc = nullptr, bool* combined = nullptr) const;
+  // The same for at most kMxIdsRows flat rows of mxfp4 experts, which need no
+  // dispatch: the launches group the ids, and the first sets *status.
+  Status experts_direct(const uint16_t* x, int64_t T, int64_t K, const int32_t* indices,
+                        uint16_t* y, Carve& ws, int32_t* status, hipStream_t s) const;
   // Whether a SwiGLU shared expert can fold into this FFN's launches at T
   // tokens: same bits and hidden size, and both on the streaming decode
   // kernel or both on the M-tiled one.
