@@ -204,9 +204,8 @@ int mlxr_moe_router_topk(const void* x, int64_t T, int64_t d,
  *   loss f32 [1] = E * sum_e counts_e / (N K) * probs_e
  * all 0 when N is 0.  A row whose logits are all -inf adds no probability; an
  * index outside [0, E) is not counted and sets the workspace's status word
- * (mlxr_moe_workspace_status).  Sums are in f32 within 16 rows or more of a
- * workgroup and in f64 across them, in a fixed order: equal inputs give equal
- * bits.  E <= 1024, K <= 64. */
+ * (mlxr_moe_workspace_status).  Sums are in f32 within a workgroup's rows and
+ * in f64 across workgroups, in a fixed order: equal inputs give equal bits.  E <= 1024, K <= 64. */
 size_t mlxr_moe_router_balance_workspace_size(int64_t T, int64_t E);
 int mlxr_moe_router_balance(const void* logits, int logits_dtype, int64_t ld,
                             int64_t T, int64_t E, const int32_t* indices,

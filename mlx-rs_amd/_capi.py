@@ -29,7 +29,13 @@ class OptionalInt(Structure):
 
     @classmethod
     def of(cls, v):
-        return cls(0, 0) if v is None else cls(int(v), 1)
+        o = _OPTIONAL.get(v)
+        if o is None:
+            o = _OPTIONAL[v] = cls(0, 0) if v is None else cls(int(v), 1)
+        return o
+
+
+_OPTIONAL = {}  # passed by value, never changed
 
 
 class QLinear(Structure):

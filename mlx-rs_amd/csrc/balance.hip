@@ -15,8 +15,8 @@
 // gradient is 0.  With N = 0 everything is 0.
 //
 // One pass over the logits, a wave per row, in the summation orders fixed here
-// (no floating-point atomics): a workgroup's rows add up in registers, its four
-// waves' sums in LDS, the workgroups' in f64 by a second kernel.
+// (no floating-point atomics): a wave's rows add up in registers, a workgroup's
+// waves in LDS, the workgroups' in f64 by a second kernel.
 #include <algorithm>
 
 #include "common.hpp"
@@ -26,8 +26,11 @@
 namespace mlxr_moe {
 namespace {
 
-constexpr int kWaves = 4;        // per workgroup of the two-launch form
+constexpr int kWaves = 4;        // per workgroup of the gradient
+constexpr int kPartWaves = 16;   // of the two-launch form's first
 constexpr int kSmallWaves = 16;  // of the one-workgroup form
+constexpr int kJoinCols = 16;    // experts per workgroup of the second launch
+constexpr int kJoinRows = 64;    // partials it reads at a time
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <int CTRL>
@@ -147,60 +150,101 @@ __device__ __forceinline__ void sum_rows(const BalanceArgs& a, int64_t r0, int64
   __syncthreads();
 }
 
-// Per workgroup: partial sums [G, E], counts [G, E], tallies [G, 2].
+// Per workgroup: partial sums [G, E], counts [G, E], tallies [G, 2]; and the
+// second launch's ticket.
 template <bool BF16, int SLOTS>
-__global__ __launch_bounds__(64 * kWaves) void balance_part_kernel(BalanceArgs a, int rows,
-                                                                   float* __restrict__ sums,
-                                                                   int32_t* __restrict__ cnts,
-                                                                   int32_t* __restrict__ tallies) {
+__global__ __launch_bounds__(64 * kPartWaves) void balance_part_kernel(
+    BalanceArgs a, int rows, float* __restrict__ sums, int32_t* __restrict__ cnts,
+    int32_t* __restrict__ tallies, int32_t* __restrict__ ticket) {
   extern __shared__ float lds[];
   float* red = lds;
-  int* hist = reinterpret_cast<int*>(red + kWaves * a.E);
+  int* hist = reinterpret_cast<int*>(red + kPartWaves * a.E);
   int* tally = hist + a.E;
   const int64_t r0 = (int64_t)blockIdx.x * rows;
-  sum_rows<BF16, SLOTS, kWaves>(a, r0, min(r0 + rows, a.T), red, hist, tally);
-  for (int e = threadIdx.x; e < a.E; e += 64 * kWaves) {
+  sum_rows<BF16, SLOTS, kPartWaves>(a, r0, min(r0 + rows, a.T), red, hist, tally);
+  for (int e = threadIdx.x; e < a.E; e += 64 * kPartWaves) {
     float s = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) s += red[w * a.E + e];
+    for (int w = 0; w < kPartWaves; ++w) s += red[w * a.E + e];
     sums[(int64_t)blockIdx.x * a.E + e] = s;
     cnts[(int64_t)blockIdx.x * a.E + e] = hist[e];
   }
   if (threadIdx.x < 2) tallies[2 * blockIdx.x + threadIdx.x] = tally[threadIdx.x];
+  if (blockIdx.x == 0 && threadIdx.x == 0) *ticket = 0;
 }
 
-// 64 experts a workgroup, its waves the workgroups' partials in turns.
-__global__ __launch_bounds__(64 * kSmallWaves) void balance_join_kernel(
-    int G, int E, const float* __restrict__ sums, const int32_t* __restrict__ cnts,
-    const int32_t* __restrict__ tallies, int32_t* __restrict__ counts, float* __restrict__ probs,
-    int32_t* __restrict__ tokens, int32_t* __restrict__ status) {
-  __shared__ double s_l[kSmallWaves][64];
-  __shared__ int c_l[kSmallWaves][64], n_l[2];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int e = blockIdx.x * 64 + lane;
+// kJoinCols experts a workgroup: their partials summed in f64, kJoinRows of the
+// workgroups at a time.  The workgroup that finishes last adds up the others'
+// shares of the loss, in their order.
+__global__ __launch_bounds__(kJoinCols* kJoinRows) void balance_join_kernel(
+    int G, int E, int K, const float* __restrict__ sums, const int32_t* __restrict__ cnts,
+    const int32_t* __restrict__ tallies, double* __restrict__ shares,
+    int32_t* __restrict__ ticket, float* __restrict__ loss, int32_t* __restrict__ counts,
+    float* __restrict__ probs, int32_t* __restrict__ tokens, int32_t* __restrict__ status) {
+  __shared__ double s_l[kJoinRows][kJoinCols];
+  __shared__ int c_l[kJoinRows][kJoinCols], n_l[2], last;
+  const int tid = threadIdx.x, col = tid % kJoinCols, row = tid / kJoinCols;
+  const int e = blockIdx.x * kJoinCols + col;
   if (tid < 2) n_l[tid] = 0;
   __syncthreads();
   double s = 0.0;
   int c = 0;
-  if (e < E)
-    for (int g = wave; g < G; g += kSmallWaves) {
-      s += sums[(int64_t)g * E + e];
-      c += cnts[(int64_t)g * E + e];
+  if (e < E) {
+    constexpr int U = 4;  // partials in flight
+    for (int g0 = row; g0 < G; g0 += U * kJoinRows) {
+      float sv[U];
+      int cv[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t at = (int64_t)min(g0 + u * kJoinRows, G - 1) * E + e;
+        sv[u] = sums[at], cv[u] = cnts[at];
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (g0 + u * kJoinRows < G) s += sv[u], c += cv[u];
     }
+  }
   int n = 0, bad = 0;
-  for (int g = tid; g < G; g += 64 * kSmallWaves) n += tallies[2 * g], bad |= tallies[2 * g + 1];
+  for (int g = tid; g < G; g += kJoinCols * kJoinRows) n += tallies[2 * g], bad |= tallies[2 * g + 1];
   if (n) atomicAdd(&n_l[0], n);
   if (bad) n_l[1] = 1;
-  s_l[wave][lane] = s;
-  c_l[wave][lane] = c;
+  s_l[row][col] = s;
+  c_l[row][col] = c;
   __syncthreads();
-  n = n_l[0];
-  if (wave == 0 && e < E) {
-    for (int w = 1; w < kSmallWaves; ++w) s += s_l[w][lane], c += c_l[w][lane];
-    counts[e] = c;
-    probs[e] = n ? (float)(s / n) : 0.0f;
+#pragma unroll
+  for (int m = kJoinRows / 2; m > 0; m >>= 1) {
+    if (row < m) {
+      s_l[row][col] += s_l[row + m][col];
+      c_l[row][col] += c_l[row + m][col];
+    }
+    __syncthreads();
   }
-  if (blockIdx.x == 0 && tid == 0) {
+  n = n_l[0];
+  if (row == 0) {
+    c = c_l[0][col];
+    const float p = n ? (float)(s_l[0][col] / n) : 0.0f;
+    if (e < E) {
+      counts[e] = c;
+      probs[e] = p;
+    }
+    double share = e < E ? (double)c * p : 0.0;
+#pragma unroll
+    for (int m = kJoinCols / 2; m > 0; m >>= 1) share += __shfl_down(share, m, kJoinCols);
+    if (col == 0) {
+      __hip_atomic_store(&shares[blockIdx.x], share, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      last = __hip_atomic_fetch_add(ticket, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) ==
+             (int)gridDim.x - 1;
+    }
+  }
+  __syncthreads();
+  if (last && tid < 64) {
+    double t = 0.0;
+    for (int b = tid; b < (int)gridDim.x; b += 64)
+      t += __hip_atomic_load(&shares[b], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+    for (int m = 32; m > 0; m >>= 1) t += __shfl_down(t, m, 64);
+    if (tid != 0) return;
+    *loss = n ? (float)(t * E / ((double)n * K)) : 0.0f;
     *tokens = n;
     *status = n_l[1];
   }
@@ -220,15 +264,6 @@ __device__ __forceinline__ void loss_of(int E, int K, int n, const int32_t* coun
   }
   if (tid == 0) *loss = n ? (float)(part[0] * E / ((double)n * K)) : 0.0f;
 }
-__global__ __launch_bounds__(256) void balance_loss_kernel(int E, int K,
-                                                           const int32_t* __restrict__ counts,
-                                                           const float* __restrict__ probs,
-                                                           const int32_t* __restrict__ tokens,
-                                                           float* __restrict__ loss) {
-  __shared__ double part[256];
-  loss_of(E, K, *tokens, counts, probs, part, loss);
-}
-
 // Everything in one workgroup, for few rows.
 template <bool BF16, int SLOTS>
 __global__ __launch_bounds__(64 * kSmallWaves) void balance_small_kernel(
@@ -351,10 +386,11 @@ __global__ __launch_bounds__(64 * kWaves) void balance_vjp_kernel(
   }
 }
 
-// Rows a workgroup of the two-launch form: four per wave, more where that would
-// make over 1024 workgroups.
+// Rows a workgroup of the two-launch form: two per wave, more where that would
+// make over 256 workgroups (one a CU; c4's 32768 rows 14.8 us and 5.9 for the
+// second launch so, 14.0 and 7.1 with two a CU, 14.5 and 10.0 with four).
 int part_rows(int64_t T) {
-  return (int)std::max<int64_t>(4 * kWaves, (T + 1023) / 1024);
+  return (int)std::max<int64_t>(2 * kPartWaves, (T + 255) / 256);
 }
 int part_groups(int64_t T) { return (int)((T + part_rows(T) - 1) / part_rows(T)); }
 // One workgroup for everything: few rows
@@ -363,7 +399,8 @@ bool one_workgroup(int64_t T, int64_t E) { return T * ((E + 63) / 64) <= 256; }
 struct BalanceScratch {
   int32_t* status;
   float* sums;
-  int32_t *cnts, *tallies;
+  int32_t *cnts, *tallies, *ticket;
+  double* shares;
 };
 BalanceScratch carve_balance(Carve& c, int64_t T, int64_t E) {
   BalanceScratch b{};
@@ -373,6 +410,8 @@ BalanceScratch carve_balance(Carve& c, int64_t T, int64_t E) {
   b.sums = c.take<float>(G * E);
   b.cnts = c.take<int32_t>(G * E);
   b.tallies = c.take<int32_t>(2 * G);
+  b.ticket = c.take<int32_t>(1);
+  b.shares = c.take<double>((E + kJoinCols - 1) / kJoinCols);
   return b;
 }
 
@@ -415,17 +454,18 @@ hipError_t launch_router_balance(const void* z, bool bf16, int64_t ld, int64_t T
     return hipGetLastError();
   }
   const int G = part_groups(T), rows = part_rows(T);
-  const size_t lds = ((size_t)(kWaves + 1) * E + 2) * 4;
-#define MLXR_BAL_CALL(BF, S)                                                                \
-  balance_part_kernel<BF, S><<<G, 64 * kWaves, lds, s>>>(a, rows, b.sums, b.cnts, b.tallies)
+  const size_t lds = ((size_t)(kPartWaves + 1) * E + 2) * 4;
+#define MLXR_BAL_CALL(BF, S)                                                                 \
+  balance_part_kernel<BF, S><<<G, 64 * kPartWaves, lds, s>>>(a, rows, b.sums, b.cnts, b.tallies, \
+                                                             b.ticket)
   if (bf16)
     MLXR_BAL_SLOTS(MLXR_BAL_CALL, true);
   else
     MLXR_BAL_SLOTS(MLXR_BAL_CALL, false);
 #undef MLXR_BAL_CALL
-  balance_join_kernel<<<(unsigned)((E + 63) / 64), 64 * kSmallWaves, 0, s>>>(
-      G, (int)E, b.sums, b.cnts, b.tallies, counts, probs, tokens, b.status);
-  balance_loss_kernel<<<1, 256, 0, s>>>((int)E, (int)K, counts, probs, tokens, loss);
+  balance_join_kernel<<<(unsigned)((E + kJoinCols - 1) / kJoinCols), kJoinCols * kJoinRows, 0,
+                        s>>>(G, (int)E, (int)K, b.sums, b.cnts, b.tallies, b.shares, b.ticket,
+                             loss, counts, probs, tokens, b.status);
   return hipGetLastError();
 }
 

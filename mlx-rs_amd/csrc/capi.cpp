@@ -168,9 +168,11 @@ int run_gather(const char* op, const void* x, int64_t x_batch, int64_t M,
   // mxfp4, few rows: one launch, which groups the indices itself
   const bool direct =
       bits == kBitsMxfp4 && R <= kMxIdsRows && !nn::use_prefill_path(R, E, bits);
+  // (the status word's slot has room for the dispatch's counter beside it)
+  int32_t* counter = bits == kBitsMxfp4 ? status + 1 : nullptr;
   if (!direct)
     st = from_hip(launch_gather_prep(lhs_indices, rhs_indices, B, M, x_batch, E,
-                                     N, ids, xrow, ob, status, s),
+                                     N, ids, xrow, ob, status, s, counter),
                   (o + " prep").c_str());
   QGemmArgs a{};
   a.x = static_cast<const uint16_t*>(x);
@@ -217,7 +219,7 @@ int run_gather(const char* op, const void* x, int64_t x_batch, int64_t M,
   db.work_rows = work_rows_for(R, E, {&a});
   a.work_rows = (uint8_t)db.work_rows;
   if (st.ok)
-    st = from_hip(launch_dispatch(ids, R, E, prefill_tile_rows(R, E, bits), db, false, s),
+    st = from_hip(launch_dispatch(ids, R, E, prefill_tile_rows(R, E, bits), db, false, s, counter),
                   (o + " dispatch").c_str());
   if (!st.ok) return finish(st);
   return finish(from_hip(launch_qgemm(a, R, dispatch_max_work(R, E, db.work_rows),

@@ -390,7 +390,10 @@ __global__ __launch_bounds__(256) void dispatch_identity_kernel(
   }
 }
 
-__global__ void zero_status_kernel(int32_t* status) { *status = 0; }
+__global__ void zero_status_kernel(int32_t* status, int32_t* counter = nullptr) {
+  *status = 0;
+  if (counter) *counter = 0;
+}
 
 // gather_qmm row preparation: flat row r = b * M + m takes expert
 // rhs[b] and x row xb(b) * M + m; rows with an index out of range get
@@ -418,8 +421,8 @@ __global__ __launch_bounds__(256) void gather_prep_kernel(
 
 }  // namespace
 
-hipError_t launch_zero_status(int32_t* status, hipStream_t s) {
-  zero_status_kernel<<<1, 1, 0, s>>>(status);
+hipError_t launch_zero_status(int32_t* status, hipStream_t s, int32_t* counter) {
+  zero_status_kernel<<<1, 1, 0, s>>>(status, counter);
   return hipGetLastError();
 }
 
@@ -441,7 +444,7 @@ hipError_t launch_dispatch(const int32_t* ids, int64_t n, int64_t E,
     return hipGetLastError();
   }
   const int nb = (int)((n + kDispatchBlock - 1) / kDispatchBlock);
-  if (reset_status) zero_status_kernel<<<1, 1, 0, s>>>(b.status);
+  if (reset_status) zero_status_kernel<<<1, 1, 0, s>>>(b.status, counter);
   if (counter) {
     dispatch_rank_scan_kernel<<<nb, kDispatchBlock, (size_t)kWaves * E * sizeof(uint16_t),
                                 s>>>(ids, (int)n, (int)E, tile_rows, b, counter);
@@ -551,9 +554,10 @@ hipError_t launch_route(const float* logits, int64_t ld, int64_t T, int64_t E,
 hipError_t launch_gather_prep(const uint32_t* lhs, const uint32_t* rhs,
                               int64_t B, int64_t M, int64_t x_batch, int64_t E,
                               int64_t N, int32_t* ids, int32_t* xrow,
-                              uint16_t* out, int32_t* status, hipStream_t s) {
+                              uint16_t* out, int32_t* status, hipStream_t s,
+                              int32_t* counter) {
   const int64_t R = B * M;
-  zero_status_kernel<<<1, 1, 0, s>>>(status);
+  zero_status_kernel<<<1, 1, 0, s>>>(status, counter);
   if (R > 0)
     gather_prep_kernel<<<(unsigned)((R + 255) / 256), 256, 0, s>>>(
         lhs, rhs, B, M, x_batch, E, N, ids, xrow, out, status);

@@ -164,15 +164,17 @@ inline int64_t dispatch_max_work(int64_t n, int64_t E, int work_rows = kWorkRows
 }
 // Clears a workspace status word with a one-thread kernel (no memset node,
 // so the call stays valid under stream capture).
-hipError_t launch_zero_status(int32_t* status, hipStream_t s);
+// (With counter, that word too.)
+hipError_t launch_zero_status(int32_t* status, hipStream_t s, int32_t* counter = nullptr);
 // Ids equal to -1 are left out silently (rows excluded by the caller);
 // other ids outside [0, E) are left out and set *status = 1.  n above 1024
 // takes three kernels (rank, scan, scatter).
 hipError_t launch_dispatch(const int32_t* ids, int64_t n, int64_t E,
                            int tile_rows, const DispatchBuffers& b,
                            bool reset_status, hipStream_t s, int32_t* counter = nullptr);
-// With counter (an int that is 0 when the launch starts), more than 1024 ids
-// rank and scan in one launch (the last workgroup to finish scans).
+// With counter (an int that is 0 when the launch starts, or cleared here with
+// reset_status), more than 1024 ids rank and scan in one launch (the last
+// workgroup to finish scans).
 #ifndef MLXR_DISPATCH_FUSED
 #define MLXR_DISPATCH_FUSED 1
 #endif
@@ -189,11 +191,12 @@ hipError_t launch_route(const float* logits, int64_t ld, int64_t T, int64_t E,
                         int64_t K, bool bf16, int32_t* idx, float* wts,
                         int tile_rows, const DispatchBuffers& b,
                         hipStream_t s, int32_t* counter = nullptr);
-// gather_qmm helper: per flat row r = b*M + m the expert id and x row.
+// gather_qmm helper (clears *status, and *counter with one): per flat row r = b*M + m the expert id and x row.
 hipError_t launch_gather_prep(const uint32_t* lhs, const uint32_t* rhs,
                               int64_t B, int64_t M, int64_t x_batch, int64_t E,
                               int64_t N, int32_t* ids, int32_t* xrow,
-                              uint16_t* out, int32_t* status, hipStream_t s);
+                              uint16_t* out, int32_t* status, hipStream_t s,
+                              int32_t* counter = nullptr);
 // Identity dispatch for a dense (always-on) expert: one expert, n rows.
 hipError_t launch_dispatch_identity(int64_t n, int tile_rows,
                                     const DispatchBuffers& b, hipStream_t s);

@@ -3,7 +3,7 @@
 //
 //   out[p, n] = sum_k x[row(p), k] * w[e, n, k]
 //
-// over work items (at most 8 or 16 rows of one expert), f32 sums of exact bf16
+// over work items (at most 8 rows of one expert), f32 sums of exact bf16
 // products.  HBM-bound: 4.25 bits a weight, each read once per item.
 //
 // A workgroup is four waves: one item x (64 / KS) nb channels.  A wave owns nb
@@ -35,10 +35,10 @@ namespace {
 // timing builds: steps in flight (gated, not), waves to slice for, blocks per wave
 // and workgroups to keep
 #ifndef MLXR_MX_DG
-#define MLXR_MX_DG 4
+#define MLXR_MX_DG 2
 #endif
 #ifndef MLXR_MX_D
-#define MLXR_MX_D 6
+#define MLXR_MX_D 3
 #endif
 #ifndef MLXR_MX_KS_WAVES
 #define MLXR_MX_KS_WAVES 2048
@@ -60,10 +60,9 @@ struct MxShape {
 };
 
 // An item: rows [0, nt) of expert e; flat rows in fl, or slots from row0 on.
-template <int TT>
 struct Item {
   int e, nt, row0;
-  int fl[TT];
+  int fl[kWorkRows];
 };
 
 // The item of this workgroup from the ids, each wave for itself: equal ids form
@@ -71,9 +70,9 @@ struct Item {
 // those.  False without one.  Ids outside [0, E) are no one's: workgroup 0 sets the
 // status word, and with zero_bad every first item's workgroup clears their rows of
 // its channels [ch0, ch0 + chs).
-template <int TT>
 __device__ __forceinline__ bool find_item(const MxIds& d, int ai, bool status, int ch0, int chs,
-                                          uint16_t* out, int64_t out_ld, Item<TT>& it) {
+                                          uint16_t* out, int64_t out_ld, Item& it) {
+  constexpr int TT = kWorkRows;
   const int lane = threadIdx.x & 63;
   const bool row = lane < d.n;
   const int batch = lane / d.M;
@@ -118,23 +117,23 @@ __device__ __forceinline__ bool find_item(const MxIds& d, int ai, bool status, i
   return true;
 }
 
-template <bool GATED, int TT, int KS, int D, bool IDS>
-__global__ __launch_bounds__(64 * kWaves, TT == 8 ? 4 : 2) void mx_stream_kernel(
+template <bool GATED, int KS, int D, bool IDS>
+__global__ __launch_bounds__(64 * kWaves, 4) void mx_stream_kernel(
     QGemmArgs a, QGemmArgs a2, MxShape sh, MxIds ids) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  constexpr int NM = GATED ? 2 : 1;
+  constexpr int NM = GATED ? 2 : 1, TT = kWorkRows;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int cw = wave / KS, kq = wave % KS;
   const int n = lane & 15, q = lane >> 4;
-  Item<TT> it;
+  Item it;
   int tile;
   bool second = false;
   if constexpr (IDS) {
     const int ai = blockIdx.x / sh.tiles_n;
     tile = blockIdx.x - ai * sh.tiles_n;
     const int chs = kWaves / KS * sh.nb * 16;
-    if (!find_item<TT>(ids, ai, blockIdx.x == 0, tile * chs, chs, a.out, a.out_ld, it)) return;
+    if (!find_item(ids, ai, blockIdx.x == 0, tile * chs, chs, a.out, a.out_ld, it)) return;
   } else {
     Unit u;
     if (!decode_unit<TT>(a, sh.tiles_n, sh.units1, sh.items1, sh.rows2, u)) return;
@@ -143,7 +142,7 @@ __global__ __launch_bounds__(64 * kWaves, TT == 8 ? 4 : 2) void mx_stream_kernel
     it.e = u.wk.x, it.row0 = u.wk.y, it.nt = min(u.wk.z, TT);
     const int fl[8] = {u.fr0.x, u.fr0.y, u.fr0.z, u.fr0.w, u.fr1.x, u.fr1.y, u.fr1.z, u.fr1.w};
 #pragma unroll
-    for (int t = 0; t < TT; ++t) it.fl[t] = TT == 8 ? (t < it.nt ? fl[t & 7] : fl[0]) : 0;
+    for (int t = 0; t < TT; ++t) it.fl[t] = t < it.nt ? fl[t] : fl[0];
   }
   const RegArgs r = pick_reg(second, a2, 0, a, 0);
   const int K = a.K, G = K / kMxGroup, S = (G + 3) / 4;
@@ -186,7 +185,7 @@ __global__ __launch_bounds__(64 * kWaves, TT == 8 ? 4 : 2) void mx_stream_kernel
     } else if (r.x_by_slot) {
       xr[t] = it.row0 + min(t, nt - 1);
     } else {
-      const int f = TT == 8 ? it.fl[t] : r.sorted[it.row0 + min(t, nt - 1)];
+      const int f = it.fl[t];
       xr[t] = r.row_map ? r.row_map[f] : f / r.row_div;
     }
   }
@@ -250,13 +249,11 @@ __global__ __launch_bounds__(64 * kWaves, TT == 8 ? 4 : 2) void mx_stream_kernel
       if (t < nt) {
         const int ch = ch0 + 16 * b + n;
         int64_t orow = it.row0 + t;
-        if (IDS) {
+        if (IDS || (!GATED && r.out_by_flat)) {
           int f = it.fl[0];
 #pragma unroll
           for (int k = 1; k < TT; ++k) f = t == k ? it.fl[k] : f;
           orow = f;
-        } else if (!GATED && r.out_by_flat) {
-          orow = r.sorted[it.row0 + t];
         }
         r.out[orow * r.out_ld + ch] =
             GATED ? mx_bf16(mx_act(r.act, acc[0][i], acc[NM - 1][i])) : mx_bf16(acc[0][i]);
@@ -329,7 +326,8 @@ hipError_t launch_mx_stream(const QGemmArgs& a, int64_t max_items, const QGemmAr
                             int64_t shared_rows, const char* profile, hipStream_t s,
                             const MxIds* ids) {
   const QGemmArgs& b = shared ? *shared : a;
-  const int64_t items2 = shared ? (shared_rows + a.work_rows - 1) / a.work_rows : 0;
+  if (a.work_rows != kWorkRows) return hipErrorInvalidValue;
+  const int64_t items2 = shared ? (shared_rows + kWorkRows - 1) / kWorkRows : 0;
   const int64_t items = max_items + items2;
   const int G = a.K / kMxGroup, S = (G + 3) / 4;
   // slices: until there are 2048 waves (two per SIMD), two steps each at least
@@ -343,7 +341,7 @@ hipError_t launch_mx_stream(const QGemmArgs& a, int64_t max_items, const QGemmAr
   const int tiles_n = a.N / (16 * (kWaves / ks) * nb);
   const int nm = a.gated ? 2 : 1;
   const int sc_bytes = (nb * 16 * G + 1023) / 1024 * 1024;
-  const size_t x_lds = ((size_t)a.work_rows * (128 * S + 8) * 2 + 15) & ~size_t(15);
+  const size_t x_lds = ((size_t)kWorkRows * (128 * S + 8) * 2 + 15) & ~size_t(15);
   const size_t lds = x_lds + (size_t)kWaves * nm * sc_bytes +
                      (ks > 1 ? (size_t)kWaves * nm * 64 * sizeof(f32x4_t) : 0);
   const MxShape sh{tiles_n, nb, (int)(max_items * tiles_n), (int)max_items, (int)shared_rows,
@@ -351,31 +349,29 @@ hipError_t launch_mx_stream(const QGemmArgs& a, int64_t max_items, const QGemmAr
   const dim3 grid((unsigned)(items * tiles_n));
   const MxIds none{};
   ProfileScope prof(profile, s);
-#define MLXR_MX(G_, TT_, KS_, IDS_)                                                       \
-  mx_stream_kernel<G_, TT_, KS_, (G_) ? MLXR_MX_DG : MLXR_MX_D, IDS_>                     \
+#define MLXR_MX(G_, KS_, IDS_)                                                            \
+  mx_stream_kernel<G_, KS_, (G_) ? MLXR_MX_DG : MLXR_MX_D, IDS_>                          \
       <<<grid, 64 * kWaves, lds, s>>>(a, b, sh, IDS_ ? *ids : none)
-#define MLXR_MX_K(G_, TT_, IDS_)   \
-  do {                             \
-    if (ks == 4)                   \
-      MLXR_MX(G_, TT_, 4, IDS_);   \
-    else if (ks == 2)              \
-      MLXR_MX(G_, TT_, 2, IDS_);   \
-    else                           \
-      MLXR_MX(G_, TT_, 1, IDS_);   \
+#define MLXR_MX_K(G_, IDS_)   \
+  do {                        \
+    if (ks == 4)              \
+      MLXR_MX(G_, 4, IDS_);   \
+    else if (ks == 2)         \
+      MLXR_MX(G_, 2, IDS_);   \
+    else                      \
+      MLXR_MX(G_, 1, IDS_);   \
   } while (0)
-#define MLXR_MX_G(TT_, IDS_)       \
-  do {                             \
-    if (a.gated)                   \
-      MLXR_MX_K(true, TT_, IDS_);  \
-    else                           \
-      MLXR_MX_K(false, TT_, IDS_); \
+#define MLXR_MX_G(IDS_)       \
+  do {                        \
+    if (a.gated)              \
+      MLXR_MX_K(true, IDS_);  \
+    else                      \
+      MLXR_MX_K(false, IDS_); \
   } while (0)
   if (ids)
-    MLXR_MX_G(8, true);
-  else if (a.work_rows == kWorkRowsWide)
-    MLXR_MX_G(16, false);
+    MLXR_MX_G(true);
   else
-    MLXR_MX_G(8, false);
+    MLXR_MX_G(false);
 #undef MLXR_MX_G
 #undef MLXR_MX_K
 #undef MLXR_MX

@@ -98,6 +98,8 @@ bool use_prefill_path(int64_t rows, int64_t experts, int bits) {
   // rows makes four gate/up tiles).
   if (bits == 16)
     return rows >= (int64_t)MLXR_DENSE_TILED_ROWS * experts && rows >= 512;
+  if (bits == kBitsMxfp4)
+    return rows >= (int64_t)MLXR_MX_TILED_ROWS * experts && rows >= 512;
   // the M-tiled kernel pays once the experts average MLXR_QUANT_TILED_ROWS
   // rows and there are rows enough for its tiles to spread over the GPU
   return rows >= (int64_t)MLXR_QUANT_TILED_ROWS * experts && rows >= 512;
@@ -320,7 +322,8 @@ Status SwitchFfn::forward(const uint16_t* x, int64_t T, const int32_t* indices,
   db.work_rows = work_rows(n, nullptr);
   // (the dispatch clears *status first: no launch of its own for that)
   Status st = from_hip(
-      launch_dispatch(indices, n, E, prefill_tile_rows(n, E, sw_.bits), db, true, s),
+      launch_dispatch(indices, n, E, prefill_tile_rows(n, E, sw_.bits), db, true, s,
+                      sw_.bits == kBitsMxfp4 ? status + 1 : nullptr),
       "switch_mlp dispatch");
   if (!st.ok) return st;
   return experts(x, T, K, db, y, ws, s, nullptr, dc, combined);

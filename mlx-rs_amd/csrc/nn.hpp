@@ -86,6 +86,15 @@ namespace nn {
 #ifndef MLXR_DENSE_TILED_ROWS
 #define MLXR_DENSE_TILED_ROWS 2
 #endif
+// mxfp4 ones switch at MLXR_MX_TILED_ROWS: the tile kernel streams an expert's
+// weights by whole lines, the streaming one holds more loads in flight where
+// experts have next to no rows.  Gate/up and down, streaming then tiles: c6 T=64 (2
+// rows) 41 + 28 us and 45 + 29, c4 T=100 (2) 92 + 46 and 71 + 46, c2 T=64 (4) 42 +
+// 25 and 43 + 26, c2 T=100 (6) 57 + 26 and 46 + 27, c4 T=420 (8) 152 + 80 and 111
+// + 70; projections of c5 T=64 (4) 110 and 87.
+#ifndef MLXR_MX_TILED_ROWS
+#define MLXR_MX_TILED_ROWS 2
+#endif
 bool use_prefill_path(int64_t rows, int64_t experts, int bits = 4);
 
 // A shared expert folded into the routed decode GEMM launches (its gate/up

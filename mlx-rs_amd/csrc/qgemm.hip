@@ -533,12 +533,7 @@ int work_rows_for(int64_t n, int64_t E, std::initializer_list<const QGemmArgs*> 
   if (!wide_items_possible(n, E)) return kWorkRows;
   const int64_t items = dispatch_max_work(n, E, kWorkRowsWide);
   for (const QGemmArgs* g : gemms) {
-    if (g->bits == kBitsMxfp4) {
-      // (16 rows of x in LDS leave room for two workgroups a CU up to here)
-      if (g->K > 2048) return kWorkRows;
-      continue;
-    }
-    if (g->bits == 16 || !(g->K <= kWideWhole || g->K % kWideSlice == 0) ||
+    if (g->bits == 16 || g->bits == kBitsMxfp4 || !(g->K <= kWideWhole || g->K % kWideSlice == 0) ||
         items * (g->N / 16) < kStreamMinBlocks)
       return kWorkRows;
     if (stream_eligible(*g, *g, items) &&

@@ -207,6 +207,7 @@ class SplitSwitchFfn:
         self.gate_proj, self.up_proj, self.down_proj = gate_proj, up_proj, down_proj
         self._desc = C.SwitchGlu(gate_proj.descriptor(), up_proj.descriptor(),
                                  down_proj.descriptor())
+        self._sizes = {}  # workspace bytes by (T, K)
 
     @classmethod
     def from_dense(cls, gate_w, up_w, down_w, group_size=None, bits=4, mode="affine"):
@@ -219,13 +220,20 @@ class SplitSwitchFfn:
     def descriptor(self) -> C.SwitchGlu:
         return self._desc
 
+    def workspace_size(self, T: int, K: int) -> int:
+        n = self._sizes.get((T, K))
+        if n is None:
+            n = self._sizes[T, K] = C.lib().mlxr_moe_switch_glu_workspace_size(
+                ctypes.byref(self._desc), T, K)
+        return n
+
     def _prep(self, x, indices):
         d = self.gate_proj.input_dims
         _check_x("SplitSwitchFfn", x, d)
         ops._dev(x, indices)
         x2 = x.reshape(-1, d).contiguous()
         K = indices.shape[-1]
-        idx = indices.reshape(-1, K).to(torch.int32).contiguous()
+        idx = ops._as_u32(indices).reshape(-1, K)
         if idx.shape[0] != x2.shape[0]:
             raise MlxrMoeError("SplitSwitchFfn: indices must be [..., T, K] over x [..., T, d]")
         return x2, idx, K
@@ -235,12 +243,11 @@ class SplitSwitchFfn:
         x2, idx, K = self._prep(x, indices)
         T, d = x2.shape
         y = torch.empty((T, K, d), dtype=torch.bfloat16, device=x.device)
-        lib = C.lib()
-        ws = ops.workspace(lib.mlxr_moe_switch_glu_workspace_size(ctypes.byref(self._desc), T, K),
-                           x.device)
-        C.check(lib.mlxr_moe_switch_glu_experts(
-            ctypes.byref(self._desc), _ptr(x2), T, _ptr(idx), K, _ptr(y), _ptr(ws), ws.numel(),
-            ops._stream(x)))
+        ws = ops.workspace(self.workspace_size(T, K), x.device)
+        with ops._on(x):
+            C.check(C.lib().mlxr_moe_switch_glu_experts(
+                ctypes.byref(self._desc), _ptr(x2), T, _ptr(idx), K, _ptr(y), _ptr(ws),
+                ws.numel(), ops._stream(x)))
         self.last_workspace = ws
         return y.reshape(tuple(indices.shape) + (d,))
 
@@ -251,12 +258,11 @@ class SplitSwitchFfn:
         ops._dev(x, weights)
         w = weights.reshape(-1, K).to(torch.float32).contiguous()
         out = torch.empty((T, d), dtype=torch.float32, device=x.device)
-        lib = C.lib()
-        ws = ops.workspace(lib.mlxr_moe_switch_glu_workspace_size(ctypes.byref(self._desc), T, K),
-                           x.device)
-        C.check(lib.mlxr_moe_switch_glu_forward(
-            ctypes.byref(self._desc), _ptr(x2), T, _ptr(idx), _ptr(w), K, _ptr(out), _ptr(ws),
-            ws.numel(), ops._stream(x)))
+        ws = ops.workspace(self.workspace_size(T, K), x.device)
+        with ops._on(x):
+            C.check(C.lib().mlxr_moe_switch_glu_forward(
+                ctypes.byref(self._desc), _ptr(x2), T, _ptr(idx), _ptr(w), K, _ptr(out),
+                _ptr(ws), ws.numel(), ops._stream(x)))
         self.last_workspace = ws
         return out.reshape(tuple(x.shape[:-1]) + (d,))
 

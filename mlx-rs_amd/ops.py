@@ -14,6 +14,7 @@ runs a kernel of libmlxr_moe.so; there is no fallback.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
@@ -36,27 +37,33 @@ def _check_mode(mode: str) -> bool:
 
 
 def _p(t):
-    return None if t is None else ctypes.c_void_p(t.data_ptr())
+    return None if t is None else t.data_ptr()
 
 
 def _stream(t: torch.Tensor):
-    return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+    """The current stream of t's device, as a handle (a Stream object around it
+    costs more than the launch)."""
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
-class _on:
-    """The tensor's device as the current one (kernels are launched there)."""
-
-    def __init__(self, t: torch.Tensor):
-        self.want = t.device.index
+class _Here:
+    """The device is the current one already."""
 
     def __enter__(self):
-        self.was = torch.cuda.current_device()
-        if self.was != self.want:
-            torch.cuda.set_device(self.want)
+        pass
 
     def __exit__(self, *exc):
-        if self.was != self.want:
-            torch.cuda.set_device(self.was)
+        pass
+
+
+_HERE = _Here()
+
+
+def _on(t: torch.Tensor):
+    """t's device as the current one (kernels are launched there)."""
+    if torch._C._cuda_getDevice() == t.device.index:
+        return _HERE
+    return torch.cuda.device(t.device)
 
 
 def _code(t: torch.Tensor) -> int:
@@ -85,8 +92,16 @@ def workspace(nbytes: int, device) -> torch.Tensor:
     return torch.empty(max(int(nbytes), 1), dtype=torch.uint8, device=device)
 
 
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(name: str, *sizes) -> int:
+    """The library's workspace size for these sizes (a function of them alone)."""
+    return getattr(C.lib(), f"mlxr_moe_{name}_workspace_size")(*sizes)
+
+
 def _as_u32(idx: torch.Tensor) -> torch.Tensor:
     # mlx indices are uint32; int32 storage carries the same bits.
+    if idx.dtype == torch.int32 and idx.is_contiguous():
+        return idx
     if idx.dtype not in (torch.int32, torch.int64, torch.uint32):
         raise MlxrMoeError(f"indices must be integer, got {idx.dtype}")
     return idx.to(torch.int32).contiguous()
@@ -248,8 +263,7 @@ def gather_qmm(x, w, scales, biases=None, lhs_indices=None, rhs_indices=None,
         raise MlxrMoeError("gather_qmm: lhs and rhs indices must have the same size")
     out = torch.empty(tuple(rhs.shape) + (M, N), dtype=torch.bfloat16, device=x.device)
     lib = C.lib()
-    nbytes = lib.mlxr_moe_gather_qmm_workspace_size(B, M, E)
-    ws = workspace(nbytes, x.device)
+    ws = workspace(_workspace_bytes("gather_qmm", B, M, E), x.device)
     with _on(x):
         C.check(lib.mlxr_moe_gather_qmm(
             _p(x), _code(x), x_batch, M, K, _p(w.contiguous()), _p(scales.contiguous()),
@@ -401,7 +415,7 @@ def _balance_inputs(name, logits, indices, mask):
     if indices.ndim != logits.ndim or indices.shape[:-1] != logits.shape[:-1]:
         raise MlxrMoeError(f"{name}: indices {tuple(indices.shape)} must be [.., T, K] over "
                            f"logits {tuple(logits.shape)}")
-    z = logits.reshape(-1, E)
+    z = logits if logits.ndim == 2 else logits.reshape(-1, E)
     if z.stride(1) != 1 or z.stride(0) < E:
         z = z.contiguous()
     if mask is not None:
@@ -411,7 +425,8 @@ def _balance_inputs(name, logits, indices, mask):
             raise MlxrMoeError(f"{name}: mask {tuple(mask.shape)} must be one value per token "
                                f"of logits {tuple(logits.shape)}")
         mask = mask.reshape(-1).contiguous()
-    return z, max(z.stride(0), E), _as_u32(indices).reshape(-1, indices.shape[-1]), mask
+    idx = _as_u32(indices)
+    return z, max(z.stride(0), E), idx if idx.ndim == 2 else idx.flatten(0, -2), mask
 
 
 def router_balance(logits: torch.Tensor, indices: torch.Tensor, mask=None):
@@ -429,7 +444,7 @@ def router_balance(logits: torch.Tensor, indices: torch.Tensor, mask=None):
     counts = torch.empty(E, dtype=torch.int32, device=dev)
     tokens = torch.empty((), dtype=torch.int32, device=dev)
     lib = C.lib()
-    ws = workspace(lib.mlxr_moe_router_balance_workspace_size(T, E), dev)
+    ws = workspace(_workspace_bytes("router_balance", T, E), dev)
     with _on(z):
         C.check(lib.mlxr_moe_router_balance(
             _p(z), _code(z), ld, T, E, _p(idx), K, _p(mask), _p(loss), _p(counts), _p(probs),
