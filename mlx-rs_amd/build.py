@@ -26,6 +26,7 @@ ARCH = "gfx950"
 SOURCES = [
     "quant.hip",
     "mx_quant.hip",
+    "mx_sort.hip",
     "mx_stream.hip",
     "mx_tile.hip",
     "router.hip",

@@ -166,11 +166,15 @@ int run_gather(const char* op, const void* x, int64_t x_batch, int64_t M,
   DispatchBuffers db = carve_dispatch(c, R, E, status);
   uint16_t* ob = static_cast<uint16_t*>(out);
   // mxfp4, few rows: one launch, which groups the indices itself
-  const bool direct =
-      bits == kBitsMxfp4 && R <= kMxIdsRows && !nn::use_prefill_path(R, E, bits);
+  const bool mx = bits == kBitsMxfp4, tiled = nn::use_prefill_path(R, E, bits);
+  const bool direct = mx && R <= kMxIdsRows && !tiled;
+  // ... rows for the tiles: one launch that sorts them
+  // (they take x under 2 GB and a 16-byte aligned out)
+  const bool sorted = mx && tiled && R <= kMxSortRows && aligned(ob, 16) &&
+                      x_batch * M * K * 2 < ((int64_t)1 << 31);
   // (the status word's slot has room for the dispatch's counter beside it)
-  int32_t* counter = bits == kBitsMxfp4 ? status + 1 : nullptr;
-  if (!direct)
+  int32_t* counter = mx ? status + 1 : nullptr;
+  if (!direct && !sorted)
     st = from_hip(launch_gather_prep(lhs_indices, rhs_indices, B, M, x_batch, E,
                                      N, ids, xrow, ob, status, s, counter),
                   (o + " prep").c_str());
@@ -201,7 +205,7 @@ int run_gather(const char* op, const void* x, int64_t x_batch, int64_t M,
   a.out_ld = N;
   a.out_by_flat = true;
   a.gated = false;
-  if (direct) {
+  if (direct || sorted) {
     a.work_rows = kWorkRows;
     MxIds d{};
     d.ids = reinterpret_cast<const int32_t*>(rhs_indices);
@@ -213,8 +217,20 @@ int run_gather(const char* op, const void* x, int64_t x_batch, int64_t M,
     d.E = (int32_t)E;
     d.x_batch = (int32_t)std::min<int64_t>(x_batch, INT32_MAX);
     d.zero_bad = true;
-    return finish(from_hip(
-        launch_mx_stream(a, dispatch_max_work(R, E), nullptr, 0, "qgemm_down", s, &d), op));
+    if (direct)
+      return finish(from_hip(
+          launch_mx_stream(a, dispatch_max_work(R, E), nullptr, 0, "qgemm_down", s, &d), op));
+    a.work = nullptr;  // (no records)
+    const bool map = lhs_indices || M > 1;  // else flat row / d.div
+    if (!map) {
+      a.row_map = nullptr;
+      a.row_div = d.div;
+    }
+    st = from_hip(launch_mx_sort(d, prefill_tile_rows(R, E, bits), N, db, map ? xrow : nullptr,
+                                 ob, s),
+                  (o + " dispatch").c_str());
+    if (!st.ok) return finish(st);
+    return finish(from_hip(launch_qgemm(a, R, dispatch_max_work(R, E), true, s), op));
   }
   db.work_rows = work_rows_for(R, E, {&a});
   a.work_rows = (uint8_t)db.work_rows;

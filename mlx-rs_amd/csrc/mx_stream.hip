@@ -326,7 +326,7 @@ hipError_t launch_mx_stream(const QGemmArgs& a, int64_t max_items, const QGemmAr
                             int64_t shared_rows, const char* profile, hipStream_t s,
                             const MxIds* ids) {
   const QGemmArgs& b = shared ? *shared : a;
-  if (a.work_rows != kWorkRows) return hipErrorInvalidValue;
+  if (a.work_rows != kWorkRows || (!ids && !a.work)) return hipErrorInvalidValue;
   const int64_t items2 = shared ? (shared_rows + kWorkRows - 1) / kWorkRows : 0;
   const int64_t items = max_items + items2;
   const int G = a.K / kMxGroup, S = (G + 3) / 4;

@@ -319,6 +319,23 @@ Status SwitchFfn::forward(const uint16_t* x, int64_t T, const int32_t* indices,
   DispatchBuffers db = carve_dispatch(ws, n, E, status);
   if (sw_.bits == kBitsMxfp4 && n <= kMxIdsRows && !use_prefill_path(n, E, sw_.bits))
     return experts_direct(x, T, K, indices, y, ws, status, s);
+  if (sw_.bits == kBitsMxfp4 && n <= kMxSortRows && use_prefill_path(n, E, sw_.bits) &&
+      (reinterpret_cast<uintptr_t>(y) & 15) == 0) {
+    db.work_rows = kWorkRows;
+    db.work = nullptr;  // (no records: both products run as tiles)
+    MxIds ids{};
+    ids.ids = indices;
+    ids.status = status;
+    ids.n = (int32_t)n;
+    ids.M = 1;
+    ids.E = (int32_t)E;
+    ids.skip_minus1 = true;
+    const Status so = from_hip(launch_mx_sort(ids, prefill_tile_rows(n, E, sw_.bits), 0, db,
+                                              nullptr, nullptr, s),
+                               "switch_mlp dispatch");
+    if (!so.ok) return so;
+    return experts(x, T, K, db, y, ws, s, nullptr, dc, combined);
+  }
   db.work_rows = work_rows(n, nullptr);
   // (the dispatch clears *status first: no launch of its own for that)
   Status st = from_hip(

@@ -231,9 +231,11 @@ class SplitSwitchFfn:
         d = self.gate_proj.input_dims
         _check_x("SplitSwitchFfn", x, d)
         ops._dev(x, indices)
-        x2 = x.reshape(-1, d).contiguous()
+        x2 = (x if x.ndim == 2 else x.reshape(-1, d)).contiguous()
         K = indices.shape[-1]
-        idx = ops._as_u32(indices).reshape(-1, K)
+        idx = ops._as_u32(indices)
+        if idx.ndim != 2:
+            idx = idx.reshape(-1, K)
         if idx.shape[0] != x2.shape[0]:
             raise MlxrMoeError("SplitSwitchFfn: indices must be [..., T, K] over x [..., T, d]")
         return x2, idx, K
@@ -249,7 +251,7 @@ class SplitSwitchFfn:
                 ctypes.byref(self._desc), _ptr(x2), T, _ptr(idx), K, _ptr(y), _ptr(ws),
                 ws.numel(), ops._stream(x)))
         self.last_workspace = ws
-        return y.reshape(tuple(indices.shape) + (d,))
+        return y if indices.ndim == 2 else y.reshape(tuple(indices.shape) + (d,))
 
     def forward_with_combine(self, x, indices, weights):
         """sum_k weights * expert_k(x) -> f32 [..., d] (switch.rs:446-474)."""

@@ -79,11 +79,13 @@ def _dev(*ts):
     for t in ts:
         if t is None:
             continue
-        if t.device.type != "cuda":
+        if not t.is_cuda:
             raise MlxrMoeError("arrays must live on a ROCm device")
-        if dev is not None and t.device != dev:
+        d = t.device
+        if dev is None:
+            dev = d
+        elif d != dev:
             raise MlxrMoeError("arrays live on different devices")
-        dev = t.device
     return dev
 
 
@@ -114,6 +116,9 @@ def _check_x_batch(name: str, x_batch_shape, idx_shape):
     indices [.., T, top_k], or one x batch for all).  Other broadcasts (a
     leading singleton against a larger index axis) would pick wrong rows:
     they are rejected."""
+    if (len(x_batch_shape) == len(idx_shape) and x_batch_shape[-1:] == (1,)
+            and x_batch_shape[:-1] == idx_shape[:-1]):
+        return  # x [.., T, 1, 1, K] against indices [.., T, top_k]
     xs = list(x_batch_shape)
     while len(xs) > len(idx_shape) and xs[0] == 1:
         xs.pop(0)
