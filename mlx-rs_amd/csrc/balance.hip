@@ -205,7 +205,8 @@ __global__ __launch_bounds__(kJoinCols* kJoinRows) void balance_join_kernel(
     }
   }
   int n = 0, bad = 0;
-  for (int g = tid; g < G; g += kJoinCols * kJoinRows) n += tallies[2 * g], bad |= tallies[2 * g + 1];
+  for (int g = tid; g < G; g += kJoinCols * kJoinRows)
+    n += tallies[2 * g], bad |= tallies[2 * g + 1];
   if (n) atomicAdd(&n_l[0], n);
   if (bad) n_l[1] = 1;
   s_l[row][col] = s;

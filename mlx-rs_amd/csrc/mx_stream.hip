@@ -102,8 +102,9 @@ __device__ __forceinline__ bool find_item(const MxIds& d, int ai, bool status, i
   // the lane that starts item ai
   const uint64_t mine = __ballot(((starts >> lane) & 1) && __popcll(starts & below) == ai);
   const int s = __ffsll((unsigned long long)mine) - 1;
-  const uint64_t rows = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(peers >> 32), s) << 32) |
-                        (uint32_t)__builtin_amdgcn_readlane((int)peers, s);
+  const uint32_t rows_hi = (uint32_t)__builtin_amdgcn_readlane((int)(peers >> 32), s);
+  const uint32_t rows_lo = (uint32_t)__builtin_amdgcn_readlane((int)peers, s);
+  const uint64_t rows = (uint64_t)rows_hi << 32 | rows_lo;
   const int base = __builtin_amdgcn_readlane(rank, s);
   it.e = __builtin_amdgcn_readlane(id, s);
   it.nt = min(__popcll(rows) - base, TT);

@@ -6,17 +6,20 @@
 // owns 32 gate and the same 32 up channels, or 64 down channels, for all rows of
 // the tile.
 //
-// Weights: 128-byte lines (8 groups) of the wave's 64 rows come straight to its own
-// 8 KB of LDS, consecutive lanes on consecutive 16 bytes (loads of 32 bytes from
-// each of 32 rows cost the address path four times the cycles: gate/up of c4
-// T=2048 212 us so, 153 with whole lines), and are then read to registers: lane
-// (c, h) = (l % 32, l / 32) takes group 2 j + h of channel c in stage j, the
-// operands of four v_mfma_f32_32x32x16_bf16 whose K halves are 8 inputs of group
-// 2 j and 8 of group 2 j + 1.  One conversion instruction gives two weights, scale
-// included: as many as there are MFMAs at 128 rows.  x is staged 64 inputs (two
-// groups) at a time, three stages, straight to LDS too.
-// c2 T=4096: gate/up 203 us, 1.0 PFLOP/s; of it about 155 are the MFMAs (all loads
-// taken out).
+// Weights: pieces of 8 groups (128 bytes; 4 groups under 64-row tiles) of the wave's
+// 64 rows come straight to its own LDS, consecutive lanes on consecutive 16 bytes
+// (loads of 32 bytes from each of 32 rows cost the address path four times the
+// cycles: gate/up of c4 T=2048 212 us so, 153 with whole lines), and are then read
+// to registers: lane (c, h) = (l % 32, l / 32) takes group 2 j + h of channel c in
+// stage j, the operands of four v_mfma_f32_32x32x16_bf16 whose K halves are 8 inputs
+// of group 2 j and 8 of group 2 j + 1.  One conversion instruction gives two
+// weights, scale included: as many as there are MFMAs at 128 rows.  x is staged 64
+// inputs (two groups) at a time, three stages, straight to LDS too.
+// c2 T=4096: gate/up 195 us, 1.06 PFLOP/s, down 118; without any load (a copy of the
+// kernel, timed) 155 and 97, where the power limit holds the matrix cores: a library
+// product of 8192^3 reaches 1.46 PFLOP/s.  Without the weights' loads 172, without
+// x's 192.  c4 T=2048 (40 rows an expert): gate/up 153 us for 570 MB of weights, 3.7
+// TB/s; matrix cores 40% busy, address units 50%.
 #include <algorithm>
 
 #include "mx.hpp"
@@ -27,11 +30,17 @@ namespace {
 
 constexpr int kWaves = 4, kNT = 64 * kWaves;
 typedef __attribute__((address_space(3))) void* lds_ptr;
-constexpr int kXStages = 3;      // x stages of 64 inputs in LDS
-constexpr int kWLine = 32 * 128; // a wave's line of one side: 128 bytes of 32 rows
+constexpr int kXStages = 3;  // x stages of 64 inputs in LDS
+// Groups of a weight piece in LDS: a 128-byte line of every row, or half of one
+// under the shorter tiles, where three workgroups then fit a CU (down of c4 T=2048
+// 102 us with lines and two, 96 so; c6 down T=509 39.6 and 36.5; gate/up alike).
 template <int ROWS>
-constexpr int kTileLds = kXStages * ROWS * 128 + kWaves * 2 * kWLine;
-static_assert(2 * kTileLds<128> <= 160 * 1024, "two workgroups per CU");
+constexpr int kPiece = ROWS == 64 ? 4 : 8;
+template <int ROWS>
+constexpr int kTileLds = kXStages * ROWS * 128 + kWaves * 2 * 512 * kPiece<ROWS>;
+template <int ROWS>
+constexpr int kWgs = ROWS == 64 ? 3 : 2;  // workgroups per CU
+static_assert(2 * kTileLds<128> <= 160 * 1024 && 3 * kTileLds<64> <= 160 * 1024, "LDS");
 
 template <int N>
 __device__ __forceinline__ void wait_loads() {  // at most N loads not back
@@ -53,18 +62,21 @@ __device__ __forceinline__ void mx_unit(const RegArgs& a, int N, int K, int e, i
   constexpr int TC = GATED ? 32 * kWaves : 64 * kWaves;  // channels per N-tile
   constexpr int WC = TC / kWaves;                        // ... per wave
   constexpr int kXBytes = ROWS * 128;
+  constexpr int GL = kPiece<ROWS>, SPL = GL / 2;  // groups, x stages per piece
+  constexpr int RPL = 64 / GL;                    // rows per load
+  constexpr int kWLine = 512 * GL;                // bytes of a piece of one side
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 31, h = lane >> 5;
   const int G = K / kMxGroup, T = K >> 6;  // groups, x stages with inputs
-  const int L = (T + 3) / 4;               // lines (of four stages)
+  const int L = (T + SPL - 1) / SPL;       // pieces
   char* xl = smem;
   char* wl = smem + kXStages * kXBytes + wave * 2 * kWLine;
 
-  // ---- weights: lines straight to the wave's own LDS.  Instruction i of a side
-  // fills rows 8 i .. 8 i + 7, lane l the 16 bytes at position l % 8 of row l / 8;
-  // chunk (group) cc of row r sits at cc ^ (r & 7).  Rows past N and chunks past
-  // the row are out of range: zeros.
+  // ---- weights: pieces straight to the wave's own LDS.  Instruction i of a side
+  // fills rows RPL i .. RPL i + RPL - 1, lane l the 16 bytes at position l % GL of row
+  // l / GL; chunk (group) cc of row r sits at cc ^ wswz(r).  Rows past N and chunks
+  // past the row are out of range: zeros.
   const uint32_t row_bytes = (uint32_t)K / 2;
   const __amdgpu_buffer_rsrc_t wr0 = __builtin_amdgcn_make_buffer_rsrc(
       const_cast<uint32_t*>(a.w0.w) + (int64_t)e * a.e_rows * (row_bytes / 4), 0,
@@ -74,31 +86,33 @@ __device__ __forceinline__ void mx_unit(const RegArgs& a, int N, int K, int e, i
           (int64_t)e * a.e_rows * (row_bytes / 4),
       0, (int)(N * row_bytes), kBufFlags);
   const int och0 = nt * TC + wave * WC;  // the wave's first channel
-  const int wrow = lane >> 3, wch = (lane & 7) ^ wrow;
+  const auto wswz = [&](int r) { return GL == 8 ? r & 7 : (r >> 2) & 3; };
+  const int wrow = lane / GL;
   auto load_w = [&](int l) {
-    const bool ok = 8 * l + wch < G;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int ch = och0 + (GATED ? 0 : 32 * s) + 8 * i + wrow;
+      for (int i = 0; i < 32 / RPL; ++i) {
+        const int wch = (lane & (GL - 1)) ^ wswz(RPL * i + wrow);
+        const bool ok = GL * l + wch < G;
+        const int ch = och0 + (GATED ? 0 : 32 * s) + RPL * i + wrow;
         __builtin_amdgcn_raw_ptr_buffer_load_lds(
             s ? wr1 : wr0, (lds_ptr)(wl + s * kWLine + 1024 * i), 16,
-            ok && ch < N ? (uint32_t)ch * row_bytes + 16u * wch : kPastEnd, 128 * l, 0, 0);
+            ok && ch < N ? (uint32_t)ch * row_bytes + 16u * wch : kPastEnd, 16 * GL * l, 0, 0);
       }
     }
   };
-  constexpr int kWLoads = 8;
-  u32x4_t w[2][4];  // [side][stage of the line]: the group 2 stage + h of channel c
+  constexpr int kWLoads = GL;
+  u32x4_t w[2][SPL];  // [side][stage of the piece]: the group 2 stage + h of channel c
   auto take_w = [&]() {
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        w[s][j] = *reinterpret_cast<const u32x4_t*>(wl + s * kWLine + c * 128 +
-                                                    16 * ((2 * j + h) ^ (c & 7)));
+      for (int j = 0; j < SPL; ++j)
+        w[s][j] = *reinterpret_cast<const u32x4_t*>(wl + s * kWLine + c * 16 * GL +
+                                                    16 * ((2 * j + h) ^ wswz(c)));
   };
-  // ---- scales: 16 bytes of channel c (two lines) at a time, by aligned words; a
+  // ---- scales: 16 bytes of channel c (PPS pieces) at a time, by aligned words; a
   // row of an odd number of pairs starts in the middle of one
   const __amdgpu_buffer_rsrc_t sr0 = __builtin_amdgcn_make_buffer_rsrc(
       const_cast<uint16_t*>(a.w0.scales) + (int64_t)e * a.e_rows * (G / 2), 0, N * G, kBufFlags);
@@ -109,30 +123,32 @@ __device__ __forceinline__ void mx_unit(const RegArgs& a, int N, int K, int e, i
     u32x4_t v;
     uint32_t past;
   };
-  Scales sn[2];  // of the two lines after the current ones
-  auto load_sc = [&](int l) {  // lines l, l + 1 (l even)
+  Scales sn[2];  // of the pieces after the current ones
+  constexpr int PPS = 16 / GL;  // pieces per scale load
+  auto load_sc = [&](int l) {  // pieces l .. l + PPS - 1 (l a multiple)
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       const int ch = och0 + (GATED ? 0 : 32 * s) + c;
       const uint32_t off = (uint32_t)ch * (uint32_t)G & ~3u;
-      const bool ok = ch < N && 8 * l < G;
-      sn[s].v = __builtin_amdgcn_raw_buffer_load_b128(s ? sr1 : sr0, ok ? off : kPastEnd, 8 * l, 0);
+      const bool ok = ch < N && GL * l < G;
+      sn[s].v =
+          __builtin_amdgcn_raw_buffer_load_b128(s ? sr1 : sr0, ok ? off : kPastEnd, GL * l, 0);
       sn[s].past = __builtin_amdgcn_raw_buffer_load_b32(
-          s ? sr1 : sr0, ok && (G & 2) ? off + 16 : kPastEnd, 8 * l, 0);
+          s ? sr1 : sr0, ok && (G & 2) ? off + 16 : kPastEnd, GL * l, 0);
     }
   };
-  uint32_t sc4[2][4];  // the two lines' scale bytes, moved so that this lane's are 0 and 2
+  uint32_t sc4[2][4];  // the pieces' scale bytes, moved so that this lane's are 0 and 2
   auto take_sc = [&](int l) {
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       const int ch = och0 + (GATED ? 0 : 32 * s) + c;
-      // bytes (2 i + h) of the row from group 8 l on, in words of two such
+      // bytes (2 i + h) of the row from group GL l on, in words of two such
       const uint32_t sh = 8 * (((uint32_t)ch * (uint32_t)G) & 3u) + 8 * h;
       const uint32_t u[5] = {sn[s].v.x, sn[s].v.y, sn[s].v.z, sn[s].v.w, sn[s].past};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint32_t v = __builtin_amdgcn_alignbit(u[i + 1], u[i], sh);
-        const int left = G - 8 * l - 4 * i;  // zeros past the row
+        const int left = G - GL * l - 4 * i;  // zeros past the row
         sc4[s][i] = left >= 4 ? v : left > 0 ? v & 0xffffu : 0u;
       }
     }
@@ -204,71 +220,88 @@ __device__ __forceinline__ void mx_unit(const RegArgs& a, int N, int K, int e, i
       af[mb] = as_bf16x8(*reinterpret_cast<const u32x4_t*>(A + 4096 * mb));
   };
   bf16x8_t af[2][NMB], bf[2];
-  // side s of chunk i of stage j of the line of parity `odd`
-  auto weights = [&](int j, int i, int s, bool odd) {
-    const uint32_t v = odd ? sc4[s][2 + (j >> 1)] : sc4[s][j >> 1];
+  // side s of chunk i of stage j of the piece
+  uint32_t cur[2][GL / 4];  // of the current piece
+  auto pick_sc = [&](int l) {
+    const int p = l & (PPS - 1);
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int k = 0; k < GL / 4; ++k) {
+        cur[s][k] = sc4[s][k];
+#pragma unroll
+        for (int q = 1; q < PPS; ++q) cur[s][k] = p == q ? sc4[s][GL / 4 * q + k] : cur[s][k];
+      }
+  };
+  auto weights = [&](int j, int i, int s) {
+    const uint32_t v = cur[s][j >> 1];
     bf[s] = mx_weights(w[s][j][i], mx_scale((v >> (16 * (j & 1))) & 0xffu));
   };
   stage_barrier<0>();
   take_w();
   take_sc(0);
+  pick_sc(0);
   read_a(af[0], 0, 0);
-  weights(0, 0, 0, false);
-  weights(0, 0, 1, false);
+  weights(0, 0, 0);
+  weights(0, 0, 1);
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   __builtin_amdgcn_sched_barrier(0);
   load_w(1);
-  load_sc(2);
+  load_sc(PPS);
   __builtin_amdgcn_sched_barrier(0);
 
-  // ---- the lines, four x stages each, four chunks of 16 inputs a stage.  The
+  // ---- the pieces, SPL x stages each, four chunks of 16 inputs a stage.  The
   // operands of a chunk are read and converted during the one before it, so the
   // matrix instructions wait for neither; that is why a stage's barrier stands
   // before its last chunk, when its x has been read for good.  The x stage three
-  // ahead then takes its place, and after a line's last barrier the line after the
+  // ahead then takes its place, and after a piece's last barrier the piece after the
   // next one the place of the next, which is in registers by then.
   // Loads are back in the order of their issue: at stage j's barrier the next
   // stage's x (two barriers old) is, when no more are out than the x stage issued
-  // since, and, in a line's first two stages, the weight line issued between.
+  // since, and, in the first half of a piece's stages, the weight piece issued
+  // between; past the half the next piece is back too.
   int at = 0;
 #pragma nounroll
   for (int l = 0; l < L; ++l) {
-    const bool odd = l & 1;
+    const bool refill = (l & (PPS - 1)) == PPS - 1;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < SPL; ++j) {
       const int next = at + kXBytes < kXStages * kXBytes ? at + kXBytes : 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if (i == 3) {
-          if (j < 2)
+          if (j < SPL / 2)
             stage_barrier<NMB + kWLoads>();
           else
             stage_barrier<NMB>();
-          load_x(4 * l + j + kXStages, at);
+          load_x(SPL * l + j + kXStages, at);
           read_a(af[0], next, 0);
-          if (j == 3) take_w();
+          if (j == SPL - 1) take_w();
         } else {
           read_a(af[(i + 1) & 1], at, i + 1);
         }
         __builtin_amdgcn_sched_barrier(0);
-        if (i == 3 && j == 3 && odd) take_sc(l + 1);
+        if (i == 3 && j == SPL - 1) {
+          if (refill) take_sc(l + 1);
+          pick_sc(l + 1);
+        }
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
 #pragma unroll
           for (int mb = 0; mb < NMB; ++mb)
             acc[mb][s] = mfma32x32x16(af[i & 1][mb], bf[s], acc[mb][s]);
           if (i < 3)
-            weights(j, i + 1, s, odd);
-          else if (j < 3)
-            weights(j + 1, 0, s, odd);
+            weights(j, i + 1, s);
+          else if (j < SPL - 1)
+            weights(j + 1, 0, s);
           else
-            weights(0, 0, s, !odd);
+            weights(0, 0, s);
         }
         __builtin_amdgcn_sched_barrier(0);
-        if (i == 3 && j == 3) {
+        if (i == 3 && j == SPL - 1) {
           asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
           load_w(l + 2);
-          if (odd) load_sc(l + 3);
+          if (refill) load_sc(l + 1 + PPS);
           __builtin_amdgcn_sched_barrier(0);
         }
       }
@@ -309,7 +342,7 @@ __device__ __forceinline__ void mx_unit(const RegArgs& a, int N, int K, int e, i
 }
 
 template <bool GATED, int ROWS>
-__global__ __launch_bounds__(kNT, 2) void mx_tile_kernel(RegLaunch L) {
+__global__ __launch_bounds__(kNT, kWgs<ROWS>) void mx_tile_kernel(RegLaunch L) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   RegUnit<ROWS> u;
   if (!u.place(L, blockIdx.x)) return;

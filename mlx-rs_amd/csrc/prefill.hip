@@ -72,7 +72,8 @@ bool prefill_supported(const QGemmArgs& a, int64_t x_rows) {
   // buffer offsets are 32-bit: x, and one expert's weights, under 2 GB
   // outputs leave as 16-byte runs of a row
   const bool out16 = (reinterpret_cast<uintptr_t>(a.out) & 15) == 0 && a.out_ld % 8 == 0;
-  return (a.bits == 4 || a.bits == 8 || a.bits == 16 || a.bits == kBitsMxfp4) && a.K % 64 == 0 && a.N % 64 == 0 &&
+  const bool bits_ok = a.bits == 4 || a.bits == 8 || a.bits == 16 || a.bits == kBitsMxfp4;
+  return bits_ok && a.K % 64 == 0 && a.N % 64 == 0 &&
          a.sorted != nullptr && out16 && a.row_div >= 1 && a.row_div <= 65536 &&
          x_rows * a.x_ld * 2 < ((int64_t)1 << 31) &&
          (int64_t)a.N * a.K * weight_bits(a.bits) / 8 < ((int64_t)1 << 31);
