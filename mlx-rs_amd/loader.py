@@ -23,7 +23,7 @@ from pathlib import Path
 
 import torch
 
-from . import nn
+from . import nn, ops
 from ._capi import MlxrMoeError
 
 
@@ -58,20 +58,27 @@ def sanitize_key(key: str) -> str:
 class QuantizationConfig:
     """The `quantization` (or `quantization_config`) block of config.json:
     body group_size / bits and per-path {group_size, bits} overrides keyed
-    by the raw module prefix (quantization.rs:20-101)."""
+    by the raw module prefix (quantization.rs:20-101), each with its own
+    mode ("affine" where an override names none: the 8-bit routers of a
+    checkpoint whose experts are mxfp4)."""
 
     def __init__(self, cfg: dict):
         self.group_size = int(cfg["group_size"])
         self.bits = int(cfg["bits"])
         self.mode = cfg.get("mode", "affine")
-        self.overrides = {}
+        self.overrides, self.modes = {}, {}
         for k, v in cfg.items():
             if isinstance(v, dict) and "group_size" in v and "bits" in v:
                 self.overrides[k] = (int(v["group_size"]), int(v["bits"]))
+                self.modes[k] = v.get("mode", "affine")
 
     def for_path(self, raw_prefix: str) -> tuple[int, int]:
         """quantization.rs:51-56."""
         return self.overrides.get(raw_prefix, (self.group_size, self.bits))
+
+    def mode_for_path(self, raw_prefix: str) -> str:
+        """The quantisation mode of the module at raw_prefix."""
+        return self.modes.get(raw_prefix, self.mode)
 
     @classmethod
     def from_config(cls, config: dict):
@@ -169,11 +176,11 @@ def qwen35_moe_block(model_dir, layer: int, device, quantize_dense=None):
 
     Quantised modules keep the checkpoint's codes, scales and biases bit for
     bit, with (group_size, bits) from the config's per-path overrides
-    (quantization.rs:51-56).  Dense modules stay dense -- bf16
+    (quantization.rs:51-56), mode "mxfp4" among them.  Dense modules stay dense -- bf16
     SwitchLinear experts (gather_mm) and Linear projections, the
     MaybeQuantized::Original form -- unless quantize_dense = (group_size,
-    bits) asks to quantise them on load (try_into_quantized,
-    switch.rs:478-491).  A dense bf16 router computes in bf16 like the
+    bits) or (group_size, bits, mode) asks to quantise them on load
+    (try_into_quantized, switch.rs:478-491).  A dense bf16 router computes in bf16 like the
     reference's (nn.Linear); an f32 one in f32."""
     config = read_config(model_dir)
     tc = text_config(config)
@@ -187,14 +194,16 @@ def qwen35_moe_block(model_dir, layer: int, device, quantize_dense=None):
             w = lt.get(f"{module}.weight").to(dev, torch.bfloat16)
             if quantize_dense is None:
                 return nn.Linear(w) if cls is nn.QuantizedLinear else nn.SwitchLinear(w)
-            gs, bits = quantize_dense
             if cls is nn.QuantizedLinear:
-                return cls.try_from_linear(w, gs, bits)
-            return cls.try_from_switch_linear(w, gs, bits)
+                return cls.try_from_linear(w, *quantize_dense)
+            return cls.try_from_switch_linear(w, *quantize_dense)
         if qc is None:
             raise MlxrMoeError("weights: quantised tensors but no quantization config")
         gs, bits = qc.for_path(raw + module)
         wq = _u32_as_i32(lt.get(f"{module}.weight")).to(dev)
+        if ops._check_mode(qc.mode_for_path(raw + module)):
+            # (scale bytes as stored; no biases)
+            return cls(wq, lt.get(f"{module}.scales").to(dev), None, gs, bits, "mxfp4")
         sc = lt.get(f"{module}.scales").to(dev, torch.bfloat16)
         bi = lt.get(f"{module}.biases").to(dev, torch.bfloat16)
         return cls(wq, sc, bi, gs, bits)

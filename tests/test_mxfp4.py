@@ -189,6 +189,73 @@ def test_python_refuses(pkg):
     assert (d.bits, d.group_size, d.biases, d.input_dims) == (0x104, 32, None, 128)
 
 
+# -------------------------------------------------------------------- loader
+def write_checkpoint(path, E=8, d=256, f=128, mode="mxfp4"):
+    """One layer with mxfp4 experts and shared expert, an affine 8-bit router
+    and shared gate named by overrides."""
+    import json
+    st = pytest.importorskip("safetensors.torch")
+    g = torch.Generator().manual_seed(3)
+    pre = "language_model.model.layers.2.mlp."
+    t = {}
+    for name, shape in (("switch_mlp.gate_proj", (E, f, d)), ("switch_mlp.up_proj", (E, f, d)),
+                        ("switch_mlp.down_proj", (E, d, f)), ("shared_expert.gate_proj", (f, d)),
+                        ("shared_expert.up_proj", (f, d)), ("shared_expert.down_proj", (d, f))):
+        wq, sc = bank(g, (1,) * (3 - len(shape)) + shape)
+        t[pre + name + ".weight"] = wq.reshape(shape[:-1] + (-1,)).view(torch.uint32)
+        t[pre + name + ".scales"] = sc.reshape(shape[:-1] + (-1,))
+    q = {"group_size": 32, "bits": 4, "mode": mode}
+    for name, rows in (("gate", E), ("shared_expert_gate", 1)):
+        t[pre + name + ".weight"] = torch.randint(0, 2 ** 31 - 1, (rows, d // 4), generator=g,
+                                                  dtype=torch.int32).view(torch.uint32)
+        t[pre + name + ".scales"] = torch.full((rows, d // 64), 0.002).bfloat16()
+        t[pre + name + ".biases"] = torch.full((rows, d // 64), -0.25).bfloat16()
+        q[pre + name] = {"group_size": 64, "bits": 8}
+    st.save_file(t, str(path / "model.safetensors"), metadata={"format": "mlx"})
+    (path / "config.json").write_text(json.dumps(
+        {"quantization": q, "text_config": {"num_experts_per_tok": 4}}))
+    return t, pre
+
+
+def test_loader_reads_mxfp4(pkg, tmp_path):
+    t, pre = write_checkpoint(tmp_path)
+    b = pkg.loader.qwen35_moe_block(tmp_path, 2, "cpu")
+    up = b.switch_mlp.up_proj
+    assert (up.mode, up.group_size, up.bits, up.biases) == ("mxfp4", 32, 4, None)
+    assert torch.equal(up.weight.view(torch.uint32), t[pre + "switch_mlp.up_proj.weight"])
+    assert torch.equal(up.scales, t[pre + "switch_mlp.up_proj.scales"])
+    down = b.shared_expert.down_proj
+    assert down.mode == "mxfp4" and down.scales.shape == (1, 256, 4)
+    assert b.gate_weight.mode == "affine" and b.gate_weight.bits == 8
+    (tmp_path / "other").mkdir()
+    write_checkpoint(tmp_path / "other", mode="nvfp4")
+    with pytest.raises(pkg.MlxrMoeError, match="mode"):
+        pkg.loader.qwen35_moe_block(tmp_path / "other", 2, "cpu")
+
+
+@gpu
+@pytest.mark.parametrize("T", [1, 300])
+def test_loaded_block_runs(pkg, dev, tmp_path, T):
+    """The loaded block against its own modules: the expert rows combined
+    in the bf16 chain of a quantised router."""
+    write_checkpoint(tmp_path)
+    b = pkg.loader.qwen35_moe_block(tmp_path, 2, dev)
+    x = torch.randn((T, 256), generator=torch.Generator().manual_seed(T)).bfloat16().to(dev)
+    out = b.forward(x)
+    assert out.dtype == torch.bfloat16
+    idx, w = pkg.ops.router_topk_quantized(x, b.gate_weight, 4)
+    assert torch.equal(b.last_indices, idx)
+    y = b.switch_mlp.forward(x, idx).double()
+    sy = b.shared_expert.forward(x).double()
+    sg = b.shared_expert_gate_weight
+    sg = pkg.ops.dequantize(sg.weight[0], sg.scales[0], sg.biases[0], 64, 8, torch.float32)
+    gate = torch.sigmoid(x.double() @ sg.double().t())
+    ref = (y * w.double()[:, :, None]).sum(1) + sy * gate
+    mass = (y * w.double()[:, :, None]).abs().sum(1) + (sy * gate).abs()
+    # each row and product, the sums and the gate rounded to bf16: four steps
+    assert bool(((out.double() - ref).abs() <= 4 * 2.0 ** -7 * mass).all())
+
+
 # ------------------------------------------------------ quantise, dequantise
 @gpu
 def test_every_code_and_scale(pkg, dev):
