@@ -288,7 +288,16 @@ constexpr int kMaxInputDims = 4096;
 #ifndef MLXR_PREFILL_DENSE_ROWS
 #define MLXR_PREFILL_DENSE_ROWS 64
 #endif
+// mxfp4: 32 rows below MLXR_MX_SHORT_ROWS an expert, where the weights' bytes bound the
+// products and the shorter x stages leave LDS for whole lines of them (gate/up and
+// down in us, 64 then 32 rows: c2 T=64 (4 rows an expert) 45 + 28 and 40 + 26, c4 T=420
+// (8) 118 + 66 and 108 + 65, c2 T=300 (19) 56 + 34 and 52 + 32, c4 T=1000 (20) 136 + 77
+// and 129 + 79, c4 T=1300 (25) 140 + 80 and 139 + 86), then as the quantised ones.
+#ifndef MLXR_MX_SHORT_ROWS
+#define MLXR_MX_SHORT_ROWS 24
+#endif
 constexpr int kPrefillMinTileRows = 64;
+constexpr int kMinTileRows = 32;
 int prefill_tile_rows(int64_t rows, int64_t experts, int bits = 4);
 // max_items bounds the number of work items (dispatch_max_work); prefill
 // selects the M-tiled kernel (prefill.hip) where it applies.  Dense bf16
@@ -374,7 +383,7 @@ hipError_t launch_qgemm_prefill_tall(const QGemmArgs& a, int64_t x_rows, int64_t
 
 // ------------------------------------------- mx_stream.hip, mx_tile.hip
 // launch_qgemm's kernels for kBitsMxfp4: work items (few rows per expert), and
-// M-tiles of tile_rows (64 or 128) rows.  With ids the work items of n <= 64 rows
+// M-tiles of tile_rows (32, 64 or 128) rows.  With ids the work items of n <= 64 rows
 // are found in the kernel, from no dispatch: flat row f of batch b = f / M has
 // expert ids[b] and x row (lhs ? lhs[b] : b / div) * M + f % M, and its output row
 // is f.

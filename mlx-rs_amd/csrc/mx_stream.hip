@@ -32,22 +32,16 @@
 namespace mlxr_moe {
 namespace {
 
-// timing builds: steps in flight (gated, not), waves to slice for, blocks per wave
-// and workgroups to keep
+// timing builds: steps in flight (gated, not), and workgroups to keep with two blocks
+// a wave
 #ifndef MLXR_MX_DG
 #define MLXR_MX_DG 2
 #endif
 #ifndef MLXR_MX_D
 #define MLXR_MX_D 3
 #endif
-#ifndef MLXR_MX_KS_WAVES
-#define MLXR_MX_KS_WAVES 2048
-#endif
-#ifndef MLXR_MX_NB
-#define MLXR_MX_NB 4
-#endif
 #ifndef MLXR_MX_NB_UNITS
-#define MLXR_MX_NB_UNITS 768
+#define MLXR_MX_NB_UNITS 384
 #endif
 constexpr int kWaves = 4;
 typedef __attribute__((address_space(3))) void* lds_ptr;
@@ -331,18 +325,27 @@ hipError_t launch_mx_stream(const QGemmArgs& a, int64_t max_items, const QGemmAr
   const int64_t items2 = shared ? (shared_rows + kWorkRows - 1) / kWorkRows : 0;
   const int64_t items = max_items + items2;
   const int G = a.K / kMxGroup, S = (G + 3) / 4;
-  // slices: until there are 2048 waves (two per SIMD), two steps each at least
-  int ks = 1;
-  while (ks < kWaves && items * (a.N / 16) * ks < MLXR_MX_KS_WAVES && S >= 4 * ks) ks *= 2;
-  int nb = 1;
-  if (ks == 1)
-    while (nb < MLXR_MX_NB && a.N % (64 * 2 * nb) == 0 &&
-           items * (a.N / (64 * 2 * nb)) >= MLXR_MX_NB_UNITS)
-      nb *= 2;
-  const int tiles_n = a.N / (16 * (kWaves / ks) * nb);
   const int nm = a.gated ? 2 : 1;
-  const int sc_bytes = (nb * 16 * G + 1023) / 1024 * 1024;
   const size_t x_lds = ((size_t)kWorkRows * (128 * S + 8) * 2 + 15) & ~size_t(15);
+  // slices of the input dim, four steps each at least, while the workgroups, which
+  // all stage the whole x, still run at once (their LDS: about four a CU up to K = 2048, two
+  // above; 1, 2 and 4 slices, c5 T=1 up 18, 12.0 and 16.4 us, c5 T=2 up 14.6, 18.3 and
+  // 20.8, c2 T=4 gate/up 14.2, 13.7 and 16.8, c2 T=2 10.6 with two and 10.1 with four;
+  // shorter slices lose, down of c2 T=1 6.0 and 6.7 with two)
+  const int64_t slots = 256 * (x_lds <= 36 * 1024 ? 4 : 2);
+  int ks = 1;
+  while (ks < kWaves && items * (a.N / 64) * ks * 2 <= slots && S >= 8 * ks) ks *= 2;
+  // two blocks a wave where one is short of steps, for the staging of x and the scales
+  // to pay, with enough workgroups left: one block then two, down of c4 T=60 (4 steps)
+  // 46 us and 38, of c2 T=16 (6) 16.8 and 14.8, of c5 T=2 (12) 13.6 and 12.6, of c5 T=8
+  // 34.4 and 34.4; but longer ones make rounds of workgroups long: c4 T=60 gate/up (16)
+  // 60 and 63, c5 T=16 up (32) 52 and 67
+  const int nb = ks == 1 && S < 16 && a.N % 128 == 0 &&
+                         items * (a.N / 128) >= MLXR_MX_NB_UNITS
+                     ? 2
+                     : 1;
+  const int tiles_n = a.N / (16 * (kWaves / ks) * nb);
+  const int sc_bytes = (nb * 16 * G + 1023) / 1024 * 1024;
   const size_t lds = x_lds + (size_t)kWaves * nm * sc_bytes +
                      (ks > 1 ? (size_t)kWaves * nm * 64 * sizeof(f32x4_t) : 0);
   const MxShape sh{tiles_n, nb, (int)(max_items * tiles_n), (int)max_items, (int)shared_rows,

@@ -1,5 +1,5 @@
 // Grouped expert GEMM of microscaled 4-bit weights for many rows per expert:
-// M-tiles of 64 or 128 rows, the weights converted in registers.
+// M-tiles of 32, 64 or 128 rows, the weights converted in registers.
 //
 // Same sums as the streaming kernel (mx_stream.hip): exact bf16 products in f32,
 // in chunks of 16 inputs a matrix instruction.  A workgroup is four waves; a wave
@@ -32,15 +32,18 @@ constexpr int kWaves = 4, kNT = 64 * kWaves;
 typedef __attribute__((address_space(3))) void* lds_ptr;
 constexpr int kXStages = 3;  // x stages of 64 inputs in LDS
 // Groups of a weight piece in LDS: a 128-byte line of every row, or half of one
-// under the shorter tiles, where three workgroups then fit a CU (down of c4 T=2048
-// 102 us with lines and two, 96 so; c6 down T=509 39.6 and 36.5; gate/up alike).
+// under 64-row tiles, where three workgroups then fit a CU (down of c4 T=2048 102 us
+// with lines and two, 96 so; c6 down T=509 39.6 and 36.5; gate/up alike).  Under
+// 32-row tiles whole lines leave room for three; c6 T=100 gate/up 54 us so, 58 with
+// half lines and four, 58 with two lines and two.
 template <int ROWS>
 constexpr int kPiece = ROWS == 64 ? 4 : 8;
 template <int ROWS>
 constexpr int kTileLds = kXStages * ROWS * 128 + kWaves * 2 * 512 * kPiece<ROWS>;
 template <int ROWS>
-constexpr int kWgs = ROWS == 64 ? 3 : 2;  // workgroups per CU
-static_assert(2 * kTileLds<128> <= 160 * 1024 && 3 * kTileLds<64> <= 160 * 1024, "LDS");
+constexpr int kWgs = ROWS == 128 ? 2 : 3;  // workgroups per CU
+static_assert(2 * kTileLds<128> <= 160 * 1024 && 3 * kTileLds<64> <= 160 * 1024 &&
+                  3 * kTileLds<32> <= 160 * 1024, "LDS");
 
 template <int N>
 __device__ __forceinline__ void wait_loads() {  // at most N loads not back
@@ -359,11 +362,13 @@ __global__ __launch_bounds__(kNT, kWgs<ROWS>) void mx_tile_kernel(RegLaunch L) {
       MLXR_MXU(2);
     else
       MLXR_MXU(1);
-  } else {
+  } else if constexpr (ROWS == 64) {
     if (u.rows > 32)
       MLXR_MXU(2);
     else
       MLXR_MXU(1);
+  } else {
+    MLXR_MXU(1);
   }
 #undef MLXR_MXU
 }
@@ -373,7 +378,7 @@ __global__ __launch_bounds__(kNT, kWgs<ROWS>) void mx_tile_kernel(RegLaunch L) {
 hipError_t launch_mx_tile(const QGemmArgs& a, int64_t x_rows, int tile_rows, int64_t max_tiles,
                           const QGemmArgs* shared, int64_t rows2, const char* profile,
                           hipStream_t s) {
-  if (tile_rows != 64 && tile_rows != 128) return hipErrorInvalidValue;
+  if (tile_rows != 32 && tile_rows != 64 && tile_rows != 128) return hipErrorInvalidValue;
   const int64_t tiles2 = shared ? (rows2 + tile_rows - 1) / tile_rows : 0;
   if (max_tiles <= 0 && tiles2 <= 0) return hipSuccess;
   const QGemmArgs& b = shared ? *shared : a;
@@ -389,6 +394,11 @@ hipError_t launch_mx_tile(const QGemmArgs& a, int64_t x_rows, int tile_rows, int
       mx_tile_kernel<true, 128><<<grid, kNT, kTileLds<128>, s>>>(L);
     else
       mx_tile_kernel<false, 128><<<grid, kNT, kTileLds<128>, s>>>(L);
+  } else if (tile_rows == 32) {
+    if (a.gated)
+      mx_tile_kernel<true, 32><<<grid, kNT, kTileLds<32>, s>>>(L);
+    else
+      mx_tile_kernel<false, 32><<<grid, kNT, kTileLds<32>, s>>>(L);
   } else {
     if (a.gated)
       mx_tile_kernel<true, 64><<<grid, kNT, kTileLds<64>, s>>>(L);

@@ -79,7 +79,7 @@ DispatchBuffers carve_dispatch(Carve& c, int64_t n, int64_t E,
   b.work_rows = kWorkRows;
   b.num_work = c.take<int32_t>(1);
   b.work_first = c.take<int32_t>(E);
-  b.tiles = c.take<int32_t>(2 * dispatch_max_tiles(n, E, kPrefillMinTileRows));
+  b.tiles = c.take<int32_t>(2 * dispatch_max_tiles(n, E, kMinTileRows));
   b.num_tiles = c.take<int32_t>(1);
   b.block_hist = c.take<int32_t>(nb * E);
   b.rank = c.take<int32_t>(n);
@@ -99,7 +99,8 @@ bool use_prefill_path(int64_t rows, int64_t experts, int bits) {
   if (bits == 16)
     return rows >= (int64_t)MLXR_DENSE_TILED_ROWS * experts && rows >= 512;
   if (bits == kBitsMxfp4)
-    return rows >= (int64_t)MLXR_MX_TILED_ROWS * experts && rows >= 512;
+    return 2 * rows >= (int64_t)MLXR_MX_TILED_ROWS2 * experts &&
+           (rows >= 512 || experts >= MLXR_MX_TILED_EXPERTS);
   // the M-tiled kernel pays once the experts average MLXR_QUANT_TILED_ROWS
   // rows and there are rows enough for its tiles to spread over the GPU
   return rows >= (int64_t)MLXR_QUANT_TILED_ROWS * experts && rows >= 512;

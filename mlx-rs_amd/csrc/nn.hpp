@@ -86,14 +86,19 @@ namespace nn {
 #ifndef MLXR_DENSE_TILED_ROWS
 #define MLXR_DENSE_TILED_ROWS 2
 #endif
-// mxfp4 ones switch at MLXR_MX_TILED_ROWS: the tile kernel streams an expert's
-// weights by whole lines, the streaming one holds more loads in flight where
-// experts have next to no rows.  Gate/up and down, streaming then tiles: c6 T=64 (2
-// rows) 41 + 28 us and 45 + 29, c4 T=100 (2) 92 + 46 and 71 + 46, c2 T=64 (4) 42 +
-// 25 and 43 + 26, c2 T=100 (6) 57 + 26 and 46 + 27, c4 T=420 (8) 152 + 80 and 111
-// + 70; projections of c5 T=64 (4) 110 and 87.
-#ifndef MLXR_MX_TILED_ROWS
-#define MLXR_MX_TILED_ROWS 2
+// mxfp4 ones switch at MLXR_MX_TILED_ROWS2 / 2 rows: the tile kernel streams an
+// expert's weights by whole lines, the streaming one holds more loads in flight where
+// experts have next to no rows.  Gate/up and down in us, streaming then tiles: c6 T=32
+// (1 row) 30 + 19 and 31 + 22, c2 T=24 (1.5) 34 + 19 and 37 + 20, c6 T=48 (1.5) 40 +
+// 23 and 40 + 25, c4 T=80 (1.6) 92 + 42 and 67 + 41, c2 T=32 (2) 40 + 22 and 39 + 20,
+// c4 T=420 (8) 152 + 80 and 108 + 65; the c5 projections of T=20 (1.25) 60 and 54, of
+// T=32 (2) 101 and 76.  Few experts with few rows (a shared expert) make too few
+// tiles to fill the GPU, and the streaming kernel slices the input dim there.
+#ifndef MLXR_MX_TILED_ROWS2
+#define MLXR_MX_TILED_ROWS2 3
+#endif
+#ifndef MLXR_MX_TILED_EXPERTS
+#define MLXR_MX_TILED_EXPERTS 128
 #endif
 bool use_prefill_path(int64_t rows, int64_t experts, int bits = 4);
 

@@ -387,6 +387,32 @@ def test_gather_many_rows(pkg, dev, E, N, K, T, topk, skew):
 
 
 @gpu
+@pytest.mark.parametrize("E,N,K,T,topk", [
+    (128, 64, 64, 95, 2),       # just under the tiles' rule
+    (128, 64, 64, 96, 2),       # just on it: 1.5 rows an expert
+    (130, 192, 192, 65, 3),     # part of a line, part of an N-tile
+    (128, 320, 768, 300, 4),    # several tiles for the crowded experts
+    (140, 64, 4096, 200, 5),    # the largest input dim
+    (200, 256, 2048, 1200, 3),  # 18 rows an expert
+])
+def test_gather_short_tiles(pkg, dev, E, N, K, T, topk):
+    """Many experts with few rows each, some just at and past a tile's end."""
+    g = torch.Generator().manual_seed(E * T + K)
+    x = torch.randn((T, 1, 1, K), generator=g).bfloat16()
+    idx = torch.randint(7, E, (T, topk), generator=g, dtype=torch.int32)
+    at = 0
+    for e, rows in enumerate([32, 33, 31, 1]):  # as many as there are rows for
+        take = idx.view(-1)[at:at + rows]
+        take.fill_(e)
+        at += len(take)
+    y, wq, sc = gather_case(pkg, dev, E, N, K, idx, x, K)
+    w64 = values64(wq, sc)
+    for e in idx.unique().tolist():
+        t, k = (idx == e).nonzero(as_tuple=True)
+        check_sum(y[t, k, 0], x[t, 0, 0].double(), w64[e], K)
+
+
+@gpu
 @pytest.mark.parametrize("T", [5, 400])
 def test_gather_lhs_M_and_bad_indices(pkg, dev, T):
     """lhs indices, several rows per batch, and indices out of range: their
@@ -671,6 +697,41 @@ def test_block(pkg, dev, T, shared_mx):
         h = blk.forward_residual(xd, n)
         assert bool(torch.isfinite(h).all())
         assert torch.allclose(h, xd.float() + blk.forward(n.forward(xd)), rtol=1e-5, atol=1e-5)
+
+
+@gpu
+@pytest.mark.parametrize("T", [70, 300])
+def test_block_many_experts(pkg, dev, T):
+    """Short tiles from the block's own dispatch, the shared expert's rows in
+    the same launches, and the same block without a workspace of its own."""
+    E, d, f, K = 128, 256, 192, 4
+    nn, ops = pkg.nn, pkg.ops
+    w, x, _ = ffn_inputs(T, E, d, f, T, K)
+    g = torch.Generator().manual_seed(8)
+    gate_w = torch.randn((E, d), generator=g).to(dev) * 0.1
+    sg = torch.randn((1, d), generator=g).to(dev) * 0.1
+    dense = [(torch.randn(s, generator=g) * 0.05).bfloat16().to(dev)
+             for s in ((f, d), (f, d), (d, f))]
+    shared = nn.SwigluMlp(*[nn.QuantizedLinear.try_from_linear(v, mode="mxfp4") for v in dense])
+    m = ffn(pkg, dev, w)
+    blk = nn.Qwen35MoeBlock(gate_w, m, K, shared, sg)
+    xd = x.to(dev)
+    out = blk.forward(xd)
+    idx, wts = ops.router_topk(xd, gate_w, K)
+    y, sy = m.forward(xd, idx), shared.forward(xd)
+    sgate = torch.sigmoid((xd.float() @ sg[0]).double())[:, None]
+    terms = y.double() * wts.double()[:, :, None]
+    mass = terms.abs().sum(1) + (sy.double() * sgate).abs()
+    lerr = d * 2.0 ** -22 * (xd.double().abs() @ sg[0].double().abs())[:, None]
+    # (as test_block: the folded rows may take another slicing, a bf16 step of any y)
+    assert bool(((out.double() - terms.sum(1) - sy.double() * sgate).abs()
+                 <= mass * (2.0 ** -6 + lerr)).all())
+    C = pkg._capi
+    bare = torch.empty_like(out)
+    stream = torch.cuda.current_stream().cuda_stream
+    C.check(C.lib().mlxr_moe_block_forward_noalloc(
+        ctypes.byref(blk.descriptor()), xd.data_ptr(), T, bare.data_ptr(), None, None, stream))
+    assert torch.equal(bare, out)
 
 
 @gpu
