@@ -408,7 +408,8 @@ bool SwitchFfn::can_fold(const SwigluMlp& m, int64_t T, int64_t K) const {
   // both on the decode kernels (quantised: the streaming kernel), or both
   // on the M-tiled one
   if (!routed_tiled && !shared_tiled) return sw_.bits != 16;
-  return routed_tiled && shared_tiled;
+  // (mxfp4: any number of the shared expert's rows rides along, with one numerics)
+  return routed_tiled && (shared_tiled || sw_.bits == kBitsMxfp4);
 }
 
 Status SwitchFfn::experts(const uint16_t* x, int64_t T, int64_t K,
