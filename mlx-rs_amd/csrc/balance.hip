@@ -293,7 +293,8 @@ __global__ __launch_bounds__(64 * kSmallWaves) void balance_small_kernel(
   }
 }
 
-// The gradient, a wave per row.
+// The gradient, a wave per row.  (Stores that keep no place in the caches: T = 32768
+// by 512 28.6 us instead of 32.9, but a sum over the gradient after it 6 us more.)
 template <bool BF16, int SLOTS>
 __global__ __launch_bounds__(64 * kWaves) void balance_vjp_kernel(
     BalanceArgs a, const int32_t* __restrict__ counts, const int32_t* __restrict__ tokens,

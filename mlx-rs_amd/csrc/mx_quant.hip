@@ -22,20 +22,41 @@ __device__ __forceinline__ uint32_t dpp_u(uint32_t v) {
   return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false);
 }
 
-// 8 values from flat element e0 on, as f32.  VEC: w is 16-byte aligned.
-template <bool BF16, bool VEC>
+// How the values are reached: one by one (any alignment), by 16-byte vectors, or by
+// such that keep no place in the caches, for arrays larger than the memory-side cache
+// (256 MB), of which no reader after the kernel could find much there.  A bank of 403 MB
+// there and back 184 us a pass with vectors, 166 with such loads, 152 with such stores
+// too; smaller arrays stay where their reader finds them.
+enum { kScalar, kVector, kStreamed };
+template <int HOW, class V>
+__device__ __forceinline__ V load16(const V* p) {
+  if constexpr (HOW == kStreamed) return __builtin_nontemporal_load(p);
+  return *p;
+}
+template <int HOW, class V>
+__device__ __forceinline__ void store16(V* p, V v) {
+  if constexpr (HOW == kStreamed)
+    __builtin_nontemporal_store(v, p);
+  else
+    *p = v;
+}
+
+// 8 values from flat element e0 on, as f32.
+template <bool BF16, int HOW>
 __device__ __forceinline__ void load8(const void* w, int64_t e0, float (&v)[8]) {
-  if constexpr (VEC && BF16) {
-    const u32x4_t u = *reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(w) + e0);
+  if constexpr (HOW != kScalar && BF16) {
+    const u32x4_t u =
+        load16<HOW>(reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(w) + e0));
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       v[2 * j] = __uint_as_float(u[j] << 16);
       v[2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
     }
-  } else if constexpr (VEC) {
+  } else if constexpr (HOW != kScalar) {
     const f32x4_t* p = reinterpret_cast<const f32x4_t*>(static_cast<const float*>(w) + e0);
+    const f32x4_t a = load16<HOW>(p), b = load16<HOW>(p + 1);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = p[0][j], v[4 + j] = p[1][j];
+    for (int j = 0; j < 4; ++j) v[j] = a[j], v[4 + j] = b[j];
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -47,7 +68,7 @@ __device__ __forceinline__ void load8(const void* w, int64_t e0, float (&v)[8]) 
   }
 }
 
-template <bool BF16, bool VEC>
+template <bool BF16, int HOW>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(const void* __restrict__ w, int64_t n,
                                                           uint32_t* __restrict__ wq,
                                                           uint8_t* __restrict__ scales) {
@@ -55,7 +76,7 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(const void* __restrict
   const int64_t e0 = i * 8;
   if (e0 >= n) return;  // whole groups: 32 divides n, and a group its wave
   float v[8];
-  load8<BF16, VEC>(w, e0, v);
+  load8<BF16, HOW>(w, e0, v);
   uint32_t top = 0;
 #pragma unroll
   for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
@@ -74,7 +95,7 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(const void* __restrict
   if ((i & 3) == 0) scales[i >> 2] = (uint8_t)byte;
 }
 
-template <bool OUT_BF16, bool VEC>
+template <bool OUT_BF16, int HOW>
 __global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint32_t* __restrict__ wq,
                                                             const uint8_t* __restrict__ scales,
                                                             int64_t n, void* __restrict__ out) {
@@ -86,8 +107,8 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint32_t* __re
   if constexpr (OUT_BF16) {
     const u32x4_t v = __builtin_bit_cast(u32x4_t, mx_weights(w, sc));
     uint16_t* o = static_cast<uint16_t*>(out) + e0;
-    if constexpr (VEC) {
-      *reinterpret_cast<u32x4_t*>(o) = v;
+    if constexpr (HOW != kScalar) {
+      store16<HOW>(reinterpret_cast<u32x4_t*>(o), v);
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[2 * j] = (uint16_t)v[j], o[2 * j + 1] = (uint16_t)(v[j] >> 16);
@@ -98,9 +119,9 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint32_t* __re
     const mx_f32x2_t c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, sc, 2);
     const mx_f32x2_t d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, sc, 3);
     float* o = static_cast<float*>(out) + e0;
-    if constexpr (VEC) {
-      *reinterpret_cast<f32x4_t*>(o) = f32x4_t{a.x, a.y, b.x, b.y};
-      *reinterpret_cast<f32x4_t*>(o + 4) = f32x4_t{c.x, c.y, d.x, d.y};
+    if constexpr (HOW != kScalar) {
+      store16<HOW>(reinterpret_cast<f32x4_t*>(o), f32x4_t{a.x, a.y, b.x, b.y});
+      store16<HOW>(reinterpret_cast<f32x4_t*>(o + 4), f32x4_t{c.x, c.y, d.x, d.y});
     } else {
       const float v[8] = {a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 #pragma unroll
@@ -112,7 +133,21 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint32_t* __re
 // elements per launch (a grid holds under 2^32 threads)
 constexpr int64_t kLaunchElems = (int64_t)1 << 34;
 
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+// how to reach an array of `bytes` at p
+int how(const void* p, int64_t bytes) {
+  if (reinterpret_cast<uintptr_t>(p) & 15) return kScalar;
+  return bytes > ((int64_t)256 << 20) ? kStreamed : kVector;
+}
+
+#define MLXR_MX_HOW(CALL, BF, h) \
+  do {                           \
+    if ((h) == kStreamed)        \
+      CALL(BF, kStreamed);       \
+    else if ((h) == kVector)     \
+      CALL(BF, kVector);         \
+    else                         \
+      CALL(BF, kScalar);         \
+  } while (0)
 
 }  // namespace
 
@@ -125,14 +160,13 @@ hipError_t launch_mx_quantize(const void* w, bool w_bf16, int64_t n, uint32_t* w
     const dim3 grid((unsigned)((m / 8 + 255) / 256));
     uint32_t* q = wq + at / 8;
     uint8_t* sc = scales + at / kMxGroup;
-    if (w_bf16 && aligned16(src))
-      mx_quantize_kernel<true, true><<<grid, 256, 0, s>>>(src, m, q, sc);
-    else if (w_bf16)
-      mx_quantize_kernel<true, false><<<grid, 256, 0, s>>>(src, m, q, sc);
-    else if (aligned16(src))
-      mx_quantize_kernel<false, true><<<grid, 256, 0, s>>>(src, m, q, sc);
+    const int h = how(src, n * es);
+#define MLXR_MX_CALL(BF, H) mx_quantize_kernel<BF, H><<<grid, 256, 0, s>>>(src, m, q, sc)
+    if (w_bf16)
+      MLXR_MX_HOW(MLXR_MX_CALL, true, h);
     else
-      mx_quantize_kernel<false, false><<<grid, 256, 0, s>>>(src, m, q, sc);
+      MLXR_MX_HOW(MLXR_MX_CALL, false, h);
+#undef MLXR_MX_CALL
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
@@ -148,18 +182,18 @@ hipError_t launch_mx_dequantize(const uint32_t* wq, const uint8_t* scales, int64
     const dim3 grid((unsigned)((m / 8 + 255) / 256));
     const uint32_t* q = wq + at / 8;
     const uint8_t* sc = scales + at / kMxGroup;
-    if (out_bf16 && aligned16(dst))
-      mx_dequantize_kernel<true, true><<<grid, 256, 0, s>>>(q, sc, m, dst);
-    else if (out_bf16)
-      mx_dequantize_kernel<true, false><<<grid, 256, 0, s>>>(q, sc, m, dst);
-    else if (aligned16(dst))
-      mx_dequantize_kernel<false, true><<<grid, 256, 0, s>>>(q, sc, m, dst);
+    const int h = how(dst, n * es);
+#define MLXR_MX_CALL(BF, H) mx_dequantize_kernel<BF, H><<<grid, 256, 0, s>>>(q, sc, m, dst)
+    if (out_bf16)
+      MLXR_MX_HOW(MLXR_MX_CALL, true, h);
     else
-      mx_dequantize_kernel<false, false><<<grid, 256, 0, s>>>(q, sc, m, dst);
+      MLXR_MX_HOW(MLXR_MX_CALL, false, h);
+#undef MLXR_MX_CALL
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
   return hipSuccess;
 }
+#undef MLXR_MX_HOW
 
 }  // namespace mlxr_moe

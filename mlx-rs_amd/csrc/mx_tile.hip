@@ -21,6 +21,7 @@
 // x's 192.  c4 T=2048 (40 rows an expert): gate/up 153 us for 570 MB of weights, 3.7
 // TB/s; matrix cores 40% busy, address units 50%.
 #include <algorithm>
+#include <type_traits>
 
 #include "mx.hpp"
 #include "prefill_reg.hpp"
@@ -57,11 +58,19 @@ __device__ __forceinline__ void stage_barrier() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
-// The rows [slot0, slot0 + rows) of expert e against N-tile nt.
+// A load that keeps no place in the caches.  Under 32-row tiles an expert's last tile
+// (mostly its only one) reads the weights so, which nothing reads again: c2 T=64 72 us
+// a pass without and 65 so, c6 down T=509 46 and 42 (46 with every tile so: an expert's
+// tiles after the first then read memory again).  Whole lines only: half a line read so
+// is fetched twice.  Taller tiles gain nothing (c4 T=2048 263 and 267 us).
+constexpr int kNonTemporal = 2;
+
+// The rows [slot0, slot0 + rows) of expert e against N-tile nt; last: no later tile
+// has rows of e.
 // NMB: 32-row blocks that hold rows.
 template <bool GATED, int ROWS, int NMB>
 __device__ __forceinline__ void mx_unit(const RegArgs& a, int N, int K, int e, int slot0,
-                                        int rows, int nt, char* smem) {
+                                        int rows, bool last, int nt, char* smem) {
   constexpr int TC = GATED ? 32 * kWaves : 64 * kWaves;  // channels per N-tile
   constexpr int WC = TC / kWaves;                        // ... per wave
   constexpr int kXBytes = ROWS * 128;
@@ -91,7 +100,7 @@ __device__ __forceinline__ void mx_unit(const RegArgs& a, int N, int K, int e, i
   const int och0 = nt * TC + wave * WC;  // the wave's first channel
   const auto wswz = [&](int r) { return GL == 8 ? r & 7 : (r >> 2) & 3; };
   const int wrow = lane / GL;
-  auto load_w = [&](int l) {
+  auto load_w_as = [&](int l, auto policy) {
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
 #pragma unroll
@@ -101,9 +110,16 @@ __device__ __forceinline__ void mx_unit(const RegArgs& a, int N, int K, int e, i
         const int ch = och0 + (GATED ? 0 : 32 * s) + RPL * i + wrow;
         __builtin_amdgcn_raw_ptr_buffer_load_lds(
             s ? wr1 : wr0, (lds_ptr)(wl + s * kWLine + 1024 * i), 16,
-            ok && ch < N ? (uint32_t)ch * row_bytes + 16u * wch : kPastEnd, 16 * GL * l, 0, 0);
+            ok && ch < N ? (uint32_t)ch * row_bytes + 16u * wch : kPastEnd, 16 * GL * l, 0,
+            decltype(policy)::value);
       }
     }
+  };
+  auto load_w = [&](int l) {
+    if (ROWS == 32 && last)
+      load_w_as(l, std::integral_constant<int, kNonTemporal>{});
+    else
+      load_w_as(l, std::integral_constant<int, 0>{});
   };
   constexpr int kWLoads = GL;
   u32x4_t w[2][SPL];  // [side][stage of the piece]: the group 2 stage + h of channel c
@@ -351,8 +367,9 @@ __global__ __launch_bounds__(kNT, kWgs<ROWS>) void mx_tile_kernel(RegLaunch L) {
   if (!u.place(L, blockIdx.x)) return;
   u.find_rows(L);
   const RegArgs r = pick_reg(u.second, L.a2, L.x_bytes2, L.a, L.x_bytes);
+  const bool last = u.rows < ROWS || (!u.second && L.a.offsets[u.e + 1] <= u.slot0 + ROWS);
 #define MLXR_MXU(NMB_) \
-  mx_unit<GATED, ROWS, NMB_>(r, L.a.N, L.a.K, u.e, u.slot0, u.rows, u.nt0, smem)
+  mx_unit<GATED, ROWS, NMB_>(r, L.a.N, L.a.K, u.e, u.slot0, u.rows, last, u.nt0, smem)
   if constexpr (ROWS == 128) {
     if (u.rows > 96)
       MLXR_MXU(4);

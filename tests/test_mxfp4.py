@@ -321,6 +321,21 @@ def test_quantise_borders_and_extremes(pkg, dev, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype,rows", [(torch.bfloat16, 65601), (torch.float32, 33003)])
+def test_quantise_larger_than_the_caches(pkg, dev, dtype, rows):
+    """An array past 256 MB: the same codes, scales and values as its parts."""
+    g = torch.Generator(device=dev).manual_seed(5)
+    w = torch.randn((rows, 2080), generator=g, device=dev).to(dtype)
+    assert w.numel() * w.element_size() > 2 ** 28
+    wq, sc, _ = pkg.ops.quantize(w, mode="mxfp4")
+    v = pkg.ops.dequantize(wq, sc, mode="mxfp4", out_dtype=dtype)
+    for a, b in ((0, 1), (1, rows // 2), (rows // 2, rows)):
+        q, s, _ = pkg.ops.quantize(w[a:b], mode="mxfp4")
+        assert torch.equal(q, wq[a:b]) and torch.equal(s, sc[a:b])
+        assert torch.equal(pkg.ops.dequantize(q, s, mode="mxfp4", out_dtype=dtype), v[a:b])
+
+
+@gpu
 def test_quantise_strided_and_unaligned(pkg, dev):
     w = torch.randn(6, 128, device=dev)
     q = pkg.ops.quantize
