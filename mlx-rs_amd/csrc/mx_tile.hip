@@ -365,9 +365,24 @@ __global__ __launch_bounds__(kNT, kWgs<ROWS>) void mx_tile_kernel(RegLaunch L) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   RegUnit<ROWS> u;
   if (!u.place(L, blockIdx.x)) return;
-  u.find_rows(L);
+  // The tile's rows end where the next tile's start (the list goes by expert, as the
+  // rows do), so both records come in one step; after the last one, at the end.
+  int end, next = -1;
+  if (u.second) {
+    u.e = 0, u.slot0 = u.tile * ROWS, end = L.rows2;
+  } else {
+    const int after = min(u.tile + 1, *L.a.num_tiles - 1);
+    const int2 rec = *reinterpret_cast<const int2*>(L.a.tiles + 2 * u.tile);
+    const int2 rec2 = *reinterpret_cast<const int2*>(L.a.tiles + 2 * after);
+    const int all = L.a.offsets[L.a.E];
+    u.e = __builtin_amdgcn_readfirstlane(rec.x);
+    u.slot0 = __builtin_amdgcn_readfirstlane(rec.y);
+    end = __builtin_amdgcn_readfirstlane(after > u.tile ? rec2.y : all);
+    if (after > u.tile) next = __builtin_amdgcn_readfirstlane(rec2.x);
+  }
+  u.rows = min(ROWS, end - u.slot0);
   const RegArgs r = pick_reg(u.second, L.a2, L.x_bytes2, L.a, L.x_bytes);
-  const bool last = u.rows < ROWS || (!u.second && L.a.offsets[u.e + 1] <= u.slot0 + ROWS);
+  const bool last = u.second ? u.slot0 + ROWS >= end : next != u.e;
 #define MLXR_MXU(NMB_) \
   mx_unit<GATED, ROWS, NMB_>(r, L.a.N, L.a.K, u.e, u.slot0, u.rows, last, u.nt0, smem)
   if constexpr (ROWS == 128) {
