@@ -233,7 +233,7 @@ class SplitSwitchFfn:
         ops._dev(x, indices)
         x2 = (x if x.ndim == 2 else x.reshape(-1, d)).contiguous()
         K = indices.shape[-1]
-        idx = ops._as_u32(indices)
+        idx = indices.to(torch.int32).contiguous()
         if idx.ndim != 2:
             idx = idx.reshape(-1, K)
         if idx.shape[0] != x2.shape[0]:

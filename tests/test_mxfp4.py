@@ -656,6 +656,18 @@ def test_split_ffn(pkg, dev, E, d, f, T, K):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.int16, torch.uint8, torch.int64])
+def test_split_ffn_takes_any_integer_indices(pkg, dev, dtype):
+    w, x, idx = ffn_inputs(2, 8, 256, 128, 5, 4)
+    m = ffn(pkg, dev, w)
+    want = m.forward(x.to(dev), idx.to(dev))
+    assert torch.equal(m.forward(x.to(dev), idx.to(dtype).to(dev)), want)
+    # (a transposed tensor of them too)
+    t = idx.to(dtype).to(dev).t().contiguous().t()
+    assert torch.equal(m.forward(x.to(dev), t), want)
+
+
+@gpu
 @pytest.mark.parametrize("T", [1, 9, 260])
 @pytest.mark.parametrize("act", ["geglu", "swiglu"])
 def test_packed_ffn(pkg, dev, T, act):
