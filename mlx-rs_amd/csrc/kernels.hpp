@@ -402,7 +402,8 @@ hipError_t launch_mx_stream(const QGemmArgs& a, int64_t max_items, const QGemmAr
                             const MxIds* ids = nullptr);
 // The tile kernel's part of a dispatch (offsets, sorted, tiles, num_tiles; the
 // other buffers are not written) of the rows of ids, in one launch; with xrow each
-// row's x row too, and with ids.zero_bad rows of bad indices of out [n, N] cleared.
+// row's x row too, and with ids.zero_bad rows of bad indices of out [n, N] (16-byte
+// aligned, N % 64 == 0) cleared.
 // At most kMxSortRows rows: 20480 take 12.5 us (the general dispatch's launches 16),
 // 32768 17.4 (17).
 constexpr int kMxSortRows = 24576;

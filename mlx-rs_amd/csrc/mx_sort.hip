@@ -64,7 +64,8 @@ __global__ __launch_bounds__(kThreads) void mx_sort_kernel(MxIds d, int tile_row
       } else {
         if (!(d.skip_minus1 && e[i] == -1)) bad = 1;
         if (d.zero_bad)
-          for (int64_t k = 0; k < N; ++k) out[f * N + k] = 0;
+          for (int64_t k = 0; k < N; k += 8)  // (16-byte aligned rows, N % 64 == 0)
+            *reinterpret_cast<u32x4_t*>(out + f * N + k) = u32x4_t{0u, 0u, 0u, 0u};
       }
       if (xrow) {
         const int batch = f / d.M;

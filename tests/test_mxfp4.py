@@ -479,7 +479,8 @@ def test_gather_groups_of_rows(pkg, dev, n, kind):
 
 
 @gpu
-@pytest.mark.parametrize("T,topk,E", [(40, 16, 8), (520, 1, 2), (3000, 2, 3), (33000, 1, 5)])
+@pytest.mark.parametrize("T,topk,E", [(40, 16, 8), (520, 1, 2), (3000, 2, 3), (33000, 1, 5),
+                                      (600, 3, 1024)])
 def test_gather_sorts(pkg, dev, T, topk, E):
     """The tiles' own sort: few rows to more than it takes (then the general
     dispatch), indices out of range among them, an expert without rows."""
@@ -497,6 +498,26 @@ def test_gather_sorts(pkg, dev, T, topk, E):
     for e in range(E - 1):
         t, k = (idx == e).nonzero(as_tuple=True)
         check_sum(y[t, k, 0], x[t, 0, 0].double(), w64[e], K)
+
+
+@gpu
+@pytest.mark.parametrize("T,topk", [(3, 2), (800, 2)])
+def test_gather_weights_past_32_bits(pkg, dev, T, topk):
+    """8.6 GB of codes in one tensor: the last experts' rows, from the
+    streaming kernel and from tiles."""
+    E, N, K = 1024, 4096, 4096
+    g = torch.Generator(device=dev).manual_seed(1)
+    wq = torch.randint(-2 ** 31, 2 ** 31 - 1, (E, N, K // 8), generator=g, device=dev,
+                       dtype=torch.int32)
+    sc = torch.randint(118, 122, (E, N, K // 32), generator=g, device=dev, dtype=torch.uint8)
+    idx = torch.randint(0, E, (T, topk), generator=g, device=dev, dtype=torch.int32)
+    idx[0, 0], idx[1, 1], idx[2, 0] = E - 1, E - 2, 513
+    x = torch.randn((T, 1, 1, K), generator=g, device=dev).bfloat16()
+    y = pkg.ops.gather_qmm(x, wq, sc, rhs_indices=idx, mode="mxfp4").cpu()
+    x, idx = x.cpu().double(), idx.cpu()
+    for e in (E - 1, E - 2, 513):
+        t, k = (idx == e).nonzero(as_tuple=True)
+        check_sum(y[t, k, 0], x[t, 0, 0], values64(wq[e:e + 1].cpu(), sc[e:e + 1].cpu())[0], K)
 
 
 @gpu
