@@ -18,8 +18,9 @@
 // c2 T=4096: gate/up 195 us, 1.06 PFLOP/s, down 118; without any load (a copy of the
 // kernel, timed) 155 and 97, where the power limit holds the matrix cores: a library
 // product of 8192^3 reaches 1.46 PFLOP/s.  Without the weights' loads 172, without
-// x's 192.  c4 T=2048 (40 rows an expert): gate/up 153 us for 570 MB of weights, 3.7
-// TB/s; matrix cores 40% busy, address units 50%.
+// x's 192.  c4 T=2048 (40 rows an expert): gate/up 153 us for 570 MB of weights, 146 of
+// them without any matrix instruction: the weights' way from memory and x's, 5 TB/s in
+// all.  c2 T=64 (4 rows): gate/up 37 us, 5.7 TB/s, down 24.
 #include <algorithm>
 #include <type_traits>
 
