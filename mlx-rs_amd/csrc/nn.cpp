@@ -100,7 +100,8 @@ bool use_prefill_path(int64_t rows, int64_t experts, int bits) {
     return rows >= (int64_t)MLXR_DENSE_TILED_ROWS * experts && rows >= 512;
   if (bits == kBitsMxfp4)
     return 2 * rows >= (int64_t)MLXR_MX_TILED_ROWS2 * experts &&
-           (rows >= 512 || experts >= MLXR_MX_TILED_EXPERTS);
+           (rows >= 512 || experts >= MLXR_MX_TILED_EXPERTS ||
+            (experts >= 8 && rows >= std::min<int64_t>(MLXR_MX_TILED_FEW * experts, 320)));
   // the M-tiled kernel pays once the experts average MLXR_QUANT_TILED_ROWS
   // rows and there are rows enough for its tiles to spread over the GPU
   return rows >= (int64_t)MLXR_QUANT_TILED_ROWS * experts && rows >= 512;

@@ -92,13 +92,21 @@ namespace nn {
 // (1 row) 30 + 19 and 31 + 22, c2 T=24 (1.5) 34 + 19 and 37 + 20, c6 T=48 (1.5) 40 +
 // 23 and 40 + 25, c4 T=80 (1.6) 92 + 42 and 67 + 41, c2 T=32 (2) 40 + 22 and 39 + 20,
 // c4 T=420 (8) 152 + 80 and 108 + 65; the c5 projections of T=20 (1.25) 60 and 54, of
-// T=32 (2) 101 and 76.  Few experts with few rows (a shared expert) make too few
-// tiles to fill the GPU, and the streaming kernel slices the input dim there.
+// T=32 (2) 101 and 76.  Few experts make too few tiles to fill the GPU, and the
+// streaming kernel, which slices the input dim there, holds out longer: to
+// MLXR_MX_TILED_FEW rows an expert or 320 in all from 8 experts on, to 512 below (whole
+// banks at d = 2048, streaming then tiles: 8 experts of f = 4096, 8 rows 43 and 52, 16
+// rows 63 and 53, 50 rows 125 and 68; 16 of f = 1024, 8 rows 26 and 31, 16 rows 34 and
+// 32, 32 rows 49 and 38; 64 of f = 1408, 2 rows 67 and 72, 4.7 rows 73 and 74, 6 rows
+// 83 and 74, 8 rows 91 and 72; one of f = 512, 65 rows 15 and 38, 511 rows 34 and 47).
 #ifndef MLXR_MX_TILED_ROWS2
 #define MLXR_MX_TILED_ROWS2 3
 #endif
 #ifndef MLXR_MX_TILED_EXPERTS
 #define MLXR_MX_TILED_EXPERTS 128
+#endif
+#ifndef MLXR_MX_TILED_FEW
+#define MLXR_MX_TILED_FEW 16
 #endif
 bool use_prefill_path(int64_t rows, int64_t experts, int bits = 4);
 
