@@ -4,7 +4,8 @@ quantised expert GEMM, combine) behind the reference's op/module API.
 The kernels live in libmlxr_moe.so (HIP, gfx950) behind the C ABI of
 include/mlxr_moe.h.  This package is the Python view of that ABI:
     ops       gather_qmm / quantize / dequantize / argpartition_axis /
-              softmax_axis / router_topk / dispatch / combine
+              softmax_axis / router_topk / dispatch / combine /
+              router_balance / router_balance_vjp
     nn        QuantizedSwitchLinear / QuantizedLinear / SwigluMlp /
               SplitSwitchFfn / PackedSwitchFfn / Qwen35MoeBlock /
               GemmaRouter / GemmaMoe

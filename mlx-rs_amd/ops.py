@@ -10,6 +10,11 @@ runs a kernel of libmlxr_moe.so; there is no fallback.
     gather_qmm        crates/mlxr/src/ops/quantization.rs:171-221
     argpartition_axis crates/mlxr/src/ops/sort.rs:211-226
     softmax_axis      crates/mlxr/src/ops/arithmetic.rs:1298-1311
+
+quantize, dequantize and gather_qmm take mode "mxfp4" (microscaled 4-bit
+weights) beside "affine".  router_balance and router_balance_vjp, the router's
+load-balance loss with its per-expert counts and the router's gradients, have no
+counterpart there.
 """
 from __future__ import annotations
 
