@@ -202,8 +202,9 @@ int mlxr_moe_router_topk(const void* x, int64_t T, int64_t d,
  *   probs f32 [E]: mean of p over the counted tokens
  *   tokens int32 [1]: N
  *   loss f32 [1] = E * sum_e counts_e / (N K) * probs_e
- * all 0 when N is 0.  A row whose logits are all -inf adds no probability; an
- * index outside [0, E) is not counted and sets the workspace's status word
+ * all 0 when N is 0.  A counted row whose logits are all -inf adds no
+ * probability; NaN or +inf among them makes its p, and so probs and loss, NaN.
+ * An index outside [0, E) is not counted and sets the workspace's status word
  * (mlxr_moe_workspace_status).  Sums are in f32 within a workgroup's rows and
  * in f64 across workgroups, in a fixed order: equal inputs give equal bits.  E <= 1024, K <= 64. */
 size_t mlxr_moe_router_balance_workspace_size(int64_t T, int64_t E);
@@ -222,8 +223,9 @@ int mlxr_moe_router_balance(const void* logits, int logits_dtype, int64_t ld,
  * (an expert named twice in a row gets both terms, an index out of range
  * none).  dloss f32 [1] on the device; dloss NULL: no balance term (counts and
  * tokens are then not read); dweights NULL: no weights' term; one of them is
- * required.  Rows whose mask is 0, and terms of a row without a finite
- * maximum, get 0.  dlogits must not overlap the inputs. */
+ * required.  Rows whose mask is 0 get 0, and so does a term whose softmax is over
+ * -inf alone (the row's logits, or the chosen ones); NaN or +inf among those
+ * makes the term NaN.  dlogits must not overlap the inputs. */
 int mlxr_moe_router_balance_vjp(const void* logits, int logits_dtype,
                                 int64_t ld, int64_t T, int64_t E,
                                 const int32_t* indices, int64_t K,

@@ -11,8 +11,9 @@
 // plus the gradient of the renormalised top-k weights w[t, :] = softmax of the
 // K chosen logits (crates/mlxr-lm/src/qwen3_5/text/moe.rs:136-138),
 //   dz[t, idx[t, k]] += w[t, k] * (dw[t, k] - sum_j w[t, j] dw[t, j]).
-// A row whose largest logit is -inf has no probabilities: it adds none, and its
-// gradient is 0.  With N = 0 everything is 0.
+// A row whose logits are all -inf has no probabilities: it adds none, and its
+// gradient is 0 (w alike, over the chosen logits).  NaN or +inf among the logits
+// makes their softmax NaN.  With N = 0 everything is 0.
 //
 // One pass over the logits, a wave per row, in the summation orders fixed here
 // (no floating-point atomics): a wave's rows add up in registers, a workgroup's
@@ -77,16 +78,25 @@ __device__ __forceinline__ void load_row(const void* z, int64_t ld, int64_t t, i
     v[j] = e < E ? logit<BF16>(z, t * ld + e) : -INFINITY;
   }
 }
-// v := softmax over the wave (0 everywhere where no logit is above -inf).  NaN
-// logits make the row NaN: fmaxf leaves them out of the maximum, the sum takes
-// them up.
+// Whether logits of maximum m over the wave are all -inf (the same on every lane).
+// fmaxf leaves NaN out of a maximum, so one of -inf may hide it behind the -inf of
+// experts that are shut off and of lanes past the end; nan: this lane holds one.
+// A NaN beside a larger maximum needs no look: the softmax's sum takes it up.
+__device__ __forceinline__ bool no_softmax(float m, bool nan) {
+  return m == -INFINITY && !__any(nan);
+}
+// v := softmax over the wave (0 everywhere where all logits are -inf).  NaN or +inf
+// make the row NaN.
 template <int SLOTS>
 __device__ __forceinline__ void softmax_row(float (&v)[SLOTS]) {
   float m = v[0];
 #pragma unroll
   for (int j = 1; j < SLOTS; ++j) m = fmaxf(m, v[j]);
   m = wave_max(m);
-  const bool none = m == -INFINITY;
+  bool nan = false;
+#pragma unroll
+  for (int j = 0; j < SLOTS; ++j) nan |= v[j] != v[j];
+  const bool none = no_softmax(m, nan);
   float s = 0.0f;
 #pragma unroll
   for (int j = 0; j < SLOTS; ++j) {
@@ -332,9 +342,10 @@ __global__ __launch_bounds__(64 * kWaves) void balance_vjp_kernel(
         const float zk = in ? logit<BF16>(a.z, t * a.ld + e) : -INFINITY;
         const float dk = in ? dw[i] : 0.0f;
         const float m = wave_max(zk);
-        const float u = in && m != -INFINITY ? __builtin_amdgcn_exp2f((zk - m) * kLog2e) : 0.0f;
+        const bool none = no_softmax(m, zk != zk);
+        const float u = in && !none ? __builtin_amdgcn_exp2f((zk - m) * kLog2e) : 0.0f;
         const float s = wave_add(u);
-        const float w = m != -INFINITY ? u / s : 0.0f;
+        const float w = none ? 0.0f : u / s;
         gk = w * (dk - wave_add(w * dk));
         // one expert chosen twice: its first lane takes the sum, in order
         first = in;

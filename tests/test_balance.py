@@ -407,3 +407,58 @@ def test_router_step_over_mxfp4_experts(pkg, dev, T):
     # logits and dw are f32 sums of d terms: relative to the gradient's mass
     mass = (dz.double().abs().t() @ x.double().abs())
     assert bool(((dgate - gate64.grad).abs() <= 1e-4 * (mass + mass.mean())).all())
+
+
+@gpu
+@pytest.mark.parametrize("T", [6, 600])
+@pytest.mark.parametrize("E", [8, 60, 65, 128])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_without_a_softmax(pkg, dev, T, E, dtype):
+    """NaN and +inf logits in rows that count make the row, the loss and the
+    mean probabilities NaN, as the formula does, whether or not the experts
+    fill the lanes; the other rows' gradients are as without them, and a row of
+    -inf alone still has none."""
+    ops, K, inf, nan = pkg.ops, 4, float("inf"), float("nan")
+    z, idx, _ = inputs(T + E, T, E, K, dtype)
+    bad = z.clone()
+    bad[0] = nan                # nothing but NaN
+    bad[1] = -inf               # NaN beside experts that are shut off
+    bad[1, idx[1, 2].long()] = nan
+    bad[2, idx[2, 0].long()] = inf
+    bad[3, idx[3, 1].long()] = nan
+    bad[4] = -inf
+    idx, dw = idx.to(dev), torch.randn((T, K), generator=torch.Generator().manual_seed(E)).to(dev)
+    one = torch.ones((), device=dev)
+    _, counts, _, tokens = ops.router_balance(z.to(dev), idx)
+    for rows in ([0], [1], [2], [3], [0, 1, 2, 3, 4]):
+        zr = z.clone()
+        zr[rows] = bad[rows]
+        loss, c, probs, n = ops.router_balance(zr.to(dev), idx)
+        assert bool(torch.isnan(loss)) and bool(torch.isnan(probs).all())
+        assert torch.equal(c, counts) and int(n) == T
+    bad = bad.to(dev)
+    both = ops.router_balance_vjp(bad, idx, counts, tokens, one, None, dw)
+    loss_only = ops.router_balance_vjp(bad, idx, counts, tokens, one)
+    dw_only = ops.router_balance_vjp(bad, idx, dweights=dw)
+    assert bool(torch.isnan(both[:4]).all()) and bool(torch.isnan(loss_only[:4]).all())
+    # the weights' term reaches the chosen experts only
+    hit = torch.zeros((T, E), dtype=torch.bool, device=dev).scatter(1, idx.long(), True)
+    assert torch.equal(torch.isnan(dw_only[:4]), hit[:4])
+    for got, kw in ((both, (counts, tokens, one, None, dw)), (loss_only, (counts, tokens, one)),
+                    (dw_only, (None, None, None, None, dw))):
+        assert bool((got[4] == 0).all())
+        assert torch.equal(got[5:], ops.router_balance_vjp(z.to(dev), idx, *kw)[5:])
+
+
+@gpu
+def test_nan_outside_the_chosen_experts(pkg, dev):
+    """The weights' term is a softmax of the chosen logits alone: what the other
+    experts of the row hold does not reach it."""
+    z, idx, _ = inputs(9, 20, 60, 3)
+    dw = torch.randn((20, 3), generator=torch.Generator().manual_seed(2)).to(dev)
+    bad = z.clone()
+    hit = torch.zeros((20, 60), dtype=torch.bool).scatter(1, idx.long(), True)
+    bad[~hit] = float("nan")
+    idx = idx.to(dev)
+    assert torch.equal(pkg.ops.router_balance_vjp(bad.to(dev), idx, dweights=dw),
+                       pkg.ops.router_balance_vjp(z.to(dev), idx, dweights=dw))
