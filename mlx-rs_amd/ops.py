@@ -436,7 +436,9 @@ def _balance_inputs(name, logits, indices, mask):
                                f"of logits {tuple(logits.shape)}")
         mask = mask.reshape(-1).contiguous()
     idx = _as_u32(indices)
-    return z, max(z.stride(0), E), idx if idx.ndim == 2 else idx.flatten(0, -2), mask
+    if idx.ndim != 2:  # (one token's [K] too)
+        idx = idx.flatten(0, -2) if idx.ndim > 2 else idx[None]
+    return z, max(z.stride(0), E), idx, mask
 
 
 def router_balance(logits: torch.Tensor, indices: torch.Tensor, mask=None):

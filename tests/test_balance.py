@@ -462,3 +462,21 @@ def test_nan_outside_the_chosen_experts(pkg, dev):
     idx = idx.to(dev)
     assert torch.equal(pkg.ops.router_balance_vjp(bad.to(dev), idx, dweights=dw),
                        pkg.ops.router_balance_vjp(z.to(dev), idx, dweights=dw))
+
+
+@gpu
+def test_one_token_without_a_row_axis(pkg, dev):
+    """Logits [E] with choices [K] are one token; its mask has no axis."""
+    ops = pkg.ops
+    z, idx, _ = inputs(4, 1, 60, 3)
+    z, idx, one = z.to(dev), idx.to(dev), torch.ones((), device=dev)
+    dw = torch.randn((1, 3), generator=torch.Generator().manual_seed(6)).to(dev)
+    for m in (None, torch.ones(1, dtype=torch.bool, device=dev),
+              torch.zeros(1, dtype=torch.bool, device=dev)):
+        m0 = None if m is None else m[0]
+        want = ops.router_balance(z, idx, m)
+        got = ops.router_balance(z[0], idx[0], m0)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        dz = ops.router_balance_vjp(z, idx, want[1], want[3], one, m, dw)
+        d0 = ops.router_balance_vjp(z[0], idx[0], want[1], want[3], one, m0, dw[0])
+        assert d0.shape == (60,) and torch.equal(d0, dz[0])
