@@ -29,13 +29,7 @@ class OptionalInt(Structure):
 
     @classmethod
     def of(cls, v):
-        o = _OPTIONAL.get(v)
-        if o is None:
-            o = _OPTIONAL[v] = cls(0, 0) if v is None else cls(int(v), 1)
-        return o
-
-
-_OPTIONAL = {}  # passed by value, never changed
+        return cls(0, 0) if v is None else cls(int(v), 1)
 
 
 class QLinear(Structure):

@@ -816,3 +816,17 @@ def test_graph_and_streams(pkg, dev, T):
     torch.cuda.current_stream().wait_stream(side)
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(other, eager))
+
+
+def test_optional_int_reads_its_argument_at_every_call(pkg):
+    """Anything int() takes, and its value now, whatever a call before held."""
+    import numpy as np
+    of = pkg._capi.OptionalInt.of
+    t = torch.tensor(64)
+    assert of(t).value == 64
+    t.fill_(32)
+    assert of(t).value == 32
+    assert of(np.array(8)).value == 8 and of(np.int64(4)).value == 4 and of(4.0).value == 4
+    o = of(5)
+    o.value = 6  # the caller's own
+    assert of(5).value == 5 and of(None).has_value == 0 and of(5).has_value == 1
