@@ -65,12 +65,12 @@ class QuantizationConfig:
     def __init__(self, cfg: dict):
         self.group_size = int(cfg["group_size"])
         self.bits = int(cfg["bits"])
-        self.mode = cfg.get("mode", "affine")
+        self.mode = cfg.get("mode") or "affine"
         self.overrides, self.modes = {}, {}
         for k, v in cfg.items():
             if isinstance(v, dict) and "group_size" in v and "bits" in v:
                 self.overrides[k] = (int(v["group_size"]), int(v["bits"]))
-                self.modes[k] = v.get("mode", "affine")
+                self.modes[k] = v.get("mode") or "affine"
 
     def for_path(self, raw_prefix: str) -> tuple[int, int]:
         """quantization.rs:51-56."""

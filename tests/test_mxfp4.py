@@ -830,3 +830,13 @@ def test_optional_int_reads_its_argument_at_every_call(pkg):
     o = of(5)
     o.value = 6  # the caller's own
     assert of(5).value == 5 and of(None).has_value == 0 and of(5).has_value == 1
+
+
+@pytest.mark.parametrize("named", [{}, {"mode": None}, {"mode": "affine"}])
+def test_loader_takes_a_mode_that_says_nothing(pkg, named):
+    """A mode of null, in the body or in an override, is none: affine."""
+    pre = "model.layers.0.mlp.gate"
+    q = pkg.loader.QuantizationConfig({"group_size": 64, "bits": 4, **named,
+                                       pre: {"group_size": 64, "bits": 8, **named}})
+    assert q.mode_for_path(pre) == "affine" and q.mode_for_path("other") == "affine"
+    assert q.for_path(pre) == (64, 8)
