@@ -233,7 +233,7 @@ class SplitSwitchFfn:
         ops._dev(x, indices)
         x2 = (x if x.ndim == 2 else x.reshape(-1, d)).contiguous()
         K = indices.shape[-1]
-        idx = indices.to(torch.int32).contiguous()
+        idx = ops._as_int32(indices)
         if idx.ndim != 2:
             idx = idx.reshape(-1, K)
         if idx.shape[0] != x2.shape[0]:
@@ -304,7 +304,7 @@ class PackedSwitchFfn:
         ops._dev(x, indices)
         x2 = x.reshape(-1, d).contiguous()
         K = indices.shape[-1]
-        idx = indices.reshape(-1, K).to(torch.int32).contiguous()
+        idx = ops._as_int32(indices.reshape(-1, K))
         if idx.shape[0] != x2.shape[0]:
             raise MlxrMoeError("PackedSwitchFfn: indices must be [..., T, K] over x [..., T, d]")
         return x2, idx, K

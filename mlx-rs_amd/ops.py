@@ -111,6 +111,14 @@ def _as_u32(idx: torch.Tensor) -> torch.Tensor:
         return idx
     if idx.dtype not in (torch.int32, torch.int64, torch.uint32):
         raise MlxrMoeError(f"indices must be integer, got {idx.dtype}")
+    return _as_int32(idx)
+
+
+def _as_int32(idx: torch.Tensor) -> torch.Tensor:
+    """idx as contiguous int32.  64-bit values that do not fit go to the type's
+    ends, which are out of every range here, not to their low bits."""
+    if idx.dtype == torch.int64:
+        idx = idx.clamp(-2 ** 31, 2 ** 31 - 1)
     return idx.to(torch.int32).contiguous()
 
 

@@ -480,3 +480,21 @@ def test_one_token_without_a_row_axis(pkg, dev):
         dz = ops.router_balance_vjp(z, idx, want[1], want[3], one, m, dw)
         d0 = ops.router_balance_vjp(z[0], idx[0], want[1], want[3], one, m0, dw[0])
         assert d0.shape == (60,) and torch.equal(d0, dz[0])
+
+
+@gpu
+@pytest.mark.parametrize("T", [5, 600])
+def test_indices_past_32_bits(pkg, dev, T):
+    """64-bit indices that no 32-bit one holds are out of range: not counted,
+    without a gradient, and the status word says so."""
+    ops = pkg.ops
+    z, idx, _ = inputs(T, T, 24, 3)
+    wide, cut = idx.long(), idx.clone()
+    wide[0, 0], wide[1, 2], wide[2, 1], wide[4, 0] = 2 ** 32 + 5, -2 ** 32, 2 ** 31, 2 ** 63 - 1
+    cut[0, 0] = cut[1, 2] = cut[2, 1] = cut[4, 0] = 24
+    a, b = ops.router_balance(z.to(dev), wide.to(dev)), ops.router_balance(z.to(dev), cut.to(dev))
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    assert ops.workspace_status(a[0]._mlxr_workspace) == 1
+    dw = torch.randn((T, 3), generator=torch.Generator().manual_seed(8)).to(dev)
+    assert torch.equal(ops.router_balance_vjp(z.to(dev), wide.to(dev), dweights=dw),
+                       ops.router_balance_vjp(z.to(dev), cut.to(dev), dweights=dw))

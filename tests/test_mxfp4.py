@@ -840,3 +840,31 @@ def test_loader_takes_a_mode_that_says_nothing(pkg, named):
                                        pre: {"group_size": 64, "bits": 8, **named}})
     assert q.mode_for_path(pre) == "affine" and q.mode_for_path("other") == "affine"
     assert q.for_path(pre) == (64, 8)
+
+
+@gpu
+@pytest.mark.parametrize("T", [5, 600])
+def test_indices_past_32_bits(pkg, dev, T):
+    """64-bit indices that no 32-bit one holds are out of range, in the plain
+    product (rows cleared) and in the modules (rows left out)."""
+    w, x, idx = ffn_inputs(6, 8, 128, 64, T, 4)
+    wide, ok = idx.long(), torch.ones((T, 4), dtype=torch.bool)
+    wide[0, 1], wide[2, 3], wide[3, 0] = 2 ** 32 + 1, 2 ** 31, -2 ** 32 + 2
+    ok[0, 1] = ok[2, 3] = ok[3, 0] = False
+    m, xd = ffn(pkg, dev, w), x.to(dev)
+    up = m.up_proj
+    kw = {"rhs_indices": wide.to(dev), "mode": "mxfp4"}
+    y = pkg.ops.gather_qmm(xd[:, None, None, :], up.weight, up.scales, **kw)
+    assert pkg.ops.workspace_status(y._mlxr_workspace) == 1
+    kw["rhs_indices"] = idx.to(dev)
+    want = pkg.ops.gather_qmm(xd[:, None, None, :], up.weight, up.scales, **kw)
+    assert torch.equal(y[ok], want[ok]) and bool((y[~ok] == 0).all())
+    gu = [torch.cat([w[0][i], w[1][i]], 1).to(dev) for i in (0, 1)]
+    packed = pkg.nn.PackedSwitchFfn(pkg.nn.QuantizedSwitchLinear(*gu, mode="mxfp4"), m.down_proj,
+                                    "swiglu")
+    for mod in (m, packed):
+        a = mod.forward(xd, idx.to(dev))
+        assert pkg.ops.workspace_status(mod.last_workspace) == 0
+        b = mod.forward(xd, wide.to(dev))
+        assert pkg.ops.workspace_status(mod.last_workspace) == 1
+        assert torch.equal(a[ok], b[ok])
