@@ -151,6 +151,13 @@ int mlxr_moe_gather_mm(const void* a, int a_dtype, int64_t a_batch, int64_t M,
  * 0 = the streaming kernel, which keeps the dequantised weights in f32.
  * Both accumulate in f32.  Returns -1 for negative sizes. */
 int mlxr_moe_gather_qmm_tiled(int64_t rows, int64_t num_experts);
+/* The same for a mode ("affine" or NULL, "mxfp4"), each with a rule of its own.
+ * Mode "mxfp4" multiplies the same weights in both kernels: there the answer
+ * says which one runs, not which numerics.  (x of 2 GB and more, or an out off
+ * 16-byte alignment, takes the streaming kernel whatever the answer.)  Returns
+ * -1 for negative sizes and other modes. */
+int mlxr_moe_gather_qmm_tiled_mode(int64_t rows, int64_t num_experts,
+                                   const char* mode);
 
 /* The summation order of a router's logits for T tokens over d inputs and
  * `columns` logit columns (the experts, plus one when a shared-expert gate

@@ -402,6 +402,15 @@ int mlxr_moe_gather_qmm_tiled(int64_t rows, int64_t num_experts) {
   return nn::use_prefill_path(rows, num_experts) ? 1 : 0;
 }
 
+int mlxr_moe_gather_qmm_tiled_mode(int64_t rows, int64_t num_experts, const char* mode) {
+  if (!is_mxfp4(mode))
+    return mode && std::strcmp(mode, "affine") != 0
+               ? fail("gather_qmm_tiled: unsupported mode")
+               : mlxr_moe_gather_qmm_tiled(rows, num_experts);
+  if (rows < 0 || num_experts < 0) return -1;
+  return nn::use_prefill_path(rows, num_experts, kBitsMxfp4) ? 1 : 0;
+}
+
 int mlxr_moe_argpartition(const float* a, int64_t rows, int64_t n, int kth,
                           int axis, uint32_t* out, mlxr_moe_stream stream) {
   if (axis != -1 && axis != 1)

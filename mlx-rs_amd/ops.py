@@ -538,12 +538,14 @@ def combine(y: torch.Tensor, weights: torch.Tensor, shared_y=None, shared_logit=
     return out
 
 
-def gather_qmm_tiled(rows: int, num_experts: int) -> bool:
+def gather_qmm_tiled(rows: int, num_experts: int, mode="affine") -> bool:
     """True when a gather_qmm of `rows` flat rows over `num_experts` experts
     runs the M-tiled kernel (weights dequantised to bf16 tiles, the
     gather_mm(x, dequantize(w)) numerics), False for the streaming kernel
-    (weights dequantised in f32)."""
-    rc = C.lib().mlxr_moe_gather_qmm_tiled(int(rows), int(num_experts))
+    (weights dequantised in f32).  Mode "mxfp4" has its own rule, and the same
+    numerics in both."""
+    _check_mode(mode)
+    rc = C.lib().mlxr_moe_gather_qmm_tiled_mode(int(rows), int(num_experts), mode.encode())
     if rc < 0:
         raise MlxrMoeError("gather_qmm_tiled: negative size")
     return bool(rc)

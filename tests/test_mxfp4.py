@@ -868,3 +868,39 @@ def test_indices_past_32_bits(pkg, dev, T):
         b = mod.forward(xd, wide.to(dev))
         assert pkg.ops.workspace_status(mod.last_workspace) == 1
         assert torch.equal(a[ok], b[ok])
+
+
+def test_rule_for_tiles(pkg):
+    """Which kernel a product of mxfp4 experts takes (host logic, no GPU): tiles
+    from 1.5 rows an expert, and with fewer than 128 experts from 16 rows an expert or 320
+    in all, with fewer than 8 from 512; the affine rule beside it is its own."""
+    q, mx = pkg.ops.gather_qmm_tiled, "mxfp4"
+    assert not q(191, 128, mx) and q(192, 128, mx)
+    assert not q(1535, 1024, mx) and q(1536, 1024, mx)
+    assert not q(127, 8, mx) and q(128, 8, mx)
+    assert not q(319, 127, mx) and q(320, 127, mx)
+    assert not q(511, 7, mx) and q(512, 7, mx)
+    assert not q(511, 1, mx) and q(512, 1, mx)
+    assert not q(0, 8, mx)
+    for rows, experts in ((192, 128), (1536, 1024), (512, 1), (511, 1), (6000, 128)):
+        assert q(rows, experts) == q(rows, experts, "affine")
+    assert not q(192, 128) and q(6000, 128)
+    with pytest.raises(pkg.MlxrMoeError, match="negative"):
+        q(-1, 8, mx)
+    with pytest.raises(pkg.MlxrMoeError, match="mode"):
+        q(1, 8, "nvfp4")
+    f = pkg._capi.lib().mlxr_moe_gather_qmm_tiled_mode
+    assert f(192, 128, b"mxfp4") == 1 and f(192, 128, b"affine") == 0 and f(192, 128, None) == 0
+    assert f(192, -1, b"mxfp4") == -1 and f(192, 128, b"nvfp4") == -1
+
+
+def test_rule_of_the_tested_sizes(pkg):
+    """The products above that are meant to run as tiles do, and those meant to
+    stay just under the rule do."""
+    q = pkg.ops.gather_qmm_tiled
+    for E, rows in ((4, 600), (8, 800), (8, 600), (16, 520), (3, 666), (5, 560), (2, 777),
+                    (128, 192), (130, 195), (128, 1200), (140, 1000), (200, 3600),
+                    (8, 640), (2, 520), (3, 6000), (5, 33000), (1024, 1800), (1024, 1600)):
+        assert q(rows, E, "mxfp4"), (E, rows)
+    for E, rows in ((11, 1), (11, 8), (11, 6), (11, 72), (11, 160), (128, 190), (140, 130)):
+        assert not q(rows, E, "mxfp4"), (E, rows)
