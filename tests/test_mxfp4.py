@@ -904,3 +904,88 @@ def test_rule_of_the_tested_sizes(pkg):
         assert q(rows, E, "mxfp4"), (E, rows)
     for E, rows in ((11, 1), (11, 8), (11, 6), (11, 72), (11, 160), (128, 190), (140, 130)):
         assert not q(rows, E, "mxfp4"), (E, rows)
+
+
+@gpu
+@pytest.mark.parametrize("E,f,T,K,tiled", [
+    (8, 128, 1, 2, False),    # the input dim in four slices
+    (4, 1024, 20, 2, False),  # two
+    (4, 1024, 80, 2, False),  # one, over 64 rows: items from a dispatch
+    (8, 192, 70, 2, True),    # 32-row tiles
+    (8, 192, 130, 2, True),   # 64-row tiles
+    (8, 192, 300, 2, True),   # 128-row tiles
+])
+def test_split_ffn_widest_input(pkg, dev, E, f, T, K, tiled):
+    """Gate and up over 4096 inputs, the most there are, in every form."""
+    d = 4096
+    w, x, idx = ffn_inputs(T + f, E, d, f, T, K)
+    assert pkg.ops.gather_qmm_tiled(T * K, E, "mxfp4") == tiled
+    m = ffn(pkg, dev, w)
+    want, bound = glu64(x.double(), [values64(*b) for b in w], idx, "swiglu")
+    y = m.forward(x.to(dev), idx.to(dev))
+    assert bool(((y.cpu().double() - want).abs() <= bound).all())
+    assert torch.equal(m.forward(x.to(dev), idx.to(dev)), y)
+
+
+@gpu
+@pytest.mark.parametrize("T", [9, 300])
+def test_packed_geglu_widest_input(pkg, dev, T):
+    E, d, f, K = 8, 4096, 128, 4
+    w, x, idx = ffn_inputs(T, E, d, f, T, K)
+    lin = lambda b: pkg.nn.QuantizedSwitchLinear(b[0].to(dev), b[1].to(dev), mode="mxfp4")  # noqa: E731
+    gu = (torch.cat([w[0][0], w[1][0]], 1), torch.cat([w[0][1], w[1][1]], 1))
+    y = pkg.nn.PackedSwitchFfn(lin(gu), lin(w[2]), "geglu").forward(x.to(dev), idx.to(dev))
+    want, bound = glu64(x.double(), [values64(*b) for b in w], idx, "geglu")
+    assert bool(((y.cpu().double() - want).abs() <= bound).all())
+
+
+def shared_inputs(T, d, f):
+    w, x, _ = ffn_inputs(T, 1, d, f, T, 1)
+    idx = torch.zeros((T, 1), dtype=torch.int32)
+    return w, x, glu64(x.double(), [values64(*b) for b in w], idx, "swiglu")
+
+
+def shared_mlp(pkg, dev, w):
+    return pkg.nn.SwigluMlp(*[pkg.nn.QuantizedLinear(q[0].to(dev), s[0].to(dev), mode="mxfp4")
+                              for q, s in w])
+
+
+@gpu
+@pytest.mark.parametrize("d,f", [(256, 192), (4096, 64)])
+@pytest.mark.parametrize("T", [1, 511, 512, 650])
+def test_one_expert(pkg, dev, T, d, f):
+    """SwigluMlp alone, just under the rule for tiles, on it and past it with a
+    ragged last tile."""
+    w, x, (want, bound) = shared_inputs(T, d, f)
+    assert pkg.ops.gather_qmm_tiled(T, 1, "mxfp4") == (T >= 512)
+    y = shared_mlp(pkg, dev, w).forward(x.to(dev))
+    assert bool(((y.cpu().double() - want[:, 0]).abs() <= bound[:, 0]).all())
+
+
+@gpu
+@pytest.mark.parametrize("T", [511, 512, 650])
+def test_block_shared_expert_of_its_own(pkg, dev, T):
+    """An mxfp4 shared expert beside affine experts has launches of its own, over
+    every token in order: the block with it less the block without it."""
+    E, d, f, K = 16, 256, 192, 4
+    nn = pkg.nn
+    g = torch.Generator().manual_seed(T)
+    w, x, (want, bound) = shared_inputs(T, d, f)
+    gate_w = (torch.randn((E, d), generator=g) * 0.1).to(dev)
+    sg = (torch.randn((1, d), generator=g) * 0.1).to(dev)
+    experts = nn.SplitSwitchFfn.from_dense(*[
+        (torch.randn(s, generator=g) * 0.05).bfloat16().to(dev)
+        for s in ((E, f, d), (E, f, d), (E, d, f))])
+    xd = x.to(dev)
+    out = nn.Qwen35MoeBlock(gate_w, experts, K, shared_mlp(pkg, dev, w), sg).forward(xd)
+    plain = nn.Qwen35MoeBlock(gate_w, experts, K).forward(xd)
+    x64, s64 = x.double(), sg.cpu().double()[0]
+    gate = torch.sigmoid(x64 @ s64)[:, None]
+    # the gate's logit is an f32 sum of d products, its sigmoid changes by a quarter
+    # of that at most and is taken in f32 (a few steps); product and sum round once each
+    egate = 0.25 * d * 2.0 ** -23 * (x64.abs() @ s64.abs())[:, None] + 2.0 ** -21
+    want, bound = want[:, 0], bound[:, 0]
+    big = want.abs() + bound
+    tol = gate * bound + egate * big + 2.0 ** -23 * (big + plain.cpu().double().abs())
+    diff = out.cpu().double() - plain.cpu().double() - gate * want
+    assert bool((diff.abs() <= tol).all())
