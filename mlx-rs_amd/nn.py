@@ -31,6 +31,22 @@ def _group_size(group_size, mode):
     return ops.MXFP4_GROUP_SIZE if mode == "mxfp4" else ops.DEFAULT_GROUP_SIZE
 
 
+def _one_device(name, *devices):
+    """The device of all of a module's tensors: the kernels get their addresses
+    as they are."""
+    if any(d != devices[0] for d in devices):
+        raise MlxrMoeError(f"{name}: weights live on different devices: "
+                           f"{', '.join(map(str, devices))}")
+    return devices[0]
+
+
+def _check_on(name, device, *ts):
+    """The call's arrays live on one ROCm device, and the weights on it too."""
+    d = ops._dev(*ts)
+    if d != device:
+        raise MlxrMoeError(f"{name}: x is on {d}, the weights on {device}")
+
+
 class SwitchLinear:
     """Expert-stacked dense linear (the unquantised MaybeQuantized slot):
     weight bf16 [E, out, in], applied with gather_mm (switch.rs:84-93).  No
@@ -44,6 +60,7 @@ class SwitchLinear:
         if weight.ndim != 3:
             raise MlxrMoeError("SwitchLinear weight must be [E, out, in]")
         self.weight = weight.to(torch.bfloat16).contiguous()
+        self.device = self.weight.device
 
     @property
     def num_experts(self):
@@ -105,6 +122,8 @@ class QuantizedSwitchLinear:
                                    f"bits 4, got {group_size} and {bits}")
         elif biases is None:
             raise MlxrMoeError("QuantizedSwitchLinear: biases are required (affine mode)")
+        self.device = _one_device("QuantizedSwitchLinear", weight.device, scales.device,
+                                  weight.device if biases is None else biases.device)
         self.weight = weight.contiguous()
         self.scales = scales.contiguous()
         if mode == "mxfp4":
@@ -207,6 +226,8 @@ class SplitSwitchFfn:
         self.gate_proj, self.up_proj, self.down_proj = gate_proj, up_proj, down_proj
         self._desc = C.SwitchGlu(gate_proj.descriptor(), up_proj.descriptor(),
                                  down_proj.descriptor())
+        self.device = _one_device("SplitSwitchFfn", gate_proj.device, up_proj.device,
+                                  down_proj.device)
         self._sizes = {}  # workspace bytes by (T, K)
 
     @classmethod
@@ -230,7 +251,7 @@ class SplitSwitchFfn:
     def _prep(self, x, indices):
         d = self.gate_proj.input_dims
         _check_x("SplitSwitchFfn", x, d)
-        ops._dev(x, indices)
+        _check_on("SplitSwitchFfn", self.device, x, indices)
         x2 = (x if x.ndim == 2 else x.reshape(-1, d)).contiguous()
         K = indices.shape[-1]
         idx = ops._as_int32(indices)
@@ -284,6 +305,7 @@ class PackedSwitchFfn:
         self.gate_up_proj, self.down_proj = gate_up_proj, down_proj
         self.activation = activation
         self.hidden_dims = gate_up_proj.output_dims // 2
+        self.device = _one_device("PackedSwitchFfn", gate_up_proj.device, down_proj.device)
         self._desc = C.PackedSwitchGlu(gate_up_proj.descriptor(), down_proj.descriptor(),
                                        C.ACT_GEGLU if activation == "geglu" else C.ACT_SWIGLU)
 
@@ -301,7 +323,7 @@ class PackedSwitchFfn:
     def _prep(self, x, indices):
         d = self.gate_up_proj.input_dims
         _check_x("PackedSwitchFfn", x, d)
-        ops._dev(x, indices)
+        _check_on("PackedSwitchFfn", self.device, x, indices)
         x2 = x.reshape(-1, d).contiguous()
         K = indices.shape[-1]
         idx = ops._as_int32(indices.reshape(-1, K))
@@ -371,6 +393,8 @@ class GemmaRouter:
         root = torch.tensor(d ** -0.5, dtype=torch.float32).to(torch.bfloat16)
         self.norm_weight = (scale * root.to(scale.device)).contiguous()
         self.per_expert_scale = per_expert_scale.to(torch.bfloat16).contiguous()
+        self.device = _one_device("GemmaRouter", self.proj.device, self.norm_weight.device,
+                                  self.per_expert_scale.device)
         z = C.QLinear()
         self._desc = C.GemmaRouter(
             d, E, top_k, eps, self.norm_weight.data_ptr(),
@@ -387,7 +411,7 @@ class GemmaRouter:
         """x bf16 [..., d] -> (indices int32 [..., K], weights bf16 [..., K])."""
         d = self.hidden_size
         _check_x("GemmaRouter", x, d)
-        ops._dev(x)
+        _check_on("GemmaRouter", self.device, x)
         x2 = x.reshape(-1, d).contiguous()
         T, K = x2.shape[0], self.top_k
         if idx is None:
@@ -416,6 +440,7 @@ class GemmaMoe:
 
     def __init__(self, router: GemmaRouter, experts: PackedSwitchFfn):
         self.router, self.experts = router, experts
+        self.device = _one_device("GemmaMoe", router.device, experts.device)
         self.last_indices = self.last_weights = self.last_workspace = None
         self._ws = None
 
@@ -426,7 +451,7 @@ class GemmaMoe:
     def forward(self, x, out=None, workspace=None, keep_routing=True):
         d = self.router.hidden_size
         _check_x("GemmaMoe", x, d)
-        ops._dev(x)
+        _check_on("GemmaMoe", self.device, x)
         x2 = x.reshape(-1, d).contiguous()
         T, K = x2.shape[0], self.router.top_k
         if workspace is None:
@@ -458,6 +483,8 @@ class SwigluMlp:
     def __init__(self, gate_proj: QuantizedLinear, up_proj: QuantizedLinear,
                  down_proj: QuantizedLinear):
         self.gate_proj, self.up_proj, self.down_proj = gate_proj, up_proj, down_proj
+        self.device = _one_device("SwigluMlp", gate_proj.device, up_proj.device,
+                                  down_proj.device)
 
     def forward(self, x):
         """SwigluMlp::forward (swiglu_mlp.rs:63-70); bf16 output.  Runs as
@@ -525,6 +552,10 @@ class Qwen35MoeBlock:
         self.hidden_size = d
         f = switch_mlp.gate_proj.output_dims
         se = shared_expert
+        self.device = _one_device(
+            "Qwen35MoeBlock", *[m.device for m in (
+                self.gate_weight, self.gate_bias, switch_mlp, se, self.shared_expert_gate_weight)
+                if m is not None])
         self._desc = C.Block(
             d, E, num_experts_per_tok, f,
             0 if se is None else se.gate_proj.output_dims,
@@ -548,7 +579,7 @@ class Qwen35MoeBlock:
         [..., d], f32 (bf16 with a quantised router)."""
         d = self.hidden_size
         _check_x("Qwen35MoeBlock", x, d)
-        ops._dev(x)
+        _check_on("Qwen35MoeBlock", self.device, x)
         x2 = x.reshape(-1, d)
         if not x2.is_contiguous():
             x2 = x2.contiguous()
@@ -592,7 +623,7 @@ class Qwen35MoeBlock:
         if norm.weight.numel() != d:
             raise MlxrMoeError(f"forward_residual: the norm weight must have {d} elements, "
                                f"got {norm.weight.numel()}")
-        ops._dev(h, norm.weight)
+        _check_on("Qwen35MoeBlock.forward_residual", self.device, h, norm.weight)
         h2 = h.reshape(-1, d).contiguous()
         T, K = h2.shape[0], self.num_experts_per_tok
         if out is None:

@@ -989,3 +989,55 @@ def test_block_shared_expert_of_its_own(pkg, dev, T):
     tol = gate * bound + egate * big + 2.0 ** -23 * (big + plain.cpu().double().abs())
     diff = out.cpu().double() - plain.cpu().double() - gate * want
     assert bool((diff.abs() <= tol).all())
+
+
+def test_weights_on_one_device(pkg):
+    """A module's tensors on different devices are refused where it is made."""
+    nn, Err = pkg.nn, pkg.MlxrMoeError
+
+    def lin(device, rows=64, cols=128, scales=None):
+        return nn.QuantizedSwitchLinear(
+            torch.zeros((4, rows, cols // 8), dtype=torch.int32, device=device),
+            torch.zeros((4, rows, cols // 32), dtype=torch.uint8, device=scales or device),
+            mode="mxfp4")
+
+    with pytest.raises(Err, match="different devices"):
+        lin("cpu", scales="meta")
+    up, down = lin("cpu"), lin("cpu", 128, 64)
+    with pytest.raises(Err, match="different devices"):
+        nn.SplitSwitchFfn(up, lin("meta"), down)
+    with pytest.raises(Err, match="different devices"):
+        nn.PackedSwitchFfn(lin("cpu", 128, 128), lin("meta", 128, 64))
+    m = nn.SplitSwitchFfn(up, up, down)
+    assert m.device == torch.device("cpu")
+    with pytest.raises(Err, match="different devices"):
+        nn.Qwen35MoeBlock(torch.zeros((4, 128), device="meta"), m, 2)
+    with pytest.raises(Err, match="ROCm device"):
+        m.forward(torch.zeros((1, 128)).bfloat16(), torch.zeros((1, 2), dtype=torch.int32))
+
+
+@gpu
+def test_weights_on_the_host_are_refused(pkg, dev, tmp_path):
+    """Modules made on the host (a checkpoint opened there) take no call."""
+    nn, Err = pkg.nn, pkg.MlxrMoeError
+    w, x, idx = ffn_inputs(1, 8, 256, 128, 3, 4)
+    x, idx = x.to(dev), idx.to(dev)
+    m = ffn(pkg, torch.device("cpu"), w)
+    wts = torch.ones((3, 4), device=dev)
+    gu = [torch.cat([w[0][i], w[1][i]], 1) for i in (0, 1)]
+    packed = nn.PackedSwitchFfn(nn.QuantizedSwitchLinear(*gu, mode="mxfp4"), m.down_proj)
+    for mod in (m, packed):
+        for call in (lambda: mod.forward(x, idx), lambda: mod.forward_with_combine(x, idx, wts)):
+            with pytest.raises(Err, match="weights on cpu"):
+                call()
+    one = [nn.QuantizedLinear(q[0], s[0], mode="mxfp4") for q, s in w]
+    with pytest.raises(Err, match="weights on cpu"):
+        nn.SwigluMlp(*one).forward(x)
+    with pytest.raises(Err, match="ROCm device"):
+        one[0].forward(x)
+    write_checkpoint(tmp_path)
+    block = pkg.loader.qwen35_moe_block(tmp_path, 2, "cpu")
+    with pytest.raises(Err, match="weights on cpu"):
+        block.forward(x)
+    with pytest.raises(Err, match="weights on cpu"):
+        block.forward_residual(x, nn.RmsNorm(torch.ones(256, device=dev)))
