@@ -378,14 +378,26 @@ def softmax_axis(a: torch.Tensor, axis: int, precise=None):
     return out.movedim(-1, ax)
 
 
+def _router_rows(name, x, d):
+    """x bf16 [.., d] as rows: the C ABI reads T * d elements of that type."""
+    if x.dtype != torch.bfloat16:
+        raise MlxrMoeError(f"{name}: x must be bfloat16, got {x.dtype}")
+    if x.ndim < 1 or x.shape[-1] != d:
+        raise MlxrMoeError(f"{name}: x last dim must be {d}, got {tuple(x.shape)}")
+    return x.reshape(-1, d).contiguous()
+
+
 def router_topk(x: torch.Tensor, gate_w: torch.Tensor, k: int, return_logits=False):
     """softmax(x @ gate_w^T) -> top-k -> renormalise (moe.rs:122-138).
     Returns (indices int32 [T, k], weights f32 [T, k]), and with
     return_logits the f32 logits [T, E] too (what router_balance takes)."""
+    if gate_w.ndim != 2 or gate_w.dtype != torch.float32:
+        raise MlxrMoeError(f"router_topk: gate_w must be float32 [E, d], got {gate_w.dtype} "
+                           f"{tuple(gate_w.shape)}")
+    E, d = gate_w.shape
+    x2 = _router_rows("router_topk", x, d)
     _dev(x, gate_w)
-    x2 = x.reshape(-1, x.shape[-1]).contiguous()
-    T, d = x2.shape
-    E = gate_w.shape[0]
+    T = x2.shape[0]
     idx = torch.empty((T, k), dtype=torch.int32, device=x.device)
     wts = torch.empty((T, k), dtype=torch.float32, device=x.device)
     lib = C.lib()
@@ -410,8 +422,8 @@ def router_topk_quantized(x: torch.Tensor, gate, k: int, return_logits=False):
     (nn.Linear): bf16 logits and probabilities, top-k on the probabilities.
     Returns (indices int32 [T, k], weights [T, k] -- bf16 values held in
     f32), and with return_logits the logits [T, E] (bf16 values in f32)."""
+    x2 = _router_rows("router_topk_quantized", x, gate.input_dims)
     _dev(x, gate.weight)
-    x2 = x.reshape(-1, x.shape[-1]).contiguous()
     T = x2.shape[0]
     idx = torch.empty((T, k), dtype=torch.int32, device=x.device)
     wts = torch.empty((T, k), dtype=torch.float32, device=x.device)

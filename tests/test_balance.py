@@ -498,3 +498,75 @@ def test_indices_past_32_bits(pkg, dev, T):
     dw = torch.randn((T, 3), generator=torch.Generator().manual_seed(8)).to(dev)
     assert torch.equal(ops.router_balance_vjp(z.to(dev), wide.to(dev), dweights=dw),
                        ops.router_balance_vjp(z.to(dev), cut.to(dev), dweights=dw))
+
+
+def test_routers_refuse_other_types_and_widths(pkg):
+    """What the kernels would read past its end, or as another type."""
+    ops, nn, Err = pkg.ops, pkg.nn, pkg.MlxrMoeError
+    x, gate = torch.zeros(4, 64).bfloat16(), torch.zeros(8, 64)
+    with pytest.raises(Err, match="gate_w must be float32"):
+        ops.router_topk(x, gate.bfloat16(), 2)
+    with pytest.raises(Err, match="gate_w must be float32"):
+        ops.router_topk(x, gate[0], 2)
+    with pytest.raises(Err, match="last dim must be 32"):
+        ops.router_topk(x, gate[:, :32], 2)
+    with pytest.raises(Err, match="x must be bfloat16"):
+        ops.router_topk(x.float(), gate, 2)
+    with pytest.raises(Err, match="ROCm device"):
+        ops.router_topk(x, gate, 2)
+    bf = nn.Linear(gate.bfloat16())
+    with pytest.raises(Err, match="last dim must be 64"):
+        ops.router_topk_quantized(x[:, :32], bf, 2)
+    with pytest.raises(Err, match="x must be bfloat16"):
+        ops.router_topk_quantized(x.float(), bf, 2)
+    with pytest.raises(Err, match="ROCm device"):
+        ops.router_topk_quantized(x, bf, 2)
+
+
+@gpu
+@pytest.mark.parametrize("T,E,d,K", [(1, 8, 128, 2), (33, 60, 512, 4), (1536, 128, 2048, 8)])
+@pytest.mark.parametrize("form", ["f32", "q8", "q4", "bf16"])
+def test_logits_a_router_returns(pkg, dev, T, E, d, K, form):
+    """Every router form's logits are the products its choices were made of:
+    bf16 values where the router is one of bf16, the choices their largest, the
+    weights the softmax of those."""
+    ops, nn = pkg.ops, pkg.nn
+    g = torch.Generator().manual_seed(T + E)
+    x = torch.randn((T, d), generator=g).bfloat16().to(dev)
+    w = (torch.randn((E, d), generator=g) * 0.05).to(dev)
+    if form == "f32":
+        idx, wts, z = ops.router_topk(x, w, K, return_logits=True)
+    else:
+        lin = nn.Linear(w.bfloat16())
+        w = lin.weight[0]
+        if form != "bf16":
+            lin = nn.QuantizedLinear.try_from_linear(w, bits=int(form[1]))
+            w = ops.dequantize(lin.weight[0], lin.scales[0], lin.biases[0], bits=lin.bits,
+                               out_dtype=torch.float32)
+        idx, wts, z = ops.router_topk_quantized(x, lin, K, return_logits=True)
+        assert torch.equal(z.bfloat16().float(), z)
+    assert z.shape == (T, E) and z.dtype == torch.float32
+    want, mass = x.double() @ w.double().t(), x.double().abs() @ w.double().abs().t()
+    # an f32 sum of d products and one rounding to bf16; quantised, codes times scale and
+    # biases may be summed apart, their magnitudes |w| + 2 |bias| at most
+    if form[0] == "q":
+        bias = lin.biases[0].double().abs().repeat_interleave(64, 1)
+        mass = mass + 2 * x.double().abs() @ bias.t()
+    tol = (d + 4) * 2.0 ** -23 * mass
+    if form != "f32":
+        tol = tol + 2.0 ** -8 * (want.abs() + tol)
+    assert bool(((z.double() - want).abs() <= tol).all())
+    # the choices: no other expert's probability is larger, but by two roundings of them
+    # to bf16 where the router works in that
+    p = torch.softmax(z.double(), 1)
+    top = p.gather(1, idx.long())
+    half = 0.0 if form == "f32" else 2.0 ** -8
+    room = (1.0 + half) / (1.0 - half) * (1.0 + 2 * rel_p(z.cpu(), None))
+    rest = p.scatter(1, idx.long(), 0.0).amax(1)
+    assert bool((rest <= top.amin(1) * room).all())
+    # the weights from these logits: each probability, their sum and the quotient rounded
+    rel = 2 * rel_p(z.cpu(), None) + (K + 3) * (2.0 ** -24 if form == "f32" else 2.0 ** -8)
+    want = top / top.sum(1, keepdim=True)
+    assert bool(((wts.double() - want).abs() <= rel * want).all())
+    # and on to the balance loss
+    check_forward(ops, dev, z.cpu(), idx.cpu(), None)
