@@ -78,13 +78,12 @@ __device__ __forceinline__ void load_row(const void* z, int64_t ld, int64_t t, i
     v[j] = e < E ? logit<BF16>(z, t * ld + e) : -INFINITY;
   }
 }
-// Whether logits of maximum m over the wave are all -inf (the same on every lane).
-// fmaxf leaves NaN out of a maximum, so one of -inf may hide it behind the -inf of
-// experts that are shut off and of lanes past the end; nan: this lane holds one.
-// A NaN beside a larger maximum needs no look: the softmax's sum takes it up.
-__device__ __forceinline__ bool no_softmax(float m, bool nan) {
-  return m == -INFINITY && !__any(nan);
-}
+// What the exponents of a softmax are taken against, for logits of maximum m.  fmaxf
+// leaves NaN out of a maximum, so one of -inf may hide it behind the -inf of experts
+// that are shut off and of lanes past the end: against 0 all of those come to 0 and NaN
+// stays NaN, so the sum tells a row of nothing (0) from one of NaN.  (Any other sum is 1
+// at least.)
+__device__ __forceinline__ float softmax_base(float m) { return m == -INFINITY ? 0.0f : m; }
 // v := softmax over the wave (0 everywhere where all logits are -inf).  NaN or +inf
 // make the row NaN.
 template <int SLOTS>
@@ -92,11 +91,7 @@ __device__ __forceinline__ void softmax_row(float (&v)[SLOTS]) {
   float m = v[0];
 #pragma unroll
   for (int j = 1; j < SLOTS; ++j) m = fmaxf(m, v[j]);
-  m = wave_max(m);
-  bool nan = false;
-#pragma unroll
-  for (int j = 0; j < SLOTS; ++j) nan |= v[j] != v[j];
-  const bool none = no_softmax(m, nan);
+  m = softmax_base(wave_max(m));
   float s = 0.0f;
 #pragma unroll
   for (int j = 0; j < SLOTS; ++j) {
@@ -104,9 +99,9 @@ __device__ __forceinline__ void softmax_row(float (&v)[SLOTS]) {
     s += v[j];
   }
   s = wave_add(s);
-  const float inv = 1.0f / s;
+  const float inv = s == 0.0f ? 0.0f : 1.0f / s;
 #pragma unroll
-  for (int j = 0; j < SLOTS; ++j) v[j] = none ? 0.0f : v[j] * inv;
+  for (int j = 0; j < SLOTS; ++j) v[j] *= inv;
 }
 
 struct BalanceArgs {
@@ -341,11 +336,10 @@ __global__ __launch_bounds__(64 * kWaves) void balance_vjp_kernel(
         ek = in ? e : -1;
         const float zk = in ? logit<BF16>(a.z, t * a.ld + e) : -INFINITY;
         const float dk = in ? dw[i] : 0.0f;
-        const float m = wave_max(zk);
-        const bool none = no_softmax(m, zk != zk);
-        const float u = in && !none ? __builtin_amdgcn_exp2f((zk - m) * kLog2e) : 0.0f;
+        const float m = softmax_base(wave_max(zk));
+        const float u = in ? __builtin_amdgcn_exp2f((zk - m) * kLog2e) : 0.0f;
         const float s = wave_add(u);
-        const float w = none ? 0.0f : u / s;
+        const float w = s == 0.0f ? 0.0f : u / s;
         gk = w * (dk - wave_add(w * dk));
         // one expert chosen twice: its first lane takes the sum, in order
         first = in;
