@@ -50,7 +50,7 @@ COMMON = [
     "-std=c++17",
     "-fPIC",
     f"--offload-arch={ARCH}",
-    # packed fp32 VALU ops stay off on this hardware pool
+    # packed fp32 VALU ops stay off: some of their forms have given wrong results
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     # every multiply and add rounds separately unless the source calls fmaf
     # (hipcc's default would fuse them): the combine and softmax then match

@@ -333,8 +333,11 @@ hipError_t launch_mx_stream(const QGemmArgs& a, int64_t max_items, const QGemmAr
   const int nm = a.gated ? 2 : 1;
   const size_t x_lds = ((size_t)kWorkRows * (128 * S + 8) * 2 + 15) & ~size_t(15);
   // slices of the input dim, four steps each at least, while the workgroups, which
-  // all stage the whole x, still run at once (their LDS: about four a CU up to K = 2048, two
-  // above; 1, 2 and 4 slices, c5 T=1 up 18, 12.0 and 16.4 us, c5 T=2 up 14.6, 18.3 and
+  // all stage the whole x, are no more than four a CU up to K = 2048, two above.  (So many
+  // run at once where a product is not gated and x is whole: 37 and 74 KB of LDS.  The
+  // limit is a count of workgroups all the same: gated ones take 41 KB at K = 2048 and 82
+  // at 4096, so three and one of them fit a CU, and those of a launch near the limit run
+  // in rounds.  1, 2 and 4 slices, c5 T=1 up 18, 12.0 and 16.4 us, c5 T=2 up 14.6, 18.3 and
   // 20.8, c2 T=4 gate/up 14.2, 13.7 and 16.8, c2 T=2 10.6 with two and 10.1 with four;
   // shorter slices lose, down of c2 T=1 6.0 and 6.7 with two)
   const int64_t slots = 256 * (x_lds <= 36 * 1024 ? 4 : 2);

@@ -467,7 +467,10 @@ def router_balance(logits: torch.Tensor, indices: torch.Tensor, mask=None):
     choices that fell on expert e and P_e its mean probability, over the
     tokens whose mask (bool or uint8, None: all) is not zero.  Returns (loss
     f32 [], counts int32 [E], probs f32 [E], tokens int32 []).  An index out
-    of range is not counted and sets the workspace's status word."""
+    of range is not counted and sets the workspace's status word.  The f_e sum
+    to 1: a coefficient meant for shares of the tokens, which sum to K, is to
+    be multiplied by K.  Not recorded by autograd: the gradient is
+    router_balance_vjp's."""
     z, ld, idx, mask = _balance_inputs("router_balance", logits, indices, mask)
     (T, E), K = z.shape, idx.shape[1]
     dev = z.device
