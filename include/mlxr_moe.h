@@ -318,7 +318,9 @@ int mlxr_moe_switch_glu_forward(const mlxr_moe_switch_glu* ffn, const void* x,
                                 mlxr_moe_stream stream);
 
 /* SplitSwitchFfn::forward (switch.rs:417-442): per-expert outputs
- * y bf16 [T, K, d] before the combine.  Same workspace size as
+ * y bf16 [T, K, d] before the combine; zeros where an index names no expert
+ * (out of range, or -1, which sets no status), and the combine goes without
+ * those rows.  Same workspace size as
  * mlxr_moe_switch_glu_forward. */
 int mlxr_moe_switch_glu_experts(const mlxr_moe_switch_glu* ffn, const void* x,
                                 int64_t T, const int32_t* indices, int64_t K,

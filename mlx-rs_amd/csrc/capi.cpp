@@ -226,8 +226,8 @@ int run_gather(const char* op, const void* x, int64_t x_batch, int64_t M,
       a.row_map = nullptr;
       a.row_div = d.div;
     }
-    st = from_hip(launch_mx_sort(d, prefill_tile_rows(R, E, bits), N, db, map ? xrow : nullptr,
-                                 ob, s),
+    st = from_hip(launch_mx_sort(d, prefill_tile_rows(R, E, bits), db, map ? xrow : nullptr,
+                                 LeftOut{ob, N}, s),
                   (o + " dispatch").c_str());
     if (!st.ok) return finish(st);
     return finish(from_hip(launch_qgemm(a, R, dispatch_max_work(R, E), true, s), op));

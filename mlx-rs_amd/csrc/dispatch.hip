@@ -219,10 +219,23 @@ __global__ __launch_bounds__(kDispatchBlock) void dispatch_rank_scan_kernel(
   if (last) dispatch_scan_body<true>(n, E, (int)gridDim.x, tile_rows, b, ss);
 }
 
+// Clearing workgroup `group` (clear_groups of them) beside a sort of ids [n].
+__device__ __forceinline__ void clear_left_out(int group, const int32_t* ids, int n, int E,
+                                               LeftOut left) {
+  const int wave = group * kWaves + (int)(threadIdx.x >> 6);
+  clear_rows<kClearRows>((int64_t)kClearRows * wave, n, left.y, left.N,
+                         [&](int64_t f) { return (uint32_t)ids[f] < (uint32_t)E; });
+}
+
 // Every workgroup of the rank pass again: sorted/inv and the flat rows of
-// the work records, from the offsets and per-workgroup prefixes.
+// the work records, from the offsets and per-workgroup prefixes.  Workgroups
+// from nb on clear the rows of left.y that no expert takes.
 __global__ __launch_bounds__(kDispatchBlock) void dispatch_scatter_kernel(
-    const int32_t* __restrict__ ids, int n, int E, DispatchBuffers b) {
+    const int32_t* __restrict__ ids, int n, int E, int nb, DispatchBuffers b, LeftOut left) {
+  if ((int)blockIdx.x >= nb) {
+    clear_left_out((int)blockIdx.x - nb, ids, n, E, left);
+    return;
+  }
   const int64_t i = (int64_t)blockIdx.x * kDispatchBlock + threadIdx.x;
   if (i >= n) return;
   const int e = ids[i];
@@ -237,12 +250,17 @@ __global__ __launch_bounds__(kDispatchBlock) void dispatch_scatter_kernel(
     b.work[kWorkInts * (b.work_first[e] + (r >> work_shift(b.work_rows))) + 4 + t] = (int32_t)i;
 }
 
-// n <= 1024 ids: the whole sort in one workgroup.
+// n <= 1024 ids: the whole sort in one workgroup.  Workgroups after it clear the
+// rows of left.y that no expert takes (one would take 80 us for 1024 rows of 4 KB).
 template <int WR>
 __global__ __launch_bounds__(kDispatchBlock) void dispatch_small_kernel(
     const int32_t* __restrict__ ids, int n, int E, int tile_rows,
-    DispatchBuffers b, int reset_status) {
+    DispatchBuffers b, int reset_status, LeftOut left) {
   __shared__ DispatchScratch ls;
+  if (blockIdx.x > 0) {
+    clear_left_out((int)blockIdx.x - 1, ids, n, E, left);
+    return;
+  }
   if (reset_status && threadIdx.x == 0) *b.status = 0;
   __syncthreads();
   const int id = (int)threadIdx.x < n ? ids[threadIdx.x] : -1;
@@ -432,15 +450,16 @@ int64_t dispatch_max_tiles(int64_t n, int64_t E, int tile_rows) {
 
 hipError_t launch_dispatch(const int32_t* ids, int64_t n, int64_t E,
                            int tile_rows, const DispatchBuffers& b,
-                           bool reset_status, hipStream_t s, int32_t* counter) {
+                           bool reset_status, hipStream_t s, int32_t* counter, LeftOut left) {
   ProfileScope prof("dispatch", s);
   if (n <= kDispatchBlock) {
+    const unsigned grid = 1 + (left.y ? clear_groups(n) : 0);
     if (b.work_rows == kWorkRowsWide)
-      dispatch_small_kernel<kWorkRowsWide><<<1, kDispatchBlock, 0, s>>>(
-          ids, (int)n, (int)E, tile_rows, b, reset_status ? 1 : 0);
+      dispatch_small_kernel<kWorkRowsWide><<<grid, kDispatchBlock, 0, s>>>(
+          ids, (int)n, (int)E, tile_rows, b, reset_status ? 1 : 0, left);
     else
-      dispatch_small_kernel<kWorkRows><<<1, kDispatchBlock, 0, s>>>(
-          ids, (int)n, (int)E, tile_rows, b, reset_status ? 1 : 0);
+      dispatch_small_kernel<kWorkRows><<<grid, kDispatchBlock, 0, s>>>(
+          ids, (int)n, (int)E, tile_rows, b, reset_status ? 1 : 0, left);
     return hipGetLastError();
   }
   const int nb = (int)((n + kDispatchBlock - 1) / kDispatchBlock);
@@ -455,7 +474,8 @@ hipError_t launch_dispatch(const int32_t* ids, int64_t n, int64_t E,
     dispatch_scan_kernel<<<1, kDispatchBlock, 0, s>>>((int)n, (int)E, nb,
                                                       tile_rows, b);
   }
-  dispatch_scatter_kernel<<<nb, kDispatchBlock, 0, s>>>(ids, (int)n, (int)E, b);
+  const unsigned clears = left.y ? clear_groups(n) : 0;
+  dispatch_scatter_kernel<<<nb + clears, kDispatchBlock, 0, s>>>(ids, (int)n, (int)E, nb, b, left);
   return hipGetLastError();
 }
 

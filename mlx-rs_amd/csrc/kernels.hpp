@@ -169,9 +169,15 @@ hipError_t launch_zero_status(int32_t* status, hipStream_t s, int32_t* counter =
 // Ids equal to -1 are left out silently (rows excluded by the caller);
 // other ids outside [0, E) are left out and set *status = 1.  n above 1024
 // takes three kernels (rank, scan, scatter).
+// With left.y, rows of y [n, N] (N % 8 == 0) that are left out are cleared.
+struct LeftOut {
+  uint16_t* y;
+  int64_t N;
+};
 hipError_t launch_dispatch(const int32_t* ids, int64_t n, int64_t E,
                            int tile_rows, const DispatchBuffers& b,
-                           bool reset_status, hipStream_t s, int32_t* counter = nullptr);
+                           bool reset_status, hipStream_t s, int32_t* counter = nullptr,
+                           LeftOut left = {});
 // With counter (an int that is 0 when the launch starts, or cleared here with
 // reset_status), more than 1024 ids rank and scan in one launch (the last
 // workgroup to finish scans).
@@ -395,20 +401,19 @@ struct MxIds {
   int32_t n, M, div, E;
   int32_t x_batch;      // bound on lhs
   bool skip_minus1;     // an id of -1 is no error
-  bool zero_bad;        // rows of indices out of range are cleared
+  bool zero_bad;        // (mx_stream) rows that no expert takes are cleared
 };
 hipError_t launch_mx_stream(const QGemmArgs& a, int64_t max_items, const QGemmArgs* shared,
                             int64_t shared_rows, const char* profile, hipStream_t s,
                             const MxIds* ids = nullptr);
 // The tile kernel's part of a dispatch (offsets, sorted, tiles, num_tiles; the
 // other buffers are not written) of the rows of ids, in one launch; with xrow each
-// row's x row too, and with ids.zero_bad rows of bad indices of out [n, N] (16-byte
-// aligned, N % 64 == 0) cleared.
+// row's x row too, and with left.y the rows of y [n, N] that no expert takes cleared.
 // At most kMxSortRows rows: 20480 take 12.5 us (the general dispatch's launches 16),
 // 32768 17.4 (17).
 constexpr int kMxSortRows = 24576;
-hipError_t launch_mx_sort(const MxIds& ids, int tile_rows, int64_t N, const DispatchBuffers& b,
-                          int32_t* xrow, uint16_t* out, hipStream_t s);
+hipError_t launch_mx_sort(const MxIds& ids, int tile_rows, const DispatchBuffers& b,
+                          int32_t* xrow, LeftOut left, hipStream_t s);
 hipError_t launch_mx_tile(const QGemmArgs& a, int64_t x_rows, int tile_rows, int64_t max_tiles,
                           const QGemmArgs* shared, int64_t shared_rows, const char* profile,
                           hipStream_t s);

@@ -67,8 +67,8 @@ struct Item {
 // The item of this workgroup from the ids, each wave for itself: equal ids form
 // an expert's rows, every TT-th of them starts an item; items are in the order of
 // those.  False without one.  Ids outside [0, E) are no one's: workgroup 0 sets the
-// status word, and with zero_bad every first item's workgroup clears their rows of
-// its channels [ch0, ch0 + chs).
+// status word (skip_minus1: not for -1), and with zero_bad every first item's
+// workgroup clears their rows of its channels [ch0, ch0 + chs).
 __device__ __forceinline__ bool find_item(const MxIds& d, int ai, bool status, int ch0, int chs,
                                           uint16_t* out, int64_t out_ld, Item& it) {
   constexpr int TT = kWorkRows;
@@ -90,8 +90,8 @@ __device__ __forceinline__ bool find_item(const MxIds& d, int ai, bool status, i
   if (ai == 0) {
     const uint64_t bad = __ballot(row && !ok && !(d.skip_minus1 && id == -1));
     if (status && d.status && threadIdx.x == 0) *d.status = bad != 0;
-    if (d.zero_bad && bad) {
-      const uint64_t all = __ballot(row && !ok);
+    const uint64_t all = __ballot(row && !ok);
+    if (d.zero_bad && all) {
       for (int r = 0; r < d.n; ++r)
         if ((all >> r) & 1)
           for (int i = threadIdx.x; i < chs; i += 64 * kWaves) out[r * out_ld + ch0 + i] = 0;

@@ -319,6 +319,9 @@ Status SwitchFfn::forward(const uint16_t* x, int64_t T, const int32_t* indices,
   const int64_t E = sw_.E;
   const int64_t n = T * K;
   DispatchBuffers db = carve_dispatch(ws, n, E, status);
+  // rows of choices that name no expert: no product writes them, every reader (the
+  // combine too) finds zeros
+  const LeftOut left{y, sw_.d};
   if (sw_.bits == kBitsMxfp4 && n <= kMxIdsRows && !use_prefill_path(n, E, sw_.bits))
     return experts_direct(x, T, K, indices, y, ws, status, s);
   if (sw_.bits == kBitsMxfp4 && n <= kMxSortRows && use_prefill_path(n, E, sw_.bits) &&
@@ -332,8 +335,8 @@ Status SwitchFfn::forward(const uint16_t* x, int64_t T, const int32_t* indices,
     ids.M = 1;
     ids.E = (int32_t)E;
     ids.skip_minus1 = true;
-    const Status so = from_hip(launch_mx_sort(ids, prefill_tile_rows(n, E, sw_.bits), 0, db,
-                                              nullptr, nullptr, s),
+    const Status so = from_hip(launch_mx_sort(ids, prefill_tile_rows(n, E, sw_.bits), db,
+                                              nullptr, left, s),
                                "switch_mlp dispatch");
     if (!so.ok) return so;
     return experts(x, T, K, db, y, ws, s, nullptr, dc, combined);
@@ -342,7 +345,7 @@ Status SwitchFfn::forward(const uint16_t* x, int64_t T, const int32_t* indices,
   // (the dispatch clears *status first: no launch of its own for that)
   Status st = from_hip(
       launch_dispatch(indices, n, E, prefill_tile_rows(n, E, sw_.bits), db, true, s,
-                      sw_.bits == kBitsMxfp4 ? status + 1 : nullptr),
+                      sw_.bits == kBitsMxfp4 ? status + 1 : nullptr, left),
       "switch_mlp dispatch");
   if (!st.ok) return st;
   return experts(x, T, K, db, y, ws, s, nullptr, dc, combined);
@@ -383,6 +386,7 @@ Status SwitchFfn::experts_direct(const uint16_t* x, int64_t T, int64_t K,
   h.out_ld = sw_.d;
   ids.status = nullptr;
   ids.div = 1;
+  ids.zero_bad = true;
   return from_hip(launch_mx_stream(h, items, nullptr, 0, "qgemm_down", s, &ids),
                   "switch_mlp down");
 }

@@ -1041,3 +1041,58 @@ def test_weights_on_the_host_are_refused(pkg, dev, tmp_path):
         block.forward(x)
     with pytest.raises(Err, match="weights on cpu"):
         block.forward_residual(x, nn.RmsNorm(torch.ones(256, device=dev)))
+
+
+@gpu
+@pytest.mark.parametrize("mode", ["affine", "mxfp4"])
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("T", [1, 3, 40, 300, 600, 7000])
+def test_rows_left_out_are_zero(pkg, dev, T, packed, mode):
+    """Choices that name no expert, -1 or out of range: their rows of the expert
+    outputs are zeros and the weighted sum goes without them, whatever outputs and
+    workspace held before; from one token to more rows than the tiles' sort takes."""
+    E, d, f, K = 8, 256, 128, 4
+    C, lib = pkg._capi, pkg._capi.lib()
+    g = torch.Generator().manual_seed(T)
+    w = [(torch.randn(s, generator=g) * 0.05).bfloat16().to(dev)
+         for s in ((E, f, d), (E, f, d), (E, d, f))]
+    if packed:
+        m = pkg.nn.PackedSwitchFfn.from_dense(torch.cat(w[:2], 1), w[2], mode=mode)
+        experts, forward = lib.mlxr_moe_packed_switch_glu_experts, \
+            lib.mlxr_moe_packed_switch_glu_forward
+    else:
+        m = pkg.nn.SplitSwitchFfn.from_dense(*w, mode=mode)
+        experts, forward = lib.mlxr_moe_switch_glu_experts, lib.mlxr_moe_switch_glu_forward
+    x = torch.randn((T, d), generator=g).bfloat16().to(dev)
+    full = torch.randint(0, E, (T, K), generator=g, dtype=torch.int32)
+    out_of = torch.rand((T, K), generator=g) < 0.3
+    out_of[0, 1], out_of[0, 0] = True, False
+    out_of[T // 2 + 1:T // 2 + 20] = True  # tokens without any expert
+    wts = torch.randn((T, K), generator=g).to(dev)
+    want = m.forward(x, full.to(dev))
+    n = lib.mlxr_moe_packed_switch_glu_workspace_size if packed else \
+        lib.mlxr_moe_switch_glu_workspace_size
+    ws = torch.empty(n(ctypes.byref(m.descriptor()), T, K), dtype=torch.uint8, device=dev)
+    stream = torch.cuda.current_stream().cuda_stream
+    for value, status in ((-1, 0), (E + 3, 1), (-7, 1)):
+        idx = torch.where(out_of, value, full).to(dev)
+        y = torch.full((T, K, d), float("nan"), dtype=torch.bfloat16, device=dev)
+        ws.fill_(255)
+        C.check(experts(ctypes.byref(m.descriptor()), x.data_ptr(), T, idx.data_ptr(), K,
+                        y.data_ptr(), ws.data_ptr(), ws.numel(), stream))
+        assert pkg.ops.workspace_status(ws) == status
+        assert bool((y[out_of] == 0).all())
+        # (the kernels may group the rows that are left in another form: an f32 sum and a
+        # bf16 step of it)
+        keep = ~out_of
+        gap = (y[keep].double() - want[keep].double()).abs()
+        assert float(gap.norm()) <= 2.0 ** -7 * float(want[keep].double().norm())
+        out = torch.full((T, d), float("nan"), device=dev)
+        ws.fill_(255)
+        kind = (C.FLOAT32,) if packed else ()
+        C.check(forward(ctypes.byref(m.descriptor()), x.data_ptr(), T, idx.data_ptr(),
+                        wts.data_ptr(), *kind, K, out.data_ptr(), ws.data_ptr(), ws.numel(),
+                        stream))
+        terms = y.double() * wts.double()[:, :, None]
+        assert bool(((out.double() - terms.sum(1)).abs()
+                     <= 2 * K * 2.0 ** -24 * terms.abs().sum(1)).all())
