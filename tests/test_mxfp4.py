@@ -1096,3 +1096,26 @@ def test_rows_left_out_are_zero(pkg, dev, T, packed, mode):
         terms = y.double() * wts.double()[:, :, None]
         assert bool(((out.double() - terms.sum(1)).abs()
                      <= 2 * K * 2.0 ** -24 * terms.abs().sum(1)).all())
+
+
+@gpu
+@pytest.mark.parametrize("T", [3, 40, 300])
+def test_outputs_at_any_address(pkg, dev, T):
+    """Expert outputs at an address the tiles do not take (two bytes past an
+    aligned one): the streaming kernel runs, and rows left out are cleared too."""
+    E, d, f, K = 8, 256, 128, 4
+    C, lib = pkg._capi, pkg._capi.lib()
+    w, x, idx = ffn_inputs(T, E, d, f, T, K)
+    want, bound = glu64(x.double(), [values64(*b) for b in w], idx, "swiglu")
+    m, xd = ffn(pkg, dev, w), x.to(dev)
+    cut = torch.zeros((T, K), dtype=torch.bool)
+    cut[T // 2, 1] = cut[T - 1] = True
+    store = torch.full((1 + T * K * d,), float("nan"), dtype=torch.bfloat16, device=dev)
+    ws = torch.empty(m.workspace_size(T, K), dtype=torch.uint8, device=dev)
+    ids = torch.where(cut, -1, idx).to(dev)
+    C.check(lib.mlxr_moe_switch_glu_experts(
+        ctypes.byref(m.descriptor()), xd.data_ptr(), T, ids.data_ptr(), K, store[1:].data_ptr(),
+        ws.data_ptr(), ws.numel(), torch.cuda.current_stream().cuda_stream))
+    y = store[1:].view(T, K, d).cpu().double()
+    assert bool(torch.isnan(store[0])) and bool((y[cut] == 0).all())
+    assert bool(((y - want).abs() <= bound)[~cut].all())
