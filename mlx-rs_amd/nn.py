@@ -340,9 +340,10 @@ class PackedSwitchFfn:
         T, d = x2.shape
         y = torch.empty((T, K, d), dtype=torch.bfloat16, device=x.device)
         ws = ops.workspace(self.workspace_size(T, K), x.device)
-        C.check(C.lib().mlxr_moe_packed_switch_glu_experts(
-            ctypes.byref(self._desc), _ptr(x2), T, _ptr(idx), K, _ptr(y), _ptr(ws), ws.numel(),
-            ops._stream(x)))
+        with ops._on(x):
+            C.check(C.lib().mlxr_moe_packed_switch_glu_experts(
+                ctypes.byref(self._desc), _ptr(x2), T, _ptr(idx), K, _ptr(y), _ptr(ws), ws.numel(),
+                ops._stream(x)))
         self.last_workspace = ws
         return y.reshape(tuple(indices.shape) + (d,))
 
@@ -363,10 +364,11 @@ class PackedSwitchFfn:
             _check_out("PackedSwitchFfn", out, T, d, odt, x.device)
         if workspace is None:
             workspace = ops.workspace(self.workspace_size(T, K), x.device)
-        C.check(C.lib().mlxr_moe_packed_switch_glu_forward(
-            ctypes.byref(self._desc), _ptr(x2), T, _ptr(idx), _ptr(w),
-            C.BFLOAT16 if bf16 else C.FLOAT32, K, _ptr(out), _ptr(workspace), workspace.numel(),
-            ops._stream(x)))
+        with ops._on(x):
+            C.check(C.lib().mlxr_moe_packed_switch_glu_forward(
+                ctypes.byref(self._desc), _ptr(x2), T, _ptr(idx), _ptr(w),
+                C.BFLOAT16 if bf16 else C.FLOAT32, K, _ptr(out), _ptr(workspace), workspace.numel(),
+                ops._stream(x)))
         self.last_workspace = workspace
         return out.reshape(tuple(x.shape[:-1]) + (d,))
 
@@ -420,9 +422,10 @@ class GemmaRouter:
             weights = torch.empty((T, K), dtype=torch.bfloat16, device=x.device)
         if workspace is None:
             workspace = ops.workspace(self.workspace_size(T), x.device)
-        C.check(C.lib().mlxr_moe_gemma_router_forward(
-            ctypes.byref(self._desc), _ptr(x2), T, _ptr(idx), _ptr(weights), _ptr(workspace),
-            workspace.numel(), ops._stream(x)))
+        with ops._on(x):
+            C.check(C.lib().mlxr_moe_gemma_router_forward(
+                ctypes.byref(self._desc), _ptr(x2), T, _ptr(idx), _ptr(weights), _ptr(workspace),
+                workspace.numel(), ops._stream(x)))
         lead = tuple(x.shape[:-1])
         return idx.reshape(lead + (K,)), weights.reshape(lead + (K,))
 
@@ -600,9 +603,10 @@ class Qwen35MoeBlock:
         if keep_routing:
             idx = torch.empty((T, K), dtype=torch.int32, device=x.device)
             wts = torch.empty((T, K), dtype=torch.float32, device=x.device)
-        C.check(C.lib().mlxr_moe_block_forward(
-            ctypes.byref(self._desc), _ptr(x2), T, _ptr(out), _ptr(idx), _ptr(wts),
-            _ptr(workspace), workspace.numel(), ops._stream(x)))
+        with ops._on(x):
+            C.check(C.lib().mlxr_moe_block_forward(
+                ctypes.byref(self._desc), _ptr(x2), T, _ptr(out), _ptr(idx), _ptr(wts),
+                _ptr(workspace), workspace.numel(), ops._stream(x)))
         self.last_indices, self.last_weights = idx, wts
         self.last_workspace = workspace
         return out.reshape(tuple(x.shape[:-1]) + (d,))
@@ -638,9 +642,10 @@ class Qwen35MoeBlock:
         if keep_routing:
             idx = torch.empty((T, K), dtype=torch.int32, device=h.device)
             wts = torch.empty((T, K), dtype=torch.float32, device=h.device)
-        C.check(C.lib().mlxr_moe_block_forward_residual(
-            ctypes.byref(self._desc), _ptr(norm.weight), norm.eps, _ptr(h2), T, _ptr(out),
-            _ptr(idx), _ptr(wts), _ptr(workspace), workspace.numel(), ops._stream(h)))
+        with ops._on(h):
+            C.check(C.lib().mlxr_moe_block_forward_residual(
+                ctypes.byref(self._desc), _ptr(norm.weight), norm.eps, _ptr(h2), T, _ptr(out),
+                _ptr(idx), _ptr(wts), _ptr(workspace), workspace.numel(), ops._stream(h)))
         self.last_indices, self.last_weights = idx, wts
         self.last_workspace = workspace
         return out.reshape(tuple(h.shape[:-1]) + (d,))
@@ -666,8 +671,9 @@ class RmsNorm:
         x2 = x.reshape(-1, d).contiguous()
         ops._dev(x2, self.weight)
         out = torch.empty_like(x2, dtype=torch.bfloat16)
-        C.check(C.lib().mlxr_moe_rms_norm(_ptr(x2), x2.shape[0], d, _ptr(self.weight), self.eps,
-                                          _ptr(out), ops._stream(x)))
+        with ops._on(x):
+            C.check(C.lib().mlxr_moe_rms_norm(_ptr(x2), x2.shape[0], d, _ptr(self.weight), self.eps,
+                                              _ptr(out), ops._stream(x)))
         return out.reshape(x.shape)
 
     __call__ = forward

@@ -168,9 +168,10 @@ def quantize(w: torch.Tensor, group_size=None, bits=None, mode="affine"):
         bi = torch.empty_like(sc)
     else:  # let the library produce the error message
         wq = sc = bi = torch.empty(1, device=w.device)
-    C.check(C.lib().mlxr_moe_quantize(
-        _p(w), _code(w), rows, cols, C.OptionalInt.of(group_size), C.OptionalInt.of(bits),
-        b"affine", _p(wq), _p(sc), _p(bi), _stream(w)))
+    with _on(w):
+        C.check(C.lib().mlxr_moe_quantize(
+            _p(w), _code(w), rows, cols, C.OptionalInt.of(group_size), C.OptionalInt.of(bits),
+            b"affine", _p(wq), _p(sc), _p(bi), _stream(w)))
     return wq, sc, bi
 
 
@@ -238,11 +239,12 @@ def dequantize(w: torch.Tensor, scales: torch.Tensor, biases=None, group_size=No
     rows = w.numel() // w.shape[-1]
     out_dtype = out_dtype or scales.dtype
     out = torch.empty(tuple(w.shape[:-1]) + (cols,), dtype=out_dtype, device=w.device)
-    C.check(C.lib().mlxr_moe_dequantize(
-        _p(w.contiguous()), _p(scales.contiguous()),
-        _p(None if biases is None else biases.contiguous()), _code(scales), rows, cols,
-        C.OptionalInt.of(group_size), C.OptionalInt.of(bits), b"affine", _p(out),
-        _code(out), _stream(w)))
+    with _on(w):
+        C.check(C.lib().mlxr_moe_dequantize(
+            _p(w.contiguous()), _p(scales.contiguous()),
+            _p(None if biases is None else biases.contiguous()), _code(scales), rows, cols,
+            C.OptionalInt.of(group_size), C.OptionalInt.of(bits), b"affine", _p(out),
+            _code(out), _stream(w)))
     return out
 
 
@@ -326,9 +328,10 @@ def gather_mm(a, b, lhs_indices=None, rhs_indices=None, sorted_indices=False,
     lib = C.lib()
     ws = workspace(lib.mlxr_moe_gather_mm_workspace_size(B, M, E), a.device)
     bc = b.contiguous()
-    C.check(lib.mlxr_moe_gather_mm(
-        _p(a), _code(a), a_batch, M, K, _p(bc), _code(bc), E, N, 1, _p(lhs), _p(rhs), B,
-        int(bool(sorted_indices)), _p(out), C.BFLOAT16, _p(ws), ws.numel(), _stream(a)))
+    with _on(a):
+        C.check(lib.mlxr_moe_gather_mm(
+            _p(a), _code(a), a_batch, M, K, _p(bc), _code(bc), E, N, 1, _p(lhs), _p(rhs), B,
+            int(bool(sorted_indices)), _p(out), C.BFLOAT16, _p(ws), ws.numel(), _stream(a)))
     out._mlxr_workspace = ws  # keep the status word alive with the result
     return out
 
@@ -356,7 +359,8 @@ def argpartition_axis(a: torch.Tensor, kth: int, axis: int):
     src = a.movedim(ax, -1).contiguous()
     out = torch.empty(src.shape, dtype=torch.int32, device=a.device)
     rows = src.numel() // n if n else 0
-    C.check(C.lib().mlxr_moe_argpartition(_p(src), rows, n, kth, -1, _p(out), _stream(a)))
+    with _on(a):
+        C.check(C.lib().mlxr_moe_argpartition(_p(src), rows, n, kth, -1, _p(out), _stream(a)))
     return out.movedim(-1, ax)
 
 
@@ -373,8 +377,9 @@ def softmax_axis(a: torch.Tensor, axis: int, precise=None):
     src = a.movedim(ax, -1).contiguous()
     n = src.shape[-1]
     out = torch.empty_like(src)
-    C.check(C.lib().mlxr_moe_softmax(_p(src), src.numel() // max(n, 1), n, -1,
-                                     int(bool(precise)), _p(out), _stream(a)))
+    with _on(a):
+        C.check(C.lib().mlxr_moe_softmax(_p(src), src.numel() // max(n, 1), n, -1,
+                                         int(bool(precise)), _p(out), _stream(a)))
     return out.movedim(-1, ax)
 
 
@@ -402,8 +407,9 @@ def router_topk(x: torch.Tensor, gate_w: torch.Tensor, k: int, return_logits=Fal
     wts = torch.empty((T, k), dtype=torch.float32, device=x.device)
     lib = C.lib()
     ws = workspace(lib.mlxr_moe_router_workspace_size(T, E), x.device)
-    C.check(lib.mlxr_moe_router_topk(_p(x2), T, d, _p(gate_w.contiguous()), E, k, _p(idx),
-                                     _p(wts), _p(ws), ws.numel(), _stream(x)))
+    with _on(x):
+        C.check(lib.mlxr_moe_router_topk(_p(x2), T, d, _p(gate_w.contiguous()), E, k, _p(idx),
+                                         _p(wts), _p(ws), ws.numel(), _stream(x)))
     return _routing(x, k, E, idx, wts, ws, return_logits)
 
 
@@ -430,8 +436,9 @@ def router_topk_quantized(x: torch.Tensor, gate, k: int, return_logits=False):
     lib = C.lib()
     ws = workspace(lib.mlxr_moe_router_workspace_size(T, gate.output_dims), x.device)
     desc = gate.descriptor()
-    C.check(lib.mlxr_moe_router_topk_quantized(_p(x2), T, ctypes.byref(desc), k, _p(idx),
-                                               _p(wts), _p(ws), ws.numel(), _stream(x)))
+    with _on(x):
+        C.check(lib.mlxr_moe_router_topk_quantized(_p(x2), T, ctypes.byref(desc), k, _p(idx),
+                                                   _p(wts), _p(ws), ws.numel(), _stream(x)))
     return _routing(x, k, gate.output_dims, idx, wts, ws, return_logits)
 
 
@@ -533,8 +540,9 @@ def dispatch(ids: torch.Tensor, num_experts: int):
     inv = torch.empty(n, dtype=torch.int32, device=dev)
     lib = C.lib()
     ws = workspace(lib.mlxr_moe_dispatch_workspace_size(n, num_experts), dev)
-    C.check(lib.mlxr_moe_dispatch(_p(flat), n, num_experts, _p(counts), _p(offsets),
-                                  _p(order), _p(inv), _p(ws), ws.numel(), _stream(ids)))
+    with _on(ids):
+        C.check(lib.mlxr_moe_dispatch(_p(flat), n, num_experts, _p(counts), _p(offsets),
+                                      _p(order), _p(inv), _p(ws), ws.numel(), _stream(ids)))
     order._mlxr_workspace = ws
     return counts, offsets, order, inv
 
@@ -545,11 +553,12 @@ def combine(y: torch.Tensor, weights: torch.Tensor, shared_y=None, shared_logit=
     _dev(y, weights, shared_y, shared_logit)
     T, K, d = y.shape
     out = torch.empty((T, d), dtype=torch.float32, device=y.device)
-    C.check(C.lib().mlxr_moe_combine(
-        _p(y.contiguous()), _p(weights.contiguous()), T, K, d,
-        _p(None if shared_y is None else shared_y.contiguous()),
-        _p(None if shared_logit is None else shared_logit.contiguous()), _p(out),
-        _stream(y)))
+    with _on(y):
+        C.check(C.lib().mlxr_moe_combine(
+            _p(y.contiguous()), _p(weights.contiguous()), T, K, d,
+            _p(None if shared_y is None else shared_y.contiguous()),
+            _p(None if shared_logit is None else shared_logit.contiguous()), _p(out),
+            _stream(y)))
     return out
 
 
@@ -580,7 +589,8 @@ def router_matrix_order(T: int, d: int, columns: int) -> bool:
 def workspace_status(ws: torch.Tensor) -> int:
     """Device status word of a call's workspace (1 = an index was out of
     range).  Synchronises the current stream."""
-    rc = C.lib().mlxr_moe_workspace_status(_p(ws), ws.numel(), _stream(ws))
+    with _on(ws):
+        rc = C.lib().mlxr_moe_workspace_status(_p(ws), ws.numel(), _stream(ws))
     if rc < 0:
         raise MlxrMoeError(C.last_error())
     return rc

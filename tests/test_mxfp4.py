@@ -1119,3 +1119,53 @@ def test_outputs_at_any_address(pkg, dev, T):
     y = store[1:].view(T, K, d).cpu().double()
     assert bool(torch.isnan(store[0])) and bool((y[cut] == 0).all())
     assert bool(((y - want).abs() <= bound)[~cut].all())
+
+
+@gpu
+def test_calls_make_their_device_the_current_one(pkg, dev, monkeypatch):
+    """Every call launches with its arrays' device current, whichever was before."""
+    ops, nn = pkg.ops, pkg.nn
+    real, seen = ops._on, []
+
+    def on(t):
+        seen.append(t.device)
+        return real(t)
+
+    monkeypatch.setattr(ops, "_on", on)
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn((4, 128), generator=g).bfloat16().to(dev)
+    gate = torch.randn((8, 128), generator=g).to(dev)
+    w = [torch.randn(s, generator=g).bfloat16().to(dev) * 0.1
+         for s in ((8, 64, 128), (8, 64, 128), (8, 128, 64))]
+    idx, wts, z = ops.router_topk(x, gate, 2, return_logits=True)
+    bf = nn.Linear(gate.bfloat16())
+    norm = nn.RmsNorm(torch.ones(128, device=dev))
+    for mode in ("affine", "mxfp4"):
+        wq, sc, bi = ops.quantize(w[0], mode=mode)
+        split = nn.SplitSwitchFfn.from_dense(*w, mode=mode)
+        packed = nn.PackedSwitchFfn.from_dense(torch.cat(w[:2], 1), w[2], mode=mode)
+        block = nn.Qwen35MoeBlock(gate, split, 2)
+        y = split.forward(x, idx)
+        _, counts, _, tokens = ops.router_balance(z, idx)
+        router = nn.GemmaRouter(gate, torch.ones(128, device=dev), torch.ones(8, device=dev), 2)
+        calls = [
+            lambda: ops.quantize(w[0], mode=mode),
+            lambda: ops.dequantize(wq, sc, bi, mode=mode),
+            lambda: ops.gather_qmm(x[:, None, None], wq, sc, bi, rhs_indices=idx, mode=mode),
+            lambda: ops.gather_mm(x[:, None, None], w[0], rhs_indices=idx),
+            lambda: ops.argpartition_axis(gate, 2, -1), lambda: ops.softmax_axis(gate, -1),
+            lambda: ops.router_topk(x, gate, 2), lambda: ops.router_topk_quantized(x, bf, 2),
+            lambda: ops.dispatch(idx.reshape(-1), 8), lambda: ops.combine(y, wts),
+            lambda: ops.router_balance(z, idx),
+            lambda: ops.router_balance_vjp(z, idx, counts, tokens, dweights=wts),
+            lambda: ops.workspace_status(split.last_workspace),
+            lambda: split.forward(x, idx), lambda: split.forward_with_combine(x, idx, wts),
+            lambda: packed.forward(x, idx), lambda: packed.forward_with_combine(x, idx, wts),
+            lambda: block.forward(x), lambda: block.forward_residual(x, norm),
+            lambda: norm.forward(x), lambda: router.forward(x),
+            lambda: nn.GemmaMoe(router, packed).forward(x),
+        ]
+        for i, call in enumerate(calls):
+            seen.clear()
+            call()
+            assert seen and all(d == x.device for d in seen), i
