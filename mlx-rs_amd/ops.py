@@ -192,6 +192,12 @@ def _quantize_mxfp4(w, group_size, bits):
     return wq, sc, None
 
 
+def _dense(*ts):
+    """The tensors as contiguous ones, for the caller to hold until its call is made:
+    the memory of a copy that nothing holds is the next copy's."""
+    return [None if t is None else t.contiguous() for t in ts]
+
+
 def _aligned(t, nbytes):
     """t, or a copy of it where its address is not a multiple of nbytes."""
     return t if t.data_ptr() % nbytes == 0 else t.clone()
@@ -234,6 +240,7 @@ def dequantize(w: torch.Tensor, scales: torch.Tensor, biases=None, group_size=No
     if _check_mode(mode):
         return _dequantize_mxfp4(w, scales, biases, group_size, bits, out_dtype)
     _dev(w, scales, biases)
+    w, scales, biases = _dense(w, scales, biases)
     b = DEFAULT_BITS if bits is None else bits
     cols = w.shape[-1] * 32 // b
     rows = w.numel() // w.shape[-1]
@@ -241,8 +248,7 @@ def dequantize(w: torch.Tensor, scales: torch.Tensor, biases=None, group_size=No
     out = torch.empty(tuple(w.shape[:-1]) + (cols,), dtype=out_dtype, device=w.device)
     with _on(w):
         C.check(C.lib().mlxr_moe_dequantize(
-            _p(w.contiguous()), _p(scales.contiguous()),
-            _p(None if biases is None else biases.contiguous()), _code(scales), rows, cols,
+            _p(w), _p(scales), _p(biases), _code(scales), rows, cols,
             C.OptionalInt.of(group_size), C.OptionalInt.of(bits), b"affine", _p(out),
             _code(out), _stream(w)))
     return out
@@ -284,10 +290,10 @@ def gather_qmm(x, w, scales, biases=None, lhs_indices=None, rhs_indices=None,
     out = torch.empty(tuple(rhs.shape) + (M, N), dtype=torch.bfloat16, device=x.device)
     lib = C.lib()
     ws = workspace(_workspace_bytes("gather_qmm", B, M, E), x.device)
+    w, scales, biases = _dense(w, scales, biases)
     with _on(x):
         C.check(lib.mlxr_moe_gather_qmm(
-            _p(x), _code(x), x_batch, M, K, _p(w.contiguous()), _p(scales.contiguous()),
-            _p(None if biases is None else biases.contiguous()),
+            _p(x), _code(x), x_batch, M, K, _p(w), _p(scales), _p(biases),
             C.UINT8 if mx else _code(scales), E, N,
             _p(lhs), _p(rhs), B, int(bool(transpose)), C.OptionalInt.of(group_size),
             C.OptionalInt.of(bits), mode.encode(), int(bool(sorted_indices)), _p(out),
@@ -400,6 +406,7 @@ def router_topk(x: torch.Tensor, gate_w: torch.Tensor, k: int, return_logits=Fal
         raise MlxrMoeError(f"router_topk: gate_w must be float32 [E, d], got {gate_w.dtype} "
                            f"{tuple(gate_w.shape)}")
     E, d = gate_w.shape
+    gate_w, = _dense(gate_w)
     x2 = _router_rows("router_topk", x, d)
     _dev(x, gate_w)
     T = x2.shape[0]
@@ -408,7 +415,7 @@ def router_topk(x: torch.Tensor, gate_w: torch.Tensor, k: int, return_logits=Fal
     lib = C.lib()
     ws = workspace(lib.mlxr_moe_router_workspace_size(T, E), x.device)
     with _on(x):
-        C.check(lib.mlxr_moe_router_topk(_p(x2), T, d, _p(gate_w.contiguous()), E, k, _p(idx),
+        C.check(lib.mlxr_moe_router_topk(_p(x2), T, d, _p(gate_w), E, k, _p(idx),
                                          _p(wts), _p(ws), ws.numel(), _stream(x)))
     return _routing(x, k, E, idx, wts, ws, return_logits)
 
@@ -551,14 +558,12 @@ def combine(y: torch.Tensor, weights: torch.Tensor, shared_y=None, shared_logit=
     """sum_k w * y over the top-k axis (combine_with_weights, switch.rs:
     223-234), plus shared_y * sigmoid(shared_logit) when given."""
     _dev(y, weights, shared_y, shared_logit)
+    y, weights, shared_y, shared_logit = _dense(y, weights, shared_y, shared_logit)
     T, K, d = y.shape
     out = torch.empty((T, d), dtype=torch.float32, device=y.device)
     with _on(y):
         C.check(C.lib().mlxr_moe_combine(
-            _p(y.contiguous()), _p(weights.contiguous()), T, K, d,
-            _p(None if shared_y is None else shared_y.contiguous()),
-            _p(None if shared_logit is None else shared_logit.contiguous()), _p(out),
-            _stream(y)))
+            _p(y), _p(weights), T, K, d, _p(shared_y), _p(shared_logit), _p(out), _stream(y)))
     return out
 
 

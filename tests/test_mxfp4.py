@@ -1169,3 +1169,34 @@ def test_calls_make_their_device_the_current_one(pkg, dev, monkeypatch):
             seen.clear()
             call()
             assert seen and all(d == x.device for d in seen), i
+
+
+@gpu
+@pytest.mark.parametrize("mode", ["affine", "mxfp4"])
+@pytest.mark.parametrize("E,N,K", [(6, 64, 128), (12, 512, 1024)])
+def test_strided_weights(pkg, dev, mode, E, N, K):
+    """Weights, scales and biases that are views in another order, all at once: the
+    copies a call makes of them live until it is done."""
+    ops = pkg.ops
+    g = torch.Generator(device=dev).manual_seed(K)
+    w = torch.randn((E, N, K), generator=g, device=dev).bfloat16()
+    parts = ops.quantize(w, mode=mode)
+    x = torch.randn((5, 1, K), generator=g, device=dev).bfloat16()
+    idx = torch.arange(5, dtype=torch.int32, device=dev)
+
+    def turned(t):  # the same values, rows not one after another
+        return None if t is None else t.transpose(0, 1).contiguous().transpose(0, 1)
+
+    for _ in range(3):
+        views = [turned(t) for t in parts]
+        torch.cuda.synchronize()
+        assert torch.equal(ops.dequantize(*views, mode=mode), ops.dequantize(*parts, mode=mode))
+        a = ops.gather_qmm(x, *views, rhs_indices=idx, mode=mode)
+        assert torch.equal(a, ops.gather_qmm(x, *parts, rhs_indices=idx, mode=mode))
+    y = torch.randn((40, 4, K), generator=g, device=dev).bfloat16()
+    wts = torch.rand((40, 4), generator=g, device=dev)
+    sy = torch.randn((40, K), generator=g, device=dev).bfloat16()
+    z = torch.randn((40,), generator=g, device=dev)
+    flat = [t.t().contiguous().t() for t in (wts, sy)]
+    wide = torch.stack([z, z], 1)[:, 0]
+    assert torch.equal(ops.combine(turned(y), flat[0], flat[1], wide), ops.combine(y, wts, sy, z))
