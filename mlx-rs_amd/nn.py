@@ -215,6 +215,13 @@ def _check_out(name: str, out, T: int, d: int, dtype, device):
         raise MlxrMoeError(f"{name}: out must be on {device}, got {out.device}")
 
 
+def _check_weights(name: str, weights, indices):
+    """One routing weight per choice: the C ABI reads that many."""
+    if weights.shape[-1:] != indices.shape[-1:] or weights.numel() != indices.numel():
+        raise MlxrMoeError(f"{name}: weights {tuple(weights.shape)} must match indices "
+                           f"{tuple(indices.shape)}")
+
+
 class SplitSwitchFfn:
     """SplitSwitchFfn<SwigluActivation>: gate_proj, up_proj [E, f, d],
     down_proj [E, d, f]; all three QuantizedSwitchLinear or all three dense
@@ -276,6 +283,7 @@ class SplitSwitchFfn:
 
     def forward_with_combine(self, x, indices, weights):
         """sum_k weights * expert_k(x) -> f32 [..., d] (switch.rs:446-474)."""
+        _check_weights("SplitSwitchFfn", weights, indices)
         x2, idx, K = self._prep(x, indices)
         T, d = x2.shape
         ops._dev(x, weights)
@@ -350,6 +358,7 @@ class PackedSwitchFfn:
     def forward_with_combine(self, x, indices, weights, out=None, workspace=None):
         """sum_k weights * expert_k(x) (switch.rs:316-335): f32 weights give
         an f32 [..., d], bf16 weights (gemma4's router) a bf16 one."""
+        _check_weights("PackedSwitchFfn", weights, indices)
         x2, idx, K = self._prep(x, indices)
         T, d = x2.shape
         bf16 = weights.dtype == torch.bfloat16

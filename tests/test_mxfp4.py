@@ -1200,3 +1200,22 @@ def test_strided_weights(pkg, dev, mode, E, N, K):
     flat = [t.t().contiguous().t() for t in (wts, sy)]
     wide = torch.stack([z, z], 1)[:, 0]
     assert torch.equal(ops.combine(turned(y), flat[0], flat[1], wide), ops.combine(y, wts, sy, z))
+
+
+def test_combine_takes_a_weight_per_choice(pkg):
+    nn, Err = pkg.nn, pkg.MlxrMoeError
+
+    def lin(rows, cols):
+        return nn.QuantizedSwitchLinear(torch.zeros((4, rows, cols // 8), dtype=torch.int32),
+                                        torch.zeros((4, rows, cols // 32), dtype=torch.uint8),
+                                        mode="mxfp4")
+
+    split = nn.SplitSwitchFfn(lin(64, 128), lin(64, 128), lin(128, 64))
+    packed = nn.PackedSwitchFfn(lin(128, 128), lin(128, 64))
+    x, idx = torch.zeros((6, 128)).bfloat16(), torch.zeros((6, 2), dtype=torch.int32)
+    for m in (split, packed):
+        for bad in (torch.ones(5, 2), torch.ones(6, 1), torch.ones(4, 3), torch.ones(6)):
+            with pytest.raises(Err, match="must match indices"):
+                m.forward_with_combine(x, idx, bad)
+        with pytest.raises(Err, match="ROCm device"):
+            m.forward_with_combine(x, idx, torch.ones(6, 2))
