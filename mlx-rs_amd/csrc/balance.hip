@@ -394,8 +394,8 @@ __global__ __launch_bounds__(64 * kWaves) void balance_vjp_kernel(
 }
 
 // Rows a workgroup of the two-launch form: two per wave, more where that would
-// make over 256 workgroups (one a CU; c4's 32768 rows 14.8 us and 5.9 for the
-// second launch so, 14.0 and 7.1 with two a CU, 14.5 and 10.0 with four).
+// make over 256 workgroups (one a CU; c4's 32768 rows 14.1 us and 6.0 for the
+// second launch so, 13.5 and 6.8 with two a CU, 15.3 and 9.9 with four).
 int part_rows(int64_t T) {
   return (int)std::max<int64_t>(2 * kPartWaves, (T + 255) / 256);
 }
