@@ -209,12 +209,14 @@ int mlxr_moe_router_topk(const void* x, int64_t T, int64_t d,
  *   probs f32 [E]: mean of p over the counted tokens
  *   tokens int32 [1]: N
  *   loss f32 [1] = E * sum_e counts_e / (N K) * probs_e
- * all 0 when N is 0.  (f_e = counts_e / (N K) sums to 1.  A coefficient meant for
- * counts_e / N, whose f_e sum to K, is to be multiplied by K here.)  A counted row whose logits are all -inf adds no
- * probability; NaN or +inf among them makes its p, and so probs and loss, NaN.
- * An index outside [0, E) is not counted and sets the workspace's status word
- * (mlxr_moe_workspace_status).  Sums are in f32 within a workgroup's rows and
- * in f64 across workgroups, in a fixed order: equal inputs give equal bits.  E <= 1024, K <= 64, T <= 2^25 - 1. */
+ * all 0 when N is 0.  (f_e = counts_e / (N K) sums to 1.  A coefficient meant
+ * for counts_e / N, whose f_e sum to K, is to be multiplied by K here.)  A
+ * counted row whose logits are all -inf adds no probability; NaN or +inf among
+ * them makes its p, and so probs and loss, NaN.  An index outside [0, E) is not
+ * counted and sets the workspace's status word (mlxr_moe_workspace_status).
+ * Sums are in f32 within a workgroup's rows and in f64 across workgroups, in a
+ * fixed order: equal inputs give equal bits.  E <= 1024, K <= 64,
+ * T <= 2^25 - 1. */
 size_t mlxr_moe_router_balance_workspace_size(int64_t T, int64_t E);
 int mlxr_moe_router_balance(const void* logits, int logits_dtype, int64_t ld,
                             int64_t T, int64_t E, const int32_t* indices,
