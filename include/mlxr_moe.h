@@ -31,7 +31,9 @@
  * "mxfp4", group_size 32 and bits 4 (their defaults there): microscaled 4-bit
  * floating point, codes of sign, two exponent bits and a mantissa bit (0, 0.5,
  * 1, 1.5, 2, 3, 4, 6) packed as the affine ones, one scale byte b per group
- * standing for 2^(b - 127) (255: NaN), no biases.
+ * standing for 2^(b - 127) (255: NaN), no biases.  quantize and dequantize also
+ * take mode "mxfp8", group_size 32 and bits 8: e4m3 codes (sign, four exponent
+ * bits of bias 7, three mantissa bits), four to a word, scales as mxfp4's.
  */
 #ifndef MLXR_MOE_H
 #define MLXR_MOE_H
@@ -72,7 +74,8 @@ int mlxr_moe_version(void);
  * biases NULL; a group's scale is 2^(floor(log2 max|w|) - 2), at least 2^-127,
  * its codes the nearest ones to w / scale (ties to the even code, magnitudes
  * above 6 to 6); a group holding an infinity or a NaN gets scale byte 255 (NaN)
- * and codes 0. */
+ * and codes 0.  Mode "mxfp8" alike with the scale 2^(floor(log2 max|w|) - 8) and
+ * magnitudes above 448 to 448. */
 int mlxr_moe_quantize(const void* w, int w_dtype, int64_t rows, int64_t cols,
                       mlxr_moe_optional_int group_size,
                       mlxr_moe_optional_int bits, const char* mode,
@@ -84,7 +87,8 @@ int mlxr_moe_quantize(const void* w, int w_dtype, int64_t rows, int64_t cols,
  * dequantize_device (crates/mlxr/src/ops/quantization.rs:118-146).
  * biases are required for mode "affine".  Mode "mxfp4": code * scale, exact
  * (past the output type's range an infinity); sb_dtype MLXR_MOE_UINT8, biases
- * NULL. */
+ * NULL.  Mode "mxfp8": the same, exact in f32 and, in bf16, from its smallest
+ * normal value on (rounded below). */
 int mlxr_moe_dequantize(const uint32_t* wq, const void* scales,
                         const void* biases, int sb_dtype, int64_t rows,
                         int64_t cols, mlxr_moe_optional_int group_size,
@@ -472,6 +476,40 @@ int mlxr_moe_block_forward_noalloc(const mlxr_moe_block* block, const void* x,
 int mlxr_moe_rms_norm(const void* x, int64_t T, int64_t d, const void* weight,
                       float eps, void* out, mlxr_moe_stream stream);
 
+/* The add in front of that norm and the norm in one pass (the attention half's
+ * h.add(..) and post_attention_layernorm, crates/mlxr-lm/src/qwen3_5/text/
+ * layer.rs:128-137):
+ *   h = x + residual,   y_j = w_j h_j / sqrt(sum_j h_j^2 / d + eps)
+ * x [T, d] f32 or bf16; residual [T, d] f32 or bf16, h in its type (the norm is
+ * over h as rounded to it); weight bf16 [d].  mode NULL: out bf16 [T, d], y
+ * rounded once (mlxr_moe_rms_norm rounds the normalised value too), scales NULL.
+ * mode "mxfp8": out uint32 [T, d/4] and scales uint8 [T, d/32] as
+ * mlxr_moe_quantize makes them of y in f32 (32 divides d): what
+ * mlxr_moe_grouped_qmm takes.  Rows holding NaN or an infinity, and rows of h
+ * whose squares pass f32's range, follow the formula in f32.  Any d up to 2^20,
+ * T up to 2^24 - 1; arrays aligned to their elements (16-byte alignment and 8
+ * dividing d are faster).  h and out must not overlap each other or the inputs. */
+int mlxr_moe_add_rms_norm(const void* x, int x_dtype, const void* residual,
+                          int residual_dtype, int64_t T, int64_t d,
+                          const void* weight, float eps, const char* mode,
+                          void* h, void* out, void* scales,
+                          mlxr_moe_stream stream);
+/* Its gradients (no counterpart in the reference's inference path).  h as the
+ * forward call returned it; dy [T, d] f32 or bf16, the gradient of y; dh [T, d] in
+ * h's type or NULL, what comes to h from the residual stream:
+ *   g = dy w,  r = 1 / sqrt(sum_j h_j^2 / d + eps)
+ *   dx_j = r (g_j - h_j r^2 sum_i g_i h_i / d) + dh_j   [T, d], h's type: the
+ *          gradient of x and of the residual
+ *   dweight_j = sum_t dy_tj h_tj r_t                    f32 [d] (0 for T = 0)
+ * Sums in f32 within a workgroup's rows, in f64 across workgroups, in a fixed
+ * order: equal inputs give equal bits.  dx must not overlap the inputs. */
+size_t mlxr_moe_add_rms_norm_vjp_workspace_size(int64_t T, int64_t d);
+int mlxr_moe_add_rms_norm_vjp(const void* dy, int dy_dtype, const void* h,
+                              int h_dtype, int64_t T, int64_t d,
+                              const void* weight, float eps, const void* dh,
+                              void* dx, float* dweight, void* workspace,
+                              size_t workspace_size, mlxr_moe_stream stream);
+
 /* The MoE half of a Qwen3.5 / Qwen3.6 decoder layer (DecoderLayer::forward,
  * crates/mlxr-lm/src/qwen3_5/text/layer.rs:134-138):
  *   out = h + block(rms_norm(h, norm_weight, eps))
@@ -505,7 +543,7 @@ int mlxr_moe_workspace_status(const void* workspace, size_t workspace_size,
  * on the stream it is launched on.  Names: "router_logits", "router_topk",
  * "dispatch", "qgemm_gated", "qgemm_down", "combine", the shared
  * expert's GEMMs "shared_gated", "shared_down", "rms_norm",
- * "router_balance", "router_balance_vjp", and
+ * "router_balance", "router_balance_vjp", "add_rms_norm", "add_rms_norm_vjp", and
  * "read_probe" (mlxr_moe_profile_read).  NULL disarms.  Not for use while
  * the stream is being captured into a graph. */
 int mlxr_moe_profile_start(const char* kernel);

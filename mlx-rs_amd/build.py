@@ -38,6 +38,7 @@ SOURCES = [
     "prefill_tall.hip",
     "combine.hip",
     "balance.hip",
+    "add_norm.hip",
     "nn.cpp",
     "profile.cpp",
     "capi.cpp",

@@ -1,0 +1,490 @@
+// The residual add with the RMSNorm behind it, and its gradients, on gfx950.
+//
+// Over rows x, residual [T, d] and a weight w [d]:
+//   h = x + residual                (rounded to the residual's type: the stream)
+//   r = 1 / sqrt(sum_j h_j^2 / d + eps)
+//   y_j = w_j h_j r
+// y in bf16, rounded once, or in mode "mxfp8": e4m3 codes with a power-of-two scale
+// per 32 (mx.hpp), each rounded once from the f32 value.  With dy the gradient of y
+// and dh what comes to h from elsewhere,
+//   g_j  = dy_j w_j,  c = sum_j g_j h_j / d
+//   dx_j = r (g_j - h_j r^2 c) + dh_j      (of x and of the residual alike)
+//   dw_j = sum_t dy_tj h_tj r_t
+// All sums in f32 (the weight gradient's over workgroups in f64), in fixed orders.
+//
+// HBM-bound: one pass over the rows, a row held in registers, by a wave (many rows)
+// or by a workgroup of four (few rows, or wide ones); 16-byte accesses where d and
+// the addresses allow, single values in a kernel of its own otherwise.
+#include <algorithm>
+
+#include "common.hpp"
+#include "kernels.hpp"
+#include "mx.hpp"
+#include "nn.hpp"
+
+namespace mlxr_moe {
+namespace {
+
+constexpr int kNT = 256;
+
+// 8 values from element e on, as f32
+template <bool F32>
+__device__ __forceinline__ void load8(const void* p, int64_t e, float (&v)[8]) {
+  if constexpr (F32) {
+    const f32x4_t* q = reinterpret_cast<const f32x4_t*>(static_cast<const float*>(p) + e);
+    const f32x4_t a = q[0], b = q[1];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = a[j], v[4 + j] = b[j];
+  } else {
+    const u32x4_t u = *reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(p) + e);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[2 * j] = __uint_as_float(u[j] << 16);
+      v[2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
+    }
+  }
+}
+template <bool F32>
+__device__ __forceinline__ void store8(void* p, int64_t e, const float (&v)[8]) {
+  if constexpr (F32) {
+    f32x4_t* q = reinterpret_cast<f32x4_t*>(static_cast<float*>(p) + e);
+    q[0] = f32x4_t{v[0], v[1], v[2], v[3]};
+    q[1] = f32x4_t{v[4], v[5], v[6], v[7]};
+  } else {
+    u32x4_t u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      u[j] = (uint32_t)f32_to_bf16(v[2 * j]) | ((uint32_t)f32_to_bf16(v[2 * j + 1]) << 16);
+    *reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(p) + e) = u;
+  }
+}
+template <bool F32>
+__device__ __forceinline__ float load1(const void* p, int64_t e) {
+  if constexpr (F32)
+    return static_cast<const float*>(p)[e];
+  else
+    return bf16_to_f32(static_cast<const uint16_t*>(p)[e]);
+}
+template <bool F32>
+__device__ __forceinline__ void store1(void* p, int64_t e, float v) {
+  if constexpr (F32)
+    static_cast<float*>(p)[e] = v;
+  else
+    static_cast<uint16_t*>(p)[e] = f32_to_bf16(v);
+}
+template <bool F32>
+__device__ __forceinline__ float round_to(float v) {
+  return F32 ? v : bf16_round(v);
+}
+
+// The sum over a row's threads (64: a wave; 256: the workgroup), the same on all.
+template <int TPR>
+__device__ __forceinline__ float row_sum(float v, float* red) {
+  v = wave_sum_butterfly(v);
+  if constexpr (TPR == 64) return v;
+  const int wave = threadIdx.x >> 6;
+  __syncthreads();  // (red may hold the sum before)
+  if ((threadIdx.x & 63) == 0) red[wave] = v;
+  __syncthreads();
+  return (red[0] + red[1]) + (red[2] + red[3]);
+}
+
+struct NormArgs {
+  const void *x, *res;
+  const uint16_t* w;
+  void* h;
+  void* out;        // bf16 rows, or words of codes
+  uint8_t* scales;  // mxfp8
+  int64_t T;
+  int d;
+  float eps;
+};
+
+// A row by TPR threads, each C pieces of 8 values.
+template <bool XF32, bool HF32, bool MX, int TPR, int C>
+__global__ __launch_bounds__(kNT) void add_rms_norm_kernel(NormArgs a) {
+  __shared__ float red[4];
+  const int lane = threadIdx.x & (TPR - 1);
+  const int64_t t = (int64_t)blockIdx.x * (kNT / TPR) + (TPR == 64 ? threadIdx.x >> 6 : 0);
+  if (t >= a.T) return;  // (whole rows: a wave's, or the workgroup's)
+  const int64_t row = t * a.d;
+  float v[C][8];
+  u32x4_t wv[C];
+  float ss = 0.0f;
+#pragma unroll
+  for (int i = 0; i < C; ++i) {
+    const int j = 8 * (lane + TPR * i);
+    float r[8];
+    if (j < a.d) {
+      load8<XF32>(a.x, row + j, v[i]);
+      load8<HF32>(a.res, row + j, r);
+      wv[i] = *reinterpret_cast<const u32x4_t*>(a.w + j);
+#pragma unroll
+      for (int c = 0; c < 8; ++c) v[i][c] = round_to<HF32>(v[i][c] + r[c]);
+    } else {
+      wv[i] = u32x4_t{0, 0, 0, 0};
+#pragma unroll
+      for (int c = 0; c < 8; ++c) v[i][c] = 0.0f;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < C; ++i) {
+    const int j = 8 * (lane + TPR * i);
+    if (j < a.d) store8<HF32>(a.h, row + j, v[i]);
+#pragma unroll
+    for (int c = 0; c < 8; ++c) ss = __builtin_fmaf(v[i][c], v[i][c], ss);
+  }
+  const float r = 1.0f / sqrtf(row_sum<TPR>(ss, red) / (float)a.d + a.eps);
+#pragma unroll
+  for (int i = 0; i < C; ++i) {
+    const int j = 8 * (lane + TPR * i);
+    float y[8];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      y[2 * c] = v[i][2 * c] * r * __uint_as_float(wv[i][c] << 16);
+      y[2 * c + 1] = v[i][2 * c + 1] * r * __uint_as_float(wv[i][c] & 0xffff0000u);
+    }
+    if constexpr (MX) {
+      // a group is four neighbouring lanes'
+      uint2 q;
+      const uint32_t byte = mx8_group8(y, q);
+      if (j < a.d) {
+        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.out) + row + j) = q;
+        if ((lane & 3) == 0) a.scales[(row + j) >> 5] = (uint8_t)byte;
+      }
+    } else {
+      if (j < a.d) store8<false>(a.out, row + j, y);
+    }
+  }
+}
+
+// Any d and alignment, a workgroup per row: h is written, then read back by the
+// thread that wrote it.  mxfp8: 32 divides d, and a group is half a wave's.
+template <bool XF32, bool HF32, bool MX>
+__global__ __launch_bounds__(kNT) void add_rms_norm_any_kernel(NormArgs a) {
+  __shared__ float red[4];
+  const int64_t row = (int64_t)blockIdx.x * a.d;
+  float ss = 0.0f;
+  for (int j = threadIdx.x; j < a.d; j += kNT) {
+    const float v = round_to<HF32>(load1<XF32>(a.x, row + j) + load1<HF32>(a.res, row + j));
+    store1<HF32>(a.h, row + j, v);
+    ss = __builtin_fmaf(v, v, ss);
+  }
+  const float r = 1.0f / sqrtf(row_sum<kNT>(ss, red) / (float)a.d + a.eps);
+  for (int j = threadIdx.x; j < a.d; j += kNT) {
+    const float y = load1<HF32>(a.h, row + j) * r * bf16_to_f32(a.w[j]);
+    if constexpr (MX) {
+      uint32_t top = __float_as_uint(y) & 0x7fffffffu;
+#pragma unroll
+      for (int m = 16; m >= 1; m >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, m, 64));
+      const uint32_t byte = mx8_byte(top);
+      static_cast<uint8_t*>(a.out)[row + j] = (uint8_t)mx8_pair(y, 0.0f, byte);
+      if ((j & 31) == 0) a.scales[(row + j) >> 5] = (uint8_t)byte;
+    } else {
+      store1<false>(a.out, row + j, y);
+    }
+  }
+}
+
+struct NormVjpArgs {
+  const void *dy, *h, *dh;  // dh may be null
+  const uint16_t* w;
+  void* dx;
+  float* part;  // [gridDim.x, d]: sums of the weight's gradient
+  int64_t T;
+  int d;
+  float eps;
+};
+
+// Rows by TPR threads each, C pieces of 8 values a thread; a thread's columns stay
+// its own, so the weight's gradient adds up in registers.
+template <bool YF32, bool HF32, int TPR, int C>
+__global__ __launch_bounds__(kNT) void add_rms_norm_vjp_kernel(NormVjpArgs a) {
+  constexpr int RPW = kNT / TPR;
+  extern __shared__ float lds[];  // TPR == 64: the waves' weight gradients [4][d]
+  __shared__ float red[8];
+  const int lane = threadIdx.x & (TPR - 1), wave = threadIdx.x >> 6;
+  float dw[C][8];
+  u32x4_t wv[C];
+#pragma unroll
+  for (int i = 0; i < C; ++i) {
+    const int j = 8 * (lane + TPR * i);
+    wv[i] = j < a.d ? *reinterpret_cast<const u32x4_t*>(a.w + j) : u32x4_t{0, 0, 0, 0};
+#pragma unroll
+    for (int c = 0; c < 8; ++c) dw[i][c] = 0.0f;
+  }
+  const auto weight = [&](int i, int c) {
+    const uint32_t u = wv[i][c >> 1];
+    return __uint_as_float(c & 1 ? u & 0xffff0000u : u << 16);
+  };
+  for (int64_t t = (int64_t)blockIdx.x * RPW + (TPR == 64 ? wave : 0); t < a.T;
+       t += (int64_t)gridDim.x * RPW) {
+    const int64_t row = t * a.d;
+    float h[C][8], dy[C][8];
+    float ss = 0.0f, gh = 0.0f;
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+      const int j = 8 * (lane + TPR * i);
+      if (j < a.d) {
+        load8<HF32>(a.h, row + j, h[i]);
+        load8<YF32>(a.dy, row + j, dy[i]);
+      } else {
+#pragma unroll
+        for (int c = 0; c < 8; ++c) h[i][c] = dy[i][c] = 0.0f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < C; ++i)
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        ss = __builtin_fmaf(h[i][c], h[i][c], ss);
+        gh = __builtin_fmaf(dy[i][c] * weight(i, c), h[i][c], gh);
+      }
+    if constexpr (TPR == 64) {
+      ss = wave_sum_butterfly(ss);
+      gh = wave_sum_butterfly(gh);
+    } else {
+      ss = wave_sum_butterfly(ss);
+      gh = wave_sum_butterfly(gh);
+      __syncthreads();
+      if ((threadIdx.x & 63) == 0) red[wave] = ss, red[4 + wave] = gh;
+      __syncthreads();
+      ss = (red[0] + red[1]) + (red[2] + red[3]);
+      gh = (red[4] + red[5]) + (red[6] + red[7]);
+    }
+    const float r = 1.0f / sqrtf(ss / (float)a.d + a.eps);
+    const float k = r * r * (gh / (float)a.d);
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+      const int j = 8 * (lane + TPR * i);
+      float o[8], e[8];
+      if (a.dh && j < a.d) {
+        load8<HF32>(a.dh, row + j, e);
+      } else {
+#pragma unroll
+        for (int c = 0; c < 8; ++c) e[c] = 0.0f;
+      }
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        o[c] = __builtin_fmaf(r, dy[i][c] * weight(i, c) - h[i][c] * k, e[c]);
+        dw[i][c] = __builtin_fmaf(dy[i][c], h[i][c] * r, dw[i][c]);
+      }
+      if (j < a.d) store8<HF32>(a.dx, row + j, o);
+    }
+  }
+  float* part = a.part + (int64_t)blockIdx.x * a.d;
+  if constexpr (TPR == 64) {
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+      const int j = 8 * (lane + TPR * i);
+      if (j < a.d) {
+        f32x4_t* q = reinterpret_cast<f32x4_t*>(lds + wave * a.d + j);
+        q[0] = f32x4_t{dw[i][0], dw[i][1], dw[i][2], dw[i][3]};
+        q[1] = f32x4_t{dw[i][4], dw[i][5], dw[i][6], dw[i][7]};
+      }
+    }
+    __syncthreads();
+    for (int j = 4 * threadIdx.x; j < a.d; j += 4 * kNT) {
+      const f32x4_t* q = reinterpret_cast<const f32x4_t*>(lds + j);
+      const int s = a.d / 4;
+      *reinterpret_cast<f32x4_t*>(part + j) = (q[0] + q[s]) + (q[2 * s] + q[3 * s]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+      const int j = 8 * (lane + TPR * i);
+      if (j < a.d) store8<true>(part, j, dw[i]);
+    }
+  }
+}
+
+// Any d and alignment, in two kernels: r and r^3 c of every row, then the columns,
+// a thread each, over a slice of the rows.
+template <bool YF32, bool HF32>
+__global__ __launch_bounds__(kNT) void norm_vjp_rows_kernel(NormVjpArgs a, float2* coef) {
+  __shared__ float red[4];
+  const int64_t row = (int64_t)blockIdx.x * a.d;
+  float ss = 0.0f, gh = 0.0f;
+  for (int j = threadIdx.x; j < a.d; j += kNT) {
+    const float h = load1<HF32>(a.h, row + j);
+    ss = __builtin_fmaf(h, h, ss);
+    gh = __builtin_fmaf(load1<YF32>(a.dy, row + j) * bf16_to_f32(a.w[j]), h, gh);
+  }
+  ss = row_sum<kNT>(ss, red);
+  gh = row_sum<kNT>(gh, red);
+  const float r = 1.0f / sqrtf(ss / (float)a.d + a.eps);
+  if (threadIdx.x == 0) coef[blockIdx.x] = make_float2(r, r * r * (gh / (float)a.d));
+}
+template <bool YF32, bool HF32>
+__global__ __launch_bounds__(kNT) void norm_vjp_cols_kernel(NormVjpArgs a, const float2* coef,
+                                                            int rows) {
+  const int j = blockIdx.y * kNT + threadIdx.x;
+  if (j >= a.d) return;
+  const int64_t t0 = (int64_t)blockIdx.x * rows, t1 = min(t0 + rows, a.T);
+  const float w = bf16_to_f32(a.w[j]);
+  float dw = 0.0f;
+  for (int64_t t = t0; t < t1; ++t) {
+    const float2 c = coef[t];
+    const float h = load1<HF32>(a.h, t * a.d + j), dy = load1<YF32>(a.dy, t * a.d + j);
+    const float e = a.dh ? load1<HF32>(a.dh, t * a.d + j) : 0.0f;
+    store1<HF32>(a.dx, t * a.d + j, __builtin_fmaf(c.x, dy * w - h * c.y, e));
+    dw = __builtin_fmaf(dy, h * c.x, dw);
+  }
+  a.part[(int64_t)blockIdx.x * a.d + j] = dw;
+}
+
+// dweight [d] = the sum of part [G, d] over its rows, in f64: 16 columns by 64
+// slices of the rows a workgroup.
+constexpr int kJoinCols = 16, kJoinRows = 64;
+__global__ __launch_bounds__(kJoinCols * kJoinRows) void norm_vjp_join_kernel(const float* part,
+                                                                              int G, int d,
+                                                                              float* dw) {
+  __shared__ double red[kJoinRows][kJoinCols + 1];
+  const int c = threadIdx.x % kJoinCols, s = threadIdx.x / kJoinCols;
+  const int j = blockIdx.x * kJoinCols + c;
+  double v = 0.0;
+  if (j < d)
+    for (int g = s; g < G; g += kJoinRows) v += (double)part[(int64_t)g * d + j];
+  red[s][c] = v;
+  __syncthreads();
+#pragma unroll
+  for (int n = kJoinRows / 2; n >= 1; n >>= 1) {
+    if (s < n) red[s][c] += red[s + n][c];
+    __syncthreads();
+  }
+  if (s == 0 && j < d) dw[j] = (float)red[0][c];
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// How a call's rows are split.
+struct RowForm {
+  bool any;  // single values
+  int tpr;   // threads per row
+  int c;     // pieces of 8 a thread
+};
+// A wave per row holds up to 4096 values and needs rows enough to fill the chip;
+// a workgroup per row up to 16384.
+RowForm row_form(int64_t T, int64_t d, bool vec) {
+  if (!vec || d % 8 || d > 16384) return {true, kNT, 0};
+  const int tpr = d <= 4096 && T >= kNormWaveRows ? 64 : kNT;
+  const int need = (int)((d / 8 + tpr - 1) / tpr);
+  return {false, tpr, need <= 1 ? 1 : need <= 2 ? 2 : need <= 4 ? 4 : 8};
+}
+
+#define MLXR_NORM_FORM(CALL, f)     \
+  do {                              \
+    if (f.tpr == 64) {              \
+      switch (f.c) {                \
+        case 1: CALL(64, 1); break; \
+        case 2: CALL(64, 2); break; \
+        case 4: CALL(64, 4); break; \
+        default: CALL(64, 8);       \
+      }                             \
+    } else {                        \
+      switch (f.c) {                \
+        case 1: CALL(256, 1); break;\
+        case 2: CALL(256, 2); break;\
+        case 4: CALL(256, 4); break;\
+        default: CALL(256, 8);      \
+      }                             \
+    }                               \
+  } while (0)
+
+template <bool XF32, bool HF32, bool MX>
+void run_norm(const NormArgs& a, const RowForm& f, hipStream_t s) {
+  if (f.any) {
+    add_rms_norm_any_kernel<XF32, HF32, MX><<<(unsigned)a.T, kNT, 0, s>>>(a);
+    return;
+  }
+  const int rpw = kNT / f.tpr;
+  const unsigned grid = (unsigned)((a.T + rpw - 1) / rpw);
+#define MLXR_NORM_CALL(TPR, C) \
+  add_rms_norm_kernel<XF32, HF32, MX, TPR, C><<<grid, kNT, 0, s>>>(a)
+  MLXR_NORM_FORM(MLXR_NORM_CALL, f);
+#undef MLXR_NORM_CALL
+}
+
+// Workgroups of the gradient's one-pass form; row slices of the other.
+int vjp_groups(int64_t T, const RowForm& f) {
+  if (f.any) return (int)std::min<int64_t>((T + 63) / 64, 1024);
+  const int rpw = kNT / f.tpr;
+  return (int)std::min<int64_t>((T + rpw - 1) / rpw, kNormVjpGroups);
+}
+struct VjpScratch {
+  float* part;
+  float2* coef;
+};
+VjpScratch carve_vjp(Carve& c, int64_t T, int64_t d) {
+  // room for either form: which one it is goes by the arrays' alignment too
+  const RowForm one = row_form(T, d, true), any = row_form(T, d, false);
+  VjpScratch v;
+  v.part = c.take<float>(std::max(vjp_groups(T, one), vjp_groups(T, any)) * d);
+  v.coef = c.take<float2>(T);
+  return v;
+}
+
+template <bool YF32, bool HF32>
+void run_norm_vjp(const NormVjpArgs& a, const RowForm& f, int G, float2* coef, hipStream_t s) {
+  if (f.any) {
+    const int rows = (int)((a.T + G - 1) / G);
+    norm_vjp_rows_kernel<YF32, HF32><<<(unsigned)a.T, kNT, 0, s>>>(a, coef);
+    norm_vjp_cols_kernel<YF32, HF32>
+        <<<dim3((unsigned)G, (unsigned)((a.d + kNT - 1) / kNT)), kNT, 0, s>>>(a, coef, rows);
+    return;
+  }
+  const size_t lds = f.tpr == 64 ? (size_t)16 * a.d : 0;
+#define MLXR_NORM_CALL(TPR, C) \
+  add_rms_norm_vjp_kernel<YF32, HF32, TPR, C><<<(unsigned)G, kNT, lds, s>>>(a)
+  MLXR_NORM_FORM(MLXR_NORM_CALL, f);
+#undef MLXR_NORM_CALL
+}
+
+}  // namespace
+
+hipError_t launch_add_rms_norm(const void* x, bool x_f32, const void* residual, bool h_f32,
+                               int64_t T, int64_t d, const uint16_t* w, float eps, void* h,
+                               void* out, uint8_t* scales, hipStream_t s) {
+  if (T == 0) return hipSuccess;
+  const bool vec = aligned16(x) && aligned16(residual) && aligned16(w) && aligned16(h) &&
+                   aligned16(out);
+  const RowForm f = row_form(T, d, vec);
+  const NormArgs a{x, residual, w, h, out, scales, T, (int)d, eps};
+  ProfileScope prof("add_rms_norm", s);
+#define MLXR_NORM_TYPES(XF, HF) \
+  (scales ? run_norm<XF, HF, true>(a, f, s) : run_norm<XF, HF, false>(a, f, s))
+  if (x_f32)
+    h_f32 ? MLXR_NORM_TYPES(true, true) : MLXR_NORM_TYPES(true, false);
+  else
+    h_f32 ? MLXR_NORM_TYPES(false, true) : MLXR_NORM_TYPES(false, false);
+#undef MLXR_NORM_TYPES
+  return hipGetLastError();
+}
+
+void plan_add_rms_norm_vjp(Carve& c, int64_t T, int64_t d) { (void)carve_vjp(c, T, d); }
+
+hipError_t launch_add_rms_norm_vjp(const void* dy, bool dy_f32, const void* h, bool h_f32,
+                                   int64_t T, int64_t d, const uint16_t* w, float eps,
+                                   const void* dh, void* dx, float* dweight, Carve ws,
+                                   hipStream_t s) {
+  const VjpScratch v = carve_vjp(ws, T, d);
+  const bool vec = aligned16(dy) && aligned16(h) && aligned16(w) && aligned16(dx) &&
+                   aligned16(dh);
+  const RowForm f = row_form(T, d, vec);
+  const int G = T ? vjp_groups(T, f) : 0;
+  const NormVjpArgs a{dy, h, dh, w, dx, v.part, T, (int)d, eps};
+  ProfileScope prof("add_rms_norm_vjp", s);
+  if (T) {
+    if (dy_f32)
+      h_f32 ? run_norm_vjp<true, true>(a, f, G, v.coef, s)
+            : run_norm_vjp<true, false>(a, f, G, v.coef, s);
+    else
+      h_f32 ? run_norm_vjp<false, true>(a, f, G, v.coef, s)
+            : run_norm_vjp<false, false>(a, f, G, v.coef, s);
+  }
+  norm_vjp_join_kernel<<<(unsigned)((d + kJoinCols - 1) / kJoinCols), kJoinCols * kJoinRows, 0,
+                         s>>>(v.part, G, (int)d, dweight);
+  return hipGetLastError();
+}
+
+}  // namespace mlxr_moe

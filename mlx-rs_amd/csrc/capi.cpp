@@ -42,6 +42,16 @@ bool dtype_ok(int dt) { return dt == MLXR_MOE_FLOAT32 || dt == MLXR_MOE_BFLOAT16
 static_assert(MLXR_MOE_BITS_MXFP4 == kBitsMxfp4, "one code for both");
 
 bool is_mxfp4(const char* mode) { return mode && std::strcmp(mode, "mxfp4") == 0; }
+bool is_mxfp8(const char* mode) { return mode && std::strcmp(mode, "mxfp8") == 0; }
+
+// group_size and bits of mode "mxfp8": 32 and 8, given or not
+Status resolve_mxfp8(mlxr_moe_optional_int gs, mlxr_moe_optional_int bits) {
+  const int g = gs.has_value ? gs.value : 32, b = bits.has_value ? bits.value : 8;
+  if (g != 32 || b != 8)
+    return Status::error("mode mxfp8 takes group_size 32 and bits 8, got " +
+                         std::to_string(g) + " and " + std::to_string(b));
+  return Status{};
+}
 
 // group_size and bits of mode "mxfp4": 32 and 4, given or not
 Status resolve_mxfp4(mlxr_moe_optional_int gs, mlxr_moe_optional_int bits) {
@@ -257,9 +267,10 @@ int mlxr_moe_quantize(const void* w, int w_dtype, int64_t rows, int64_t cols,
                       uint32_t* wq, void* scales, void* biases,
                       mlxr_moe_stream stream) {
   int g = 32, b = 4;
-  const bool mx = is_mxfp4(mode);
-  Status st = mx ? resolve_mxfp4(group_size, bits)
-                 : resolve_quant(mode, group_size, bits, false, &g, &b);
+  const bool mx8 = is_mxfp8(mode), mx = mx8 || is_mxfp4(mode);
+  Status st = mx8  ? resolve_mxfp8(group_size, bits)
+              : mx ? resolve_mxfp4(group_size, bits)
+                   : resolve_quant(mode, group_size, bits, false, &g, &b);
   if (!st.ok) return finish(st);
   if (!dtype_ok(w_dtype)) return fail("quantize: w dtype must be f32 or bf16");
   if (rows < 0 || cols <= 0) return fail("quantize: bad shape");
@@ -267,10 +278,15 @@ int mlxr_moe_quantize(const void* w, int w_dtype, int64_t rows, int64_t cols,
     return fail("quantize: last dim " + std::to_string(cols) +
                 " is not a multiple of group_size " + std::to_string(g));
   if (mx) {
-    if (biases) return fail("quantize: mode mxfp4 has no biases");
+    if (biases) return fail(std::string("quantize: mode ") + mode + " has no biases");
     if (rows && (!w || !wq || !scales)) return fail("quantize: null array");
     if (!aligned(w, w_dtype == MLXR_MOE_BFLOAT16 ? 2 : 4) || !aligned(wq, 4))
       return fail("quantize: w must be aligned to its elements, wq to 4 bytes");
+    if (mx8)
+      return finish(from_hip(launch_mx8_quantize(w, w_dtype == MLXR_MOE_BFLOAT16, rows * cols, wq,
+                                                 static_cast<uint8_t*>(scales),
+                                                 as_stream(stream)),
+                             "quantize"));
     return finish(from_hip(launch_mx_quantize(w, w_dtype == MLXR_MOE_BFLOAT16, rows * cols, wq,
                                               static_cast<uint8_t*>(scales),
                                               as_stream(stream)),
@@ -289,16 +305,23 @@ int mlxr_moe_dequantize(const uint32_t* wq, const void* scales,
                         int64_t cols, mlxr_moe_optional_int group_size,
                         mlxr_moe_optional_int bits, const char* mode,
                         void* out, int out_dtype, mlxr_moe_stream stream) {
-  if (is_mxfp4(mode)) {
-    const Status st = resolve_mxfp4(group_size, bits);
+  if (is_mxfp4(mode) || is_mxfp8(mode)) {
+    const std::string m(mode);
+    const bool mx8 = is_mxfp8(mode);
+    const Status st = mx8 ? resolve_mxfp8(group_size, bits) : resolve_mxfp4(group_size, bits);
     if (!st.ok) return finish(st);
     if (sb_dtype != MLXR_MOE_UINT8 || !dtype_ok(out_dtype))
-      return fail("dequantize: mode mxfp4 takes uint8 scales and a f32 or bf16 out");
+      return fail("dequantize: mode " + m + " takes uint8 scales and a f32 or bf16 out");
     if (rows < 0 || cols <= 0 || cols % 32) return fail("dequantize: bad shape");
-    if (biases) return fail("dequantize: mode mxfp4 has no biases");
+    if (biases) return fail("dequantize: mode " + m + " has no biases");
     if (rows && (!wq || !scales || !out)) return fail("dequantize: null array");
     if (!aligned(out, out_dtype == MLXR_MOE_BFLOAT16 ? 2 : 4) || !aligned(wq, 4))
       return fail("dequantize: out must be aligned to its elements, wq to 4 bytes");
+    if (mx8)
+      return finish(from_hip(
+          launch_mx8_dequantize(wq, static_cast<const uint8_t*>(scales), rows * cols, out,
+                                out_dtype == MLXR_MOE_BFLOAT16, as_stream(stream)),
+          "dequantize"));
     return finish(from_hip(
         launch_mx_dequantize(wq, static_cast<const uint8_t*>(scales), rows * cols, out,
                              out_dtype == MLXR_MOE_BFLOAT16, as_stream(stream)),
@@ -990,12 +1013,85 @@ int mlxr_moe_block_forward_residual(const mlxr_moe_block* block,
   return finish(m.forward(hb, T, out, topk_idx, topk_w, c, s, hb, &nm));
 }
 
+// What add_rms_norm and its gradient share.
+static Status check_norm(const char* op, int64_t T, int64_t d, const void* weight, float eps) {
+  const std::string o(op);
+  if (T < 0 || d <= 0) return Status::error(o + ": bad shape");
+  if (T > kMaxNormRows || d > kMaxNormDims)
+    return Status::error(o + ": at most " + std::to_string(kMaxNormRows) + " rows of " +
+                         std::to_string(kMaxNormDims));
+  if (!(eps >= 0.0f)) return Status::error(o + ": eps must be >= 0");
+  if (T && !weight) return Status::error(o + ": null array");
+  if (!aligned(weight, 2)) return Status::error(o + ": weight must be aligned to its elements");
+  return Status{};
+}
+
+int mlxr_moe_add_rms_norm(const void* x, int x_dtype, const void* residual, int residual_dtype,
+                          int64_t T, int64_t d, const void* weight, float eps, const char* mode,
+                          void* h, void* out, void* scales, mlxr_moe_stream stream) {
+  Status st = check_norm("add_rms_norm", T, d, weight, eps);
+  if (!st.ok) return finish(st);
+  if (!dtype_ok(x_dtype) || !dtype_ok(residual_dtype))
+    return fail("add_rms_norm: x and residual must be f32 or bf16");
+  const bool mx = is_mxfp8(mode);
+  if (mode && !mx)
+    return fail(std::string("add_rms_norm: unsupported mode '") + mode + "' (NULL or 'mxfp8')");
+  if (mx && d % 32)
+    return fail("add_rms_norm: mode mxfp8 takes rows of whole groups of 32, got " +
+                std::to_string(d));
+  if (!mx && scales) return fail("add_rms_norm: scales go with mode mxfp8");
+  if (T && (!x || !residual || !h || !out || (mx && !scales)))
+    return fail("add_rms_norm: null array");
+  const size_t xa = x_dtype == MLXR_MOE_BFLOAT16 ? 2 : 4;
+  const size_t ha = residual_dtype == MLXR_MOE_BFLOAT16 ? 2 : 4;
+  if (!aligned(x, xa) || !aligned(residual, ha) || !aligned(h, ha) || !aligned(out, mx ? 4 : 2))
+    return fail("add_rms_norm: arrays must be aligned to their elements");
+  return finish(from_hip(
+      launch_add_rms_norm(x, x_dtype == MLXR_MOE_FLOAT32, residual,
+                          residual_dtype == MLXR_MOE_FLOAT32, T, d,
+                          static_cast<const uint16_t*>(weight), eps, h, out,
+                          static_cast<uint8_t*>(scales), as_stream(stream)),
+      "add_rms_norm"));
+}
+
+size_t mlxr_moe_add_rms_norm_vjp_workspace_size(int64_t T, int64_t d) {
+  Carve c(nullptr);
+  if (T >= 0 && d > 0 && T <= kMaxNormRows && d <= kMaxNormDims) plan_add_rms_norm_vjp(c, T, d);
+  return c.off;
+}
+
+int mlxr_moe_add_rms_norm_vjp(const void* dy, int dy_dtype, const void* h, int h_dtype, int64_t T,
+                              int64_t d, const void* weight, float eps, const void* dh, void* dx,
+                              float* dweight, void* workspace, size_t workspace_size,
+                              mlxr_moe_stream stream) {
+  Status st = check_norm("add_rms_norm_vjp", T, d, weight, eps);
+  if (!st.ok) return finish(st);
+  if (!dtype_ok(dy_dtype) || !dtype_ok(h_dtype))
+    return fail("add_rms_norm_vjp: dy and h must be f32 or bf16");
+  if ((T && (!dy || !h || !dx)) || !dweight) return fail("add_rms_norm_vjp: null array");
+  const size_t ya = dy_dtype == MLXR_MOE_BFLOAT16 ? 2 : 4;
+  const size_t ha = h_dtype == MLXR_MOE_BFLOAT16 ? 2 : 4;
+  if (!aligned(dy, ya) || !aligned(h, ha) || !aligned(dh, ha) || !aligned(dx, ha) ||
+      !aligned(dweight, 4))
+    return fail("add_rms_norm_vjp: arrays must be aligned to their elements");
+  Carve plan(nullptr);
+  plan_add_rms_norm_vjp(plan, T, d);
+  st = check_workspace(plan, workspace, workspace_size);
+  if (!st.ok) return finish(st);
+  return finish(from_hip(
+      launch_add_rms_norm_vjp(dy, dy_dtype == MLXR_MOE_FLOAT32, h, h_dtype == MLXR_MOE_FLOAT32, T,
+                              d, static_cast<const uint16_t*>(weight), eps, dh, dx, dweight,
+                              Carve(workspace), as_stream(stream)),
+      "add_rms_norm_vjp"));
+}
+
 int mlxr_moe_profile_start(const char* kernel) {
   static const char* const kNames[] = {"router_logits", "router_topk",
                                        "dispatch",      "qgemm_gated",
                                        "qgemm_down",    "combine",
                                        "shared_gated",  "shared_down",
-                                       "rms_norm",      "read_probe"};
+                                       "rms_norm",      "add_rms_norm",
+                                       "add_rms_norm_vjp", "read_probe"};
   if (kernel && *kernel) {
     bool known = false;
     for (const char* n : kNames) known = known || std::strcmp(n, kernel) == 0;

@@ -47,6 +47,11 @@ hipError_t launch_mx_quantize(const void* w, bool w_bf16, int64_t n, uint32_t* w
                               uint8_t* scales, hipStream_t s);
 hipError_t launch_mx_dequantize(const uint32_t* wq, const uint8_t* scales, int64_t n, void* out,
                                 bool out_bf16, hipStream_t s);
+// ... and mode "mxfp8", four codes to a word.
+hipError_t launch_mx8_quantize(const void* w, bool w_bf16, int64_t n, uint32_t* wq,
+                               uint8_t* scales, hipStream_t s);
+hipError_t launch_mx8_dequantize(const uint32_t* wq, const uint8_t* scales, int64_t n, void* out,
+                                 bool out_bf16, hipStream_t s);
 
 // --------------------------------------------------------------- router.hip
 // Router weights: an f32 Linear [E, d] (bits == 0), a bf16 Linear (bits ==

@@ -1,4 +1,5 @@
-// Microscaled 4-bit weights (mode "mxfp4"): device helpers.
+// Microscaled 4-bit weights and 8-bit activations (modes "mxfp4", "mxfp8"): device
+// helpers.
 //
 // A group of 32 values of a row shares one scale byte b, the power of two
 // 2^(b - 127); b = 255 is NaN.  A value is a 4-bit e2m1 code -- sign, two
@@ -7,6 +8,10 @@
 // v1.0).  Eight codes to a 32-bit word, the first lowest.  Every such weight is a
 // bf16 value exactly while the product stays in bf16's range (b < 253), so the
 // products below multiply the same weights whichever kernel runs.
+//
+// Mode "mxfp8" (MXFP8 of the same) has 8-bit e4m3 codes -- sign, four exponent bits
+// of bias 7, three mantissa bits, magnitudes up to 448 -- four to a word, and the
+// same scales.
 #pragma once
 
 #include "common.hpp"
@@ -55,6 +60,42 @@ __device__ __forceinline__ float mx_act(int act, float g, float u) {
 }
 __device__ __forceinline__ uint16_t mx_bf16(float v) {
   return __builtin_bit_cast(uint16_t, (__bf16)v);
+}
+
+// ---- mode "mxfp8"
+// The scale byte of a group whose largest magnitude has the bits `top`: its exponent
+// less e4m3's own largest (8), at least 0; 255 where an infinity or a NaN is among
+// them (integers compare NaN largest).
+__device__ __forceinline__ uint32_t mx8_byte(uint32_t top) {
+  const uint32_t ex = top >> 23;
+  return ex == 255 ? 255u : ex > 8 ? ex - 8 : 0u;
+}
+// The codes of a and b, low byte first, under that scale: the nearest ones (ties to
+// the even code), magnitudes above 448 to 448; 0 under 255.  The division by the
+// power of two is exact.
+__device__ __forceinline__ uint32_t mx8_pair(float a, float b, uint32_t byte) {
+  if (byte == 255) return 0;
+  const float inv = __uint_as_float((254u - byte) << 23);
+  a = __builtin_amdgcn_fmed3f(a * inv, -448.0f, 448.0f);
+  b = __builtin_amdgcn_fmed3f(b * inv, -448.0f, 448.0f);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false) & 0xffffu;
+}
+// 8 values of a lane, a group being four neighbouring lanes': their codes and the
+// group's scale byte.
+__device__ __forceinline__ uint32_t mx8_group8(const float (&v)[8], uint2& q) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
+  top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0xB1, 0xf, 0xf, false));
+  top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x4E, 0xf, 0xf, false));
+  const uint32_t byte = mx8_byte(top);
+  q.x = mx8_pair(v[0], v[1], byte) | (mx8_pair(v[2], v[3], byte) << 16);
+  q.y = mx8_pair(v[4], v[5], byte) | (mx8_pair(v[6], v[7], byte) << 16);
+  return byte;
+}
+// The value of a scale byte, exactly.
+__device__ __forceinline__ float mx8_scale(uint32_t byte) {
+  return __uint_as_float(byte == 0 ? 0x00400000u : byte == 255 ? 0x7fc00000u : byte << 23);
 }
 
 }  // namespace mlxr_moe

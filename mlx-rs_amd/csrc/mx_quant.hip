@@ -1,4 +1,4 @@
-// Quantise to and from microscaled 4-bit weights (format in mx.hpp).
+// Quantise to and from microscaled 4-bit weights and 8-bit values (formats in mx.hpp).
 //
 // quantise: the scale byte of a group is its largest magnitude's exponent less
 // e2m1's own largest (2), in [0, 254]: 2^(floor(log2 max) - 2); each value
@@ -7,6 +7,9 @@
 // infinity or a NaN gets byte 255 and codes 0: it reads back as NaN.
 // dequantise: code * scale, exact in f32, and in bf16 (past bf16's range an
 // infinity).
+// Mode "mxfp8" alike: the scale is 2^(floor(log2 max) - 8), magnitudes above 448 go
+// to 448, and the values read back are exact in f32 (in bf16 rounded where they lie
+// below its normal range, an infinity past it).
 // HBM-bound, one pass: a lane takes 8 values (16 bytes of bf16, 32 of f32), one
 // word of codes; the four lanes of a group find its maximum by DPP moves, as
 // integers, so that NaN compares largest.  A bank of 128 x 768 x 2048 bf16 weights: 81
@@ -131,6 +134,64 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint32_t* __re
   }
 }
 
+template <bool BF16, int HOW>
+__global__ __launch_bounds__(256) void mx8_quantize_kernel(const void* __restrict__ w, int64_t n,
+                                                           uint32_t* __restrict__ wq,
+                                                           uint8_t* __restrict__ scales) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (8 * i >= n) return;
+  float v[8];
+  load8<BF16, HOW>(w, 8 * i, v);
+  uint2 q;
+  const uint32_t byte = mx8_group8(v, q);
+  if constexpr (HOW != kScalar) {
+    *reinterpret_cast<uint2*>(wq + 2 * i) = q;
+  } else {
+    wq[2 * i] = q.x;
+    wq[2 * i + 1] = q.y;
+  }
+  if ((i & 3) == 0) scales[i >> 2] = (uint8_t)byte;
+}
+
+template <bool OUT_BF16, int HOW>
+__global__ __launch_bounds__(256) void mx8_dequantize_kernel(const uint32_t* __restrict__ wq,
+                                                             const uint8_t* __restrict__ scales,
+                                                             int64_t n, void* __restrict__ out) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (8 * i >= n) return;
+  const float sc = mx8_scale(scales[i >> 2]);
+  float v[8];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const uint32_t u = wq[2 * i + k];
+    const mx_f32x2_t a = __builtin_amdgcn_cvt_pk_f32_fp8((int)u, false);
+    const mx_f32x2_t b = __builtin_amdgcn_cvt_pk_f32_fp8((int)u, true);
+    v[4 * k] = a.x * sc, v[4 * k + 1] = a.y * sc, v[4 * k + 2] = b.x * sc, v[4 * k + 3] = b.y * sc;
+  }
+  if constexpr (OUT_BF16) {
+    uint16_t* o = static_cast<uint16_t*>(out) + 8 * i;
+    u32x4_t u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      u[j] = (uint32_t)f32_to_bf16(v[2 * j]) | ((uint32_t)f32_to_bf16(v[2 * j + 1]) << 16);
+    if constexpr (HOW != kScalar) {
+      store16<HOW>(reinterpret_cast<u32x4_t*>(o), u);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[2 * j] = (uint16_t)u[j], o[2 * j + 1] = (uint16_t)(u[j] >> 16);
+    }
+  } else {
+    float* o = static_cast<float*>(out) + 8 * i;
+    if constexpr (HOW != kScalar) {
+      store16<HOW>(reinterpret_cast<f32x4_t*>(o), f32x4_t{v[0], v[1], v[2], v[3]});
+      store16<HOW>(reinterpret_cast<f32x4_t*>(o + 4), f32x4_t{v[4], v[5], v[6], v[7]});
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) o[j] = v[j];
+    }
+  }
+}
+
 // elements per launch (a grid holds under 2^32 threads)
 constexpr int64_t kLaunchElems = (int64_t)1 << 34;
 
@@ -185,6 +246,50 @@ hipError_t launch_mx_dequantize(const uint32_t* wq, const uint8_t* scales, int64
     const uint8_t* sc = scales + at / kMxGroup;
     const int h = how(dst, n * es);
 #define MLXR_MX_CALL(BF, H) mx_dequantize_kernel<BF, H><<<grid, 256, 0, s>>>(q, sc, m, dst)
+    if (out_bf16)
+      MLXR_MX_HOW(MLXR_MX_CALL, true, h);
+    else
+      MLXR_MX_HOW(MLXR_MX_CALL, false, h);
+#undef MLXR_MX_CALL
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
+hipError_t launch_mx8_quantize(const void* w, bool w_bf16, int64_t n, uint32_t* wq,
+                               uint8_t* scales, hipStream_t s) {
+  const int64_t es = w_bf16 ? 2 : 4;
+  for (int64_t at = 0; at < n; at += kLaunchElems) {
+    const int64_t m = std::min(n - at, kLaunchElems);
+    const char* src = static_cast<const char*>(w) + at * es;
+    const dim3 grid((unsigned)((m / 8 + 255) / 256));
+    uint32_t* q = wq + at / 4;
+    uint8_t* sc = scales + at / kMxGroup;
+    const int h = (reinterpret_cast<uintptr_t>(q) & 7) ? kScalar : how(src, n * es);
+#define MLXR_MX_CALL(BF, H) mx8_quantize_kernel<BF, H><<<grid, 256, 0, s>>>(src, m, q, sc)
+    if (w_bf16)
+      MLXR_MX_HOW(MLXR_MX_CALL, true, h);
+    else
+      MLXR_MX_HOW(MLXR_MX_CALL, false, h);
+#undef MLXR_MX_CALL
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
+hipError_t launch_mx8_dequantize(const uint32_t* wq, const uint8_t* scales, int64_t n, void* out,
+                                 bool out_bf16, hipStream_t s) {
+  const int64_t es = out_bf16 ? 2 : 4;
+  for (int64_t at = 0; at < n; at += kLaunchElems) {
+    const int64_t m = std::min(n - at, kLaunchElems);
+    char* dst = static_cast<char*>(out) + at * es;
+    const dim3 grid((unsigned)((m / 8 + 255) / 256));
+    const uint32_t* q = wq + at / 4;
+    const uint8_t* sc = scales + at / kMxGroup;
+    const int h = how(dst, n * es);
+#define MLXR_MX_CALL(BF, H) mx8_dequantize_kernel<BF, H><<<grid, 256, 0, s>>>(q, sc, m, dst)
     if (out_bf16)
       MLXR_MX_HOW(MLXR_MX_CALL, true, h);
     else

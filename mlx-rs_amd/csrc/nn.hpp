@@ -52,6 +52,27 @@ Status from_hip(hipError_t e, const char* where);
 DispatchBuffers carve_dispatch(Carve& c, int64_t n, int64_t E,
                                int32_t* status);
 
+// ------------------------------------------------------------ add_norm.hip
+// h = x + residual [T, d] (each f32 or bf16, h as the residual) and its RMSNorm with
+// weight w bf16 [d]: out bf16, or with scales the words and scale bytes of mode
+// "mxfp8" (32 divides d).
+hipError_t launch_add_rms_norm(const void* x, bool x_f32, const void* residual, bool h_f32,
+                               int64_t T, int64_t d, const uint16_t* w, float eps, void* h,
+                               void* out, uint8_t* scales, hipStream_t s);
+// Its gradients: dx [T, d] (h's type) of x and residual, dweight [d], for dy and dh
+// (h's type, or null); ws as plan_add_rms_norm_vjp carves it.
+void plan_add_rms_norm_vjp(Carve& c, int64_t T, int64_t d);
+hipError_t launch_add_rms_norm_vjp(const void* dy, bool dy_f32, const void* h, bool h_f32,
+                                   int64_t T, int64_t d, const uint16_t* w, float eps,
+                                   const void* dh, void* dx, float* dweight, Carve ws,
+                                   hipStream_t s);
+// Rows from which a wave takes a row (a workgroup one below), and the workgroups of
+// the gradient's one pass.
+constexpr int64_t kNormWaveRows = 2048;
+constexpr int64_t kNormVjpGroups = 1024;
+// The most rows and values a row of these calls (a grid holds under 2^32 threads).
+constexpr int64_t kMaxNormRows = (1 << 24) - 1, kMaxNormDims = 1 << 20;
+
 // ------------------------------------------------------------- balance.hip
 // The balance loss over logits z [T, E] (rows ld apart, f32 or bf16) and
 // choices idx [T, K]; ws as plan_router_balance carves it, its first word the

@@ -32,6 +32,8 @@ DEFAULT_BITS = 4
 # mode "mxfp4": e2m1 codes, a power-of-two scale byte per 32
 MXFP4_GROUP_SIZE = 32
 MODES = ("affine", "mxfp4")
+# mode "mxfp8" of quantize, dequantize and add_rms_norm: e4m3 codes, the same scales
+MXFP8_GROUP_SIZE = 32
 
 
 def _check_mode(mode: str) -> bool:
@@ -152,9 +154,12 @@ def quantize(w: torch.Tensor, group_size=None, bits=None, mode="affine"):
     """(w_q, scales, biases) of MLX affine quantisation along the last axis.
     w_q is int32 storage of mlx's uint32 words.  Mode "mxfp4" (group_size 32,
     4 bits): e2m1 codes, scales uint8 (the exponent of a power of two plus
-    127; 255 is NaN), biases None."""
+    127; 255 is NaN), biases None.  Mode "mxfp8" (group_size 32, 8 bits): e4m3
+    codes, four to a word, and the same scales."""
+    if mode == "mxfp8":
+        return _quantize_mx(w, group_size, bits, mode, 4)
     if _check_mode(mode):
-        return _quantize_mxfp4(w, group_size, bits)
+        return _quantize_mx(w, group_size, bits, mode, 8)
     _dev(w)
     w = w.contiguous()
     gs = DEFAULT_GROUP_SIZE if group_size is None else group_size
@@ -175,20 +180,21 @@ def quantize(w: torch.Tensor, group_size=None, bits=None, mode="affine"):
     return wq, sc, bi
 
 
-def _quantize_mxfp4(w, group_size, bits):
+def _quantize_mx(w, group_size, bits, mode, per_word):
     _dev(w)
     w = w.contiguous()
     cols = w.shape[-1] if w.ndim else 0
     rows = w.numel() // cols if cols else 0
     lead = tuple(w.shape[:-1])
     ok = cols > 0 and cols % MXFP4_GROUP_SIZE == 0  # (else the library says what is wrong)
-    wq = torch.empty(lead + (cols // 8,) if ok else 1, dtype=torch.int32, device=w.device)
+    wq = torch.empty(lead + (cols // per_word,) if ok else 1, dtype=torch.int32,
+                     device=w.device)
     sc = torch.empty(lead + (cols // MXFP4_GROUP_SIZE,) if ok else 1, dtype=torch.uint8,
                      device=w.device)
     with _on(w):
         C.check(C.lib().mlxr_moe_quantize(
             _p(w), _code(w), rows, cols, C.OptionalInt.of(group_size), C.OptionalInt.of(bits),
-            b"mxfp4", _p(wq), _p(sc), None, _stream(w)))
+            mode.encode(), _p(wq), _p(sc), None, _stream(w)))
     return wq, sc, None
 
 
@@ -203,42 +209,46 @@ def _aligned(t, nbytes):
     return t if t.data_ptr() % nbytes == 0 else t.clone()
 
 
-def _check_mxfp4(name, w, scales, biases):
-    """w [.., K/8] words and scales [.., K/32] bytes of the same rows: the C
-    ABI reads that much of both."""
+def _check_mxfp4(name, w, scales, biases, mode="mxfp4", per_word=8):
+    """w [.., K/8] words (mxfp8: K/4) and scales [.., K/32] bytes of the same rows:
+    the C ABI reads that much of both."""
     if biases is not None:
-        raise MlxrMoeError(f"{name}: mode mxfp4 has no biases")
+        raise MlxrMoeError(f"{name}: mode {mode} has no biases")
     if w.dtype not in (torch.int32, torch.uint32) or scales.dtype != torch.uint8:
-        raise MlxrMoeError(f"{name}: mode mxfp4 takes 32-bit words and uint8 scales, got "
+        raise MlxrMoeError(f"{name}: mode {mode} takes 32-bit words and uint8 scales, got "
                            f"{w.dtype} and {scales.dtype}")
     if (w.ndim < 1 or w.ndim != scales.ndim or w.shape[:-1] != scales.shape[:-1]
-            or w.shape[-1] * 8 != scales.shape[-1] * MXFP4_GROUP_SIZE):
+            or w.shape[-1] * per_word != scales.shape[-1] * MXFP4_GROUP_SIZE):
         raise MlxrMoeError(f"{name}: scales {tuple(scales.shape)} must hold one byte for each "
-                           f"four words of w {tuple(w.shape)}")
+                           f"{'four' if per_word == 8 else 'eight'} words of w "
+                           f"{tuple(w.shape)}")
 
 
-def _dequantize_mxfp4(w, scales, biases, group_size, bits, out_dtype):
+def _dequantize_mx(w, scales, biases, group_size, bits, out_dtype, mode, per_word):
     _dev(w, scales)
-    _check_mxfp4("dequantize", w, scales, biases)
+    _check_mxfp4("dequantize", w, scales, biases, mode, per_word)
     w, scales = w.contiguous(), scales.contiguous()
-    cols = w.shape[-1] * 8
+    cols = w.shape[-1] * per_word
     rows = w.numel() // w.shape[-1] if cols else 0
     out = torch.empty(tuple(w.shape[:-1]) + (cols,), dtype=out_dtype or torch.bfloat16,
                       device=w.device)
     with _on(w):
         C.check(C.lib().mlxr_moe_dequantize(
             _p(w), _p(scales), None, C.UINT8, rows, cols, C.OptionalInt.of(group_size),
-            C.OptionalInt.of(bits), b"mxfp4", _p(out), _code(out), _stream(w)))
+            C.OptionalInt.of(bits), mode.encode(), _p(out), _code(out), _stream(w)))
     return out
 
 
 def dequantize(w: torch.Tensor, scales: torch.Tensor, biases=None, group_size=None,
                bits=None, out_dtype=None, mode="affine"):
     """code * scale + bias (one fused multiply-add, rounded once) in scales'
-    dtype unless out_dtype is given.  Mode "mxfp4": code * scale, exact, in
-    bf16 unless out_dtype is given."""
+    dtype unless out_dtype is given.  Modes "mxfp4" and "mxfp8": code * scale,
+    exact, in bf16 unless out_dtype is given (mxfp8's values below bf16's normal
+    range are rounded there)."""
+    if mode == "mxfp8":
+        return _dequantize_mx(w, scales, biases, group_size, bits, out_dtype, mode, 4)
     if _check_mode(mode):
-        return _dequantize_mxfp4(w, scales, biases, group_size, bits, out_dtype)
+        return _dequantize_mx(w, scales, biases, group_size, bits, out_dtype, mode, 8)
     _dev(w, scales, biases)
     w, scales, biases = _dense(w, scales, biases)
     b = DEFAULT_BITS if bits is None else bits
@@ -532,6 +542,71 @@ def router_balance_vjp(logits: torch.Tensor, indices: torch.Tensor, counts=None,
             _p(z), _code(z), ld, T, E, _p(idx), K, _p(mask), _p(counts), _p(tokens), _p(dloss),
             _p(dweights), _p(dz), _stream(z)))
     return dz.reshape(logits.shape)
+
+
+def _norm_weight(name, weight, d):
+    if weight.dtype != torch.bfloat16 or weight.shape != (d,):
+        raise MlxrMoeError(f"{name}: weight must be bfloat16 [{d}], got {weight.dtype} "
+                           f"{tuple(weight.shape)}")
+    return weight.contiguous()
+
+
+def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps=1e-6,
+                 mode=None):
+    """h = x + residual (residual's dtype: f32 or bf16, as x) and y = rms_norm(h,
+    weight, eps), x and residual [.., d], weight bf16 [d].  Returns (h, y), y bf16
+    rounded once; with mode "mxfp8" (32 divides d) (h, codes int32 [.., d/4], scales
+    uint8 [.., d/32]), as quantize makes them of y in f32.  Not recorded by autograd:
+    the gradients are add_rms_norm_vjp's."""
+    if mode not in (None, "mxfp8"):
+        raise MlxrMoeError(f"add_rms_norm: unsupported mode {mode!r} (None or 'mxfp8')")
+    _dev(x, residual, weight)
+    d = x.shape[-1] if x.ndim else 0
+    if d < 1 or x.shape != residual.shape:
+        raise MlxrMoeError(f"add_rms_norm: x {tuple(x.shape)} and residual "
+                           f"{tuple(residual.shape)} must be the same [.., d]")
+    w = _norm_weight("add_rms_norm", weight, d)
+    if mode and d % MXFP8_GROUP_SIZE:
+        raise MlxrMoeError(f"add_rms_norm: mode mxfp8 takes rows of whole groups of 32, got {d}")
+    x, res = x.contiguous(), residual.contiguous()
+    h = torch.empty_like(res)
+    if mode:
+        lead = tuple(x.shape[:-1])
+        out = torch.empty(lead + (d // 4,), dtype=torch.int32, device=x.device)
+        sc = torch.empty(lead + (d // MXFP8_GROUP_SIZE,), dtype=torch.uint8, device=x.device)
+    else:
+        out, sc = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device), None
+    with _on(x):
+        C.check(C.lib().mlxr_moe_add_rms_norm(
+            _p(x), _code(x), _p(res), _code(res), x.numel() // d, d, _p(w), eps,
+            mode and mode.encode(), _p(h), _p(out), _p(sc), _stream(x)))
+    return (h, out, sc) if mode else (h, out)
+
+
+def add_rms_norm_vjp(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, eps=1e-6, dh=None):
+    """The gradients of add_rms_norm for dy [.., d] (f32 or bf16), that of y, and dh
+    (h's dtype, None: none), what comes to h from the residual stream; h as the
+    forward call returned it.  Returns (dx, dweight): dx in h's dtype, of x and of
+    the residual alike, and dweight f32 [d]."""
+    _dev(dy, h, weight, dh)
+    d = h.shape[-1] if h.ndim else 0
+    if d < 1 or dy.shape != h.shape:
+        raise MlxrMoeError(f"add_rms_norm_vjp: dy {tuple(dy.shape)} and h {tuple(h.shape)} must "
+                           "be the same [.., d]")
+    w = _norm_weight("add_rms_norm_vjp", weight, d)
+    if dh is not None and (dh.shape != h.shape or dh.dtype != h.dtype):
+        raise MlxrMoeError(f"add_rms_norm_vjp: dh must be {h.dtype} {tuple(h.shape)}, got "
+                           f"{dh.dtype} {tuple(dh.shape)}")
+    dy, h, dh = _dense(dy, h, dh)
+    T = h.numel() // d
+    dx = torch.empty_like(h)
+    dw = torch.empty(d, dtype=torch.float32, device=h.device)
+    ws = workspace(_workspace_bytes("add_rms_norm_vjp", T, d), h.device)
+    with _on(h):
+        C.check(C.lib().mlxr_moe_add_rms_norm_vjp(
+            _p(dy), _code(dy), _p(h), _code(h), T, d, _p(w), eps, _p(dh), _p(dx), _p(dw),
+            _p(ws), ws.numel(), _stream(h)))
+    return dx, dw
 
 
 def dispatch(ids: torch.Tensor, num_experts: int):
