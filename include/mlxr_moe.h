@@ -258,6 +258,49 @@ int mlxr_moe_dispatch(const int32_t* ids, int64_t n, int64_t E,
                       int32_t* inv, void* workspace, size_t workspace_size,
                       mlxr_moe_stream stream);
 
+/* Products over rows sorted by expert, as mlxr_moe_dispatch sorts them: expert e has
+ * the rows offsets[e] .. offsets[e + 1] - 1 of R (offsets int32 [E + 1] on the device,
+ * ascending from 0; groups may be empty).  gather_mm and gather_qmm
+ * (crates/mlxr/src/ops/arithmetic.rs:1577-1613, quantization.rs:171-221) sort their
+ * rows at every call and give them in the callers' order; these take them sorted
+ * once for all projections and gradients of a layer.
+ *   y[r] = x[rows[r]] @ w[e(r)]^T   (rows int32 [R], or NULL: x has R rows, r's own)
+ * Rows behind the last group come out as zeros, and so do rows whose index is
+ * outside [0, x_rows) (their x is taken as zeros).  offsets are clamped to [0, R];
+ * where they do not ascend, what comes out is not specified, but nothing outside
+ * the arrays is read or written.
+ * grouped_mm: x bf16 [x_rows, K], w bf16 [E, N, K], out [R, N] bf16 or f32, sums in
+ * f32.  K and N multiples of 8, up to 2^16; E <= 1024; N * K < 2^30; arrays 16-byte
+ * aligned; x under 4 GB where rows are given. */
+int mlxr_moe_grouped_mm(const void* x, int64_t x_rows, int64_t K, const void* w,
+                        int64_t num_experts, int64_t N, const int32_t* offsets,
+                        const int32_t* rows, int64_t R, void* out, int out_dtype,
+                        mlxr_moe_stream stream);
+/* Its gradients for dy bf16 [R, N]:
+ *   dx[r]    = dy[r] @ w[e(r)]                 bf16 [R, K], of each sorted row's x
+ *              (zeros behind the last group); tokens named by several rows sum theirs
+ *   dw[e]    = sum over r of e: dy[r]^T x[rows[r]]   f32 or bf16 [E, N, K]; zeros for
+ *              experts without rows
+ * dx or dw may be NULL (not computed; w, or x, is then not read). */
+size_t mlxr_moe_grouped_mm_vjp_workspace_size(int64_t R, int64_t num_experts, int64_t N,
+                                              int64_t K);
+int mlxr_moe_grouped_mm_vjp(const void* dy, const void* x, int64_t x_rows, int64_t K,
+                            const void* w, int64_t num_experts, int64_t N,
+                            const int32_t* offsets, const int32_t* rows, int64_t R,
+                            void* dx, void* dw, int dw_dtype, void* workspace,
+                            size_t workspace_size, mlxr_moe_stream stream);
+/* grouped_mm with x in mode "mxfp8" (words [x_rows, K/4], scales uint8 [x_rows, K/32])
+ * and w in mode "mxfp4" (words [E, N, K/8], scales uint8 [E, N, K/32]): out [R, N] bf16
+ * or f32.  K a multiple of 32, N of 8.  The matrix instructions multiply the codes as
+ * they are; they keep a product down to 2^-13 of the largest of the few products that
+ * they add at a time, and add those sums in f32: against the rounding of x to 8 bits,
+ * 2^-4 of each value, that is nothing. */
+int mlxr_moe_grouped_qmm(const uint32_t* x, const uint8_t* x_scales, int64_t x_rows,
+                         int64_t K, const uint32_t* w, const uint8_t* w_scales,
+                         int64_t num_experts, int64_t N, const int32_t* offsets,
+                         const int32_t* rows, int64_t R, void* out, int out_dtype,
+                         mlxr_moe_stream stream);
+
 /* out f32 [T, d] = sum_k w[t,k] * y[t,k,:] (+ shared_y[t,:] *
  * sigmoid(shared_logit[t])).  y bf16 [T, K, d]; shared_y bf16 [T, d] or
  * NULL.  Replaces combine_with_weights (crates/mlxr-lm/src/nn/switch.rs:
@@ -543,8 +586,8 @@ int mlxr_moe_workspace_status(const void* workspace, size_t workspace_size,
  * on the stream it is launched on.  Names: "router_logits", "router_topk",
  * "dispatch", "qgemm_gated", "qgemm_down", "combine", the shared
  * expert's GEMMs "shared_gated", "shared_down", "rms_norm",
- * "router_balance", "router_balance_vjp", "add_rms_norm", "add_rms_norm_vjp", and
- * "read_probe" (mlxr_moe_profile_read).  NULL disarms.  Not for use while
+ * "router_balance", "router_balance_vjp", "add_rms_norm", "add_rms_norm_vjp",
+ * "grouped_mm", "grouped_dx", "grouped_dw", "grouped_qmm", and "read_probe" (mlxr_moe_profile_read).  NULL disarms.  Not for use while
  * the stream is being captured into a graph. */
 int mlxr_moe_profile_start(const char* kernel);
 /* Waits for the armed kernel's last launch, returns the number of launches

@@ -124,6 +124,16 @@ SIGNATURES = {
         [P, c_int, c_int64, c_int64, c_int64, P, c_int64, P, P, P, P, P, P, P]),
     "mlxr_moe_dispatch_workspace_size": (c_size_t, [c_int64, c_int64]),
     "mlxr_moe_dispatch": (c_int, [P, c_int64, c_int64, P, P, P, P, P, c_size_t, P]),
+    "mlxr_moe_grouped_mm": (
+        c_int,
+        [P, c_int64, c_int64, P, c_int64, c_int64, P, P, c_int64, P, c_int, P]),
+    "mlxr_moe_grouped_mm_vjp_workspace_size": (c_size_t, [c_int64, c_int64, c_int64, c_int64]),
+    "mlxr_moe_grouped_mm_vjp": (
+        c_int,
+        [P, P, c_int64, c_int64, P, c_int64, c_int64, P, P, c_int64, P, P, c_int, P, c_size_t, P]),
+    "mlxr_moe_grouped_qmm": (
+        c_int,
+        [P, P, c_int64, c_int64, P, P, c_int64, c_int64, P, P, c_int64, P, c_int, P]),
     "mlxr_moe_combine": (c_int, [P, P, c_int64, c_int64, c_int64, P, P, P, P]),
     "mlxr_moe_switch_glu_workspace_size": (c_size_t, [POINTER(SwitchGlu), c_int64, c_int64]),
     "mlxr_moe_switch_glu_forward": (

@@ -39,9 +39,11 @@ SOURCES = [
     "combine.hip",
     "balance.hip",
     "add_norm.hip",
+    "grouped_tile.hip",
     "nn.cpp",
     "profile.cpp",
     "capi.cpp",
+    "capi_grouped.cpp",
     "noalloc.hip",
     "probe.hip",
 ]

@@ -1091,7 +1091,9 @@ int mlxr_moe_profile_start(const char* kernel) {
                                        "qgemm_down",    "combine",
                                        "shared_gated",  "shared_down",
                                        "rms_norm",      "add_rms_norm",
-                                       "add_rms_norm_vjp", "read_probe"};
+                                       "add_rms_norm_vjp", "grouped_mm",
+                                       "grouped_dx",    "grouped_dw",
+                                       "grouped_qmm",   "read_probe"};
   if (kernel && *kernel) {
     bool known = false;
     for (const char* n : kNames) known = known || std::strcmp(n, kernel) == 0;

@@ -629,6 +629,104 @@ def dispatch(ids: torch.Tensor, num_experts: int):
     return counts, offsets, order, inv
 
 
+def _grouped_inputs(name, x, K, E, offsets, rows):
+    """(x rows, rows int32 or None, offsets int32, R) of the products over sorted rows."""
+    if offsets.ndim != 1 or offsets.numel() != E + 1:
+        raise MlxrMoeError(f"{name}: offsets must be [{E + 1}] for {E} experts, got "
+                           f"{tuple(offsets.shape)}")
+    if x.ndim < 1 or x.shape[-1] != K:
+        raise MlxrMoeError(f"{name}: x last dim must be {K}, got {tuple(x.shape)}")
+    x = (x if x.ndim == 2 else x.reshape(-1, K)).contiguous()
+    if rows is not None:
+        if rows.ndim != 1:
+            raise MlxrMoeError(f"{name}: rows must be [R], got {tuple(rows.shape)}")
+        rows = _as_u32(rows)
+    return _aligned(x, 16), rows, _as_u32(offsets), x.shape[0] if rows is None else rows.numel()
+
+
+def _grouped_weight(name, w):
+    if w.ndim != 3 or w.dtype != torch.bfloat16:
+        raise MlxrMoeError(f"{name}: w must be bfloat16 [E, N, K], got {w.dtype} "
+                           f"{tuple(w.shape)}")
+    return _aligned(w.contiguous(), 16)
+
+
+def _bf16(name, what, t):
+    if t.dtype != torch.bfloat16:
+        raise MlxrMoeError(f"{name}: {what} must be bfloat16, got {t.dtype}")
+
+
+def grouped_mm(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, rows=None,
+               out_dtype=torch.bfloat16):
+    """y[r] = x[rows[r]] @ w[e(r)]^T over R rows sorted by expert: expert e has the
+    rows offsets[e] .. offsets[e + 1] (as dispatch gives them), w bf16 [E, N, K].
+    With rows [R] x is bf16 [.., K] of any number of rows (a token's row taken by
+    each of its choices), without it x's rows are the sorted ones.  Returns [R, N]
+    in out_dtype (bf16 or f32); zeros behind the last group and where rows names no
+    row of x.  K and N multiples of 8.  Not recorded by autograd: the gradients are
+    grouped_mm_vjp's."""
+    _dev(x, w, offsets, rows)
+    w = _grouped_weight("grouped_mm", w)
+    _bf16("grouped_mm", "x", x)
+    E, N, K = w.shape
+    x, rows, offsets, R = _grouped_inputs("grouped_mm", x, K, E, offsets, rows)
+    out = torch.empty((R, N), dtype=out_dtype, device=x.device)
+    with _on(x):
+        C.check(C.lib().mlxr_moe_grouped_mm(
+            _p(x), x.shape[0], K, _p(w), E, N, _p(offsets), _p(rows), R, _p(out), _code(out),
+            _stream(x)))
+    return out
+
+
+def grouped_mm_vjp(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor,
+                   rows=None, dw_dtype=torch.bfloat16, need_dx=True, need_dw=True):
+    """The gradients of grouped_mm for dy bf16 [R, N]: (dx, dw), dx bf16 [R, K] of each
+    sorted row's x (a token's choices sum theirs: combine with weights of 1), dw
+    [E, N, K] in dw_dtype (bf16 or f32), zeros for experts without rows.  None where
+    not needed."""
+    _dev(dy, x, w, offsets, rows)
+    w = _grouped_weight("grouped_mm_vjp", w)
+    _bf16("grouped_mm_vjp", "x", x)
+    _bf16("grouped_mm_vjp", "dy", dy)
+    E, N, K = w.shape
+    x, rows, offsets, R = _grouped_inputs("grouped_mm_vjp", x, K, E, offsets, rows)
+    if dy.shape != (R, N):
+        raise MlxrMoeError(f"grouped_mm_vjp: dy must be ({R}, {N}), got {tuple(dy.shape)}")
+    dy = _aligned(dy.contiguous(), 16)
+    dx = torch.empty((R, K), dtype=torch.bfloat16, device=x.device) if need_dx else None
+    dw = torch.empty((E, N, K), dtype=dw_dtype, device=x.device) if need_dw else None
+    if not (need_dx or need_dw):
+        return None, None
+    ws = workspace(_workspace_bytes("grouped_mm_vjp", R, E, N, K), x.device)
+    with _on(x):
+        C.check(C.lib().mlxr_moe_grouped_mm_vjp(
+            _p(dy), _p(x), x.shape[0], K, _p(w), E, N, _p(offsets), _p(rows), R, _p(dx), _p(dw),
+            _code(dw) if need_dw else C.BFLOAT16, _p(ws), ws.numel(), _stream(x)))
+    return dx, dw
+
+
+def grouped_qmm(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor,
+                offsets: torch.Tensor, rows=None, out_dtype=torch.bfloat16):
+    """grouped_mm with x in mode "mxfp8" (words [.., K/4] and scales [.., K/32], as
+    quantize or add_rms_norm give them) and w in mode "mxfp4" (words [E, N, K/8], scales
+    [E, N, K/32]).  K a multiple of 32, N of 8."""
+    _dev(x, x_scales, w, w_scales, offsets, rows)
+    _check_mxfp4("grouped_qmm", w, w_scales, None)
+    _check_mxfp4("grouped_qmm", x, x_scales, None, "mxfp8", 4)
+    if w.ndim != 3:
+        raise MlxrMoeError("grouped_qmm: w must be [E, N, K/8]")
+    E, N, K = w.shape[0], w.shape[1], w.shape[2] * 8
+    x, rows, offsets, R = _grouped_inputs("grouped_qmm", x, K // 4, E, offsets, rows)
+    x_scales, w, w_scales = _dense(x_scales, w, w_scales)
+    x_scales, w, w_scales = _aligned(x_scales, 4), _aligned(w, 16), _aligned(w_scales, 4)
+    out = torch.empty((R, N), dtype=out_dtype, device=x.device)
+    with _on(x):
+        C.check(C.lib().mlxr_moe_grouped_qmm(
+            _p(x), _p(x_scales), x.shape[0], K, _p(w), _p(w_scales), E, N, _p(offsets), _p(rows),
+            R, _p(out), _code(out), _stream(x)))
+    return out
+
+
 def combine(y: torch.Tensor, weights: torch.Tensor, shared_y=None, shared_logit=None):
     """sum_k w * y over the top-k axis (combine_with_weights, switch.rs:
     223-234), plus shared_y * sigmoid(shared_logit) when given."""
