@@ -47,6 +47,19 @@ Status check_shape(const char* op, int64_t x_rows, int64_t K, int64_t E, int64_t
   return Status{};
 }
 
+// dW's plan, and the parts of groups that are summed in several.
+struct VjpScratch {
+  int32_t* plan;
+  float* parts;
+};
+VjpScratch plan_vjp(Carve& c, int64_t R, int64_t E, int64_t N, int64_t K) {
+  const int64_t chunk = grouped_chunk_rows(R, N, K), slices = grouped_slices(R, chunk);
+  VjpScratch v;
+  v.plan = c.take<int32_t>(plan_words(grouped_chunks(R, E, chunk), slices));
+  v.parts = c.take<float>(slices * N * K);
+  return v;
+}
+
 }  // namespace
 
 extern "C" {
@@ -69,8 +82,9 @@ int mlxr_moe_grouped_mm(const void* x, int64_t x_rows, int64_t K, const void* w,
 }
 
 size_t mlxr_moe_grouped_mm_vjp_workspace_size(int64_t R, int64_t E, int64_t N, int64_t K) {
-  (void)R, (void)E, (void)N, (void)K;
-  return 0;
+  Carve c(nullptr);
+  if (R >= 0 && E > 0 && N > 0 && K > 0) plan_vjp(c, R, E, N, K);
+  return c.off;
 }
 
 int mlxr_moe_grouped_mm_vjp(const void* dy, const void* x, int64_t x_rows, int64_t K,
@@ -86,7 +100,16 @@ int mlxr_moe_grouped_mm_vjp(const void* dy, const void* x, int64_t x_rows, int64
   if (!aligned(dy, 16) || !aligned(x, 16) || !aligned(w, 16) || !aligned(dx, 16) ||
       !aligned(dw, 16))
     return capi_fail("grouped_mm_vjp: arrays must be 16-byte aligned");
-  (void)workspace, (void)workspace_size;
+  Carve plan(nullptr);
+  plan_vjp(plan, R, E, N, K);
+  if (dw) {
+    if (plan.off > workspace_size)
+      return capi_fail("grouped_mm_vjp: workspace too small: need " + std::to_string(plan.off) +
+                       " bytes, got " + std::to_string(workspace_size));
+    if (!workspace) return capi_fail("grouped_mm_vjp: workspace is NULL");
+    if (!aligned(workspace, 256))
+      return capi_fail("grouped_mm_vjp: workspace must be 256-byte aligned");
+  }
   hipStream_t s = as_stream(stream);
   if (dx && R) {
     GroupedArgs a{};
@@ -100,6 +123,11 @@ int mlxr_moe_grouped_mm_vjp(const void* dy, const void* x, int64_t x_rows, int64
     a.m = dy, a.j = x, a.offsets = offsets, a.rows = rows, a.out = dw;
     a.R = R, a.x_rows = x_rows, a.E = (int32_t)E, a.J = (int32_t)K, a.C = (int32_t)N;
     a.out_f32 = dw_dtype == MLXR_MOE_FLOAT32;
+    Carve c(workspace);
+    const VjpScratch v = plan_vjp(c, R, E, N, K);
+    a.plan = v.plan, a.parts = v.parts;
+    a.chunk = (int32_t)grouped_chunk_rows(R, N, K);
+    a.slices = (int32_t)grouped_slices(R, a.chunk);
     st = from_hip(launch_grouped_dw(a, s), "grouped_mm_vjp dw");
   }
   return finish(st);

@@ -3,6 +3,8 @@
 // Expert e has the rows offsets[e] .. offsets[e + 1] of R (offsets clamped to R).
 #pragma once
 
+#include <algorithm>
+
 #include "common.hpp"
 #include "kernels.hpp"
 #include "mx.hpp"
@@ -28,74 +30,158 @@ struct GroupedArgs {
   int32_t tiles_j;  // column tiles
   int32_t tiles_m;  // row tiles of one expert (dW)
   int32_t out_f32;
+  int32_t chunk;   // dW: rows of a group that one tile sums over at most
+  int32_t slices;  // dW: of `parts`
+  int32_t max_parts;
+  float* parts;    // [slices, C, J]: groups summed over in several parts
+  int32_t* plan;   // dW: kPlanHead words, max_parts records, 2 words a slice
 };
 
-// A tile's group and rows.
-struct GroupedTile {
-  int e;  // E: rows that no group has
-  int64_t slot0, rows;
-};
-
-__device__ __forceinline__ int64_t group_at(const GroupedArgs& a, int e) {
-  return min(max((int64_t)a.offsets[e], (int64_t)0), a.R);
+// dW's plan, which a kernel of its own writes: where each XCD's parts start (words 0 .. 8),
+// the parts' records (expert, first row, rows, slice of a.parts or -1), and of every slice
+// the expert and how many it is the first of (0: it is not the first of an expert's).
+constexpr int kPlanHead = 16;
+inline int64_t plan_words(int64_t max_parts, int64_t slices) {
+  return kPlanHead + 4 * max_parts + 2 * slices;
 }
 
-// Workgroup b's unit of those that the groups' tiles of TM rows make with tiles_j
-// column tiles each, the rows behind the last group (expert E) among them.  Every wave
-// does this by itself: lane l counts the tiles of a run of groups, a scan over the
-// lanes places them.  Units go to the XCDs in runs, so that one L2 sees an expert's.
-// False: no such unit.
+// How a group's rows are cut: into n tiles of `each` rows (the last may have fewer).
+struct GroupCut {
+  int n, each;
+};
+// Forward and dx: tiles of TM rows at most, of equal numbers of 32-row blocks.
 template <int TM>
-__device__ __forceinline__ bool find_tile(const GroupedArgs& a, int b, GroupedTile& t, int& tj) {
-  const int lane = threadIdx.x & 63;
-  const int per = (a.E + 64) / 64;  // groups a lane, of E + 1
-  const int g0 = lane * per, g1 = min(g0 + per, a.E + 1);
-  int count = 0;
-  if (g0 < g1) {
-    int64_t at = group_at(a, g0);
-    for (int g = g0; g < g1; ++g) {
-      const int64_t end = g < a.E ? group_at(a, g + 1) : a.R;
-      if (end > at) count += (int)((end - at + TM - 1) / TM);
-      at = end;
-    }
+__device__ __forceinline__ GroupCut cut_tiles(int rows) {
+  const int n = (rows + TM - 1) / TM;
+  return {n, n > 1 ? ((rows + n - 1) / n + 31) & ~31 : rows};
+}
+// dW: parts of `chunk` rows at most, of equal numbers of 64 rows; one for a group without
+// rows, too (its dW is zeros).
+__device__ __forceinline__ GroupCut cut_chunks(int rows, int chunk) {
+  const int n = rows > chunk ? (rows + chunk - 1) / chunk : 1;
+  return {n, n > 1 ? ((rows + n - 1) / n + 63) & ~63 : rows};
+}
+
+// A unit's place: a part of a group and a tile.
+struct GroupedUnit {
+  int e;            // a.E: rows that no group has
+  int slot0, rows;  // the part's sorted rows
+  int slice;        // dW: the slice of a.parts that it is summed in (-1: none)
+  int tile;
+};
+
+// Where the groups' parts lie in the order of all parts (DW: of a.E groups, else with the
+// rows behind the last as one more), in LDS: kGroupWords words at `lds`, by all of the
+// workgroup's threads.
+constexpr int kGroupWords = 4 * (kMaxExperts + 4) + 64;
+template <bool DW, int TM>
+struct Groups {
+  static constexpr int kStep = kMaxExperts + 4;
+  const GroupedArgs& a;
+  int *tab, *parts, *slices, *weights;  // offsets; parts, slices, weights before each group
+  int groups;
+
+  __device__ __forceinline__ int rows(int g) const {
+    return max((g < a.E ? tab[g + 1] : (int)a.R) - tab[g], 0);
   }
-  int incl = count;
+  __device__ __forceinline__ GroupCut cut(int g) const {
+    return DW ? cut_chunks(rows(g), a.chunk) : cut_tiles<TM>(rows(g));
+  }
+  // dW: what a part costs in each of its tiles, in 32-row blocks: its own and what it costs
+  // however few it has
+  static __device__ __forceinline__ int weigh(GroupCut c) { return (c.each + 31) / 32 + 9; }
+
+  __device__ __forceinline__ Groups(const GroupedArgs& a_, int* lds) : a(a_) {
+    tab = lds, parts = lds + kStep, slices = lds + 2 * kStep, weights = lds + 3 * kStep;
+    int* totals = lds + 4 * kStep;
+    groups = DW ? a.E : a.E + 1;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    for (int e = tid; e <= a.E; e += blockDim.x) tab[e] = min(max(a.offsets[e], 0), (int)a.R);
+    __syncthreads();
+    const int per = (groups + blockDim.x - 1) / blockDim.x;
+    const int g0 = min(tid * per, groups), g1 = min(g0 + per, groups);
+    int n = 0, s = 0, w = 0;
+    for (int g = g0; g < g1; ++g) {
+      const GroupCut c = cut(g);
+      n += c.n;
+      if (DW && c.n > 1) s += c.n;
+      if (DW) w += c.n * weigh(c);
+    }
+    int ni = n, si = s, wi = w;  // inclusive scans over the wave
 #pragma unroll
-  for (int s = 1; s < 64; s <<= 1) {
-    const int v = __shfl_up(incl, s, 64);
-    if (lane >= s) incl += v;
-  }
-  const int total = __builtin_amdgcn_readlane(incl, 63);
-  const int units = total * a.tiles_j;
-  const int per_x = (units + (int)kXcds - 1) / (int)kXcds;
-  const int u = (b % (int)kXcds) * per_x + b / (int)kXcds;
-  if (b / (int)kXcds >= per_x || u >= units) return false;
-  const int tile = u / a.tiles_j;
-  tj = u - tile * a.tiles_j;
-  const uint64_t mine = __ballot(incl > tile);
-  const int owner = __builtin_ctzll(mine);
-  int e = 0, part = 0;
-  if (lane == owner) {
-    int left = tile - (incl - count);
-    int64_t at = group_at(a, g0);
-    for (int g = g0; g < g1; ++g) {
-      const int64_t end = g < a.E ? group_at(a, g + 1) : a.R;
-      const int n = end > at ? (int)((end - at + TM - 1) / TM) : 0;
-      if (left < n) {
-        e = g, part = left;
-        break;
-      }
-      left -= n;
-      at = end;
+    for (int k = 1; k < 64; k <<= 1) {
+      const int x = __shfl_up(ni, k, 64), y = DW ? __shfl_up(si, k, 64) : 0;
+      const int z = DW ? __shfl_up(wi, k, 64) : 0;
+      if (lane >= k) ni += x, si += y, wi += z;
     }
+    if (lane == 63) totals[wave] = ni, totals[16 + wave] = si, totals[32 + wave] = wi;
+    __syncthreads();
+    n = ni - n, s = si - s, w = wi - w;
+    for (int k = 0; k < wave; ++k) n += totals[k], s += totals[16 + k], w += totals[32 + k];
+    for (int g = g0; g < g1; ++g) {
+      const GroupCut c = cut(g);
+      parts[g] = n;
+      n += c.n;
+      if (DW) {
+        slices[g] = s, weights[g] = w;
+        if (c.n > 1) s += c.n;
+        w += c.n * weigh(c);
+      }
+    }
+    if (tid == (int)blockDim.x - 1) parts[groups] = n, slices[groups] = s, weights[groups] = w;
+    __syncthreads();
   }
-  e = __builtin_amdgcn_readlane(e, owner);
-  part = __builtin_amdgcn_readlane(part, owner);
-  const int64_t at = group_at(a, e), end = e < a.E ? group_at(a, e + 1) : a.R;
-  t.e = e;
-  t.slot0 = at + (int64_t)part * TM;
-  t.rows = min(end - t.slot0, (int64_t)TM);
-  return true;
+  // The last group whose entry of t is at most v.
+  __device__ __forceinline__ int search(const int* t, int v) const {
+    int lo = 0, hi = groups - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (t[mid] <= v)
+        lo = mid;
+      else
+        hi = mid - 1;
+    }
+    return lo;
+  }
+  // The part that XCD x's start with: an eighth of all parts is before it, dW of their
+  // weight, as far as `cap` parts an XCD allow.
+  __device__ __forceinline__ int start(int x, int cap) const {
+    const int all = parts[groups];
+    if (x == 0) return 0;
+    if (!DW) return (int)((int64_t)all * x / kXcds);
+    const int w = (int)((int64_t)weights[groups] * x / kXcds);
+    const int g = search(weights, w);
+    const GroupCut c = cut(g);
+    const int p = min(parts[g] + (w - weights[g]) / weigh(c), all);
+    return max(min(p, cap * x), all - cap * ((int)kXcds - x));
+  }
+  // Workgroup b's unit: a part and one of `tiles` tiles of each.  Parts go to the XCDs in
+  // runs, so that one L2 sees an expert's.  False: no such unit.
+  __device__ __forceinline__ bool find(int b, int tiles, GroupedUnit& u) const {
+    const int i = b / kXcds, cap = (int)(gridDim.x / kXcds) / tiles;
+    const int part = start(b % kXcds, cap) + i / tiles;
+    if (part >= start(b % kXcds + 1, cap)) return false;
+    u.tile = i % tiles;
+    // (parts before a group without any are those before the next one: the last one counts)
+    const int g = __builtin_amdgcn_readfirstlane(search(parts, part));
+    const int n = rows(g), k = part - parts[g];
+    const GroupCut c = cut(g);
+    u.e = g;
+    u.slot0 = __builtin_amdgcn_readfirstlane(tab[g] + k * c.each);
+    u.rows = __builtin_amdgcn_readfirstlane(min(max(n - k * c.each, 0), c.each));
+    u.slice = __builtin_amdgcn_readfirstlane(DW && c.n > 1 ? slices[g] + k : -1);
+    return true;
+  }
+};
+
+// Upper bounds of the parts, and of the slices.
+inline int64_t grouped_chunks(int64_t R, int64_t E, int64_t chunk) { return R / chunk + E; }
+inline int64_t grouped_slices(int64_t R, int64_t chunk) { return R > chunk ? 2 * (R / chunk) : 0; }
+// Rows that one tile of dW sums over at most: a 128th of all tiles' rows, so that a group
+// that has most rows is spread over the chip, and 1024 at least.
+inline int64_t grouped_chunk_rows(int64_t R, int64_t N, int64_t K) {
+  const int64_t tiles = ((N + 255) / 256) * ((K + 255) / 256);
+  return std::max<int64_t>(1024, (R * tiles / 128 + 63) / 64 * 64);
 }
 
 // Upper bound of the tiles of TM rows (find_tile's total).

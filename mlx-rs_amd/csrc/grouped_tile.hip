@@ -5,12 +5,12 @@
 // in bf16 with f32 sums, and the forward product of e4m3 rows by e2m1 weights, each
 // with a power-of-two scale per 32 (modes mxfp8 and mxfp4).
 //
-// One kernel body.  An output tile is TM x TJ; a stage of 64 inputs (128 of the 8- and
-// 4-bit ones) of both operands goes straight to LDS by 16-byte loads while the stage
-// before is multiplied.  An operand whose inputs run along memory (x and W forward, dy
+// One kernel body.  An output tile is TM x TJ; a stage of SI inputs of both operands goes
+// straight to LDS by 16-byte loads while the stages before are multiplied.  An operand whose inputs run along memory (x and W forward, dy
 // of dx) lies in LDS as 128-byte rows; one whose inputs run across rows (W of dx, both
 // of dW) as rows of columns, read transposed by ds_read_b64_tr_b16.
 #include <algorithm>
+#include <type_traits>
 
 #include "grouped.hpp"
 #include "nn.hpp"
@@ -29,18 +29,39 @@ constexpr bool kMTrans = KIND == kDw;
 template <int KIND>
 constexpr bool kJTrans = KIND == kDw || KIND == kDx;
 
-// Bytes of a stage.  8-bit: TJ rows of 64 bytes of weights.
+// A stage has SI inputs: bytes of a row of either operand that runs along them ...
+template <int KIND, int SI>
+constexpr int kMRow = KIND == kForward8 ? SI : 2 * SI;
+template <int KIND, int SI>
+constexpr int kJRow = KIND == kForward8 ? SI / 2 : 2 * SI;
+// ... and of both operands (as much where they run across rows)
+template <int KIND, int TM, int TJ, int SI>
+constexpr int kStage = TM * kMRow<KIND, SI> + TJ * kJRow<KIND, SI>;
+// 8-bit: the scales of 512 inputs, 16 bytes a row, twice.  dW: indices of x's rows.
+constexpr int kIndexRows = 512;
 template <int KIND, int TM, int TJ>
-constexpr int kStage = TM * 128 + TJ * (KIND == kForward8 ? 64 : 128);
-// ... and of the scales of four stages: 16 bytes a row
-template <int KIND, int TM, int TJ>
-constexpr int kScales = KIND == kForward8 ? 16 * (TM + TJ) : 0;
-template <int KIND, int TM, int TJ, int STAGES>
-constexpr int kTileLds = STAGES * kStage<KIND, TM, TJ> + 2 * kScales<KIND, TM, TJ>;
+constexpr int kExtra = KIND == kForward8 ? 2 * 16 * (TM + TJ) : KIND == kDw ? 2 * 4 * kIndexRows
+                                                                            : 0;
+template <int KIND, int TM, int TJ, int SI, int STAGES>
+constexpr int kTileLds = STAGES * kStage<KIND, TM, TJ, SI> + kExtra<KIND, TM, TJ>;
 
-// Where 32-byte piece p of row r of a transposed operand lies: at p ^ tkey(r).  The four
-// rows and the two neighbouring pieces that half a wave reads at once lie in eight
-// different eighths of 256 bytes so.
+// Waves a SIMD: of as many workgroups as LDS holds (two at most)
+template <int KIND, int TM, int TJ, int WM, int WJ, int SI, int STAGES>
+constexpr int kWavesPerSimd = std::max(
+    1, WM * WJ / 4 * (2 * kTileLds<KIND, TM, TJ, SI, STAGES> <= 160 * 1024 ? 2 : 1));
+// LDS that a wave's output rows pass through, 32 at a time
+template <int TJ, int WJ>
+constexpr int kOutBytes = 32 * (4 * (TJ / WJ) + 16);
+
+// An operand in rows of P 16-byte pieces: piece p of row r lies at p ^ rkey<P>(r), so that
+// the 16 rows that a quarter of a wave reads a piece of lie in all 256 bytes of the banks.
+template <int P>
+__device__ __forceinline__ int rkey(int r) {
+  return (r / (16 / P)) & (P - 1);
+}
+// A transposed operand: 32-byte piece p of row r at p ^ tkey(r).  The four rows and the two
+// neighbouring pieces that half a wave reads at once lie in eight different eighths of 256
+// bytes so.
 __device__ __forceinline__ int tkey(int r) { return (r & 3) | ((r & 1) << 2); }
 
 // One load of 16 bytes a lane to consecutive LDS
@@ -53,167 +74,203 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const char* p, int64_t by
                                                               (int64_t)0xFFFFF000),
                                            kBufFlags);
 }
+// The workgroup's barrier, when at most N of this wave's loads are not back and its reads
+// and writes of LDS are.
+template <int N>
+__device__ __forceinline__ void stage_barrier() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
 
-// The tile of output rows [row0, row0 + rows) and columns [col0, ..): rows of the group
-// (forward, dx) or of dW.  slot0, len: the group's first row and rows (dW).
-template <int KIND, int TM, int TJ, int WM, int WJ, int STAGES, int NMB>
-__device__ __forceinline__ void tile_unit(const GroupedArgs& a, int e, int64_t slot0, int64_t len,
-                                          int row0, int rows, int col0, char* smem) {
+// A tile's place.
+struct TileAt {
+  int e;           // expert
+  int64_t slot0;   // forward, dx: the tile's first sorted row.  dW: the first summed over
+  int64_t len;     // dW: sorted rows summed over
+  int row0, rows;  // dW: output rows.  Else 0 and the tile's sorted rows
+  int col0;        // first column
+  void* out;       // of column 0 of the tile's first row
+  bool f32;
+};
+
+template <int KIND, int TM, int TJ, int WM, int WJ, int SI, int STAGES, int NMB>
+__device__ __forceinline__ void tile_unit(const GroupedArgs& a, const TileAt& at, char* smem) {
   constexpr bool F8 = KIND == kForward8, MT = kMTrans<KIND>, JT = kJTrans<KIND>;
   constexpr int NW = WM * WJ;
   constexpr int MB = TM / WM / 32, NB = TJ / WJ / 32;  // 32 x 32 blocks of a wave
   constexpr int NA = NMB > 0 ? NMB : 1;
-  constexpr int kM = TM * 128;  // the J operand's place in a stage
-  constexpr int ML = TM / 8 / NW, JL = (F8 ? TJ / 16 : TJ / 8) / NW;  // loads a wave
-  static_assert(ML >= 1 && JL >= 1 && MB >= 1 && NB >= 1, "tile");
-  const int tid = threadIdx.x, lane = tid & 63;
+  constexpr int MR = kMRow<KIND, SI>, JR = kJRow<KIND, SI>;
+  constexpr int MP = MT ? TM / 8 : MR / 16, JP = JT ? TJ / 8 : JR / 16;  // pieces a row
+  constexpr int kM = TM * MR, kS = kStage<KIND, TM, TJ, SI>;
+  constexpr int ML = kM / 1024 / NW, JL = TJ * JR / 1024 / NW;  // loads a wave and stage
+  static_assert(ML >= 1 && JL >= 1 && MB >= 1 && NB >= 1 && SI % 32 == 0, "tile");
+  static_assert((!MT || TM >= 128) && (!JT || TJ >= 128), "eight 32-byte pieces a row");
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));
+  const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WJ, wj = wave % WJ;
   const int c = lane & 31, h = lane >> 5;
+  const int rows = at.rows;
 
   // ---- where the operands start, how far apart their rows are, how many stages
-  const int esM = F8 ? 1 : 2;
-  const int64_t ldm = MT ? (int64_t)a.C * 2 : (int64_t)a.C * esM;  // bytes
+  const int64_t ldm = F8 ? (int64_t)a.C : (int64_t)a.C * 2;  // bytes
   const int64_t ldj = JT ? (int64_t)a.J * 2 : F8 ? (int64_t)a.C / 2 : (int64_t)a.C * 2;
   const bool mapped = a.rows != nullptr;  // x's rows (M forward, J of dW)
-  const int64_t cn = MT ? len : a.C;      // inputs
-  constexpr int SI = F8 ? 128 : 64;       // a stage's
-  const int T = (int)((cn + SI - 1) / SI);
+  const int T = (int)(((MT ? at.len : a.C) + SI - 1) / SI);
+  char* extra = smem + STAGES * kS;
 
   // ---- M
-  const char* mp;
+  const char* mp = static_cast<const char*>(a.m);
   int64_t mbytes;
   uint32_t moff[ML];
+  const auto mrow = [&](int i) { return (wave * ML + i) * (64 / MP) + lane / MP; };
   if constexpr (MT) {
-    mp = static_cast<const char*>(a.m) + slot0 * ldm + 2 * (int64_t)row0;
-    mbytes = len * ldm - 2 * (int64_t)row0;
-    constexpr int P = TM / 8;  // 16-byte pieces a row
+    mp += at.slot0 * ldm + 2 * (int64_t)at.row0;
+    mbytes = at.len * ldm - 2 * (int64_t)at.row0;
 #pragma unroll
     for (int i = 0; i < ML; ++i) {
-      const int r = (wave * ML + i) * (64 / P) + lane / P, p = lane % P;
+      const int r = mrow(i), p = lane % MP;
       moff[i] = (uint32_t)(r * ldm) + 32 * ((p >> 1) ^ tkey(r)) + 16 * (p & 1);
     }
   } else {
     const bool map = mapped && KIND != kDx;
-    mp = static_cast<const char*>(a.m) + (map ? 0 : (slot0 + row0) * ldm);
+    if (!map) mp += at.slot0 * ldm;
     mbytes = map ? a.x_rows * ldm : rows * ldm;
 #pragma unroll
     for (int i = 0; i < ML; ++i) {
-      const int r = (wave * ML + i) * 8 + (lane >> 3);
-      int64_t at = (int64_t)r * ldm;
+      const int r = mrow(i);
+      int64_t x = r;
       bool ok = r < rows;
       if (map) {
-        const int x = as_global<const int32_t>(a.rows)[slot0 + row0 + min(r, rows - 1)];
+        x = as_global<const int32_t>(a.rows)[at.slot0 + min(r, rows - 1)];
         ok = ok && x >= 0 && x < a.x_rows;
-        at = x * ldm;
       }
-      moff[i] = ok ? (uint32_t)at + 16 * ((lane & 7) ^ swz(r)) : kPastEnd;
+      moff[i] = ok ? (uint32_t)(x * ldm) + 16 * ((lane % MP) ^ rkey<MP>(r)) : kPastEnd;
     }
   }
   // ---- J
-  const char* jp;
+  const char* jp = static_cast<const char*>(a.j);
   int64_t jbytes;
   uint32_t joff[JL];
+  const auto jrow = [&](int i) { return (wave * JL + i) * (64 / JP) + lane / JP; };
   if constexpr (JT) {
     const bool map = KIND == kDw && mapped;
-    jp = static_cast<const char*>(a.j) + 2 * (int64_t)col0 +
-         (KIND == kDw ? (map ? 0 : slot0 * ldj) : (int64_t)e * a.C * ldj);
-    jbytes = (KIND == kDw ? (map ? a.x_rows : len) : (int64_t)a.C) * ldj - 2 * (int64_t)col0;
-    constexpr int P = TJ / 8;
+    jp += 2 * (int64_t)at.col0 +
+          (KIND == kDw ? (map ? 0 : at.slot0 * ldj) : (int64_t)at.e * a.C * ldj);
+    jbytes = (KIND == kDw ? (map ? a.x_rows : at.len) : (int64_t)a.C) * ldj - 2 * (int64_t)at.col0;
 #pragma unroll
     for (int i = 0; i < JL; ++i) {
-      const int r = (wave * JL + i) * (64 / P) + lane / P, p = lane % P;
+      const int r = jrow(i), p = lane % JP;
       joff[i] = (map ? 0u : (uint32_t)(r * ldj)) + 32 * ((p >> 1) ^ tkey(r)) + 16 * (p & 1);
     }
   } else {
-    jp = static_cast<const char*>(a.j) + ((int64_t)e * a.J + col0) * ldj;
-    jbytes = (int64_t)(a.J - col0) * ldj;
+    jp += ((int64_t)at.e * a.J + at.col0) * ldj;
+    jbytes = (int64_t)(a.J - at.col0) * ldj;
 #pragma unroll
     for (int i = 0; i < JL; ++i) {
-      const int r = F8 ? (wave * JL + i) * 16 + (lane >> 2) : (wave * JL + i) * 8 + (lane >> 3);
-      const int p = F8 ? (lane & 3) ^ ((r >> 2) & 3) : (lane & 7) ^ swz(r);
-      joff[i] = (uint32_t)(r * ldj) + 16 * p;
+      const int r = jrow(i);
+      joff[i] = (uint32_t)(r * ldj) + 16 * ((lane % JP) ^ rkey<JP>(r));
     }
   }
-  // the rows of x of a stage of dW, found a stage ahead
-  int xrow[KIND == kDw ? JL : 1];
-  auto find_x = [&](int t) {
+  // ---- dW: kIndexRows indices of x's rows from sorted row q kIndexRows of the group on,
+  // straight to LDS (past the rows 0, of rows that are not read)
+  auto issue_index = [&](int q) {
     if constexpr (KIND == kDw) {
-      if (mapped) {
-        constexpr int P = TJ / 8;
+      const int64_t from = (int64_t)q * kIndexRows;
+      const __amdgpu_buffer_rsrc_t r =
+          rsrc(reinterpret_cast<const char*>(a.rows + at.slot0 + from), 4 * (at.len - from));
+      for (int i = wave; i < kIndexRows / 64; i += NW)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            r, (lds_ptr)(extra + 4 * kIndexRows * (q & 1) + 256 * i), 4, 256 * i + 4 * lane, 0, 0,
+            0);
+    }
+  };
+  // ---- 8-bit: the scales of inputs 512 q .. 512 q + 511, 16 bytes a row
+  const int G = a.C / 32;
+  auto issue_scales = [&](int q) {
+    if constexpr (F8) {
+      char* S = extra + 16 * (TM + TJ) * (q & 1);
+      if ((G & 3) == 0) {
+        // by aligned words, 64 rows a load
+        const __amdgpu_buffer_rsrc_t mr =
+            rsrc(reinterpret_cast<const char*>(a.ms) + (mapped ? 0 : at.slot0 * G) + 16 * q,
+                 (mapped ? a.x_rows : rows) * (int64_t)G - 16 * q);
+        const __amdgpu_buffer_rsrc_t jr =
+            rsrc(reinterpret_cast<const char*>(a.js) + ((int64_t)at.e * a.J + at.col0) * G + 16 * q,
+                 (int64_t)(a.J - at.col0) * G - 16 * q);
+        for (int i = wave; i < (TM + TJ) / 64; i += NW) {
+          const bool isj = i >= TM / 64;
+          const int r = 64 * i + lane - (isj ? TM : 0);
+          uint32_t off = (uint32_t)r * G;
+          if (!isj) {
+            if (r >= rows) off = kPastEnd;
+            if (mapped && r < rows) {
+              const int x = as_global<const int32_t>(a.rows)[at.slot0 + r];
+              off = x >= 0 && x < a.x_rows ? (uint32_t)x * G : kPastEnd;
+            }
+          }
+          load_lds(isj ? jr : mr, S + 1024 * i, off);
+        }
+      } else {
+        // rows at any address, byte by byte; zeros past the row
+        for (int r = tid; r < TM + TJ; r += 64 * NW) {
+          const uint8_t* p = nullptr;
+          if (r >= TM) {
+            if (at.col0 + r - TM < a.J) p = a.js + ((int64_t)at.e * a.J + at.col0 + r - TM) * G;
+          } else if (r < rows) {
+            int64_t x = at.slot0 + r;
+            if (mapped) x = as_global<const int32_t>(a.rows)[x];
+            if (x >= 0 && x < a.x_rows) p = a.ms + x * G;
+          }
+          uint32_t v[4] = {0, 0, 0, 0};
+          if (p) {
 #pragma unroll
-        for (int i = 0; i < JL; ++i) {
-          const int64_t r = (int64_t)t * 64 + (wave * JL + i) * (64 / P) + lane / P;
-          xrow[i] = r < len ? as_global<const int32_t>(a.rows)[slot0 + r] : -1;
+            for (int i = 0; i < 16; ++i)
+              if (16 * q + i < G) v[i >> 2] |= (uint32_t)p[16 * q + i] << (8 * (i & 3));
+          }
+          *reinterpret_cast<u32x4_t*>(S + 16 * r) = u32x4_t{v[0], v[1], v[2], v[3]};
         }
       }
     }
   };
 
-  // ---- a stage's loads
-  const int mchunks = F8 ? a.C / 16 : a.C / 8;  // 16-byte pieces of an M row, of a J row
-  const int jchunks = F8 ? a.C / 32 : a.C / 8;
-  auto issue = [&](int t, char* S) {
-    const int64_t mo = MT ? (int64_t)t * 64 * ldm : (int64_t)t * 128;
-    const __amdgpu_buffer_rsrc_t mr = rsrc(mp + mo, mbytes - mo);
+  // ---- a stage's loads, always as many (past the last stage of nothing)
+  const int mpieces = (int)(ldm / 16), jpieces = (int)(ldj / 16);
+  auto issue_m = [&](int t, char* S) {
+    if (F8 && t % (512 / SI) == 0 && t < T) issue_scales(t / (512 / SI));
+    const int64_t mo = MT ? (int64_t)t * SI * ldm : (int64_t)t * MR;
+    const __amdgpu_buffer_rsrc_t mr = rsrc(mp + mo, t < T ? mbytes - mo : 0);
 #pragma unroll
     for (int i = 0; i < ML; ++i) {
       bool ok = true;
-      if constexpr (!MT)
-        ok = 8 * t + ((lane & 7) ^ swz((wave * ML + i) * 8 + (lane >> 3))) < mchunks;
+      if constexpr (!MT) ok = MP * t + ((lane % MP) ^ rkey<MP>(mrow(i))) < mpieces;
       load_lds(mr, S + (wave * ML + i) * 1024, ok ? moff[i] : kPastEnd);
     }
+  };
+  auto issue_j = [&](int t, char* S) {
     if constexpr (KIND == kDw) {
       if (mapped) {
-        const __amdgpu_buffer_rsrc_t jr = rsrc(jp, jbytes);
+        constexpr int kPer = kIndexRows / SI;  // stages a part of the indices
+        if (t % kPer == 0 && t > 0) issue_index(t / kPer + 1);
+        const __amdgpu_buffer_rsrc_t jr = rsrc(jp, t < T ? jbytes : 0);
+        const int* xi = reinterpret_cast<const int*>(extra) + t * SI % (2 * kIndexRows);
 #pragma unroll
-        for (int i = 0; i < JL; ++i)
+        for (int i = 0; i < JL; ++i) {
+          const int64_t x = xi[jrow(i)];
+          const bool ok = x >= 0 && x < a.x_rows && (int64_t)t * SI + jrow(i) < at.len;
           load_lds(jr, S + kM + (wave * JL + i) * 1024,
-                   xrow[i] >= 0 && xrow[i] < a.x_rows ? joff[i] + (uint32_t)(xrow[i] * ldj)
-                                                      : kPastEnd);
+                   ok ? joff[i] + (uint32_t)(x * ldj) : kPastEnd);
+        }
         return;
       }
     }
-    const int64_t jo = JT ? (int64_t)t * 64 * ldj : (int64_t)t * (F8 ? 64 : 128);
-    const __amdgpu_buffer_rsrc_t jr = rsrc(jp + jo, jbytes - jo);
+    const int64_t jo = JT ? (int64_t)t * SI * ldj : (int64_t)t * JR;
+    const __amdgpu_buffer_rsrc_t jr = rsrc(jp + jo, t < T ? jbytes - jo : 0);
 #pragma unroll
     for (int i = 0; i < JL; ++i) {
       bool ok = true;
-      if constexpr (!JT) {
-        const int r = F8 ? (wave * JL + i) * 16 + (lane >> 2) : (wave * JL + i) * 8 + (lane >> 3);
-        const int p = F8 ? (lane & 3) ^ ((r >> 2) & 3) : (lane & 7) ^ swz(r);
-        ok = (F8 ? 4 : 8) * t + p < jchunks;
-      }
+      if constexpr (!JT) ok = JP * t + ((lane % JP) ^ rkey<JP>(jrow(i))) < jpieces;
       load_lds(jr, S + kM + (wave * JL + i) * 1024, ok ? joff[i] : kPastEnd);
-    }
-  };
-  // ---- the scales of stages 4 q .. 4 q + 3, 16 bytes a row (zeros past the row's)
-  const int G = a.C / 32;
-  char* scl = smem + STAGES * kStage<KIND, TM, TJ>;
-  auto issue_scales = [&](int q, char* S) {
-    if constexpr (F8) {
-      for (int r = tid; r < TM + TJ; r += 64 * NW) {
-        const bool isj = r >= TM;
-        const int rr = isj ? r - TM : r;
-        const uint8_t* p = nullptr;
-        if (isj) {
-          if (col0 + rr < a.J) p = a.js + ((int64_t)e * a.J + col0 + rr) * G;
-        } else if (rr < rows) {
-          int64_t x = slot0 + row0 + rr;
-          if (mapped) {
-            x = as_global<const int32_t>(a.rows)[x];
-            if (x < 0 || x >= a.x_rows) x = -1;
-          }
-          if (x >= 0) p = a.ms + x * G;
-        }
-        uint32_t v[4] = {0, 0, 0, 0};
-        if (p) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (16 * q + i < G) v[i >> 2] |= (uint32_t)p[16 * q + i] << (8 * (i & 3));
-        }
-        *reinterpret_cast<u32x4_t*>(S + 16 * r) = u32x4_t{v[0], v[1], v[2], v[3]};
-      }
     }
   };
 
@@ -225,14 +282,13 @@ __device__ __forceinline__ void tile_unit(const GroupedArgs& a, int e, int64_t s
     for (int j = 0; j < NB; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
-  const int m0 = wm * MB, j0 = wj * NB;  // the wave's first blocks
+  // the wave's blocks: rows 32 (wm + WM i), so that a short tile's are spread over the
+  // waves; columns 32 (j0 + j)
+  const int j0 = wj * NB;
   // transposed: byte of the lane's four values of block 0, rows 8 h + (lane % 16) / 4
   const int ti = lane & 15, tg = (lane >> 4) & 1;
   const int tlow = ((tg ^ tkey(ti >> 2)) << 5) + 8 * (ti & 3);
-  auto frag = [&](const char* O, int blk, int ks, bool trans, int row_bytes) -> bf16x8_t {
-    if (!trans)
-      return as_bf16x8(*reinterpret_cast<const u32x4_t*>(O + blk * 4096 + c * 128 +
-                                                         16 * ((2 * ks + h) ^ swz(c))));
+  const auto trans = [&](const char* O, int blk, int ks, int row_bytes) -> bf16x8_t {
     const char* p = O + (8 * h + (ti >> 2) + 16 * ks) * row_bytes + (tlow ^ (blk << 6));
     typedef __attribute__((address_space(3))) s16x4_t* tptr;
     const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tptr)(lds_ptr)p);
@@ -240,96 +296,136 @@ __device__ __forceinline__ void tile_unit(const GroupedArgs& a, int e, int64_t s
     const u32x2_t l2 = __builtin_bit_cast(u32x2_t, lo), h2 = __builtin_bit_cast(u32x2_t, hi);
     return as_bf16x8(u32x4_t{l2.x, l2.y, h2.x, h2.y});
   };
-  auto products = [&](const char* S, const char* SC, int sub) {
-    if constexpr (NMB > 0) {
-      if constexpr (!F8) {
+  // The operands of a step: 16 inputs, or 64 of the 8- and 4-bit ones and their scales.
+  constexpr int KS = SI / (F8 ? 64 : 16);
+  static_assert(KS % 2 == 0, "two sets of operands");
+  typedef std::conditional_t<F8, i32x8_t, bf16x8_t> Op;
+  Op mf[2][NA], jf[2][NB];
+  uint32_t ms[2][NA], js[2][NB];
+  // of step ks of the stage t at S into set p
+  auto read = [&](const char* S, int t, int ks, int p) {
+    if constexpr (NMB > 0 && !F8) {
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-          bf16x8_t mf[NA], jf[NB];
+      for (int j = 0; j < NB; ++j) {
+        if constexpr (JT)
+          jf[p][j] = trans(S + kM, j0 + j, ks, 2 * TJ);
+        else
+          jf[p][j] = as_bf16x8(*reinterpret_cast<const u32x4_t*>(
+              S + kM + (32 * (j0 + j) + c) * JR + 16 * ((2 * ks + h) ^ rkey<JP>(c))));
+      }
 #pragma unroll
-          for (int j = 0; j < NB; ++j) jf[j] = frag(S + kM, j0 + j, ks, JT, 2 * TJ);
-#pragma unroll
-          for (int i = 0; i < NA; ++i) mf[i] = frag(S, m0 + i, ks, MT, 2 * TM);
-#pragma unroll
-          for (int i = 0; i < NA; ++i)
-#pragma unroll
-            for (int j = 0; j < NB; ++j) acc[i][j] = mfma32x32x16(jf[j], mf[i], acc[i][j]);
-        }
-      } else {
-        uint32_t ms[NA], js[NB];
+      for (int i = 0; i < NA; ++i) {
+        if constexpr (MT)
+          mf[p][i] = trans(S, wm + WM * i, ks, 2 * TM);
+        else
+          mf[p][i] = as_bf16x8(*reinterpret_cast<const u32x4_t*>(
+              S + (32 * (wm + WM * i) + c) * MR + 16 * ((2 * ks + h) ^ rkey<MP>(c))));
+      }
+    } else if constexpr (NMB > 0) {
+      // lane half h: 4-bit inputs 32 h .. 32 h + 31 of 64; 8-bit ones 16 h .. + 15 and
+      // 32 + 16 h .. + 15; the scales of inputs 32 h .. + 31
+      if (ks == 0) {
+        const char* SC =
+            extra + 16 * (TM + TJ) * (t / (512 / SI) & 1) + t % (512 / SI) * (SI / 32);
 #pragma unroll
         for (int i = 0; i < NA; ++i)
-          ms[i] = *reinterpret_cast<const uint32_t*>(SC + 16 * (32 * (m0 + i) + c) + 4 * sub) >>
-                  (8 * h);
+          ms[0][i] = *reinterpret_cast<const uint32_t*>(SC + 16 * (32 * (wm + WM * i) + c));
 #pragma unroll
         for (int j = 0; j < NB; ++j)
-          js[j] = *reinterpret_cast<const uint32_t*>(SC + 16 * (TM + 32 * (j0 + j) + c) +
-                                                     4 * sub) >>
-                  (8 * h);
+          js[0][j] = *reinterpret_cast<const uint32_t*>(SC + 16 * (TM + 32 * (j0 + j) + c));
+      }
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          i32x8_t mf[NA], jf[NB];
+      for (int j = 0; j < NB; ++j) {
+        const i32x4_t v = *reinterpret_cast<const i32x4_t*>(
+            S + kM + (32 * (j0 + j) + c) * JR + 16 * ((2 * ks + h) ^ rkey<JP>(c)));
+        jf[p][j] = i32x8_t{v.x, v.y, v.z, v.w, 0, 0, 0, 0};
+      }
 #pragma unroll
-          for (int j = 0; j < NB; ++j) {
-            const int r = 32 * (j0 + j) + c;
-            const i32x4_t v = *reinterpret_cast<const i32x4_t*>(
-                S + kM + 64 * r + 16 * ((2 * s + h) ^ ((r >> 2) & 3)));
-            jf[j] = i32x8_t{v.x, v.y, v.z, v.w, 0, 0, 0, 0};
-          }
-#pragma unroll
-          for (int i = 0; i < NA; ++i) {
-            const char* p = S + 4096 * (m0 + i) + 128 * c;
-            const i32x4_t lo =
-                *reinterpret_cast<const i32x4_t*>(p + 16 * ((4 * s + h) ^ swz(c)));
-            const i32x4_t hi =
-                *reinterpret_cast<const i32x4_t*>(p + 16 * ((4 * s + 2 + h) ^ swz(c)));
-            mf[i] = i32x8_t{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-          }
-#pragma unroll
-          for (int i = 0; i < NA; ++i)
-#pragma unroll
-            for (int j = 0; j < NB; ++j) {
-              if (s == 0)
-                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-                    jf[j], mf[i], acc[i][j], 4, 0, 0, js[j], 0, ms[i]);
-              else
-                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-                    jf[j], mf[i], acc[i][j], 4, 0, 2, js[j], 2, ms[i]);
-            }
-        }
+      for (int i = 0; i < NA; ++i) {
+        const char* q = S + (32 * (wm + WM * i) + c) * MR;
+        const i32x4_t lo = *reinterpret_cast<const i32x4_t*>(q + 16 * ((4 * ks + h) ^ rkey<MP>(c)));
+        const i32x4_t hi =
+            *reinterpret_cast<const i32x4_t*>(q + 16 * ((4 * ks + 2 + h) ^ rkey<MP>(c)));
+        mf[p][i] = i32x8_t{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
       }
     }
   };
-
-  find_x(0);
-  if (T > 0) {
-    issue(0, smem);
-    if (F8) issue_scales(0, scl);
-    find_x(1);
-  }
-  for (int t = 0; t < T; ++t) {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (t + 1 < T) {
-      issue(t + 1, smem + ((t + 1) & 1) * kStage<KIND, TM, TJ>);
-      if (F8 && ((t + 1) & 3) == 0)
-        issue_scales((t + 1) >> 2, scl + (((t + 1) >> 2) & 1) * kScales<KIND, TM, TJ>);
-      find_x(t + 2);
+  // step ks of a stage, from set p
+  auto multiply = [&](int ks, int p) {
+    if constexpr (NMB > 0) {
+      if (F8 && ks == 0) {
+        // this half's scales of the stage, at bytes 0 and 2
+#pragma unroll
+        for (int i = 0; i < NA; ++i) ms[1][i] = ms[0][i] >> (8 * h);
+#pragma unroll
+        for (int j = 0; j < NB; ++j) js[1][j] = js[0][j] >> (8 * h);
+      }
+#pragma unroll
+      for (int i = 0; i < NA; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+          if constexpr (!F8)
+            acc[i][j] = mfma32x32x16(jf[p][j], mf[p][i], acc[i][j]);
+          else if (ks == 0)
+            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+                jf[p][j], mf[p][i], acc[i][j], 4, 0, 0, js[1][j], 0, ms[1][i]);
+          else
+            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+                jf[p][j], mf[p][i], acc[i][j], 4, 0, 2, js[1][j], 2, ms[1][i]);
+        }
     }
-    products(smem + (t & 1) * kStage<KIND, TM, TJ>,
-             scl + ((t >> 2) & 1) * kScales<KIND, TM, TJ>, t & 3);
+  };
+
+  if (KIND == kDw && mapped) {
+    issue_index(0);
+    issue_index(1);
+    stage_barrier<0>();
   }
-  __syncthreads();
+  // ---- The operands of a step are read during the step before it, so a stage's barrier
+  // stands before its last step, when all waves have read the stage for good; the stage
+  // STAGES ahead then takes its place.  A stage's loads are back when no more are out than
+  // the later stages' (what else is loaded on the way only makes it wait for more).
+#pragma unroll
+  for (int t = 0; t < STAGES; ++t) {
+    issue_m(t, smem + t * kS);
+    issue_j(t, smem + t * kS);
+  }
+  stage_barrier<(STAGES - 1) * (ML + JL)>();
+  read(smem, 0, 0, 0);
+  int from = 0, last = (STAGES - 1) * kS;  // this stage's place, the one's before
+#pragma nounroll
+  for (int t = 0; t < T; ++t) {
+    const int next = from + kS < STAGES * kS ? from + kS : 0;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      if (ks == KS - 1) {
+        stage_barrier<(STAGES - 2) * (ML + JL)>();
+        read(smem + next, t + 1, 0, 0);
+        issue_m(t + STAGES, smem + from);
+      } else {
+        read(smem + from, t, ks + 1, (ks + 1) & 1);
+        if (ks == 0 && t > 0) issue_j(t - 1 + STAGES, smem + last);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(ks, ks & 1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    last = from;
+    from = next;
+  }
+  // nothing may be on its way to LDS when it is used again
+  stage_barrier<0>();
 
   // ---- out, 32 rows at a time through the wave's own LDS: lane (c, h) holds output row
   // c and columns 8 q + 4 h .. + 3 of each 32; rows leave by 16-byte stores
   if constexpr (NMB > 0) {
     constexpr int WC = 32 * NB;  // the wave's columns
-    char* O = smem + wave * (32 * (4 * WC + 16));
-    const int wcol0 = col0 + 32 * j0;
+    char* O = smem + wave * kOutBytes<TJ, WJ>;
+    const int wcol0 = 32 * j0, cols = a.J - at.col0;
 #pragma unroll
     for (int i = 0; i < NA; ++i) {
-      const int row1 = 32 * (m0 + i);
-      const int es = a.out_f32 ? 4 : 2, stride = WC * es + 16;
+      const int row1 = 32 * (wm + WM * i);
+      const int es = at.f32 ? 4 : 2, stride = WC * es + 16;
 #pragma unroll
       for (int j = 0; j < NB; ++j)
 #pragma unroll
@@ -337,21 +433,18 @@ __device__ __forceinline__ void tile_unit(const GroupedArgs& a, int e, int64_t s
           const f32x4_t v{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2],
                           acc[i][j][4 * q + 3]};
           char* p = O + c * stride + (32 * j + 8 * q + 4 * h) * es;
-          if (a.out_f32)
+          if (at.f32)
             *reinterpret_cast<f32x4_t*>(p) = v;
           else
             *reinterpret_cast<u32x2_t*>(p) = u32x2_t{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
         }
       wave_sync();
       const int cpr = WC * es / 16;  // 16-byte runs a row
-      const int64_t obase =
-          (KIND == kDw ? (int64_t)e * a.C + row0 : slot0 + row0) * (int64_t)a.J;
       for (int id = lane; id < 32 * cpr; id += 64) {
         const int r = id / cpr, cc = id - r * cpr;
         const int col = wcol0 + cc * 16 / es;
-        if (row1 + r < rows && col < a.J)
-          *(gptr<u32x4_t>)(as_global<char>(a.out) +
-                           (obase + (int64_t)(row1 + r) * a.J + col) * es) =
+        if (row1 + r < rows && col < cols)
+          *(gptr<u32x4_t>)(as_global<char>(at.out) + ((int64_t)(row1 + r) * a.J + col) * es) =
               *reinterpret_cast<const u32x4_t*>(O + r * stride + 16 * cc);
       }
       wave_sync();
@@ -371,54 +464,67 @@ __device__ __forceinline__ void zero_rows(const GroupedArgs& a, int64_t slot0, i
   }
 }
 
-template <int KIND, int TM, int TJ, int WM, int WJ, int STAGES>
-__global__ __launch_bounds__(64 * WM * WJ, 2) void grouped_tile_kernel(GroupedArgs a) {
+template <int KIND, int TM, int TJ, int WM, int WJ, int SI, int STAGES>
+__global__ __launch_bounds__(64 * WM * WJ, (kWavesPerSimd<KIND, TM, TJ, WM, WJ, SI, STAGES>))
+void grouped_tile_kernel(GroupedArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   constexpr int MB = TM / WM / 32;
-  int e, row0 = 0, rows, tj;
-  int64_t slot0, len = 0;
-  if constexpr (KIND == kDw) {
-    const int units = a.E * a.tiles_m * a.tiles_j;
-    const int per_x = (units + (int)kXcds - 1) / (int)kXcds;
-    const int b = blockIdx.x, u = (b % (int)kXcds) * per_x + b / (int)kXcds;
-    if (b / (int)kXcds >= per_x || u >= units) return;
-    const int tile = u / a.tiles_j;
-    tj = u - tile * a.tiles_j;
-    e = tile / a.tiles_m;
-    row0 = (tile - e * a.tiles_m) * TM;
-    rows = min(TM, a.C - row0);
-    slot0 = group_at(a, e);
-    len = max(group_at(a, e + 1) - slot0, (int64_t)0);
+  constexpr bool DW = KIND == kDw;
+  GroupedUnit u;
+  if constexpr (DW) {
+    const int tiles = a.tiles_m * a.tiles_j, x = blockIdx.x % kXcds, i = blockIdx.x / kXcds;
+    const int part = a.plan[x] + i / tiles;
+    if (part >= a.plan[x + 1]) return;
+    const int4 r = reinterpret_cast<const int4*>(a.plan + kPlanHead)[part];
+    u.tile = i % tiles;
+    u.e = r.x, u.slot0 = r.y, u.rows = r.z, u.slice = r.w;
   } else {
-    GroupedTile t;
-    if (!find_tile<TM>(a, blockIdx.x, t, tj)) return;
-    if (t.e == a.E) {
-      zero_rows(a, t.slot0, (int)t.rows, tj * TJ, TJ);
+    const Groups<DW, TM> groups(a, reinterpret_cast<int*>(smem));
+    const bool found = groups.find(blockIdx.x, a.tiles_j, u);
+    __syncthreads();  // (the stages take its place)
+    if (!found) return;
+  }
+  TileAt at;
+  at.e = u.e, at.slot0 = u.slot0;
+  at.f32 = a.out_f32;
+  if constexpr (DW) {
+    const int tn = u.tile / a.tiles_j;
+    at.len = u.rows;
+    at.row0 = tn * TM, at.rows = min(TM, a.C - at.row0);
+    at.col0 = (u.tile - tn * a.tiles_j) * TJ;
+    // a part of a group of several: its sums in f32, to be joined
+    int64_t first = ((int64_t)at.e * a.C + at.row0) * a.J + at.col0;
+    at.out = a.out;
+    if (u.slice >= 0) {
+      if (u.slice >= a.slices) return;
+      first = ((int64_t)u.slice * a.C + at.row0) * a.J + at.col0;
+      at.out = a.parts;
+      at.f32 = true;
+    }
+    at.out = static_cast<char*>(at.out) + first * (at.f32 ? 4 : 2);
+  } else {
+    at.len = 0, at.row0 = 0, at.rows = u.rows;
+    at.col0 = u.tile * TJ;
+    if (u.e == a.E) {
+      zero_rows(a, u.slot0, u.rows, at.col0, TJ);
       return;
     }
-    e = t.e, slot0 = t.slot0, rows = (int)t.rows;
+    at.out = static_cast<char*>(a.out) + ((int64_t)u.slot0 * a.J + at.col0) * (at.f32 ? 4 : 2);
   }
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // 32-row blocks that hold rows of this wave's
-  const int nmb = min(max((rows + 31) / 32 - (wave / WJ) * MB, 0), MB);
-#define MLXR_GT_UNIT(N) \
-  tile_unit<KIND, TM, TJ, WM, WJ, STAGES, N>(a, e, slot0, len, row0, rows, tj * TJ, smem)
-  if constexpr (MB == 4) {
-    if (nmb == 4)
-      MLXR_GT_UNIT(4);
-    else if (nmb == 3)
-      MLXR_GT_UNIT(3);
-    else if (nmb == 2)
+  const int nmb = max((at.rows + 31) / 32 - wave / WJ + WM - 1, 0) / WM;
+#define MLXR_GT_UNIT(N) tile_unit<KIND, TM, TJ, WM, WJ, SI, STAGES, N>(a, at, smem)
+  if constexpr (MB == 2) {
+    if (nmb == 2)
       MLXR_GT_UNIT(2);
     else if (nmb == 1)
       MLXR_GT_UNIT(1);
     else
       MLXR_GT_UNIT(0);
   } else {
-    static_assert(MB == 2, "wave tiles of 64 or 128 rows");
-    if (nmb == 2)
-      MLXR_GT_UNIT(2);
-    else if (nmb == 1)
+    static_assert(MB == 1, "wave tiles of 32 or 64 rows");
+    if (nmb == 1)
       MLXR_GT_UNIT(1);
     else
       MLXR_GT_UNIT(0);
@@ -426,46 +532,120 @@ __global__ __launch_bounds__(64 * WM * WJ, 2) void grouped_tile_kernel(GroupedAr
 #undef MLXR_GT_UNIT
 }
 
-template <int KIND, int TM, int TJ, int WM, int WJ, int STAGES>
+// dW's plan, in one workgroup (every workgroup of the products finding its part by itself
+// took 80 us of 310 at 128 experts of 768 x 2048); cap: parts an XCD that the grid holds.
+__global__ __launch_bounds__(1024) void grouped_plan_kernel(GroupedArgs a, int cap) {
+  __shared__ int lds[kGroupWords];
+  const Groups<true, 64> groups(a, lds);
+  const int tid = threadIdx.x;
+  if (tid <= (int)kXcds) a.plan[tid] = min(groups.start(tid, cap), a.max_parts);
+  int4* records = reinterpret_cast<int4*>(a.plan + kPlanHead);
+  int2* first = reinterpret_cast<int2*>(a.plan + kPlanHead + 4 * a.max_parts);
+  const int all = min(groups.parts[groups.groups], a.max_parts);
+  for (int p = tid; p < all; p += 1024) {
+    const int g = groups.search(groups.parts, p), k = p - groups.parts[g];
+    const GroupCut c = groups.cut(g);
+    const int slice = c.n > 1 ? groups.slices[g] + k : -1;
+    records[p] = make_int4(g, groups.tab[g] + k * c.each,
+                           min(max(groups.rows(g) - k * c.each, 0), c.each), slice);
+    if (slice >= 0 && slice < a.slices) first[slice] = make_int2(g, k ? 0 : c.n);
+  }
+  // (slices that no expert has)
+  for (int s = groups.slices[groups.groups] + tid; s < a.slices; s += 1024)
+    first[s] = make_int2(0, 0);
+}
+
+// The parts of dW of the groups that are summed in several, added in order.  Workgroup b
+// takes slice b / kJoinParts' group, if the slice is the group's first, and part b %
+// kJoinParts of it.
+constexpr int kJoinParts = 64;
+__global__ __launch_bounds__(256) void grouped_join_kernel(GroupedArgs a) {
+  const int slice = blockIdx.x / kJoinParts;
+  const int2 r = reinterpret_cast<const int2*>(a.plan + kPlanHead + 4 * a.max_parts)[slice];
+  const int e = r.x, n = r.y;
+  if (n <= 1 || slice + n > a.slices) return;
+  const int64_t size = (int64_t)a.C * a.J;  // (8 divides it)
+  const f32x4_t* p = reinterpret_cast<const f32x4_t*>(a.parts + slice * size);
+  const int64_t o = (int64_t)e * size;
+  for (int64_t i = (blockIdx.x % kJoinParts) * 256 + threadIdx.x; i < size / 4;
+       i += kJoinParts * 256) {
+    f32x4_t v = p[i];
+    for (int k = 1; k < n; ++k) v += p[k * (size / 4) + i];
+    if (a.out_f32)
+      *reinterpret_cast<f32x4_t*>(static_cast<float*>(a.out) + o + 4 * i) = v;
+    else
+      *reinterpret_cast<u32x2_t*>(static_cast<uint16_t*>(a.out) + o + 4 * i) =
+          u32x2_t{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+  }
+}
+
+template <int KIND, int TM, int TJ, int WM, int WJ, int SI, int STAGES>
 hipError_t run_tiles(GroupedArgs a, hipStream_t s) {
-  constexpr int lds = kTileLds<KIND, TM, TJ, STAGES>;
-  static_assert(lds <= 160 * 1024 && WM * WJ * 32 * (4 * (TJ / WJ) + 16) <= lds, "LDS");
+  constexpr int lds = kTileLds<KIND, TM, TJ, SI, STAGES>;
+  static_assert(lds <= 160 * 1024 && WM * WJ * kOutBytes<TJ, WJ> <= lds && 4 * kGroupWords <= lds,
+                "LDS");
   a.tiles_j = (a.J + TJ - 1) / TJ;
   a.tiles_m = KIND == kDw ? (a.C + TM - 1) / TM : 0;
-  const int64_t units = KIND == kDw ? (int64_t)a.E * a.tiles_m * a.tiles_j
-                                    : grouped_tiles(a.R, a.E, TM) * a.tiles_j;
+  const int64_t units = KIND == kDw
+                            ? grouped_chunks(a.R, a.E, a.chunk) * a.tiles_m * a.tiles_j
+                            : grouped_tiles(a.R, a.E, TM) * a.tiles_j;
   if (units <= 0) return hipSuccess;
-  const int64_t grid = (units + kXcds - 1) / kXcds * kXcds;
+  // dW: room for XCDs whose parts are lighter to take a quarter more of them
+  const int64_t tiles = KIND == kDw ? (int64_t)a.tiles_m * a.tiles_j : a.tiles_j;
+  const int64_t parts = units / tiles;
+  const int64_t per = (parts + kXcds - 1) / kXcds + (KIND == kDw ? (parts + 31) / 32 : 0);
+  const int64_t grid = per * tiles * kXcds;
   if (grid * 64 * WM * WJ > UINT32_MAX) return hipErrorInvalidValue;  // (the callers check)
-  grouped_tile_kernel<KIND, TM, TJ, WM, WJ, STAGES>
+  if (KIND == kDw) {
+    a.max_parts = (int32_t)parts;
+    grouped_plan_kernel<<<1, 1024, 0, s>>>(a, (int)per);
+  }
+  grouped_tile_kernel<KIND, TM, TJ, WM, WJ, SI, STAGES>
       <<<(unsigned)grid, 64 * WM * WJ, lds, s>>>(a);
+  if (KIND == kDw && a.slices)
+    grouped_join_kernel<<<(unsigned)(a.slices * kJoinParts), 256, 0, s>>>(a);
   return hipGetLastError();
 }
 
-// Rows a group, from which 256-row tiles are taken instead of 64-row ones.
-bool tall(int64_t R, int64_t E) { return R >= 96 * E; }
+// Whether 128-row tiles are left to fill half of the chip, at two workgroups a CU.
+bool few_tiles(int64_t R, int64_t E, int64_t J, int64_t TJ) {
+  return grouped_tiles(R, E, 128) * ((J + TJ - 1) / TJ) < 256;
+}
 
 }  // namespace
 
+// 128 x 256 tiles by eight waves, two workgroups a CU (128 registers a lane): of the tiles
+// that fit the best in all but the smallest calls.  At c2's down projection over 32768 rows
+// (128 experts, J 2048, C 768): 185 us, 256 x 256 200, 256 x 128 214, 128 x 128 by four
+// waves 203; dx of its up projection 206, 224, 242, 234.
+//
+// 64 x 128 by four waves where these are few: 1024 rows of 8 experts, J 768, C 2048 18.5 us
+// against 33.2, its dx 16.6 against 20.6; 4096 rows 25.5 against 35.1, but dx, J 2048, with
+// 328 tiles, 43.9 against 26.7.  Forward also where a group has few rows: 64 a group of 256
+// experts (J 512, C 2048) 136 us against 147, 96 a group 143 against 129.  (dx reads the
+// weights' rows, 256 bytes of them in these tiles: 64 a group 181 us against 130.)
 hipError_t launch_grouped_mm(const GroupedArgs& a, hipStream_t s) {
-  ProfileScope prof("grouped_mm", s);
-  return tall(a.R, a.E) ? run_tiles<kForward, 256, 256, 2, 4, 2>(a, s)
-                        : run_tiles<kForward, 64, 256, 1, 4, 2>(a, s);
+  if (a.R <= 64 * (int64_t)a.E || few_tiles(a.R, a.E, a.J, 256))
+    return run_tiles<kForward, 64, 128, 1, 4, 64, 3>(a, s);
+  return run_tiles<kForward, 128, 256, 2, 4, 32, 3>(a, s);
 }
 hipError_t launch_grouped_dx(const GroupedArgs& a, hipStream_t s) {
-  ProfileScope prof("grouped_dx", s);
-  return tall(a.R, a.E) ? run_tiles<kDx, 256, 256, 2, 4, 2>(a, s)
-                        : run_tiles<kDx, 64, 256, 1, 4, 2>(a, s);
+  if (few_tiles(a.R, a.E, a.J, 256)) return run_tiles<kDx, 64, 128, 1, 4, 64, 3>(a, s);
+  return run_tiles<kDx, 128, 256, 2, 4, 32, 3>(a, s);
 }
+// (128 x 128 tiles by four waves: 14.9 us against 16.2 at 1527 rows of 13 experts of 424 x
+// 1032, 23.1 against 22.9 at 1024 rows of 8 of 768 x 2048, 297 against 269 at c2's.)
 hipError_t launch_grouped_dw(const GroupedArgs& a, hipStream_t s) {
-  ProfileScope prof("grouped_dw", s);
-  return tall(a.R, a.E) ? run_tiles<kDw, 256, 256, 2, 4, 2>(a, s)
-                        : run_tiles<kDw, 128, 128, 2, 2, 2>(a, s);
+  return run_tiles<kDw, 128, 256, 2, 4, 32, 3>(a, s);
 }
+// 128 x 128 by four waves, one a SIMD: at c2's up projection over 32768 rows 97 us, 128 x
+// 256 by eight 102, 64 x 256 by four 135.  64 x 128 where a group has few rows (16 a group
+// of 256 experts, J 512, C 2048: 32.0 us against 35.1; 64: 51 against 46) or the tiles are few
+// (1024 rows of 8 experts, J 768: 14.3 against 18.1).
 hipError_t launch_grouped_qmm(const GroupedArgs& a, hipStream_t s) {
-  ProfileScope prof("grouped_qmm", s);
-  return tall(a.R, a.E) ? run_tiles<kForward8, 256, 256, 2, 4, 2>(a, s)
-                        : run_tiles<kForward8, 64, 256, 1, 4, 2>(a, s);
+  if (a.R <= 32 * (int64_t)a.E || few_tiles(a.R, a.E, a.J, 128))
+    return run_tiles<kForward8, 64, 128, 1, 4, 128, 3>(a, s);
+  return run_tiles<kForward8, 128, 128, 2, 2, 128, 3>(a, s);
 }
 
 }  // namespace mlxr_moe
