@@ -5,7 +5,7 @@
 //   r = 1 / sqrt(sum_j h_j^2 / d + eps)
 //   y_j = w_j h_j r
 // y in bf16, rounded once, or in mode "mxfp8": e4m3 codes with a power-of-two scale
-// per 32 (mx.hpp), each rounded once from the f32 value.  With dy the gradient of y
+// per 32 (mx.hpp), each the nearest of the value in f64.  With dy the gradient of y
 // and dh what comes to h from elsewhere,
 //   g_j  = dy_j w_j,  c = sum_j g_j h_j / d
 //   dx_j = r (g_j - h_j r^2 c) + dh_j      (of x and of the residual alike)
@@ -16,6 +16,7 @@
 // or by a workgroup of four (few rows, or wide ones); 16-byte accesses where d and
 // the addresses allow, single values in a kernel of its own otherwise.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.hpp"
 #include "kernels.hpp"
@@ -89,6 +90,32 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
   return (red[0] + red[1]) + (red[2] + red[3]);
 }
 
+template <int TPR>
+__device__ __forceinline__ double row_sum(double v, double* red) {
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
+  if constexpr (TPR == 64) return v;
+  const int wave = threadIdx.x >> 6;
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[wave] = v;
+  __syncthreads();
+  return (red[0] + red[1]) + (red[2] + red[3]);
+}
+
+// Codes of 4 bits show an f32's rounding: of a row's values some lie nearer to the middle of
+// two codes than f32 tells apart (one in 2^18), and then the codes would go by the order of
+// the sums.  So mode "mxfp8" norms in f64 and rounds once: the value goes on as f32 rounded
+// to odd (the last of 24 bits set if any behind it is), which no middle of two codes is and
+// no power of two that the scale goes by.
+template <bool MX>
+using norm_t = std::conditional_t<MX, double, float>;
+__device__ __forceinline__ float to_odd(double y) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, y);
+  const uint32_t lo = (uint32_t)u;
+  const uint32_t odd = (lo & 0xe0000000u) | ((lo & 0x1fffffffu) ? 0x20000000u : 0u);
+  return (float)__builtin_bit_cast(double, (u & 0xffffffff00000000ull) | odd);
+}
+
 struct NormArgs {
   const void *x, *res;
   const uint16_t* w;
@@ -103,14 +130,15 @@ struct NormArgs {
 // A row by TPR threads, each C pieces of 8 values.
 template <bool XF32, bool HF32, bool MX, int TPR, int C>
 __global__ __launch_bounds__(kNT) void add_rms_norm_kernel(NormArgs a) {
-  __shared__ float red[4];
+  typedef norm_t<MX> sum_t;
+  __shared__ sum_t red[4];
   const int lane = threadIdx.x & (TPR - 1);
   const int64_t t = (int64_t)blockIdx.x * (kNT / TPR) + (TPR == 64 ? threadIdx.x >> 6 : 0);
   if (t >= a.T) return;  // (whole rows: a wave's, or the workgroup's)
   const int64_t row = t * a.d;
   float v[C][8];
   u32x4_t wv[C];
-  float ss = 0.0f;
+  sum_t ss = 0;
 #pragma unroll
   for (int i = 0; i < C; ++i) {
     const int j = 8 * (lane + TPR * i);
@@ -132,17 +160,34 @@ __global__ __launch_bounds__(kNT) void add_rms_norm_kernel(NormArgs a) {
     const int j = 8 * (lane + TPR * i);
     if (j < a.d) store8<HF32>(a.h, row + j, v[i]);
 #pragma unroll
-    for (int c = 0; c < 8; ++c) ss = __builtin_fmaf(v[i][c], v[i][c], ss);
+    for (int c = 0; c < 8; ++c) {
+      if constexpr (MX)
+        ss = __builtin_fma((double)v[i][c], (double)v[i][c], ss);
+      else
+        ss = __builtin_fmaf(v[i][c], v[i][c], ss);
+    }
   }
-  const float r = 1.0f / sqrtf(row_sum<TPR>(ss, red) / (float)a.d + a.eps);
+  sum_t r;
+  if constexpr (MX)
+    r = 1.0 / sqrt(row_sum<TPR>(ss, red) / a.d + a.eps);
+  else
+    r = 1.0f / sqrtf(row_sum<TPR>(ss, red) / (float)a.d + a.eps);
 #pragma unroll
   for (int i = 0; i < C; ++i) {
     const int j = 8 * (lane + TPR * i);
     float y[8];
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      y[2 * c] = v[i][2 * c] * r * __uint_as_float(wv[i][c] << 16);
-      y[2 * c + 1] = v[i][2 * c + 1] * r * __uint_as_float(wv[i][c] & 0xffff0000u);
+      const float w0 = __uint_as_float(wv[i][c] << 16);
+      const float w1 = __uint_as_float(wv[i][c] & 0xffff0000u);
+      if constexpr (MX) {
+        // (v w is exact of a bf16 row, and of an f32 one)
+        y[2 * c] = to_odd((double)v[i][2 * c] * (double)w0 * r);
+        y[2 * c + 1] = to_odd((double)v[i][2 * c + 1] * (double)w1 * r);
+      } else {
+        y[2 * c] = v[i][2 * c] * r * w0;
+        y[2 * c + 1] = v[i][2 * c + 1] * r * w1;
+      }
     }
     if constexpr (MX) {
       // a group is four neighbouring lanes'
@@ -162,18 +207,27 @@ __global__ __launch_bounds__(kNT) void add_rms_norm_kernel(NormArgs a) {
 // thread that wrote it.  mxfp8: 32 divides d, and a group is half a wave's.
 template <bool XF32, bool HF32, bool MX>
 __global__ __launch_bounds__(kNT) void add_rms_norm_any_kernel(NormArgs a) {
-  __shared__ float red[4];
+  typedef norm_t<MX> sum_t;
+  __shared__ sum_t red[4];
   const int64_t row = (int64_t)blockIdx.x * a.d;
-  float ss = 0.0f;
+  sum_t ss = 0;
   for (int j = threadIdx.x; j < a.d; j += kNT) {
     const float v = round_to<HF32>(load1<XF32>(a.x, row + j) + load1<HF32>(a.res, row + j));
     store1<HF32>(a.h, row + j, v);
-    ss = __builtin_fmaf(v, v, ss);
+    if constexpr (MX)
+      ss = __builtin_fma((double)v, (double)v, ss);
+    else
+      ss = __builtin_fmaf(v, v, ss);
   }
-  const float r = 1.0f / sqrtf(row_sum<kNT>(ss, red) / (float)a.d + a.eps);
+  sum_t r;
+  if constexpr (MX)
+    r = 1.0 / sqrt(row_sum<kNT>(ss, red) / a.d + a.eps);
+  else
+    r = 1.0f / sqrtf(row_sum<kNT>(ss, red) / (float)a.d + a.eps);
   for (int j = threadIdx.x; j < a.d; j += kNT) {
-    const float y = load1<HF32>(a.h, row + j) * r * bf16_to_f32(a.w[j]);
+    const float h = load1<HF32>(a.h, row + j), w = bf16_to_f32(a.w[j]);
     if constexpr (MX) {
+      const float y = to_odd((double)h * (double)w * r);
       uint32_t top = __float_as_uint(y) & 0x7fffffffu;
 #pragma unroll
       for (int m = 16; m >= 1; m >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, m, 64));
@@ -181,7 +235,7 @@ __global__ __launch_bounds__(kNT) void add_rms_norm_any_kernel(NormArgs a) {
       static_cast<uint8_t*>(a.out)[row + j] = (uint8_t)mx8_pair(y, 0.0f, byte);
       if ((j & 31) == 0) a.scales[(row + j) >> 5] = (uint8_t)byte;
     } else {
-      store1<false>(a.out, row + j, y);
+      store1<false>(a.out, row + j, h * r * w);
     }
   }
 }
@@ -333,9 +387,9 @@ __global__ __launch_bounds__(kNT) void norm_vjp_cols_kernel(NormVjpArgs a, const
   a.part[(int64_t)blockIdx.x * a.d + j] = dw;
 }
 
-// dweight [d] = the sum of part [G, d] over its rows, in f64: 16 columns by 64
-// slices of the rows a workgroup.
-constexpr int kJoinCols = 16, kJoinRows = 64;
+// dweight [d] = the sum of part [G, d] over its rows, in f64: 32 columns
+// (a line of 128 bytes) by 32 slices of the rows a workgroup.
+constexpr int kJoinCols = 32, kJoinRows = 32;
 __global__ __launch_bounds__(kJoinCols * kJoinRows) void norm_vjp_join_kernel(const float* part,
                                                                               int G, int d,
                                                                               float* dw) {
@@ -343,8 +397,23 @@ __global__ __launch_bounds__(kJoinCols * kJoinRows) void norm_vjp_join_kernel(co
   const int c = threadIdx.x % kJoinCols, s = threadIdx.x / kJoinCols;
   const int j = blockIdx.x * kJoinCols + c;
   double v = 0.0;
-  if (j < d)
-    for (int g = s; g < G; g += kJoinRows) v += (double)part[(int64_t)g * d + j];
+  if (j < d) {
+    // 16 loads at a time (one after the other 9.6 us of 1024 rows of 2048, so 6.4; 5.0 of 512)
+    int g = s;
+    for (; g + 15 * kJoinRows < G; g += 16 * kJoinRows) {
+      float x[16];
+#pragma unroll
+      for (int k = 0; k < 16; ++k) x[k] = part[(int64_t)(g + k * kJoinRows) * d + j];
+#pragma unroll
+      for (int k = 0; k < 16; ++k) v += (double)x[k];
+    }
+    float x[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k)
+      x[k] = g + k * kJoinRows < G ? part[(int64_t)(g + k * kJoinRows) * d + j] : 0.0f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) v += (double)x[k];
+  }
   red[s][c] = v;
   __syncthreads();
 #pragma unroll

@@ -370,3 +370,20 @@ def test_python_refusals_on_the_device(pkg, dev):
     q, sc, _ = ops.quantize(torch.zeros((2, 64), device=dev), mode="mxfp8")
     with pytest.raises(E, match="eight words"):
         ops.dequantize(q, sc[:, :1], mode="mxfp8")
+
+
+# The codes go by the value in 64 bits: f32 would put one value in 2^18 on the wrong side of
+# the middle of two codes, dozens of these.
+@gpu
+@pytest.mark.parametrize("ht", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T,d,shift", [(4096, 2048, 0), (600, 8192, 0), (512, 2048, 1)])
+def test_codes_are_the_nearest(pkg, dev, T, d, shift, ht):
+    x, res, w = (t.to(dev) for t in inputs(77, T, d, torch.float32, ht))
+    if shift:  # a weight off 16 bytes: the kernel for single values
+        w = torch.cat([w[:shift], w])[shift:]
+        assert w.data_ptr() % 16
+    h, q, sc = pkg.ops.add_rms_norm(x, res, w, EPS, mode="mxfp8")
+    y = norm64(h.cpu(), w.cpu())
+    byte = scale_bytes8(y)
+    assert torch.equal(sc.cpu().long(), byte.long())
+    assert torch.equal(decode8(q.cpu(), sc.cpu()), nearest8(y, byte))
