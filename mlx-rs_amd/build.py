@@ -39,7 +39,7 @@ SOURCES = [
     "combine.hip",
     "balance.hip",
     "add_norm.hip",
-    "grouped_tile.hip",
+    "grouped_stream.hip", "grouped_tile.hip",
     "nn.cpp",
     "profile.cpp",
     "capi.cpp",

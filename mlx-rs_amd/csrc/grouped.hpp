@@ -49,11 +49,12 @@ inline int64_t plan_words(int64_t max_parts, int64_t slices) {
 struct GroupCut {
   int n, each;
 };
-// Forward and dx: tiles of TM rows at most, of equal numbers of 32-row blocks.
+// Forward and dx: tiles of TM rows at most, of equal numbers of blocks of 32 (16).
 template <int TM>
 __device__ __forceinline__ GroupCut cut_tiles(int rows) {
   const int n = (rows + TM - 1) / TM;
-  return {n, n > 1 ? ((rows + n - 1) / n + 31) & ~31 : rows};
+  constexpr int kBlock = TM < 32 ? TM : 32;
+  return {n, n > 1 ? ((rows + n - 1) / n + kBlock - 1) & ~(kBlock - 1) : rows};
 }
 // dW: parts of `chunk` rows at most, of equal numbers of 64 rows; one for a group without
 // rows, too (its dW is zeros).
@@ -196,6 +197,10 @@ hipError_t launch_grouped_mm(const GroupedArgs& a, hipStream_t s);
 hipError_t launch_grouped_dx(const GroupedArgs& a, hipStream_t s);
 hipError_t launch_grouped_dw(const GroupedArgs& a, hipStream_t s);
 hipError_t launch_grouped_qmm(const GroupedArgs& a, hipStream_t s);
+// grouped_mm and grouped_qmm (a.ms given) where groups have few rows (grouped_stream.hip),
+// and whether they are that few.
+bool grouped_streams(const GroupedArgs& a);
+hipError_t launch_grouped_stream(const GroupedArgs& a, hipStream_t s);
 
 // Rows, inputs and outputs that the kernels' grids hold: R rows by J columns.
 constexpr int64_t kMaxGroupedRows = 1 << 24, kMaxGroupedDims = 1 << 16;

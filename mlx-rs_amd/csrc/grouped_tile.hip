@@ -625,6 +625,7 @@ bool few_tiles(int64_t R, int64_t E, int64_t J, int64_t TJ) {
 // experts (J 512, C 2048) 136 us against 147, 96 a group 143 against 129.  (dx reads the
 // weights' rows, 256 bytes of them in these tiles: 64 a group 181 us against 130.)
 hipError_t launch_grouped_mm(const GroupedArgs& a, hipStream_t s) {
+  if (grouped_streams(a)) return launch_grouped_stream(a, s);
   if (a.R <= 64 * (int64_t)a.E || few_tiles(a.R, a.E, a.J, 256))
     return run_tiles<kForward, 64, 128, 1, 4, 64, 3>(a, s);
   return run_tiles<kForward, 128, 256, 2, 4, 32, 3>(a, s);
@@ -643,6 +644,7 @@ hipError_t launch_grouped_dw(const GroupedArgs& a, hipStream_t s) {
 // of 256 experts, J 512, C 2048: 32.0 us against 35.1; 64: 51 against 46) or the tiles are few
 // (1024 rows of 8 experts, J 768: 14.3 against 18.1).
 hipError_t launch_grouped_qmm(const GroupedArgs& a, hipStream_t s) {
+  if (grouped_streams(a)) return launch_grouped_stream(a, s);
   if (a.R <= 32 * (int64_t)a.E || few_tiles(a.R, a.E, a.J, 128))
     return run_tiles<kForward8, 64, 128, 1, 4, 128, 3>(a, s);
   return run_tiles<kForward8, 128, 128, 2, 2, 128, 3>(a, s);
