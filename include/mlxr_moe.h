@@ -281,7 +281,10 @@ int mlxr_moe_grouped_mm(const void* x, int64_t x_rows, int64_t K, const void* w,
  *              (zeros behind the last group); tokens named by several rows sum theirs
  *   dw[e]    = sum over r of e: dy[r]^T x[rows[r]]   f32 or bf16 [E, N, K]; zeros for
  *              experts without rows
- * dx or dw may be NULL (not computed; w, or x, is then not read). */
+ * dx or dw may be NULL (not computed; w, or x, is then not read).  Groups of more
+ * rows than a tile sums are summed in parts (f32, in the workspace), added in the
+ * rows' order: equal inputs give equal bits.  workspace is dw's (256-byte aligned;
+ * not read where dw is NULL). */
 size_t mlxr_moe_grouped_mm_vjp_workspace_size(int64_t R, int64_t num_experts, int64_t N,
                                               int64_t K);
 int mlxr_moe_grouped_mm_vjp(const void* dy, const void* x, int64_t x_rows, int64_t K,
@@ -527,9 +530,9 @@ int mlxr_moe_rms_norm(const void* x, int64_t T, int64_t d, const void* weight,
  * over h as rounded to it); weight bf16 [d].  mode NULL: out bf16 [T, d], y
  * rounded once (mlxr_moe_rms_norm rounds the normalised value too), scales NULL.
  * mode "mxfp8": out uint32 [T, d/4] and scales uint8 [T, d/32] as
- * mlxr_moe_quantize makes them of y in f32 (32 divides d): what
- * mlxr_moe_grouped_qmm takes.  Rows holding NaN or an infinity, and rows of h
- * whose squares pass f32's range, follow the formula in f32.  Any d up to 2^20,
+ * mlxr_moe_quantize makes them, but of y in f64 (32 divides d): what
+ * mlxr_moe_grouped_qmm takes.  Rows holding NaN or an infinity, and without a
+ * mode rows of h whose squares pass f32's range, follow the formula in f32.  Any d up to 2^20,
  * T up to 2^24 - 1; arrays aligned to their elements (16-byte alignment and 8
  * dividing d are faster).  h and out must not overlap each other or the inputs. */
 int mlxr_moe_add_rms_norm(const void* x, int x_dtype, const void* residual,
@@ -587,8 +590,9 @@ int mlxr_moe_workspace_status(const void* workspace, size_t workspace_size,
  * "dispatch", "qgemm_gated", "qgemm_down", "combine", the shared
  * expert's GEMMs "shared_gated", "shared_down", "rms_norm",
  * "router_balance", "router_balance_vjp", "add_rms_norm", "add_rms_norm_vjp",
- * "grouped_mm", "grouped_dx", "grouped_dw", "grouped_qmm", and "read_probe" (mlxr_moe_profile_read).  NULL disarms.  Not for use while
- * the stream is being captured into a graph. */
+ * "grouped_mm", "grouped_dx" and "grouped_dw" (grouped_mm_vjp's halves),
+ * "grouped_qmm", and "read_probe" (mlxr_moe_profile_read).  NULL disarms.  Not
+ * for use while the stream is being captured into a graph. */
 int mlxr_moe_profile_start(const char* kernel);
 /* Waits for the armed kernel's last launch, returns the number of launches
  * and their elapsed time (total / min / max, milliseconds), and disarms. */

@@ -1090,7 +1090,8 @@ int mlxr_moe_profile_start(const char* kernel) {
                                        "dispatch",      "qgemm_gated",
                                        "qgemm_down",    "combine",
                                        "shared_gated",  "shared_down",
-                                       "rms_norm",      "add_rms_norm",
+                                       "rms_norm",      "router_balance",
+                                       "router_balance_vjp", "add_rms_norm",
                                        "add_rms_norm_vjp", "grouped_mm",
                                        "grouped_dx",    "grouped_dw",
                                        "grouped_qmm",   "read_probe"};

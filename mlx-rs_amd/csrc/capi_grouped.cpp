@@ -78,6 +78,7 @@ int mlxr_moe_grouped_mm(const void* x, int64_t x_rows, int64_t K, const void* w,
   a.m = x, a.j = w, a.offsets = offsets, a.rows = rows, a.out = out;
   a.R = R, a.x_rows = x_rows, a.E = (int32_t)E, a.J = (int32_t)N, a.C = (int32_t)K;
   a.out_f32 = out_dtype == MLXR_MOE_FLOAT32;
+  ProfileScope prof("grouped_mm", as_stream(stream));
   return finish(from_hip(launch_grouped_mm(a, as_stream(stream)), "grouped_mm"));
 }
 
@@ -115,6 +116,7 @@ int mlxr_moe_grouped_mm_vjp(const void* dy, const void* x, int64_t x_rows, int64
     GroupedArgs a{};
     a.m = dy, a.j = w, a.offsets = offsets, a.out = dx;
     a.R = R, a.x_rows = R, a.E = (int32_t)E, a.J = (int32_t)K, a.C = (int32_t)N;
+    ProfileScope prof("grouped_dx", s);
     st = from_hip(launch_grouped_dx(a, s), "grouped_mm_vjp dx");
     if (!st.ok) return finish(st);
   }
@@ -128,6 +130,7 @@ int mlxr_moe_grouped_mm_vjp(const void* dy, const void* x, int64_t x_rows, int64
     a.plan = v.plan, a.parts = v.parts;
     a.chunk = (int32_t)grouped_chunk_rows(R, N, K);
     a.slices = (int32_t)grouped_slices(R, a.chunk);
+    ProfileScope prof("grouped_dw", s);
     st = from_hip(launch_grouped_dw(a, s), "grouped_mm_vjp dw");
   }
   return finish(st);
@@ -151,6 +154,7 @@ int mlxr_moe_grouped_qmm(const uint32_t* x, const uint8_t* x_scales, int64_t x_r
   a.out = out;
   a.R = R, a.x_rows = x_rows, a.E = (int32_t)E, a.J = (int32_t)N, a.C = (int32_t)K;
   a.out_f32 = out_dtype == MLXR_MOE_FLOAT32;
+  ProfileScope prof("grouped_qmm", as_stream(stream));
   return finish(from_hip(launch_grouped_qmm(a, as_stream(stream)), "grouped_qmm"));
 }
 

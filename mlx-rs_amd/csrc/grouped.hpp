@@ -145,24 +145,20 @@ struct Groups {
     return lo;
   }
   // The part that XCD x's start with: an eighth of all parts is before it, dW of their
-  // weight, as far as `cap` parts an XCD allow.
-  __device__ __forceinline__ int start(int x, int cap) const {
+  // weight.
+  __device__ __forceinline__ int start(int x) const {
     const int all = parts[groups];
-    if (x == 0) return 0;
     if (!DW) return (int)((int64_t)all * x / kXcds);
     const int w = (int)((int64_t)weights[groups] * x / kXcds);
     const int g = search(weights, w);
-    const GroupCut c = cut(g);
-    const int p = min(parts[g] + (w - weights[g]) / weigh(c), all);
-    return max(min(p, cap * x), all - cap * ((int)kXcds - x));
+    return min(parts[g] + (w - weights[g]) / weigh(cut(g)), all);
   }
   // Workgroup b's unit: a part and one of `tiles` tiles of each.  Parts go to the XCDs in
   // runs, so that one L2 sees an expert's.  False: no such unit.
   __device__ __forceinline__ bool find(int b, int tiles, GroupedUnit& u) const {
-    const int i = b / kXcds, cap = (int)(gridDim.x / kXcds) / tiles;
-    const int part = start(b % kXcds, cap) + i / tiles;
-    if (part >= start(b % kXcds + 1, cap)) return false;
-    u.tile = i % tiles;
+    const int part = start(b % kXcds) + b / (int)kXcds / tiles;
+    if (part >= start(b % kXcds + 1)) return false;
+    u.tile = b / (int)kXcds % tiles;
     // (parts before a group without any are those before the next one: the last one counts)
     const int g = __builtin_amdgcn_readfirstlane(search(parts, part));
     const int n = rows(g), k = part - parts[g];

@@ -536,9 +536,10 @@ void grouped_tile_kernel(GroupedArgs a) {
 // took 80 us of 310 at 128 experts of 768 x 2048); cap: parts an XCD that the grid holds.
 __global__ __launch_bounds__(1024) void grouped_plan_kernel(GroupedArgs a, int cap) {
   __shared__ int lds[kGroupWords];
+  __shared__ int starts[kXcds + 1];
   const Groups<true, 64> groups(a, lds);
   const int tid = threadIdx.x;
-  if (tid <= (int)kXcds) a.plan[tid] = min(groups.start(tid, cap), a.max_parts);
+  if (tid <= (int)kXcds) starts[tid] = groups.start(tid);
   int4* records = reinterpret_cast<int4*>(a.plan + kPlanHead);
   int2* first = reinterpret_cast<int2*>(a.plan + kPlanHead + 4 * a.max_parts);
   const int all = min(groups.parts[groups.groups], a.max_parts);
@@ -549,6 +550,16 @@ __global__ __launch_bounds__(1024) void grouped_plan_kernel(GroupedArgs a, int c
     records[p] = make_int4(g, groups.tab[g] + k * c.each,
                            min(max(groups.rows(g) - k * c.each, 0), c.each), slice);
     if (slice >= 0 && slice < a.slices) first[slice] = make_int2(g, k ? 0 : c.n);
+  }
+  __syncthreads();
+  if (tid == 0) {
+    // at most cap parts each, and few enough left for the XCDs behind
+    int at = 0;
+    a.plan[0] = 0;
+    for (int x = 1; x <= (int)kXcds; ++x) {
+      at = max(max(min(min(starts[x], all), at + cap), all - cap * ((int)kXcds - x)), at);
+      a.plan[x] = at;
+    }
   }
   // (slices that no expert has)
   for (int s = groups.slices[groups.groups] + tid; s < a.slices; s += 1024)

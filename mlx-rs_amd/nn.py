@@ -78,6 +78,16 @@ class SwitchLinear:
         """SwitchLinear::apply (switch.rs:84-93)."""
         return ops.gather_mm(x, self.weight, None, indices, sorted)
 
+    def apply_grouped(self, x, offsets, rows=None, out_dtype=torch.bfloat16):
+        """apply to rows sorted by expert once (ops.dispatch) for all of a layer's
+        projections: ops.grouped_mm."""
+        return ops.grouped_mm(x, self.weight, offsets, rows, out_dtype)
+
+    def vjp_grouped(self, dy, x, offsets, rows=None, dw_dtype=torch.bfloat16, need_dx=True,
+                    need_dw=True):
+        """The gradients (dx, dw) of apply_grouped: ops.grouped_mm_vjp."""
+        return ops.grouped_mm_vjp(dy, x, self.weight, offsets, rows, dw_dtype, need_dx, need_dw)
+
     def try_into_quantized(self, group_size=None, bits=4, mode="affine"):
         """Quantizable::try_into_quantized (switch.rs:96-113)."""
         return QuantizedSwitchLinear.try_from_switch_linear(self.weight, group_size, bits, mode)
@@ -155,6 +165,14 @@ class QuantizedSwitchLinear:
         """QuantizedSwitchLinear::apply (switch.rs:148-167)."""
         return ops.gather_qmm(x, self.weight, self.scales, self.biases, None, indices, True,
                               self.group_size, self.bits, sorted, self.mode)
+
+    def apply_grouped(self, x, x_scales, offsets, rows=None, out_dtype=torch.bfloat16):
+        """apply to rows sorted by expert, quantised in mode "mxfp8" (ops.quantize,
+        RmsNorm.forward_add): ops.grouped_qmm.  Mode "mxfp4" only."""
+        if self.mode != "mxfp4":
+            raise MlxrMoeError("QuantizedSwitchLinear: apply_grouped takes weights in mode mxfp4, "
+                               f"got {self.mode}")
+        return ops.grouped_qmm(x, x_scales, self.weight, self.scales, offsets, rows, out_dtype)
 
     def descriptor(self) -> C.QLinear:
         return C.QLinear(self.weight.data_ptr(), self.scales.data_ptr(), _ptr(self.biases),
@@ -684,5 +702,15 @@ class RmsNorm:
             C.check(C.lib().mlxr_moe_rms_norm(_ptr(x2), x2.shape[0], d, _ptr(self.weight), self.eps,
                                               _ptr(out), ops._stream(x)))
         return out.reshape(x.shape)
+
+    def forward_add(self, x, residual, mode=None):
+        """h = x + residual and the norm of h, in one pass (the attention half's add and
+        the norm behind it, crates/mlxr-lm/src/qwen3_5/text/layer.rs:128-137):
+        ops.add_rms_norm."""
+        return ops.add_rms_norm(x, residual, self.weight, self.eps, mode)
+
+    def vjp(self, dy, h, dh=None):
+        """The gradients (dx, dweight) of forward_add: ops.add_rms_norm_vjp."""
+        return ops.add_rms_norm_vjp(dy, h, self.weight, self.eps, dh)
 
     __call__ = forward

@@ -556,7 +556,7 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, 
     """h = x + residual (residual's dtype: f32 or bf16, as x) and y = rms_norm(h,
     weight, eps), x and residual [.., d], weight bf16 [d].  Returns (h, y), y bf16
     rounded once; with mode "mxfp8" (32 divides d) (h, codes int32 [.., d/4], scales
-    uint8 [.., d/32]), as quantize makes them of y in f32.  Not recorded by autograd:
+    uint8 [.., d/32]), as quantize makes them, of y in f64.  Not recorded by autograd:
     the gradients are add_rms_norm_vjp's."""
     if mode not in (None, "mxfp8"):
         raise MlxrMoeError(f"add_rms_norm: unsupported mode {mode!r} (None or 'mxfp8')")

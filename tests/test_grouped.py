@@ -397,3 +397,98 @@ def test_python_refusals_on_the_device(pkg, dev):
         ops.grouped_qmm(q, sc[:, :1], wq, wsc, offsets, rows)
     with pytest.raises(E, match="four words"):
         ops.grouped_qmm(q, sc, wq, wsc[..., :1], offsets, rows)
+
+
+# Groups of few rows (the kernel that streams the weights): its 16-row parts' edges, many
+# experts, inputs shorter and longer than a chunk, rows that name none.
+FEW = {
+    "one": [1],
+    "eight": [0, 1, 1, 1, 0, 1, 1, 1, 1, 1] + [0] * 30,
+    "edges": [15, 16, 17, 0, 1, 33] + [0] * 30,
+    "spread": [(5 * e) % 4 for e in range(90)],
+    "last": [0] * 511 + [40],
+}
+
+
+@gpu
+@pytest.mark.parametrize("groups", sorted(FEW))
+@pytest.mark.parametrize("K,N", [(8, 8), (264, 520), (512, 136), (2056, 24), (4104, 16)])
+@pytest.mark.parametrize("mapped", [None, 37])
+def test_few_rows(pkg, dev, groups, K, N, mapped):
+    counts = FEW[groups]
+    if len(counts) > 100:
+        K, N = min(K, 520), min(N, 24)
+    x, w, _, offsets, rows = problem(K + N, counts, K, N, tail=4, mapped=mapped)
+    if mapped:
+        rows[::5] = mapped
+    out_dtype = BF16 if K % 3 else F32
+    got = pkg.ops.grouped_mm(*to(dev, x, w, offsets, rows), out_dtype=out_dtype)
+    near(got, *forward64(taken(x, rows), w, offsets), K)
+    assert bool((got[sum(counts):] == 0).all())
+    K = (K + 31) // 32 * 32
+    x, w, _, offsets, rows = problem(K + N, counts, K, N, tail=4, mapped=mapped)
+    if mapped:
+        rows[::5] = -1
+    q, sc, _ = [None if t is None else t.cpu()
+                for t in pkg.ops.quantize((3 * x).to(dev), mode="mxfp8")]
+    wq, wsc, _ = [None if t is None else t.cpu()
+                  for t in pkg.ops.quantize(w.to(dev), mode="mxfp4")]
+    got = check_qmm(pkg, dev, q, sc, wq, wsc, offsets, rows, out_dtype)
+    assert bool((got[sum(counts):] == 0).all())
+
+
+@gpu
+@pytest.mark.parametrize("K,N,counts", [(72, 40, [3000, 0, 5, 1100]), (264, 520, [0, 2500]),
+                                        (64, 64, [1024, 1025]), (8, 8, [20000]),
+                                        (128, 136, [1] * 700 + [4000])])
+def test_weight_gradients_of_long_groups(pkg, dev, K, N, counts):
+    """Groups summed in several parts; the same bits at every call."""
+    x, w, dy, offsets, rows = problem(sum(counts), counts, K, N, tail=9, mapped=500)
+    args = to(dev, dy, x, w, offsets, rows)
+    _, dw = pkg.ops.grouped_mm_vjp(*args, dw_dtype=F32, need_dx=False)
+    xs, g = taken(x, rows), dy.double()
+    for e in range(len(counts)):
+        s = slice(int(offsets[e]), int(offsets[e + 1]))
+        near(dw[e], g[s].t() @ xs[s], g[s].abs().t() @ xs[s].abs(), counts[e] + 1)
+    _, half = pkg.ops.grouped_mm_vjp(*args, need_dx=False)
+    assert torch.equal(half, dw.to(BF16))
+    for _ in range(3):
+        _, again = pkg.ops.grouped_mm_vjp(*args, dw_dtype=F32, need_dx=False)
+        assert torch.equal(again, dw)
+
+
+def test_workspace_refusals(pkg):
+    lib, C, err = pkg._capi.lib(), pkg._capi, pkg._capi.last_error
+    need = lib.mlxr_moe_grouped_mm_vjp_workspace_size(4096, 4, 64, 64)
+    assert need > 0
+    # (long groups need room for their parts)
+    assert lib.mlxr_moe_grouped_mm_vjp_workspace_size(1 << 20, 4, 64, 64) > need
+
+    def vjp(ws, n, dw=16):
+        return lib.mlxr_moe_grouped_mm_vjp(16, 16, 4096, 64, 16, 4, 64, 16, None, 4096, None, dw,
+                                           C.BFLOAT16, ws, n, None)
+
+    assert vjp(256, need - 1) == -1 and "workspace too small" in err()
+    assert vjp(None, need) == -1 and "workspace is NULL" in err()
+    assert vjp(128, need) == -1 and "256-byte aligned" in err()
+
+
+@gpu
+def test_two_streams_at_once(pkg, dev):
+    """Calls on two streams share nothing."""
+    ops = pkg.ops
+    sets = [to(dev, *problem(20 + i, [2000, 3, 0, 1500 + i], 136, 72, mapped=300))
+            for i in range(2)]
+    want = [(ops.grouped_mm(x, w, o, r), *ops.grouped_mm_vjp(dy, x, w, o, r))
+            for x, w, dy, o, r in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[], []]
+    for _ in range(4):
+        for i, (x, w, dy, o, r) in enumerate(sets):
+            with torch.cuda.stream(streams[i]):
+                got[i].append((ops.grouped_mm(x, w, o, r), *ops.grouped_mm_vjp(dy, x, w, o, r)))
+    torch.cuda.synchronize()
+    for outs, right in zip(got, want):
+        for out in outs:
+            assert all(torch.equal(a, b) for a, b in zip(out, right))
