@@ -71,33 +71,92 @@ struct GroupedUnit {
   int tile;
 };
 
-// Where the groups' parts lie in the order of all parts (DW: of a.E groups, else with the
-// rows behind the last as one more), in LDS: kGroupWords words at `lds`, by all of the
-// workgroup's threads.
+__device__ __forceinline__ int clamped_offset(const GroupedArgs& a, int e) {
+  return min(max(as_global<const int32_t>(a.offsets)[e], 0), (int)a.R);
+}
+// The inclusive sums over a wave's lanes.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // of the row's lanes: one
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);  // before, two, four, eight
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // the row's before
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // the half's before
+  return v;
+}
+
+// Forward and dx: the unit of a workgroup.  The groups (and the rows behind the last as one
+// more) are cut into parts of TM rows; `pick(all, u)`, of how many there are, gives u.tile and
+// the part, or -1 for none.  The thread whose group has that part says where it is: two
+// barriers behind the offsets (a table of all parts, searched by halves: one token through 8
+// of 256 experts 8.4 us, so 7.1).
+// kFindWords words of LDS.
+constexpr int kFindWords = 32;
+template <int TM, class Pick>
+__device__ __forceinline__ bool find_part(const GroupedArgs& a, int* lds, GroupedUnit& u,
+                                          Pick pick) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
+  const int groups = a.E + 1, per = (groups + blockDim.x - 1) / blockDim.x;
+  const int g0 = min(tid * per, groups), g1 = min(g0 + per, groups);
+  const auto end = [&](int g) { return g < a.E ? clamped_offset(a, g + 1) : (int)a.R; };
+  const int first = g0 < groups ? clamped_offset(a, g0) : 0;
+  int n = 0;
+  for (int g = g0, at = first; g < g1; ++g) {
+    const int to = end(g);
+    n += cut_tiles<TM>(max(to - at, 0)).n;
+    at = to;
+  }
+  const int upto = wave_scan(n);
+  if (lane == 63) lds[wave] = upto;
+  __syncthreads();
+  int before = upto - n, all = 0;
+  for (int k = 0; k < waves; ++k) {
+    const int t = lds[k];
+    if (k < wave) before += t;
+    all += t;
+  }
+  const int part = pick(__builtin_amdgcn_readfirstlane(all), u);
+  if (part < 0) return false;
+  if (part >= before && part < before + n) {
+    int k = part - before, g = g0, at = first, to = end(g);
+    GroupCut c = cut_tiles<TM>(max(to - at, 0));
+    while (k >= c.n) {
+      k -= c.n;
+      at = to, to = end(++g);
+      c = cut_tiles<TM>(max(to - at, 0));
+    }
+    lds[16] = g, lds[17] = at + k * c.each;
+    lds[18] = min(to - at - k * c.each, c.each);
+  }
+  __syncthreads();
+  u.e = __builtin_amdgcn_readfirstlane(lds[16]);
+  u.slot0 = __builtin_amdgcn_readfirstlane(lds[17]);
+  u.rows = __builtin_amdgcn_readfirstlane(lds[18]);
+  u.slice = -1;
+  return true;
+}
+
+// dW: where the experts' parts lie in the order of all parts, in LDS: kGroupWords words at
+// `lds`, by all of the workgroup's threads.
 constexpr int kGroupWords = 4 * (kMaxExperts + 4) + 64;
-template <bool DW, int TM>
 struct Groups {
   static constexpr int kStep = kMaxExperts + 4;
   const GroupedArgs& a;
   int *tab, *parts, *slices, *weights;  // offsets; parts, slices, weights before each group
   int groups;
 
-  __device__ __forceinline__ int rows(int g) const {
-    return max((g < a.E ? tab[g + 1] : (int)a.R) - tab[g], 0);
-  }
-  __device__ __forceinline__ GroupCut cut(int g) const {
-    return DW ? cut_chunks(rows(g), a.chunk) : cut_tiles<TM>(rows(g));
-  }
-  // dW: what a part costs in each of its tiles, in 32-row blocks: its own and what it costs
+  __device__ __forceinline__ int rows(int g) const { return max(tab[g + 1] - tab[g], 0); }
+  __device__ __forceinline__ GroupCut cut(int g) const { return cut_chunks(rows(g), a.chunk); }
+  // what a part costs in each of its tiles, in 32-row blocks: its own and what it costs
   // however few it has
   static __device__ __forceinline__ int weigh(GroupCut c) { return (c.each + 31) / 32 + 9; }
 
   __device__ __forceinline__ Groups(const GroupedArgs& a_, int* lds) : a(a_) {
     tab = lds, parts = lds + kStep, slices = lds + 2 * kStep, weights = lds + 3 * kStep;
     int* totals = lds + 4 * kStep;
-    groups = DW ? a.E : a.E + 1;
+    groups = a.E;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    for (int e = tid; e <= a.E; e += blockDim.x) tab[e] = min(max(a.offsets[e], 0), (int)a.R);
+    for (int e = tid; e <= a.E; e += blockDim.x) tab[e] = clamped_offset(a, e);
     __syncthreads();
     const int per = (groups + blockDim.x - 1) / blockDim.x;
     const int g0 = min(tid * per, groups), g1 = min(g0 + per, groups);
@@ -105,29 +164,20 @@ struct Groups {
     for (int g = g0; g < g1; ++g) {
       const GroupCut c = cut(g);
       n += c.n;
-      if (DW && c.n > 1) s += c.n;
-      if (DW) w += c.n * weigh(c);
+      if (c.n > 1) s += c.n;
+      w += c.n * weigh(c);
     }
-    int ni = n, si = s, wi = w;  // inclusive scans over the wave
-#pragma unroll
-    for (int k = 1; k < 64; k <<= 1) {
-      const int x = __shfl_up(ni, k, 64), y = DW ? __shfl_up(si, k, 64) : 0;
-      const int z = DW ? __shfl_up(wi, k, 64) : 0;
-      if (lane >= k) ni += x, si += y, wi += z;
-    }
+    const int ni = wave_scan(n), si = wave_scan(s), wi = wave_scan(w);
     if (lane == 63) totals[wave] = ni, totals[16 + wave] = si, totals[32 + wave] = wi;
     __syncthreads();
     n = ni - n, s = si - s, w = wi - w;
     for (int k = 0; k < wave; ++k) n += totals[k], s += totals[16 + k], w += totals[32 + k];
     for (int g = g0; g < g1; ++g) {
       const GroupCut c = cut(g);
-      parts[g] = n;
+      parts[g] = n, slices[g] = s, weights[g] = w;
       n += c.n;
-      if (DW) {
-        slices[g] = s, weights[g] = w;
-        if (c.n > 1) s += c.n;
-        w += c.n * weigh(c);
-      }
+      if (c.n > 1) s += c.n;
+      w += c.n * weigh(c);
     }
     if (tid == (int)blockDim.x - 1) parts[groups] = n, slices[groups] = s, weights[groups] = w;
     __syncthreads();
@@ -144,30 +194,11 @@ struct Groups {
     }
     return lo;
   }
-  // The part that XCD x's start with: an eighth of all parts is before it, dW of their
-  // weight.
+  // The part that XCD x's start with: an eighth of all parts' weight is before it.
   __device__ __forceinline__ int start(int x) const {
-    const int all = parts[groups];
-    if (!DW) return (int)((int64_t)all * x / kXcds);
     const int w = (int)((int64_t)weights[groups] * x / kXcds);
     const int g = search(weights, w);
-    return min(parts[g] + (w - weights[g]) / weigh(cut(g)), all);
-  }
-  // Workgroup b's unit: a part and one of `tiles` tiles of each.  Parts go to the XCDs in
-  // runs, so that one L2 sees an expert's.  False: no such unit.
-  __device__ __forceinline__ bool find(int b, int tiles, GroupedUnit& u) const {
-    const int part = start(b % kXcds) + b / (int)kXcds / tiles;
-    if (part >= start(b % kXcds + 1)) return false;
-    u.tile = b / (int)kXcds % tiles;
-    // (parts before a group without any are those before the next one: the last one counts)
-    const int g = __builtin_amdgcn_readfirstlane(search(parts, part));
-    const int n = rows(g), k = part - parts[g];
-    const GroupCut c = cut(g);
-    u.e = g;
-    u.slot0 = __builtin_amdgcn_readfirstlane(tab[g] + k * c.each);
-    u.rows = __builtin_amdgcn_readfirstlane(min(max(n - k * c.each, 0), c.each));
-    u.slice = __builtin_amdgcn_readfirstlane(DW && c.n > 1 ? slices[g] + k : -1);
-    return true;
+    return min(parts[g] + (w - weights[g]) / weigh(cut(g)), parts[groups]);
   }
 };
 

@@ -34,7 +34,7 @@ __global__ __launch_bounds__(64 * kWaves) void grouped_stream_kernel(GroupedArgs
   constexpr int CH = F8 ? 2 : 4;       // steps of a chunk
   constexpr int XL = F8 ? 2 : 1;       // loads of x a step
   __shared__ union {
-    int words[kGroupWords];
+    int words[kFindWords];
     f32x4_t sums[2][kWaves][64];
   } lds;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -44,23 +44,18 @@ __global__ __launch_bounds__(64 * kWaves) void grouped_stream_kernel(GroupedArgs
   // ---- the workgroup's unit: a part and `per` column tiles.  XCDs take runs of them (a
   // part's, one part after the other): an expert of several parts is read by one of them.
   const int runs = (a.tiles_j + per - 1) / per;
-  int e, slot0, rows, tile0;
-  {
-    const Groups<false, kRows> groups(a, lds.words);
+  GroupedUnit u;
+  const bool found = find_part<kRows>(a, lds.words, u, [&](int parts, auto& v) {
     const int x = blockIdx.x % kXcds, i = blockIdx.x / kXcds;
-    const int64_t all = (int64_t)groups.parts[groups.groups] * runs;
-    const int64_t u = all * x / kXcds + i;
-    const bool none = u >= all * (x + 1) / kXcds;
-    const int part = none ? 0 : (int)(u / runs);
-    tile0 = __builtin_amdgcn_readfirstlane((int)(u - (int64_t)part * runs) * per);
-    e = __builtin_amdgcn_readfirstlane(groups.search(groups.parts, part));
-    const int n = groups.rows(e), k = part - groups.parts[e];
-    const GroupCut cut = groups.cut(e);
-    slot0 = __builtin_amdgcn_readfirstlane(groups.tab[e] + k * cut.each);
-    rows = __builtin_amdgcn_readfirstlane(min(max(n - k * cut.each, 0), cut.each));
-    __syncthreads();  // (the sums take its place)
-    if (none || !rows) return;
-  }
+    const int64_t all = (int64_t)parts * runs, at = all * x / kXcds + i;
+    const int part = (int)(at / runs);
+    v.tile = (int)(at - (int64_t)part * runs) * per;
+    return at < all * (x + 1) / kXcds ? part : -1;
+  });
+  if (!found) return;
+  __syncthreads();  // (the sums take the words' place)
+  const int e = u.e, slot0 = u.slot0, rows = u.rows;
+  const int tile0 = __builtin_amdgcn_readfirstlane(u.tile);
   const int tiles = min(per, a.tiles_j - tile0);
   const int wcol0 = (tile0 * csplit + wave % csplit) * 16;  // the wave's columns: of tile t
   const int es = a.out_f32 ? 4 : 2;                         // from 16 csplit t on

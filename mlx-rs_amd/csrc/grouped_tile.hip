@@ -479,10 +479,15 @@ void grouped_tile_kernel(GroupedArgs a) {
     u.tile = i % tiles;
     u.e = r.x, u.slot0 = r.y, u.rows = r.z, u.slice = r.w;
   } else {
-    const Groups<DW, TM> groups(a, reinterpret_cast<int*>(smem));
-    const bool found = groups.find(blockIdx.x, a.tiles_j, u);
-    __syncthreads();  // (the stages take its place)
+    // parts go to the XCDs in runs, so that one L2 sees an expert's
+    const bool found = find_part<TM>(a, reinterpret_cast<int*>(smem), u, [&](int all, auto& v) {
+      const int x = blockIdx.x % kXcds, i = blockIdx.x / kXcds;
+      const int part = (int)((int64_t)all * x / kXcds) + i / a.tiles_j;
+      v.tile = i % a.tiles_j;
+      return part < (int)((int64_t)all * (x + 1) / kXcds) ? part : -1;
+    });
     if (!found) return;
+    __syncthreads();  // (the stages take the words' place)
   }
   TileAt at;
   at.e = u.e, at.slot0 = u.slot0;
@@ -537,7 +542,7 @@ void grouped_tile_kernel(GroupedArgs a) {
 __global__ __launch_bounds__(1024) void grouped_plan_kernel(GroupedArgs a, int cap) {
   __shared__ int lds[kGroupWords];
   __shared__ int starts[kXcds + 1];
-  const Groups<true, 64> groups(a, lds);
+  const Groups groups(a, lds);
   const int tid = threadIdx.x;
   if (tid <= (int)kXcds) starts[tid] = groups.start(tid);
   int4* records = reinterpret_cast<int4*>(a.plan + kPlanHead);
@@ -593,8 +598,7 @@ __global__ __launch_bounds__(256) void grouped_join_kernel(GroupedArgs a) {
 template <int KIND, int TM, int TJ, int WM, int WJ, int SI, int STAGES>
 hipError_t run_tiles(GroupedArgs a, hipStream_t s) {
   constexpr int lds = kTileLds<KIND, TM, TJ, SI, STAGES>;
-  static_assert(lds <= 160 * 1024 && WM * WJ * kOutBytes<TJ, WJ> <= lds && 4 * kGroupWords <= lds,
-                "LDS");
+  static_assert(lds <= 160 * 1024 && WM * WJ * kOutBytes<TJ, WJ> <= lds, "LDS");
   a.tiles_j = (a.J + TJ - 1) / TJ;
   a.tiles_m = KIND == kDw ? (a.C + TM - 1) / TM : 0;
   const int64_t units = KIND == kDw
