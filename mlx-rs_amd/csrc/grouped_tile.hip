@@ -119,11 +119,23 @@ __device__ __forceinline__ void tile_unit(const GroupedArgs& a, const TileAt& at
   const int T = (int)(((MT ? at.len : a.C) + SI - 1) / SI);
   char* extra = smem + STAGES * kS;
 
+  // ---- the rows' indices: asked for first, waited for behind the first loads of J (a wait
+  // for the last load asked for is one for all before it)
+  const auto mrow = [&](int i) { return (wave * ML + i) * (64 / MP) + lane / MP; };
+  constexpr bool kMap = KIND == kForward || F8;
+  int xi[ML] = {}, sx = 0;
+  const int srow = 64 * wave + lane;  // 8-bit: the row (of x, then of W) whose scales it loads
+  if (kMap && mapped) {
+#pragma unroll
+    for (int i = 0; i < ML; ++i)
+      xi[i] = as_global<const int32_t>(a.rows)[at.slot0 + min(mrow(i), rows - 1)];
+    if (F8) sx = as_global<const int32_t>(a.rows)[at.slot0 + min(srow, rows - 1)];
+  }
+
   // ---- M
   const char* mp = static_cast<const char*>(a.m);
   int64_t mbytes;
   uint32_t moff[ML];
-  const auto mrow = [&](int i) { return (wave * ML + i) * (64 / MP) + lane / MP; };
   if constexpr (MT) {
     mp += at.slot0 * ldm + 2 * (int64_t)at.row0;
     mbytes = at.len * ldm - 2 * (int64_t)at.row0;
@@ -133,21 +145,20 @@ __device__ __forceinline__ void tile_unit(const GroupedArgs& a, const TileAt& at
       moff[i] = (uint32_t)(r * ldm) + 32 * ((p >> 1) ^ tkey(r)) + 16 * (p & 1);
     }
   } else {
-    const bool map = mapped && KIND != kDx;
+    const bool map = mapped && kMap;
     if (!map) mp += at.slot0 * ldm;
     mbytes = map ? a.x_rows * ldm : rows * ldm;
-#pragma unroll
-    for (int i = 0; i < ML; ++i) {
-      const int r = mrow(i);
-      int64_t x = r;
-      bool ok = r < rows;
-      if (map) {
-        x = as_global<const int32_t>(a.rows)[at.slot0 + min(r, rows - 1)];
-        ok = ok && x >= 0 && x < a.x_rows;
-      }
-      moff[i] = ok ? (uint32_t)(x * ldm) + 16 * ((lane % MP) ^ rkey<MP>(r)) : kPastEnd;
-    }
   }
+  const auto place_m = [&] {
+    if constexpr (!MT) {
+#pragma unroll
+      for (int i = 0; i < ML; ++i) {
+        const int r = mrow(i), x = kMap && mapped ? xi[i] : r;
+        const bool ok = r < rows && (!(kMap && mapped) || (x >= 0 && x < a.x_rows));
+        moff[i] = ok ? (uint32_t)x * (uint32_t)ldm + 16 * ((lane % MP) ^ rkey<MP>(r)) : kPastEnd;
+      }
+    }
+  };
   // ---- J
   const char* jp = static_cast<const char*>(a.j);
   int64_t jbytes;
@@ -198,18 +209,13 @@ __device__ __forceinline__ void tile_unit(const GroupedArgs& a, const TileAt& at
         const __amdgpu_buffer_rsrc_t jr =
             rsrc(reinterpret_cast<const char*>(a.js) + ((int64_t)at.e * a.J + at.col0) * G + 16 * q,
                  (int64_t)(a.J - at.col0) * G - 16 * q);
-        for (int i = wave; i < (TM + TJ) / 64; i += NW) {
-          const bool isj = i >= TM / 64;
-          const int r = 64 * i + lane - (isj ? TM : 0);
-          uint32_t off = (uint32_t)r * G;
-          if (!isj) {
-            if (r >= rows) off = kPastEnd;
-            if (mapped && r < rows) {
-              const int x = as_global<const int32_t>(a.rows)[at.slot0 + r];
-              off = x >= 0 && x < a.x_rows ? (uint32_t)x * G : kPastEnd;
-            }
-          }
-          load_lds(isj ? jr : mr, S + 1024 * i, off);
+        static_assert(!F8 || (TM + TJ) / 64 <= NW, "one load a wave");
+        if (wave < (TM + TJ) / 64) {
+          const bool isj = wave >= TM / 64;
+          uint32_t off = (uint32_t)(srow - (isj ? TM : 0)) * G;
+          if (!isj && mapped) off = sx >= 0 && sx < a.x_rows ? (uint32_t)sx * G : kPastEnd;
+          if (!isj && srow >= rows) off = kPastEnd;
+          load_lds(isj ? jr : mr, S + 1024 * wave, off);
         }
       } else {
         // rows at any address, byte by byte; zeros past the row
@@ -385,8 +391,12 @@ __device__ __forceinline__ void tile_unit(const GroupedArgs& a, const TileAt& at
   // stands before its last step, when all waves have read the stage for good; the stage
   // STAGES ahead then takes its place.  A stage's loads are back when no more are out than
   // the later stages' (what else is loaded on the way only makes it wait for more).
+  issue_j(0, smem);
+  __builtin_amdgcn_sched_barrier(0);
+  place_m();
+  issue_m(0, smem);
 #pragma unroll
-  for (int t = 0; t < STAGES; ++t) {
+  for (int t = 1; t < STAGES; ++t) {
     issue_m(t, smem + t * kS);
     issue_j(t, smem + t * kS);
   }
