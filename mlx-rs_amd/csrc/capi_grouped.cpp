@@ -112,26 +112,29 @@ int mlxr_moe_grouped_mm_vjp(const void* dy, const void* x, int64_t x_rows, int64
       return capi_fail("grouped_mm_vjp: workspace must be 256-byte aligned");
   }
   hipStream_t s = as_stream(stream);
+  GroupedArgs g{};  // dW
+  if (dw) {
+    g.m = dy, g.j = x, g.offsets = offsets, g.rows = rows, g.out = dw;
+    g.R = R, g.x_rows = x_rows, g.E = (int32_t)E, g.J = (int32_t)K, g.C = (int32_t)N;
+    g.out_f32 = dw_dtype == MLXR_MOE_FLOAT32;
+    Carve c(workspace);
+    const VjpScratch v = plan_vjp(c, R, E, N, K);
+    g.plan = v.plan, g.parts = v.parts;
+    g.chunk = (int32_t)grouped_chunk_rows(R, N, K);
+    g.slices = (int32_t)grouped_slices(R, g.chunk);
+  }
+  const bool both = dx && R && dw;
   if (dx && R) {
     GroupedArgs a{};
     a.m = dy, a.j = w, a.offsets = offsets, a.out = dx;
     a.R = R, a.x_rows = R, a.E = (int32_t)E, a.J = (int32_t)K, a.C = (int32_t)N;
     ProfileScope prof("grouped_dx", s);
-    st = from_hip(launch_grouped_dx(a, s), "grouped_mm_vjp dx");
+    st = from_hip(launch_grouped_dx(a, both ? &g : nullptr, s), "grouped_mm_vjp dx");
     if (!st.ok) return finish(st);
   }
   if (dw) {
-    GroupedArgs a{};
-    a.m = dy, a.j = x, a.offsets = offsets, a.rows = rows, a.out = dw;
-    a.R = R, a.x_rows = x_rows, a.E = (int32_t)E, a.J = (int32_t)K, a.C = (int32_t)N;
-    a.out_f32 = dw_dtype == MLXR_MOE_FLOAT32;
-    Carve c(workspace);
-    const VjpScratch v = plan_vjp(c, R, E, N, K);
-    a.plan = v.plan, a.parts = v.parts;
-    a.chunk = (int32_t)grouped_chunk_rows(R, N, K);
-    a.slices = (int32_t)grouped_slices(R, a.chunk);
     ProfileScope prof("grouped_dw", s);
-    st = from_hip(launch_grouped_dw(a, s), "grouped_mm_vjp dw");
+    st = from_hip(launch_grouped_dw(g, both, s), "grouped_mm_vjp dw");
   }
   return finish(st);
 }

@@ -32,12 +32,13 @@ struct GroupedArgs {
   int32_t out_f32;
   int32_t chunk;   // dW: rows of a group that one tile sums over at most
   int32_t slices;  // dW: of `parts`
-  int32_t max_parts;
+  int32_t max_parts, max_run;  // dW: of all groups, and of one XCD
   float* parts;    // [slices, C, J]: groups summed over in several parts
-  int32_t* plan;   // dW: kPlanHead words, max_parts records, 2 words a slice
+  int32_t* plan;   // dW: kPlanHead words, max_parts records, 2 words a slice.  dx: null, or
+                   // dW's, to be written (with dW's chunk, slices, max_parts and max_run)
 };
 
-// dW's plan, which a kernel of its own writes: where each XCD's parts start (words 0 .. 8),
+// dW's plan, written by one workgroup of dx or of a launch of its own: where each XCD's parts start (words 0 .. 8),
 // the parts' records (expert, first row, rows, slice of a.parts or -1), and of every slice
 // the expert and how many it is the first of (0: it is not the first of an expert's).
 constexpr int kPlanHead = 16;
@@ -221,8 +222,9 @@ inline int64_t grouped_tiles(int64_t R, int64_t E, int64_t TM) {
 // Forward: m = x, j = W [E, J, C]; dx: m = dy, j = W [E, C, J]; dW: m = dy [R, C],
 // j = x, out [E, C, J].
 hipError_t launch_grouped_mm(const GroupedArgs& a, hipStream_t s);
-hipError_t launch_grouped_dx(const GroupedArgs& a, hipStream_t s);
-hipError_t launch_grouped_dw(const GroupedArgs& a, hipStream_t s);
+// dw: dW's arguments, whose plan dx is to write on the way, or null.  planned: it has.
+hipError_t launch_grouped_dx(const GroupedArgs& a, const GroupedArgs* dw, hipStream_t s);
+hipError_t launch_grouped_dw(const GroupedArgs& a, bool planned, hipStream_t s);
 hipError_t launch_grouped_qmm(const GroupedArgs& a, hipStream_t s);
 // grouped_mm and grouped_qmm (a.ms given) where groups have few rows (grouped_stream.hip),
 // and whether they are that few.

@@ -474,6 +474,45 @@ __device__ __forceinline__ void zero_rows(const GroupedArgs& a, int64_t slot0, i
   }
 }
 
+// dW's plan, by one workgroup (every workgroup of the products finding its part by itself
+// took 80 us of 310 at 128 experts of 768 x 2048): block 0 of dx where that is asked for, too
+// (a launch of its own is 4 us), else of grouped_plan_kernel.  kPlanWords words of LDS.
+constexpr int kPlanWords = kGroupWords + kXcds + 1;
+__device__ void write_plan(const GroupedArgs& a, int* lds) {
+  int* starts = lds + kGroupWords;
+  const Groups groups(a, lds);
+  const int tid = threadIdx.x, threads = blockDim.x, cap = a.max_run;
+  if (tid <= (int)kXcds) starts[tid] = groups.start(tid);
+  int4* records = reinterpret_cast<int4*>(a.plan + kPlanHead);
+  int2* first = reinterpret_cast<int2*>(a.plan + kPlanHead + 4 * a.max_parts);
+  const int all = min(groups.parts[groups.groups], a.max_parts);
+  for (int p = tid; p < all; p += threads) {
+    const int g = groups.search(groups.parts, p), k = p - groups.parts[g];
+    const GroupCut c = groups.cut(g);
+    const int slice = c.n > 1 ? groups.slices[g] + k : -1;
+    records[p] = make_int4(g, groups.tab[g] + k * c.each,
+                           min(max(groups.rows(g) - k * c.each, 0), c.each), slice);
+    if (slice >= 0 && slice < a.slices) first[slice] = make_int2(g, k ? 0 : c.n);
+  }
+  __syncthreads();
+  if (tid == 0) {
+    // at most cap parts each, and few enough left for the XCDs behind
+    int at = 0;
+    a.plan[0] = 0;
+    for (int x = 1; x <= (int)kXcds; ++x) {
+      at = max(max(min(min(starts[x], all), at + cap), all - cap * ((int)kXcds - x)), at);
+      a.plan[x] = at;
+    }
+  }
+  // (slices that no expert has)
+  for (int s = groups.slices[groups.groups] + tid; s < a.slices; s += threads)
+    first[s] = make_int2(0, 0);
+}
+__global__ __launch_bounds__(1024) void grouped_plan_kernel(GroupedArgs a) {
+  __shared__ int lds[kPlanWords];
+  write_plan(a, lds);
+}
+
 template <int KIND, int TM, int TJ, int WM, int WJ, int SI, int STAGES>
 __global__ __launch_bounds__(64 * WM * WJ, (kWavesPerSimd<KIND, TM, TJ, WM, WJ, SI, STAGES>))
 void grouped_tile_kernel(GroupedArgs a) {
@@ -489,9 +528,17 @@ void grouped_tile_kernel(GroupedArgs a) {
     u.tile = i % tiles;
     u.e = r.x, u.slot0 = r.y, u.rows = r.z, u.slice = r.w;
   } else {
+    int block = blockIdx.x;
+    if (KIND == kDx && a.plan) {
+      if (block == 0) {
+        write_plan(a, reinterpret_cast<int*>(smem));
+        return;
+      }
+      --block;
+    }
     // parts go to the XCDs in runs, so that one L2 sees an expert's
     const bool found = find_part<TM>(a, reinterpret_cast<int*>(smem), u, [&](int all, auto& v) {
-      const int x = blockIdx.x % kXcds, i = blockIdx.x / kXcds;
+      const int x = block % (int)kXcds, i = block / (int)kXcds;
       const int part = (int)((int64_t)all * x / kXcds) + i / a.tiles_j;
       v.tile = i % a.tiles_j;
       return part < (int)((int64_t)all * (x + 1) / kXcds) ? part : -1;
@@ -547,40 +594,6 @@ void grouped_tile_kernel(GroupedArgs a) {
 #undef MLXR_GT_UNIT
 }
 
-// dW's plan, in one workgroup (every workgroup of the products finding its part by itself
-// took 80 us of 310 at 128 experts of 768 x 2048); cap: parts an XCD that the grid holds.
-__global__ __launch_bounds__(1024) void grouped_plan_kernel(GroupedArgs a, int cap) {
-  __shared__ int lds[kGroupWords];
-  __shared__ int starts[kXcds + 1];
-  const Groups groups(a, lds);
-  const int tid = threadIdx.x;
-  if (tid <= (int)kXcds) starts[tid] = groups.start(tid);
-  int4* records = reinterpret_cast<int4*>(a.plan + kPlanHead);
-  int2* first = reinterpret_cast<int2*>(a.plan + kPlanHead + 4 * a.max_parts);
-  const int all = min(groups.parts[groups.groups], a.max_parts);
-  for (int p = tid; p < all; p += 1024) {
-    const int g = groups.search(groups.parts, p), k = p - groups.parts[g];
-    const GroupCut c = groups.cut(g);
-    const int slice = c.n > 1 ? groups.slices[g] + k : -1;
-    records[p] = make_int4(g, groups.tab[g] + k * c.each,
-                           min(max(groups.rows(g) - k * c.each, 0), c.each), slice);
-    if (slice >= 0 && slice < a.slices) first[slice] = make_int2(g, k ? 0 : c.n);
-  }
-  __syncthreads();
-  if (tid == 0) {
-    // at most cap parts each, and few enough left for the XCDs behind
-    int at = 0;
-    a.plan[0] = 0;
-    for (int x = 1; x <= (int)kXcds; ++x) {
-      at = max(max(min(min(starts[x], all), at + cap), all - cap * ((int)kXcds - x)), at);
-      a.plan[x] = at;
-    }
-  }
-  // (slices that no expert has)
-  for (int s = groups.slices[groups.groups] + tid; s < a.slices; s += 1024)
-    first[s] = make_int2(0, 0);
-}
-
 // The parts of dW of the groups that are summed in several, added in order.  Workgroup b
 // takes slice b / kJoinParts' group, if the slice is the group's first, and part b %
 // kJoinParts of it.
@@ -605,30 +618,35 @@ __global__ __launch_bounds__(256) void grouped_join_kernel(GroupedArgs a) {
   }
 }
 
+// dW's tiles and what its plan holds: parts, of one XCD a quarter more than an eighth, so
+// that those whose parts are lighter take more of them.
+constexpr int kDwTM = 128, kDwTJ = 256;
+GroupedArgs with_plan(GroupedArgs a) {
+  a.tiles_m = (a.C + kDwTM - 1) / kDwTM;
+  a.tiles_j = (a.J + kDwTJ - 1) / kDwTJ;
+  const int64_t parts = grouped_chunks(a.R, a.E, a.chunk);
+  a.max_parts = (int32_t)parts;
+  a.max_run = (int32_t)((parts + kXcds - 1) / kXcds + (parts + 31) / 32);
+  return a;
+}
+
 template <int KIND, int TM, int TJ, int WM, int WJ, int SI, int STAGES>
 hipError_t run_tiles(GroupedArgs a, hipStream_t s) {
   constexpr int lds = kTileLds<KIND, TM, TJ, SI, STAGES>;
-  static_assert(lds <= 160 * 1024 && WM * WJ * kOutBytes<TJ, WJ> <= lds, "LDS");
-  a.tiles_j = (a.J + TJ - 1) / TJ;
-  a.tiles_m = KIND == kDw ? (a.C + TM - 1) / TM : 0;
-  const int64_t units = KIND == kDw
-                            ? grouped_chunks(a.R, a.E, a.chunk) * a.tiles_m * a.tiles_j
-                            : grouped_tiles(a.R, a.E, TM) * a.tiles_j;
-  if (units <= 0) return hipSuccess;
-  // dW: room for XCDs whose parts are lighter to take a quarter more of them
-  const int64_t tiles = KIND == kDw ? (int64_t)a.tiles_m * a.tiles_j : a.tiles_j;
-  const int64_t parts = units / tiles;
-  const int64_t per = (parts + kXcds - 1) / kXcds + (KIND == kDw ? (parts + 31) / 32 : 0);
-  const int64_t grid = per * tiles * kXcds;
-  if (grid * 64 * WM * WJ > UINT32_MAX) return hipErrorInvalidValue;  // (the callers check)
-  if (KIND == kDw) {
-    a.max_parts = (int32_t)parts;
-    grouped_plan_kernel<<<1, 1024, 0, s>>>(a, (int)per);
+  static_assert(lds <= 160 * 1024 && WM * WJ * kOutBytes<TJ, WJ> <= lds && 4 * kPlanWords <= lds,
+                "LDS");
+  int64_t grid;
+  if constexpr (KIND == kDw) {
+    static_assert(TM == kDwTM && TJ == kDwTJ, "the plan's");
+    grid = (int64_t)a.max_run * a.tiles_m * a.tiles_j * kXcds;
+  } else {
+    a.tiles_j = (a.J + TJ - 1) / TJ;
+    const int64_t parts = grouped_tiles(a.R, a.E, TM);
+    grid = (parts + kXcds - 1) / kXcds * a.tiles_j * kXcds + (KIND == kDx && a.plan ? 1 : 0);
   }
+  if (grid * 64 * WM * WJ > UINT32_MAX) return hipErrorInvalidValue;  // (the callers check)
   grouped_tile_kernel<KIND, TM, TJ, WM, WJ, SI, STAGES>
       <<<(unsigned)grid, 64 * WM * WJ, lds, s>>>(a);
-  if (KIND == kDw && a.slices)
-    grouped_join_kernel<<<(unsigned)(a.slices * kJoinParts), 256, 0, s>>>(a);
   return hipGetLastError();
 }
 
@@ -655,14 +673,25 @@ hipError_t launch_grouped_mm(const GroupedArgs& a, hipStream_t s) {
     return run_tiles<kForward, 64, 128, 1, 4, 64, 3>(a, s);
   return run_tiles<kForward, 128, 256, 2, 4, 32, 3>(a, s);
 }
-hipError_t launch_grouped_dx(const GroupedArgs& a, hipStream_t s) {
+hipError_t launch_grouped_dx(const GroupedArgs& given, const GroupedArgs* dw, hipStream_t s) {
+  GroupedArgs a = given;
+  if (dw) {
+    const GroupedArgs p = with_plan(*dw);
+    a.plan = p.plan, a.chunk = p.chunk, a.slices = p.slices;
+    a.max_parts = p.max_parts, a.max_run = p.max_run;
+  }
   if (few_tiles(a.R, a.E, a.J, 256)) return run_tiles<kDx, 64, 128, 1, 4, 64, 3>(a, s);
   return run_tiles<kDx, 128, 256, 2, 4, 32, 3>(a, s);
 }
 // (128 x 128 tiles by four waves: 14.9 us against 16.2 at 1527 rows of 13 experts of 424 x
 // 1032, 23.1 against 22.9 at 1024 rows of 8 of 768 x 2048, 297 against 269 at c2's.)
-hipError_t launch_grouped_dw(const GroupedArgs& a, hipStream_t s) {
-  return run_tiles<kDw, 128, 256, 2, 4, 32, 3>(a, s);
+hipError_t launch_grouped_dw(const GroupedArgs& given, bool planned, hipStream_t s) {
+  const GroupedArgs a = with_plan(given);
+  if (!planned) grouped_plan_kernel<<<1, 1024, 0, s>>>(a);
+  const hipError_t e = run_tiles<kDw, kDwTM, kDwTJ, 2, 4, 32, 3>(a, s);
+  if (e != hipSuccess || !a.slices) return e;
+  grouped_join_kernel<<<(unsigned)(a.slices * kJoinParts), 256, 0, s>>>(a);
+  return hipGetLastError();
 }
 // 128 x 128 by four waves, one a SIMD: at c2's up projection over 32768 rows 97 us, 128 x
 // 256 by eight 102, 64 x 256 by four 135.  64 x 128 where a group has few rows (16 a group
