@@ -8,6 +8,9 @@
 // calls by the latency from the offsets to the last load: a wave asks for all of its chunk
 // before it waits.  The inputs of a row are split over `ksplit` of a workgroup's eight
 // waves, whose sums are joined in LDS in order.
+//
+// Measured: one token's 8 experts of 512 x 2048 7 us (3.5 at a copy's rate), in 8 by 4 bits 8
+// of 768 x 2048 7 us; 640 rows of 512 experts of 2048 x 512 in 8 by 4 bits 50 us, floor 43.
 #include <algorithm>
 
 #include "grouped.hpp"
