@@ -271,7 +271,7 @@ int mlxr_moe_dispatch(const int32_t* ids, int64_t n, int64_t E,
  * the arrays is read or written.
  * grouped_mm: x bf16 [x_rows, K], w bf16 [E, N, K], out [R, N] bf16 or f32, sums in
  * f32.  K and N multiples of 8, up to 2^16; E <= 1024; N * K < 2^30; arrays 16-byte
- * aligned; x under 4 GB where rows are given. */
+ * aligned; x under 4 GB where rows are given; out must not overlap the inputs. */
 int mlxr_moe_grouped_mm(const void* x, int64_t x_rows, int64_t K, const void* w,
                         int64_t num_experts, int64_t N, const int32_t* offsets,
                         const int32_t* rows, int64_t R, void* out, int out_dtype,

@@ -210,7 +210,7 @@ inline int64_t grouped_slices(int64_t R, int64_t chunk) { return R > chunk ? 2 *
 // that has most rows is spread over the chip, and 1024 at least.
 inline int64_t grouped_chunk_rows(int64_t R, int64_t N, int64_t K) {
   const int64_t tiles = ((N + 255) / 256) * ((K + 255) / 256);
-  return std::max<int64_t>(1024, (R * tiles / 128 + 63) / 64 * 64);
+  return std::max<int64_t>(1024, (std::min(R, R * tiles / 128) + 63) / 64 * 64);
 }
 
 // Upper bound of the tiles of TM rows (find_tile's total).

@@ -13,9 +13,9 @@
 // Measured (one MI355X; c2: 128 experts, 4096 tokens of 8 choices, 768 x 2048): down 181 us,
 // its bytes at a copy's rate 122; dx 204, dW 257; 8 by 4 bits up 88, floor 36; 256 experts of
 // 512 x 2048, 2048 tokens of 8 choices 133, floor 117.  With 4 to 32 equal groups 770-910
-// TFLOP/s.  What bounds the ragged ones: loads and their barriers (c2 down without loads 110,
-// with the matrix instructions left out the same), and a workgroup's start and end (40 with
-// no stage in between).
+// TFLOP/s.  What bounds the ragged ones: loads and their barriers (of c2 down's 198 us by the
+// profiler's clock 195 are left without matrix instructions, 110 without loads), and the
+// workgroups' starts and ends (40 with no stage in between).
 #include <algorithm>
 #include <type_traits>
 
@@ -666,9 +666,9 @@ bool few_tiles(int64_t R, int64_t E, int64_t J, int64_t TJ) {
 
 // 128 x 256 tiles by eight waves, two workgroups a CU (128 registers a lane): of the tiles
 // that fit the best in all but the smallest calls.  At c2's down projection over 32768 rows
-// (128 experts, J 2048, C 768; these and the next as measured one after the other, a few us
-// above today's): 185 us, 256 x 256 200, 256 x 128 214, 128 x 128 by four
-// waves 203; dx of its up projection 206, 224, 242, 234.
+// (128 experts, J 2048, C 768; these and the next before steps that took a few us off each):
+// 185 us, 256 x 256 200, 256 x 128 214, 128 x 128 by four waves 203; dx of its up projection
+// 206, 224, 242, 234.
 //
 // 64 x 128 by four waves where these are few: 1024 rows of 8 experts, J 768, C 2048 18.5 us
 // against 33.2, its dx 16.6 against 20.6; 4096 rows 25.5 against 35.1, but dx, J 2048, with

@@ -492,3 +492,54 @@ def test_two_streams_at_once(pkg, dev):
     for outs, right in zip(got, want):
         for out in outs:
             assert all(torch.equal(a, b) for a, b in zip(out, right))
+
+
+@gpu
+def test_few_rows_with_nan_and_loose_offsets(pkg, dev):
+    """The streaming kernel: what is not finite stays in its row and column; offsets that
+    descend or pass the rows stay inside the arrays."""
+    x, w, _, offsets, _ = problem(31, [1, 2, 0, 3] + [0] * 28, 264, 40)
+    x[2, 263], w[3, 5, 7] = torch.nan, torch.inf
+    bad = ~torch.isfinite(pkg.ops.grouped_mm(*to(dev, x, w, offsets)).cpu())
+    assert bool(bad[2].all()) and bool(bad[3:, 5].all())
+    bad[2], bad[3:, 5] = False, False
+    assert not bool(bad.any())
+    x, w, _, offsets, _ = problem(32, [1, 2, 0, 3] + [0] * 28, 160, 40)
+    x[2, 159], w[3, 5, 7] = torch.nan, torch.nan
+    q, sc, _ = pkg.ops.quantize(x.to(dev), mode="mxfp8")
+    wq, wsc, _ = pkg.ops.quantize(w.to(dev), mode="mxfp4")
+    bad = torch.isnan(pkg.ops.grouped_qmm(q, sc, wq, wsc, offsets.to(dev))).cpu()
+    assert bool(bad[2].all()) and bool(bad[3:, 5].all())
+    bad[2], bad[3:, 5] = False, False
+    assert not bool(bad.any())
+    g = torch.Generator().manual_seed(33)
+    for _ in range(4):
+        o = torch.randint(-3, 12, (33,), generator=g, dtype=torch.int32).to(dev)
+        assert pkg.ops.grouped_mm(x.to(dev), w.to(dev), o).shape == (6, 40)
+        assert pkg.ops.grouped_qmm(q, sc, wq, wsc, o).shape == (6, 40)
+
+
+@gpu
+def test_arrays_past_32_bits(pkg, dev):
+    """x, dy, dx and out of more than 2^32 bytes; rows at their ends."""
+    ops, R, wide = pkg.ops, 66000, 32768
+    g = torch.Generator(device=dev).manual_seed(40)
+    big = torch.randint(-2, 3, (R, wide), generator=g, device=dev, dtype=torch.int8).to(BF16)
+    w = torch.randint(-2, 3, (2, 8, wide), generator=g, device=dev, dtype=torch.int8).to(BF16)
+    offsets = torch.tensor([0, 65000, R], dtype=torch.int32, device=dev)
+    last = slice(R - 40, R)
+    # (small whole numbers: every sum is exact in f32)
+    y = ops.grouped_mm(big, w, offsets, out_dtype=F32)
+    assert torch.equal(y[last], big[last].float() @ w[1].float().t())
+    small = torch.randint(-2, 3, (R, 8), generator=g, device=dev, dtype=torch.int8).to(BF16)
+    dx, dw = ops.grouped_mm_vjp(small, big, w, offsets, dw_dtype=F32)
+    assert torch.equal(dx[last].float(), small[last].float() @ w[1].float())
+    assert torch.equal(dw[1], small[65000:].float().t() @ big[65000:].float())
+    del dx, dw, y
+    wt = w.transpose(1, 2).contiguous()
+    out = ops.grouped_mm(small, wt, offsets)
+    assert torch.equal(out[last].float(), small[last].float() @ wt[1].float().t())
+    del out
+    dx, dw = ops.grouped_mm_vjp(big, small, wt, offsets, dw_dtype=F32)
+    assert torch.equal(dx[last].float(), (big[last].float() @ wt[1].float()).to(BF16).float())
+    assert torch.equal(dw[1], big[65000:].float().t() @ small[65000:].float())
