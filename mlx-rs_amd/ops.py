@@ -217,8 +217,8 @@ def _check_mxfp4(name, w, scales, biases, mode="mxfp4", per_word=8):
     if w.dtype not in (torch.int32, torch.uint32) or scales.dtype != torch.uint8:
         raise MlxrMoeError(f"{name}: mode {mode} takes 32-bit words and uint8 scales, got "
                            f"{w.dtype} and {scales.dtype}")
-    if (w.ndim < 1 or w.ndim != scales.ndim or w.shape[:-1] != scales.shape[:-1]
-            or w.shape[-1] * per_word != scales.shape[-1] * MXFP4_GROUP_SIZE):
+    a, b = w.shape, scales.shape
+    if not a or len(a) != len(b) or a[-1] * per_word != b[-1] * MXFP4_GROUP_SIZE or a[:-1] != b[:-1]:
         raise MlxrMoeError(f"{name}: scales {tuple(scales.shape)} must hold one byte for each "
                            f"{'four' if per_word == 8 else 'eight'} words of w "
                            f"{tuple(w.shape)}")
