@@ -533,8 +533,7 @@ int mlxr_moe_rms_norm(const void* x, int64_t T, int64_t d, const void* weight,
  * mlxr_moe_quantize makes them, but of y in f64 (32 divides d): what
  * mlxr_moe_grouped_qmm takes.  Rows holding NaN or an infinity, and without a
  * mode rows of h whose squares pass f32's range, follow the formula in f32.  Any d up to 2^20,
- * T up to 2^24 - 1; arrays aligned to their elements (16-byte alignment and 8
- * dividing d are faster).  h and out must not overlap each other or the inputs. */
+ * T up to 2^24 - 1; arrays aligned to their elements.  h and out must not overlap each other or the inputs. */
 int mlxr_moe_add_rms_norm(const void* x, int x_dtype, const void* residual,
                           int residual_dtype, int64_t T, int64_t d,
                           const void* weight, float eps, const char* mode,

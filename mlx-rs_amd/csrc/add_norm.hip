@@ -13,10 +13,13 @@
 // All sums in f32 (the weight gradient's over workgroups in f64), in fixed orders.
 //
 // HBM-bound: one pass over the rows, a row held in registers, by a wave (many rows)
-// or by a workgroup of four (few rows, or wide ones); 16-byte accesses where d and
-// the addresses allow, single values in a kernel of its own otherwise.  Measured: 8192 rows
+// or by a workgroup of four (few rows, or wide ones), in 16-byte accesses; a form of the
+// kernels takes them at any address and of any length, and rows of more than 16384 values
+// or less than 8 go by single ones.  Measured: 8192 rows
 // of 2048, f32 + bf16 to bf16 and codes, 33 us (4.6 TB/s); the gradients of 32768 of 2048 in
-// f32 178 + 5 us (5.2 TB/s), of 1000 of 4096 in bf16 12 + 4; one row 2.3.
+// f32 167 + 5 us (5.6 TB/s), of 1000 of 4096 in bf16 12 + 4; one row 2.3.  Rows of 2047 as
+// those of 2048 (single values in place of their 16 bytes: 196 us against 104 forward, the
+// gradients 217 against 127, 32768 rows in bf16).
 #include <algorithm>
 #include <type_traits>
 
@@ -30,37 +33,10 @@ namespace {
 
 constexpr int kNT = 256;
 
-// 8 values from element e on, as f32
-template <bool F32>
-__device__ __forceinline__ void load8(const void* p, int64_t e, float (&v)[8]) {
-  if constexpr (F32) {
-    const f32x4_t* q = reinterpret_cast<const f32x4_t*>(static_cast<const float*>(p) + e);
-    const f32x4_t a = q[0], b = q[1];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = a[j], v[4 + j] = b[j];
-  } else {
-    const u32x4_t u = *reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(p) + e);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      v[2 * j] = __uint_as_float(u[j] << 16);
-      v[2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
-    }
-  }
-}
-template <bool F32>
-__device__ __forceinline__ void store8(void* p, int64_t e, const float (&v)[8]) {
-  if constexpr (F32) {
-    f32x4_t* q = reinterpret_cast<f32x4_t*>(static_cast<float*>(p) + e);
-    q[0] = f32x4_t{v[0], v[1], v[2], v[3]};
-    q[1] = f32x4_t{v[4], v[5], v[6], v[7]};
-  } else {
-    u32x4_t u;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      u[j] = (uint32_t)f32_to_bf16(v[2 * j]) | ((uint32_t)f32_to_bf16(v[2 * j + 1]) << 16);
-    *reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(p) + e) = u;
-  }
-}
+// 16 bytes at any element
+typedef f32x4_t f32x4_any __attribute__((aligned(4)));
+typedef u32x4_t u32x4_any __attribute__((aligned(2)));
+
 template <bool F32>
 __device__ __forceinline__ float load1(const void* p, int64_t e) {
   if constexpr (F32)
@@ -78,6 +54,58 @@ __device__ __forceinline__ void store1(void* p, int64_t e, float v) {
 template <bool F32>
 __device__ __forceinline__ float round_to(float v) {
   return F32 ? v : bf16_round(v);
+}
+
+// 8 values from element e on, as f32.  ANY: at any alignment.
+template <bool F32, bool ANY>
+__device__ __forceinline__ void load8(const void* p, int64_t e, float (&v)[8]) {
+  if constexpr (F32) {
+    typedef std::conditional_t<ANY, f32x4_any, f32x4_t> T;
+    const T* q = reinterpret_cast<const T*>(static_cast<const float*>(p) + e);
+    const f32x4_t a = q[0], b = q[1];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = a[j], v[4 + j] = b[j];
+  } else {
+    typedef std::conditional_t<ANY, u32x4_any, u32x4_t> T;
+    const u32x4_t u = *reinterpret_cast<const T*>(static_cast<const uint16_t*>(p) + e);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[2 * j] = __uint_as_float(u[j] << 16);
+      v[2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
+    }
+  }
+}
+template <bool F32, bool ANY>
+__device__ __forceinline__ void store8(void* p, int64_t e, const float (&v)[8]) {
+  if constexpr (F32) {
+    typedef std::conditional_t<ANY, f32x4_any, f32x4_t> T;
+    T* q = reinterpret_cast<T*>(static_cast<float*>(p) + e);
+    q[0] = f32x4_t{v[0], v[1], v[2], v[3]};
+    q[1] = f32x4_t{v[4], v[5], v[6], v[7]};
+  } else {
+    typedef std::conditional_t<ANY, u32x4_any, u32x4_t> T;
+    u32x4_t u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      u[j] = (uint32_t)f32_to_bf16(v[2 * j]) | ((uint32_t)f32_to_bf16(v[2 * j + 1]) << 16);
+    *reinterpret_cast<T*>(static_cast<uint16_t*>(p) + e) = u;
+  }
+}
+// 8 bf16 weights from element j on, as they are
+template <bool ANY>
+__device__ __forceinline__ u32x4_t weights8(const uint16_t* w, int j) {
+  return *reinterpret_cast<const std::conditional_t<ANY, u32x4_any, u32x4_t>*>(w + j);
+}
+// A piece of a row of d values, which is the k-th 8 of them.  ANY: a last one of fewer is the
+// row's last 8, of which the first `skip` are another piece's, too: stored alike by both,
+// summed by that one.
+struct Piece {
+  int j, skip;
+};
+template <bool ANY>
+__device__ __forceinline__ Piece piece_at(int k, int d) {
+  const int j = 8 * k, over = j + 8 - d;
+  return ANY && over > 0 && over < 8 ? Piece{d - 8, over} : Piece{j, 0};
 }
 
 // The sum over a row's threads (64: a wave; 256: the workgroup), the same on all.
@@ -130,7 +158,7 @@ struct NormArgs {
 };
 
 // A row by TPR threads, each C pieces of 8 values.
-template <bool XF32, bool HF32, bool MX, int TPR, int C>
+template <bool XF32, bool HF32, bool MX, int TPR, int C, bool ANY>
 __global__ __launch_bounds__(kNT) void add_rms_norm_kernel(NormArgs a) {
   typedef norm_t<MX> sum_t;
   __shared__ sum_t red[4];
@@ -143,12 +171,12 @@ __global__ __launch_bounds__(kNT) void add_rms_norm_kernel(NormArgs a) {
   sum_t ss = 0;
 #pragma unroll
   for (int i = 0; i < C; ++i) {
-    const int j = 8 * (lane + TPR * i);
+    const int j = piece_at<ANY>(lane + TPR * i, a.d).j;
     float r[8];
     if (j < a.d) {
-      load8<XF32>(a.x, row + j, v[i]);
-      load8<HF32>(a.res, row + j, r);
-      wv[i] = *reinterpret_cast<const u32x4_t*>(a.w + j);
+      load8<XF32, ANY>(a.x, row + j, v[i]);
+      load8<HF32, ANY>(a.res, row + j, r);
+      wv[i] = weights8<ANY>(a.w, j);
 #pragma unroll
       for (int c = 0; c < 8; ++c) v[i][c] = round_to<HF32>(v[i][c] + r[c]);
     } else {
@@ -159,14 +187,15 @@ __global__ __launch_bounds__(kNT) void add_rms_norm_kernel(NormArgs a) {
   }
 #pragma unroll
   for (int i = 0; i < C; ++i) {
-    const int j = 8 * (lane + TPR * i);
-    if (j < a.d) store8<HF32>(a.h, row + j, v[i]);
+    const auto [j, skip] = piece_at<ANY>(lane + TPR * i, a.d);
+    if (j < a.d) store8<HF32, ANY>(a.h, row + j, v[i]);
 #pragma unroll
     for (int c = 0; c < 8; ++c) {
+      const float s = c >= skip ? v[i][c] : 0.0f;
       if constexpr (MX)
-        ss = __builtin_fma((double)v[i][c], (double)v[i][c], ss);
+        ss = __builtin_fma((double)s, (double)s, ss);
       else
-        ss = __builtin_fmaf(v[i][c], v[i][c], ss);
+        ss = __builtin_fmaf(s, s, ss);
     }
   }
   sum_t r;
@@ -176,7 +205,7 @@ __global__ __launch_bounds__(kNT) void add_rms_norm_kernel(NormArgs a) {
     r = 1.0f / sqrtf(row_sum<TPR>(ss, red) / (float)a.d + a.eps);
 #pragma unroll
   for (int i = 0; i < C; ++i) {
-    const int j = 8 * (lane + TPR * i);
+    const int j = piece_at<ANY>(lane + TPR * i, a.d).j;
     float y[8];
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
@@ -196,16 +225,20 @@ __global__ __launch_bounds__(kNT) void add_rms_norm_kernel(NormArgs a) {
       uint2 q;
       const uint32_t byte = mx8_group8(y, q);
       if (j < a.d) {
-        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.out) + row + j) = q;
+        uint32_t* o = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.out) + row + j);
+        if constexpr (ANY)
+          o[0] = q.x, o[1] = q.y;
+        else
+          *reinterpret_cast<uint2*>(o) = q;
         if ((lane & 3) == 0) a.scales[(row + j) >> 5] = (uint8_t)byte;
       }
     } else {
-      if (j < a.d) store8<false>(a.out, row + j, y);
+      if (j < a.d) store8<false, ANY>(a.out, row + j, y);
     }
   }
 }
 
-// Any d and alignment, a workgroup per row: h is written, then read back by the
+// Rows that no registers hold (or no piece), a workgroup each: h is written, then read back by the
 // thread that wrote it.  mxfp8: 32 divides d, and a group is half a wave's.
 template <bool XF32, bool HF32, bool MX>
 __global__ __launch_bounds__(kNT) void add_rms_norm_any_kernel(NormArgs a) {
@@ -254,18 +287,19 @@ struct NormVjpArgs {
 
 // Rows by TPR threads each, C pieces of 8 values a thread; a thread's columns stay
 // its own, so the weight's gradient adds up in registers.
-template <bool YF32, bool HF32, int TPR, int C>
+template <bool YF32, bool HF32, int TPR, int C, bool ANY>
 __global__ __launch_bounds__(kNT) void add_rms_norm_vjp_kernel(NormVjpArgs a) {
   constexpr int RPW = kNT / TPR;
-  extern __shared__ float lds[];  // TPR == 64: the waves' weight gradients [4][d]
+  extern __shared__ float lds[];  // TPR == 64: the waves' weight gradients [4][d], d in eights
+  const int ld = (a.d + 7) & ~7;
   __shared__ float red[8];
   const int lane = threadIdx.x & (TPR - 1), wave = threadIdx.x >> 6;
   float dw[C][8];
   u32x4_t wv[C];
 #pragma unroll
   for (int i = 0; i < C; ++i) {
-    const int j = 8 * (lane + TPR * i);
-    wv[i] = j < a.d ? *reinterpret_cast<const u32x4_t*>(a.w + j) : u32x4_t{0, 0, 0, 0};
+    const int j = piece_at<ANY>(lane + TPR * i, a.d).j;
+    wv[i] = j < a.d ? weights8<ANY>(a.w, j) : u32x4_t{0, 0, 0, 0};
 #pragma unroll
     for (int c = 0; c < 8; ++c) dw[i][c] = 0.0f;
   }
@@ -280,22 +314,25 @@ __global__ __launch_bounds__(kNT) void add_rms_norm_vjp_kernel(NormVjpArgs a) {
     float ss = 0.0f, gh = 0.0f;
 #pragma unroll
     for (int i = 0; i < C; ++i) {
-      const int j = 8 * (lane + TPR * i);
+      const int j = piece_at<ANY>(lane + TPR * i, a.d).j;
       if (j < a.d) {
-        load8<HF32>(a.h, row + j, h[i]);
-        load8<YF32>(a.dy, row + j, dy[i]);
+        load8<HF32, ANY>(a.h, row + j, h[i]);
+        load8<YF32, ANY>(a.dy, row + j, dy[i]);
       } else {
 #pragma unroll
         for (int c = 0; c < 8; ++c) h[i][c] = dy[i][c] = 0.0f;
       }
     }
 #pragma unroll
-    for (int i = 0; i < C; ++i)
+    for (int i = 0; i < C; ++i) {
+      const int skip = piece_at<ANY>(lane + TPR * i, a.d).skip;
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
-        ss = __builtin_fmaf(h[i][c], h[i][c], ss);
-        gh = __builtin_fmaf(dy[i][c] * weight(i, c), h[i][c], gh);
+        const float s = c >= skip ? h[i][c] : 0.0f;
+        ss = __builtin_fmaf(s, s, ss);
+        gh = __builtin_fmaf(c >= skip ? dy[i][c] * weight(i, c) : 0.0f, s, gh);
       }
+    }
     if constexpr (TPR == 64) {
       ss = wave_sum_butterfly(ss);
       gh = wave_sum_butterfly(gh);
@@ -312,10 +349,10 @@ __global__ __launch_bounds__(kNT) void add_rms_norm_vjp_kernel(NormVjpArgs a) {
     const float k = r * r * (gh / (float)a.d);
 #pragma unroll
     for (int i = 0; i < C; ++i) {
-      const int j = 8 * (lane + TPR * i);
+      const int j = piece_at<ANY>(lane + TPR * i, a.d).j;
       float o[8], e[8];
       if (a.dh && j < a.d) {
-        load8<HF32>(a.dh, row + j, e);
+        load8<HF32, ANY>(a.dh, row + j, e);
       } else {
 #pragma unroll
         for (int c = 0; c < 8; ++c) e[c] = 0.0f;
@@ -325,16 +362,20 @@ __global__ __launch_bounds__(kNT) void add_rms_norm_vjp_kernel(NormVjpArgs a) {
         o[c] = __builtin_fmaf(r, dy[i][c] * weight(i, c) - h[i][c] * k, e[c]);
         dw[i][c] = __builtin_fmaf(dy[i][c], h[i][c] * r, dw[i][c]);
       }
-      if (j < a.d) store8<HF32>(a.dx, row + j, o);
+      if (j < a.d) store8<HF32, ANY>(a.dx, row + j, o);
     }
   }
   float* part = a.part + (int64_t)blockIdx.x * a.d;
   if constexpr (TPR == 64) {
 #pragma unroll
     for (int i = 0; i < C; ++i) {
-      const int j = 8 * (lane + TPR * i);
-      if (j < a.d) {
-        f32x4_t* q = reinterpret_cast<f32x4_t*>(lds + wave * a.d + j);
+      const auto [j, skip] = piece_at<ANY>(lane + TPR * i, a.d);
+      if (ANY && skip) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          if (c >= skip) lds[wave * ld + j + c] = dw[i][c];
+      } else if (j < a.d) {
+        f32x4_t* q = reinterpret_cast<f32x4_t*>(lds + wave * ld + j);
         q[0] = f32x4_t{dw[i][0], dw[i][1], dw[i][2], dw[i][3]};
         q[1] = f32x4_t{dw[i][4], dw[i][5], dw[i][6], dw[i][7]};
       }
@@ -342,19 +383,32 @@ __global__ __launch_bounds__(kNT) void add_rms_norm_vjp_kernel(NormVjpArgs a) {
     __syncthreads();
     for (int j = 4 * threadIdx.x; j < a.d; j += 4 * kNT) {
       const f32x4_t* q = reinterpret_cast<const f32x4_t*>(lds + j);
-      const int s = a.d / 4;
-      *reinterpret_cast<f32x4_t*>(part + j) = (q[0] + q[s]) + (q[2 * s] + q[3 * s]);
+      const int s = ld / 4;
+      const f32x4_t v = (q[0] + q[s]) + (q[2 * s] + q[3 * s]);
+      if constexpr (ANY) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (j + i < a.d) part[j + i] = v[i];
+      } else {
+        *reinterpret_cast<f32x4_t*>(part + j) = v;
+      }
     }
   } else {
 #pragma unroll
     for (int i = 0; i < C; ++i) {
-      const int j = 8 * (lane + TPR * i);
-      if (j < a.d) store8<true>(part, j, dw[i]);
+      const auto [j, skip] = piece_at<ANY>(lane + TPR * i, a.d);
+      if (ANY && skip) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          if (c >= skip) part[j + c] = dw[i][c];
+      } else if (j < a.d) {
+        store8<true, ANY>(part, j, dw[i]);
+      }
     }
   }
 }
 
-// Any d and alignment, in two kernels: r and r^3 c of every row, then the columns,
+// Rows that no registers hold (or no piece), in two kernels: r and r^3 c of every row, then the columns,
 // a thread each, over a slice of the rows.
 template <bool YF32, bool HF32>
 __global__ __launch_bounds__(kNT) void norm_vjp_rows_kernel(NormVjpArgs a, float2* coef) {
@@ -430,17 +484,21 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 
 // How a call's rows are split.
 struct RowForm {
-  bool any;  // single values
+  bool wide;  // rows that no registers hold (or no piece): single values
+  bool any;   // 16-byte accesses at any alignment, a last piece over the one before
   int tpr;   // threads per row
   int c;     // pieces of 8 a thread
 };
-// A wave per row holds up to 4096 values and needs rows enough to fill the chip;
-// a workgroup per row up to 16384.
-RowForm row_form(int64_t T, int64_t d, bool vec) {
-  if (!vec || d % 8 || d > 16384) return {true, kNT, 0};
-  const int tpr = d <= 4096 && T >= kNormWaveRows ? 64 : kNT;
-  const int need = (int)((d / 8 + tpr - 1) / tpr);
-  return {false, tpr, need <= 1 ? 1 : need <= 2 ? 2 : need <= 4 ? 4 : 8};
+// A wave per row holds up to kWaveMost values (the gradients fewer, with the weight's gradient
+// beside them: 16384 rows of 4096 in bf16 239 us by waves, 106 by workgroups; 32768 of 2048
+// 180 and 170 in f32, 127 and 125 in bf16) and needs rows enough to fill the chip; a
+// workgroup per row up to 16384.
+constexpr int64_t kWaveMost = 4096, kVjpWaveMost = 1024;
+RowForm row_form(int64_t T, int64_t d, bool vec, int64_t wave_most) {
+  if (d > 16384 || d < 8) return {true, true, kNT, 0};
+  const int tpr = d <= wave_most && T >= kNormWaveRows ? 64 : kNT;
+  const int need = (int)((d + 8 * tpr - 1) / (8 * tpr));
+  return {false, !vec || d % 8 != 0, tpr, need <= 1 ? 1 : need <= 2 ? 2 : need <= 4 ? 4 : 8};
 }
 
 #define MLXR_NORM_FORM(CALL, f)     \
@@ -464,49 +522,51 @@ RowForm row_form(int64_t T, int64_t d, bool vec) {
 
 template <bool XF32, bool HF32, bool MX>
 void run_norm(const NormArgs& a, const RowForm& f, hipStream_t s) {
-  if (f.any) {
+  if (f.wide) {
     add_rms_norm_any_kernel<XF32, HF32, MX><<<(unsigned)a.T, kNT, 0, s>>>(a);
     return;
   }
   const int rpw = kNT / f.tpr;
   const unsigned grid = (unsigned)((a.T + rpw - 1) / rpw);
-#define MLXR_NORM_CALL(TPR, C) \
-  add_rms_norm_kernel<XF32, HF32, MX, TPR, C><<<grid, kNT, 0, s>>>(a)
+#define MLXR_NORM_CALL(TPR, C)                                                  \
+  (f.any ? add_rms_norm_kernel<XF32, HF32, MX, TPR, C, true><<<grid, kNT, 0, s>>>(a) \
+         : add_rms_norm_kernel<XF32, HF32, MX, TPR, C, false><<<grid, kNT, 0, s>>>(a))
   MLXR_NORM_FORM(MLXR_NORM_CALL, f);
 #undef MLXR_NORM_CALL
 }
 
 // Workgroups of the gradient's one-pass form; row slices of the other.
 int vjp_groups(int64_t T, const RowForm& f) {
-  if (f.any) return (int)std::min<int64_t>((T + 63) / 64, 1024);
+  if (f.wide) return (int)std::min<int64_t>((T + 63) / 64, 1024);
   const int rpw = kNT / f.tpr;
-  return (int)std::min<int64_t>((T + rpw - 1) / rpw, kNormVjpGroups);
+  return (int)std::min<int64_t>((T + rpw - 1) / rpw,
+                                T < kNormVjpManyRows ? kNormVjpGroups : kNormVjpManyGroups);
 }
 struct VjpScratch {
   float* part;
   float2* coef;
 };
 VjpScratch carve_vjp(Carve& c, int64_t T, int64_t d) {
-  // room for either form: which one it is goes by the arrays' alignment too
-  const RowForm one = row_form(T, d, true), any = row_form(T, d, false);
+  const RowForm f = row_form(T, d, true, kVjpWaveMost);
   VjpScratch v;
-  v.part = c.take<float>(std::max(vjp_groups(T, one), vjp_groups(T, any)) * d);
-  v.coef = c.take<float2>(T);
+  v.part = c.take<float>(vjp_groups(T, f) * d);
+  v.coef = c.take<float2>(f.wide ? T : 0);
   return v;
 }
 
 template <bool YF32, bool HF32>
 void run_norm_vjp(const NormVjpArgs& a, const RowForm& f, int G, float2* coef, hipStream_t s) {
-  if (f.any) {
+  if (f.wide) {
     const int rows = (int)((a.T + G - 1) / G);
     norm_vjp_rows_kernel<YF32, HF32><<<(unsigned)a.T, kNT, 0, s>>>(a, coef);
     norm_vjp_cols_kernel<YF32, HF32>
         <<<dim3((unsigned)G, (unsigned)((a.d + kNT - 1) / kNT)), kNT, 0, s>>>(a, coef, rows);
     return;
   }
-  const size_t lds = f.tpr == 64 ? (size_t)16 * a.d : 0;
-#define MLXR_NORM_CALL(TPR, C) \
-  add_rms_norm_vjp_kernel<YF32, HF32, TPR, C><<<(unsigned)G, kNT, lds, s>>>(a)
+  const size_t lds = f.tpr == 64 ? (size_t)16 * ((a.d + 7) & ~7) : 0;
+#define MLXR_NORM_CALL(TPR, C)                                                       \
+  (f.any ? add_rms_norm_vjp_kernel<YF32, HF32, TPR, C, true><<<(unsigned)G, kNT, lds, s>>>(a) \
+         : add_rms_norm_vjp_kernel<YF32, HF32, TPR, C, false><<<(unsigned)G, kNT, lds, s>>>(a))
   MLXR_NORM_FORM(MLXR_NORM_CALL, f);
 #undef MLXR_NORM_CALL
 }
@@ -519,7 +579,7 @@ hipError_t launch_add_rms_norm(const void* x, bool x_f32, const void* residual, 
   if (T == 0) return hipSuccess;
   const bool vec = aligned16(x) && aligned16(residual) && aligned16(w) && aligned16(h) &&
                    aligned16(out);
-  const RowForm f = row_form(T, d, vec);
+  const RowForm f = row_form(T, d, vec, kWaveMost);
   const NormArgs a{x, residual, w, h, out, scales, T, (int)d, eps};
   ProfileScope prof("add_rms_norm", s);
 #define MLXR_NORM_TYPES(XF, HF) \
@@ -541,7 +601,7 @@ hipError_t launch_add_rms_norm_vjp(const void* dy, bool dy_f32, const void* h, b
   const VjpScratch v = carve_vjp(ws, T, d);
   const bool vec = aligned16(dy) && aligned16(h) && aligned16(w) && aligned16(dx) &&
                    aligned16(dh);
-  const RowForm f = row_form(T, d, vec);
+  const RowForm f = row_form(T, d, vec, kVjpWaveMost);
   const int G = T ? vjp_groups(T, f) : 0;
   const NormVjpArgs a{dy, h, dh, w, dx, v.part, T, (int)d, eps};
   ProfileScope prof("add_rms_norm_vjp", s);

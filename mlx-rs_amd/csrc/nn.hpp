@@ -67,10 +67,11 @@ hipError_t launch_add_rms_norm_vjp(const void* dy, bool dy_f32, const void* h, b
                                    const void* dh, void* dx, float* dweight, Carve ws,
                                    hipStream_t s);
 // Rows from which a wave takes a row (a workgroup one below), and the workgroups of
-// the gradient's one pass: of 256, 512 and 1024 it and the sum of their parts take
-// 18.3, 15.5 and 21.7 us at 1000 rows of 4096, 267, 185 and 186 at 32768 of 2048 in f32.
+// the gradient's one pass, of few rows and of kNormVjpManyRows: of 256, 512 and 1024 it and
+// the sum of their parts take 18.3, 15.5 and 21.7 us at 1000 rows of 4096; of 512 and 1024
+// 24.5 and 27.0 at 2048 in f32, 136 and 106 at 16384 in bf16, 174 and 176 in f32.
 constexpr int64_t kNormWaveRows = 2048;
-constexpr int64_t kNormVjpGroups = 512;
+constexpr int64_t kNormVjpGroups = 512, kNormVjpManyGroups = 1024, kNormVjpManyRows = 8192;
 // The most rows and values a row of these calls (a grid holds under 2^32 threads).
 constexpr int64_t kMaxNormRows = (1 << 24) - 1, kMaxNormDims = 1 << 20;
 

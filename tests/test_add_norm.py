@@ -387,3 +387,39 @@ def test_codes_are_the_nearest(pkg, dev, T, d, shift, ht):
     byte = scale_bytes8(y)
     assert torch.equal(sc.cpu().long(), byte.long())
     assert torch.equal(decode8(q.cpu(), sc.cpu()), nearest8(y, byte))
+
+
+# Rows of any length and at any address take 16-byte accesses with a shorter last piece; rows of
+# more than 16384 values single ones.
+@gpu
+@pytest.mark.parametrize("ht", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T,d,shift", [(3, 16385, 0), (2050, 2047, 1), (2050, 4095, 0), (5, 12345, 3),
+                                       (2100, 9, 1), (2048, 264, 1), (7, 520, 1), (3, 16384, 1)])
+def test_any_length_and_address(pkg, dev, T, d, shift, ht):
+    ops = pkg.ops
+
+    def off(t):  # the same values, `shift` elements off 16 bytes
+        flat = torch.zeros(t.numel() + shift, dtype=t.dtype, device=dev)
+        flat[shift:] = t.flatten().to(dev)
+        return flat[shift:].view(t.shape)
+
+    x, res, w = inputs(d + T, T, d, torch.float32, ht)
+    h, y = ops.add_rms_norm(off(x), off(res), off(w), EPS)
+    h64 = (x + res.float()).to(ht)
+    assert torch.equal(h.cpu(), h64)
+    want = norm64(h64, w)
+    assert bool(((y.cpu().double() - want).abs() <= (2.0 ** -8 + rel(d)) * want.abs()).all())
+    g = torch.Generator().manual_seed(d)
+    dy, dh = torch.randn((T, d), generator=g), torch.randn((T, d), generator=g).to(ht)
+    dx, dw = ops.add_rms_norm_vjp(off(dy), off(h64), off(w), EPS, off(dh))
+    hh, dd, w64 = h64.double(), dy.double(), w.double()
+    r = 1 / torch.sqrt((hh * hh).mean(-1, keepdim=True) + EPS)
+    gw = dd * w64
+    c = (gw * hh).mean(-1, keepdim=True)
+    want = r * (gw - hh * r * r * c) + dh.double()
+    mass = (r * (gw.abs() + hh.abs() * r * r * (gw * hh).abs().mean(-1, keepdim=True))
+            + dh.double().abs())
+    assert bool(((dx.cpu().double() - want).abs()
+                 <= HALF[ht] * want.abs() + (1 + HALF[ht]) * rel(d) * mass).all())
+    want, mass = (dd * hh * r).sum(0), (dd * hh * r).abs().sum(0)
+    assert bool(((dw.cpu().double() - want).abs() <= (rel(d) + rel(T)) * mass + 1e-30).all())
