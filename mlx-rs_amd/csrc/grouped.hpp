@@ -59,7 +59,7 @@ __device__ __forceinline__ GroupCut cut_tiles(int rows) {
 }
 // dW: parts of `chunk` rows at most, of equal numbers of 64 rows; one for a group without
 // rows, too (its dW is zeros).
-__device__ __forceinline__ GroupCut cut_chunks(int rows, int chunk) {
+__host__ __device__ __forceinline__ GroupCut cut_chunks(int rows, int chunk) {
   const int n = rows > chunk ? (rows + chunk - 1) / chunk : 1;
   return {n, n > 1 ? ((rows + n - 1) / n + 63) & ~63 : rows};
 }
@@ -75,16 +75,23 @@ struct GroupedUnit {
 __device__ __forceinline__ int clamped_offset(const GroupedArgs& a, int e) {
   return min(max(as_global<const int32_t>(a.offsets)[e], 0), (int)a.R);
 }
-// The inclusive sums over a wave's lanes.
-__device__ __forceinline__ int wave_scan(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // of the row's lanes: one
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);  // before, two, four, eight
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // the row's before
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // the half's before
+// The inclusive results of op (of values from 0 on, 0 its neutral one) over a wave's lanes.
+template <class Op>
+__device__ __forceinline__ int wave_scan(int v, Op op) {
+  v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false));  // of the row's lanes:
+  v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false));  // one before, two,
+  v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false));  // four, eight
+  v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false));
+  v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false));  // the row's before
+  v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false));  // the half's before
   return v;
 }
+struct Sum {
+  __host__ __device__ int operator()(int a, int b) const { return a + b; }
+};
+struct Most {
+  __host__ __device__ int operator()(int a, int b) const { return a > b ? a : b; }
+};
 
 // Forward and dx: the unit of a workgroup.  The groups (and the rows behind the last as one
 // more) are cut into parts of TM rows; `pick(all, u)`, of how many there are, gives u.tile and
@@ -107,7 +114,7 @@ __device__ __forceinline__ bool find_part(const GroupedArgs& a, int* lds, Groupe
     n += cut_tiles<TM>(max(to - at, 0)).n;
     at = to;
   }
-  const int upto = wave_scan(n);
+  const int upto = wave_scan(n, Sum{});
   if (lane == 63) lds[wave] = upto;
   __syncthreads();
   int before = upto - n, all = 0;
@@ -137,30 +144,90 @@ __device__ __forceinline__ bool find_part(const GroupedArgs& a, int* lds, Groupe
   return true;
 }
 
+// Upper bounds of the parts, and of the slices.
+inline int64_t grouped_chunks(int64_t R, int64_t E, int64_t chunk) { return R / chunk + E; }
+inline int64_t grouped_slices(int64_t R, int64_t chunk) { return R > chunk ? 2 * (R / chunk) : 0; }
+// Rows that one tile of dW sums over at most: a 128th of all tiles' rows, so that a group
+// that has most rows is spread over the chip, and 1024 at least.
+inline int64_t grouped_chunk_rows(int64_t R, int64_t N, int64_t K) {
+  const int64_t tiles = ((N + 255) / 256) * ((K + 255) / 256);
+  return std::max<int64_t>(1024, (std::min(R, R * tiles / 128) + 63) / 64 * 64);
+}
+
+// dW's tiles and what its plan holds: parts, of one XCD a quarter more than an eighth, so
+// that those whose parts are lighter take more of them.
+constexpr int kDwTM = 128, kDwTJ = 256;
+inline GroupedArgs with_plan(GroupedArgs a) {
+  a.tiles_m = (a.C + kDwTM - 1) / kDwTM;
+  a.tiles_j = (a.J + kDwTJ - 1) / kDwTJ;
+  const int64_t parts = grouped_chunks(a.R, a.E, a.chunk);
+  a.max_parts = (int32_t)parts;
+  a.max_run = (int32_t)((parts + kXcds - 1) / kXcds + (parts + 31) / 32);
+  return a;
+}
+
+// The threads that make a plan together: a workgroup.  (Tests make plans on the host, by one
+// thread.)
+struct PlanTeam {
+  __device__ int tid() const { return threadIdx.x; }
+  __device__ int threads() const { return blockDim.x; }
+  __device__ void sync() const { __syncthreads(); }
+  // op of the values of all threads before this one (0 of the first); 16 words of LDS
+  template <class Op>
+  __device__ int before(int v, int* words, Op op) const {
+    const int lane = tid() & 63, wave = tid() >> 6;
+    v = wave_scan(v, op);
+    if (lane == 63) words[wave] = v;
+    sync();
+    v = __shfl_up(v, 1, 64);
+    if (lane == 0) v = 0;
+    for (int k = 0; k < wave; ++k) v = op(v, words[k]);
+    return v;
+  }
+};
+
 // dW: where the experts' parts lie in the order of all parts, in LDS: kGroupWords words at
-// `lds`, by all of the workgroup's threads.
+// `lds`, by all of the team's threads.  Offsets that do not ascend are taken as the largest
+// one up to there: of groups that lie apart there are never more parts, or slices, than the
+// bounds above.
 constexpr int kGroupWords = 4 * (kMaxExperts + 4) + 64;
+template <class Team>
 struct Groups {
   static constexpr int kStep = kMaxExperts + 4;
   const GroupedArgs& a;
   int *tab, *parts, *slices, *weights;  // offsets; parts, slices, weights before each group
   int groups;
 
-  __device__ __forceinline__ int rows(int g) const { return max(tab[g + 1] - tab[g], 0); }
-  __device__ __forceinline__ GroupCut cut(int g) const { return cut_chunks(rows(g), a.chunk); }
+  __host__ __device__ __forceinline__ int rows(int g) const { return tab[g + 1] - tab[g]; }
+  __host__ __device__ __forceinline__ GroupCut cut(int g) const {
+    return cut_chunks(rows(g), a.chunk);
+  }
   // what a part costs in each of its tiles, in 32-row blocks: its own and what it costs
   // however few it has
-  static __device__ __forceinline__ int weigh(GroupCut c) { return (c.each + 31) / 32 + 9; }
+  static __host__ __device__ __forceinline__ int weigh(GroupCut c) {
+    return (c.each + 31) / 32 + 9;
+  }
 
-  __device__ __forceinline__ Groups(const GroupedArgs& a_, int* lds) : a(a_) {
+  __host__ __device__ __forceinline__ Groups(const GroupedArgs& a_, Team team, int* lds) : a(a_) {
     tab = lds, parts = lds + kStep, slices = lds + 2 * kStep, weights = lds + 3 * kStep;
     int* totals = lds + 4 * kStep;
     groups = a.E;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    for (int e = tid; e <= a.E; e += blockDim.x) tab[e] = clamped_offset(a, e);
-    __syncthreads();
-    const int per = (groups + blockDim.x - 1) / blockDim.x;
-    const int g0 = min(tid * per, groups), g1 = min(g0 + per, groups);
+    const int tid = team.tid(), threads = team.threads();
+    {
+      const int per = (groups + threads) / threads;  // (of the groups + 1 offsets)
+      const int e0 = Most{}(0, tid * per), e1 = e0 + per;
+      int most = 0;
+      for (int e = e0; e < e1 && e <= groups; ++e) {
+        const int o = a.offsets[e];
+        most = Most{}(most, o < a.R ? o : (int)a.R);
+        tab[e] = most;
+      }
+      most = team.before(most, totals + 48, Most{});
+      for (int e = e0; e < e1 && e <= groups; ++e) tab[e] = Most{}(tab[e], most);
+      team.sync();
+    }
+    const int per = (groups + threads - 1) / threads;
+    const int g0 = tid * per, g1 = g0 + per < groups ? g0 + per : groups;
     int n = 0, s = 0, w = 0;
     for (int g = g0; g < g1; ++g) {
       const GroupCut c = cut(g);
@@ -168,11 +235,9 @@ struct Groups {
       if (c.n > 1) s += c.n;
       w += c.n * weigh(c);
     }
-    const int ni = wave_scan(n), si = wave_scan(s), wi = wave_scan(w);
-    if (lane == 63) totals[wave] = ni, totals[16 + wave] = si, totals[32 + wave] = wi;
-    __syncthreads();
-    n = ni - n, s = si - s, w = wi - w;
-    for (int k = 0; k < wave; ++k) n += totals[k], s += totals[16 + k], w += totals[32 + k];
+    n = team.before(n, totals, Sum{});
+    s = team.before(s, totals + 16, Sum{});
+    w = team.before(w, totals + 32, Sum{});
     for (int g = g0; g < g1; ++g) {
       const GroupCut c = cut(g);
       parts[g] = n, slices[g] = s, weights[g] = w;
@@ -180,11 +245,11 @@ struct Groups {
       if (c.n > 1) s += c.n;
       w += c.n * weigh(c);
     }
-    if (tid == (int)blockDim.x - 1) parts[groups] = n, slices[groups] = s, weights[groups] = w;
-    __syncthreads();
+    if (tid == threads - 1) parts[groups] = n, slices[groups] = s, weights[groups] = w;
+    team.sync();
   }
   // The last group whose entry of t is at most v.
-  __device__ __forceinline__ int search(const int* t, int v) const {
+  __host__ __device__ __forceinline__ int search(const int* t, int v) const {
     int lo = 0, hi = groups - 1;
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
@@ -196,21 +261,49 @@ struct Groups {
     return lo;
   }
   // The part that XCD x's start with: an eighth of all parts' weight is before it.
-  __device__ __forceinline__ int start(int x) const {
-    const int w = (int)((int64_t)weights[groups] * x / kXcds);
+  __host__ __device__ __forceinline__ int start(int x) const {
+    const int w = (int)((int64_t)weights[groups] * x / (int)kXcds);
     const int g = search(weights, w);
-    return min(parts[g] + (w - weights[g]) / weigh(cut(g)), parts[groups]);
+    const int p = parts[g] + (w - weights[g]) / weigh(cut(g));
+    return p < parts[groups] ? p : parts[groups];
   }
 };
 
-// Upper bounds of the parts, and of the slices.
-inline int64_t grouped_chunks(int64_t R, int64_t E, int64_t chunk) { return R / chunk + E; }
-inline int64_t grouped_slices(int64_t R, int64_t chunk) { return R > chunk ? 2 * (R / chunk) : 0; }
-// Rows that one tile of dW sums over at most: a 128th of all tiles' rows, so that a group
-// that has most rows is spread over the chip, and 1024 at least.
-inline int64_t grouped_chunk_rows(int64_t R, int64_t N, int64_t K) {
-  const int64_t tiles = ((N + 255) / 256) * ((K + 255) / 256);
-  return std::max<int64_t>(1024, (std::min(R, R * tiles / 128) + 63) / 64 * 64);
+// dW's plan, by one team (every workgroup of the products finding its part by itself
+// took 80 us of 310 at 128 experts of 768 x 2048): block 0 of dx where that is asked for, too
+// (a launch of its own is 4 us), else of grouped_plan_kernel.  kPlanWords words of LDS.
+constexpr int kPlanWords = kGroupWords + kXcds + 1;
+template <class Team>
+__host__ __device__ void write_plan(const GroupedArgs& a, Team team, int* lds) {
+  int* starts = lds + kGroupWords;
+  const Groups<Team> groups(a, team, lds);
+  const int tid = team.tid(), threads = team.threads(), cap = a.max_run;
+  for (int x = tid; x <= (int)kXcds; x += threads) starts[x] = groups.start(x);
+  int4* records = reinterpret_cast<int4*>(a.plan + kPlanHead);
+  int2* first = reinterpret_cast<int2*>(a.plan + kPlanHead + 4 * a.max_parts);
+  const int all = groups.parts[groups.groups];
+  for (int p = tid; p < all; p += threads) {
+    const int g = groups.search(groups.parts, p), k = p - groups.parts[g];
+    const GroupCut c = groups.cut(g);
+    const int left = groups.rows(g) - k * c.each;
+    const int slice = c.n > 1 ? groups.slices[g] + k : -1;
+    records[p] = make_int4(g, groups.tab[g] + k * c.each, left < c.each ? left : c.each, slice);
+    if (slice >= 0) first[slice] = make_int2(g, k ? 0 : c.n);
+  }
+  team.sync();
+  if (tid == 0) {
+    // at most cap parts each, and few enough left for the XCDs behind
+    int at = 0;
+    a.plan[0] = 0;
+    for (int x = 1; x <= (int)kXcds; ++x) {
+      const int want = starts[x] < at + cap ? starts[x] : at + cap;
+      at = Most{}(Most{}(want, all - cap * ((int)kXcds - x)), at);
+      a.plan[x] = at;
+    }
+  }
+  // (slices that no expert has)
+  for (int s = groups.slices[groups.groups] + tid; s < a.slices; s += threads)
+    first[s] = make_int2(0, 0);
 }
 
 // Upper bound of the tiles of TM rows (find_tile's total).

@@ -481,43 +481,9 @@ __device__ __forceinline__ void zero_rows(const GroupedArgs& a, int64_t slot0, i
   }
 }
 
-// dW's plan, by one workgroup (every workgroup of the products finding its part by itself
-// took 80 us of 310 at 128 experts of 768 x 2048): block 0 of dx where that is asked for, too
-// (a launch of its own is 4 us), else of grouped_plan_kernel.  kPlanWords words of LDS.
-constexpr int kPlanWords = kGroupWords + kXcds + 1;
-__device__ void write_plan(const GroupedArgs& a, int* lds) {
-  int* starts = lds + kGroupWords;
-  const Groups groups(a, lds);
-  const int tid = threadIdx.x, threads = blockDim.x, cap = a.max_run;
-  if (tid <= (int)kXcds) starts[tid] = groups.start(tid);
-  int4* records = reinterpret_cast<int4*>(a.plan + kPlanHead);
-  int2* first = reinterpret_cast<int2*>(a.plan + kPlanHead + 4 * a.max_parts);
-  const int all = min(groups.parts[groups.groups], a.max_parts);
-  for (int p = tid; p < all; p += threads) {
-    const int g = groups.search(groups.parts, p), k = p - groups.parts[g];
-    const GroupCut c = groups.cut(g);
-    const int slice = c.n > 1 ? groups.slices[g] + k : -1;
-    records[p] = make_int4(g, groups.tab[g] + k * c.each,
-                           min(max(groups.rows(g) - k * c.each, 0), c.each), slice);
-    if (slice >= 0 && slice < a.slices) first[slice] = make_int2(g, k ? 0 : c.n);
-  }
-  __syncthreads();
-  if (tid == 0) {
-    // at most cap parts each, and few enough left for the XCDs behind
-    int at = 0;
-    a.plan[0] = 0;
-    for (int x = 1; x <= (int)kXcds; ++x) {
-      at = max(max(min(min(starts[x], all), at + cap), all - cap * ((int)kXcds - x)), at);
-      a.plan[x] = at;
-    }
-  }
-  // (slices that no expert has)
-  for (int s = groups.slices[groups.groups] + tid; s < a.slices; s += threads)
-    first[s] = make_int2(0, 0);
-}
 __global__ __launch_bounds__(1024) void grouped_plan_kernel(GroupedArgs a) {
   __shared__ int lds[kPlanWords];
-  write_plan(a, lds);
+  write_plan(a, PlanTeam{}, lds);
 }
 
 template <int KIND, int TM, int TJ, int WM, int WJ, int SI, int STAGES>
@@ -538,7 +504,7 @@ void grouped_tile_kernel(GroupedArgs a) {
     int block = blockIdx.x;
     if (KIND == kDx && a.plan) {
       if (block == 0) {
-        write_plan(a, reinterpret_cast<int*>(smem));
+        write_plan(a, PlanTeam{}, reinterpret_cast<int*>(smem));
         return;
       }
       --block;
@@ -623,18 +589,6 @@ __global__ __launch_bounds__(256) void grouped_join_kernel(GroupedArgs a) {
       *reinterpret_cast<u32x2_t*>(static_cast<uint16_t*>(a.out) + o + 4 * i) =
           u32x2_t{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
   }
-}
-
-// dW's tiles and what its plan holds: parts, of one XCD a quarter more than an eighth, so
-// that those whose parts are lighter take more of them.
-constexpr int kDwTM = 128, kDwTJ = 256;
-GroupedArgs with_plan(GroupedArgs a) {
-  a.tiles_m = (a.C + kDwTM - 1) / kDwTM;
-  a.tiles_j = (a.J + kDwTJ - 1) / kDwTJ;
-  const int64_t parts = grouped_chunks(a.R, a.E, a.chunk);
-  a.max_parts = (int32_t)parts;
-  a.max_run = (int32_t)((parts + kXcds - 1) / kXcds + (parts + 31) / 32);
-  return a;
 }
 
 template <int KIND, int TM, int TJ, int WM, int WJ, int SI, int STAGES>
