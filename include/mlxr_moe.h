@@ -260,12 +260,13 @@ int mlxr_moe_dispatch(const int32_t* ids, int64_t n, int64_t E,
 
 /* Products over rows sorted by expert, as mlxr_moe_dispatch sorts them: expert e has
  * the rows offsets[e] .. offsets[e + 1] - 1 of R (offsets int32 [E + 1] on the device,
- * ascending from 0; groups may be empty).  gather_mm and gather_qmm
+ * ascending; groups may be empty).  gather_mm and gather_qmm
  * (crates/mlxr/src/ops/arithmetic.rs:1577-1613, quantization.rs:171-221) sort their
  * rows at every call and give them in the callers' order; these take them sorted
  * once for all projections and gradients of a layer.
  *   y[r] = x[rows[r]] @ w[e(r)]^T   (rows int32 [R], or NULL: x has R rows, r's own)
- * Rows behind the last group come out as zeros, and so do rows whose index is
+ * Rows before the first group and behind the last (offsets[0] need not be 0: an excerpt of
+ * a larger table will do) come out as zeros, and so do rows whose index is
  * outside [0, x_rows) (their x is taken as zeros).  offsets are clamped to [0, R];
  * where they do not ascend, what comes out is not specified (of dw: as if each were
  * the largest one up to it), but nothing outside the arrays is read or written.
@@ -278,7 +279,7 @@ int mlxr_moe_grouped_mm(const void* x, int64_t x_rows, int64_t K, const void* w,
                         mlxr_moe_stream stream);
 /* Its gradients for dy bf16 [R, N]:
  *   dx[r]    = dy[r] @ w[e(r)]                 bf16 [R, K], of each sorted row's x
- *              (zeros behind the last group); tokens named by several rows sum theirs
+ *              (zeros where no group is); tokens named by several rows sum theirs
  *   dw[e]    = sum over r of e: dy[r]^T x[rows[r]]   f32 or bf16 [E, N, K]; zeros for
  *              experts without rows
  * dx or dw may be NULL (not computed; w, or x, is then not read).  Groups of more

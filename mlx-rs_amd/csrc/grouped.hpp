@@ -1,6 +1,7 @@
 // Products grouped by expert over rows sorted by expert: what their kernels share.
 //
-// Expert e has the rows offsets[e] .. offsets[e + 1] of R (offsets clamped to R).
+// Expert e has the rows offsets[e] .. offsets[e + 1] of R (offsets clamped to R); rows that no
+// expert has come out as zeros.
 #pragma once
 
 #include <algorithm>
@@ -93,21 +94,21 @@ struct Most {
   __host__ __device__ int operator()(int a, int b) const { return a > b ? a : b; }
 };
 
-// Forward and dx: the unit of a workgroup.  The groups (and the rows behind the last as one
-// more) are cut into parts of TM rows; `pick(all, u)`, of how many there are, gives u.tile and
-// the part, or -1 for none.  The thread whose group has that part says where it is: two
-// barriers behind the offsets (a table of all parts, searched by halves: one token through 8
-// of 256 experts 8.4 us, so 7.1).
+// Forward and dx: the unit of a workgroup.  The groups (the rows before the first and those
+// behind the last as one more each) are cut into parts of TM rows; `pick(all, u)`, of how many
+// there are, gives u.tile and the part, or -1 for none.  The thread whose group has that part
+// says where it is: two barriers behind the offsets (a table of all parts, searched by halves:
+// one token through 8 of 256 experts 8.4 us, so 7.1).
 // kFindWords words of LDS.
 constexpr int kFindWords = 32;
 template <int TM, class Pick>
 __device__ __forceinline__ bool find_part(const GroupedArgs& a, int* lds, GroupedUnit& u,
                                           Pick pick) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
-  const int groups = a.E + 1, per = (groups + blockDim.x - 1) / blockDim.x;
+  const int groups = a.E + 2, per = (groups + blockDim.x - 1) / blockDim.x;
   const int g0 = min(tid * per, groups), g1 = min(g0 + per, groups);
-  const auto end = [&](int g) { return g < a.E ? clamped_offset(a, g + 1) : (int)a.R; };
-  const int first = g0 < groups ? clamped_offset(a, g0) : 0;
+  const auto end = [&](int g) { return g <= a.E ? clamped_offset(a, g) : (int)a.R; };
+  const int first = g0 > 0 ? end(g0 - 1) : 0;
   int n = 0;
   for (int g = g0, at = first; g < g1; ++g) {
     const int to = end(g);
@@ -133,7 +134,7 @@ __device__ __forceinline__ bool find_part(const GroupedArgs& a, int* lds, Groupe
       at = to, to = end(++g);
       c = cut_tiles<TM>(max(to - at, 0));
     }
-    lds[16] = g, lds[17] = at + k * c.each;
+    lds[16] = g > 0 && g <= a.E ? g - 1 : a.E, lds[17] = at + k * c.each;
     lds[18] = min(to - at - k * c.each, c.each);
   }
   __syncthreads();
@@ -306,9 +307,9 @@ __host__ __device__ void write_plan(const GroupedArgs& a, Team team, int* lds) {
     first[s] = make_int2(0, 0);
 }
 
-// Upper bound of the tiles of TM rows (find_tile's total).
+// Upper bound of the parts of TM rows that find_part cuts.
 inline int64_t grouped_tiles(int64_t R, int64_t E, int64_t TM) {
-  return R / TM + (R < E + 1 ? R : E + 1);
+  return R / TM + std::min(R, E + 2);
 }
 
 // The products (grouped_tile.hip); a.tiles_m and tiles_j are the launchers' own.
@@ -327,7 +328,7 @@ hipError_t launch_grouped_stream(const GroupedArgs& a, hipStream_t s);
 // Rows, inputs and outputs that the kernels' grids hold: R rows by J columns.
 constexpr int64_t kMaxGroupedRows = 1 << 24, kMaxGroupedDims = 1 << 16;
 inline bool grouped_grid_ok(int64_t R, int64_t E, int64_t J) {
-  return (grouped_tiles(R, E, 16) + 8) * ((J + 127) / 128 + 8) < ((int64_t)1 << 24);
+  return (grouped_tiles(R, E, 16) + 7) * ((J + 127) / 128 + 8) < ((int64_t)1 << 24);
 }
 
 }  // namespace mlxr_moe

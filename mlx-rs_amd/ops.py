@@ -659,11 +659,11 @@ def _bf16(name, what, t):
 def grouped_mm(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, rows=None,
                out_dtype=torch.bfloat16):
     """y[r] = x[rows[r]] @ w[e(r)]^T over R rows sorted by expert: expert e has the
-    rows offsets[e] .. offsets[e + 1] (as dispatch gives them), w bf16 [E, N, K].
-    With rows [R] x is bf16 [.., K] of any number of rows (a token's row taken by
-    each of its choices), without it x's rows are the sorted ones.  Returns [R, N]
-    in out_dtype (bf16 or f32); zeros behind the last group and where rows names no
-    row of x.  K and N multiples of 8.  Not recorded by autograd: the gradients are
+    rows offsets[e] .. offsets[e + 1] (as dispatch gives them, or some experts' of
+    those), w bf16 [E, N, K].  With rows [R] x is bf16 [.., K] of any number of rows
+    (a token's row taken by each of its choices), without it x's rows are the sorted
+    ones.  Returns [R, N] in out_dtype (bf16 or f32); zeros in rows of no group and
+    where rows names no row of x.  K and N multiples of 8.  Not recorded by autograd: the gradients are
     grouped_mm_vjp's."""
     _dev(x, w, offsets, rows)
     w = _grouped_weight("grouped_mm", w)
