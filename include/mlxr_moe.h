@@ -267,7 +267,7 @@ int mlxr_moe_dispatch(const int32_t* ids, int64_t n, int64_t E,
  *   y[r] = x[rows[r]] @ w[e(r)]^T   (rows int32 [R], or NULL: x has R rows, r's own)
  * Rows before the first group and behind the last (offsets[0] need not be 0: an excerpt of
  * a larger table will do) come out as zeros, and so do rows whose index is
- * outside [0, x_rows) (their x is taken as zeros).  offsets are clamped to [0, R];
+ * outside [0, x_rows), whatever w holds.  offsets are clamped to [0, R];
  * where they do not ascend, what comes out is not specified (of dw: as if each were
  * the largest one up to it), but nothing outside the arrays is read or written.
  * grouped_mm: x bf16 [x_rows, K], w bf16 [E, N, K], out [R, N] bf16 or f32, sums in

@@ -62,10 +62,13 @@ __global__ __launch_bounds__(64 * kWaves) void grouped_stream_kernel(GroupedArgs
   const int tiles = min(per, a.tiles_j - tile0);
   const int wcol0 = (tile0 * csplit + wave % csplit) * 16;  // the wave's columns: of tile t
   const int es = a.out_f32 ? 4 : 2;                         // from 16 csplit t on
-  // lane: of row c columns 4 g .. + 3 of a tile
+  uint32_t xrow = c;    // the lane's row of x
+  bool xok = c < rows;  // (false, too, of an index that names none)
+  // lane: of row c columns 4 g .. + 3 of a tile; zeros where no row of x is, whatever W holds
   const auto put = [&](int t, f32x4_t v) {
     const int col = wcol0 + 16 * csplit * t + 4 * g;
     if (c >= rows || col >= a.J) return;
+    if (!xok) v = f32x4_t{0, 0, 0, 0};
     char* p = static_cast<char*>(a.out) + ((int64_t)(slot0 + c) * a.J + col) * es;
     if (a.out_f32)
       *reinterpret_cast<f32x4_t*>(p) = v;
@@ -114,8 +117,6 @@ __global__ __launch_bounds__(64 * kWaves) void grouped_stream_kernel(GroupedArgs
             wsr, ok ? r * G + at(s + i) / 32 : kPastEnd, 0, 0);
     }
   };
-  uint32_t xrow = c;
-  bool xok = c < rows;
   const auto load_x = [&](Chunk& k, int s) {
 #pragma unroll
     for (int i = 0; i < CH; ++i) {

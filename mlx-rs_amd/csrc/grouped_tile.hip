@@ -130,14 +130,18 @@ __device__ __forceinline__ void tile_unit(const GroupedArgs& a, const TileAt& at
   // for the last load asked for is one for all before it)
   const auto mrow = [&](int i) { return (wave * ML + i) * (64 / MP) + lane / MP; };
   constexpr bool kMap = KIND == kForward || F8;
-  int xi[ML] = {}, sx = 0;
+  int xi[ML] = {}, sx = 0, oi[NA] = {};  // (oi: of the output rows that the lane has)
   const int srow = 64 * wave + lane;  // 8-bit: the row (of x, then of W) whose scales it loads
   if (kMap && mapped) {
 #pragma unroll
     for (int i = 0; i < ML; ++i)
       xi[i] = as_global<const int32_t>(a.rows)[at.slot0 + min(mrow(i), rows - 1)];
     if (F8) sx = as_global<const int32_t>(a.rows)[at.slot0 + min(srow, rows - 1)];
+#pragma unroll
+    for (int i = 0; i < NMB; ++i)
+      oi[i] = as_global<const int32_t>(a.rows)[at.slot0 + min(32 * (wm + WM * i) + c, rows - 1)];
   }
+  uint64_t none[NA] = {};  // by lane: whether its index names no row of x
 
   // ---- M
   const char* mp = static_cast<const char*>(a.m);
@@ -164,6 +168,11 @@ __device__ __forceinline__ void tile_unit(const GroupedArgs& a, const TileAt& at
         const bool ok = r < rows && (!(kMap && mapped) || (x >= 0 && x < a.x_rows));
         moff[i] = ok ? (uint32_t)x * (uint32_t)ldm + 16 * ((lane % MP) ^ rkey<MP>(r)) : kPastEnd;
       }
+    }
+    if constexpr (kMap) {
+      if (mapped)
+#pragma unroll
+        for (int i = 0; i < NMB; ++i) none[i] = __ballot(oi[i] < 0 || oi[i] >= a.x_rows);
     }
   };
   // ---- J
@@ -443,12 +452,15 @@ __device__ __forceinline__ void tile_unit(const GroupedArgs& a, const TileAt& at
     for (int i = 0; i < NA; ++i) {
       const int row1 = 32 * (wm + WM * i);
       const int es = at.f32 ? 4 : 2, stride = WC * es + 16;
+      // (zeros where no row of x is, whatever W holds)
+      const bool zero = kMap && (none[i] >> lane & 1);
 #pragma unroll
       for (int j = 0; j < NB; ++j)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const f32x4_t v{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2],
-                          acc[i][j][4 * q + 3]};
+          f32x4_t v{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2],
+                    acc[i][j][4 * q + 3]};
+          if (zero) v = f32x4_t{0, 0, 0, 0};
           char* p = O + c * stride + (32 * j + 8 * q + 4 * h) * es;
           if (at.f32)
             *reinterpret_cast<f32x4_t*>(p) = v;

@@ -105,3 +105,41 @@ def test_a_slice_of_the_offsets(pkg, dev, case):
     s = slice(int(offsets[a]), int(offsets[b]))
     assert bool((got[:s.start] == 0).all()) and bool((got[s.stop:] == 0).all())
     near(got, *forward64(x.double(), w[a:b], offsets[a:b + 1]), w.shape[2])
+
+
+NONE = torch.tensor([-1, 37, 2 ** 31 - 1, -2 ** 31], dtype=torch.int32)
+
+
+def padded(case, seed):
+    """A problem over 37 rows of x in which every seventh sorted row names none."""
+    x, w, dy, offsets, rows = shifted(case, 2, 3, seed, mapped=37)
+    bad = torch.zeros(rows.numel(), dtype=torch.bool)
+    bad[1::7] = True
+    bad[2], bad[-4] = True, True  # the first and the last group's ends
+    rows[bad] = NONE.repeat(rows.numel())[: int(bad.sum())]
+    return x, w, dy, offsets, rows, bad
+
+
+@gpu
+@pytest.mark.parametrize("case", sorted(CASES))
+def test_rows_that_name_none_are_zeros_by_any_weights(pkg, dev, case):
+    """Infinities and NaN in the weights reach the rows of their group that name a row of x, and
+    no other."""
+    x, w, _, offsets, rows, bad = padded(case, 11)
+    w[0, 3, 5], w[-1, 7, 0], w[0, 8] = torch.nan, torch.inf, -torch.inf
+    c, R = Filled(pkg, dev), rows.numel()
+    xd, wd, od, rd = to(dev, x, w, offsets, rows)
+    y = c.mm(xd, wd, od, rd, R).cpu()
+    assert bool((y[bad] == 0).all())
+    ok = ~bad
+    ok[: int(offsets[0])], ok[int(offsets[-1]):] = False, False
+    last = slice(int(offsets[-2]), int(offsets[-1]))
+    assert not bool(torch.isfinite(y[last, 7][ok[last]]).any())
+    assert bool(torch.isfinite(y[:, 10]).all())
+    q, sc, _ = pkg.ops.quantize(xd, mode="mxfp8")
+    wq, wsc, _ = pkg.ops.quantize(wd, mode="mxfp4")  # (scale bytes of 255)
+    assert bool((wsc == 255).any())
+    y = c.qmm(q, sc, wq, wsc, od, rd, R).cpu()
+    assert bool((y[bad] == 0).all())
+    assert bool(torch.isnan(y[last, 7][ok[last]]).all())
+    assert bool(torch.isfinite(y[:, 10]).all())
