@@ -281,7 +281,8 @@ int mlxr_moe_grouped_mm(const void* x, int64_t x_rows, int64_t K, const void* w,
  *   dx[r]    = dy[r] @ w[e(r)]                 bf16 [R, K], of each sorted row's x
  *              (zeros where no group is); tokens named by several rows sum theirs
  *   dw[e]    = sum over r of e: dy[r]^T x[rows[r]]   f32 or bf16 [E, N, K]; zeros for
- *              experts without rows
+ *              experts without rows.  Rows whose index is outside [0, x_rows) add
+ *              nothing, whatever dy holds there (their dx is dy[r] @ w[e(r)] as the others')
  * dx or dw may be NULL (not computed; w, or x, is then not read).  Groups of more
  * rows than a tile sums are summed in parts (f32, in the workspace), added in the
  * rows' order: equal inputs give equal bits.  workspace is dw's (256-byte aligned;

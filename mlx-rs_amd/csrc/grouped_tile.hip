@@ -123,6 +123,8 @@ __device__ __forceinline__ void tile_unit(const GroupedArgs& a, const TileAt& at
   const int64_t ldm = F8 ? (int64_t)a.C : (int64_t)a.C * 2;  // bytes
   const int64_t ldj = JT ? (int64_t)a.J * 2 : F8 ? (int64_t)a.C / 2 : (int64_t)a.C * 2;
   const bool mapped = a.rows != nullptr;  // x's rows (M forward, J of dW)
+  // (negative indices are past all rows as unsigned ones)
+  const uint32_t x_rows = (uint32_t)min(a.x_rows, (int64_t)1 << 31);
   const int T = (int)(((MT ? at.len : a.C) + SI - 1) / SI);
   char* extra = smem + STAGES * kS;
 
@@ -165,14 +167,14 @@ __device__ __forceinline__ void tile_unit(const GroupedArgs& a, const TileAt& at
 #pragma unroll
       for (int i = 0; i < ML; ++i) {
         const int r = mrow(i), x = kMap && mapped ? xi[i] : r;
-        const bool ok = r < rows && (!(kMap && mapped) || (x >= 0 && x < a.x_rows));
+        const bool ok = r < rows && (!(kMap && mapped) || (uint32_t)x < x_rows);
         moff[i] = ok ? (uint32_t)x * (uint32_t)ldm + 16 * ((lane % MP) ^ rkey<MP>(r)) : kPastEnd;
       }
     }
     if constexpr (kMap) {
       if (mapped)
 #pragma unroll
-        for (int i = 0; i < NMB; ++i) none[i] = __ballot(oi[i] < 0 || oi[i] >= a.x_rows);
+        for (int i = 0; i < NMB; ++i) none[i] = __ballot((uint32_t)oi[i] >= x_rows);
     }
   };
   // ---- J
@@ -212,6 +214,10 @@ __device__ __forceinline__ void tile_unit(const GroupedArgs& a, const TileAt& at
             0);
     }
   };
+  // ... of stage t's rows (past the last stage of any: nothing of it is read)
+  const auto stage_index = [&](int t) {
+    return reinterpret_cast<const int*>(extra) + t * SI % (2 * kIndexRows);
+  };
   // ---- 8-bit: the scales of inputs 512 q .. 512 q + 511, 16 bytes a row
   const int G = a.C / 32;
   auto issue_scales = [&](int q) {
@@ -229,7 +235,7 @@ __device__ __forceinline__ void tile_unit(const GroupedArgs& a, const TileAt& at
         if (wave < (TM + TJ) / 64) {
           const bool isj = wave >= TM / 64;
           uint32_t off = (uint32_t)(srow - (isj ? TM : 0)) * G;
-          if (!isj && mapped) off = sx >= 0 && sx < a.x_rows ? (uint32_t)sx * G : kPastEnd;
+          if (!isj && mapped) off = (uint32_t)sx < x_rows ? (uint32_t)sx * G : kPastEnd;
           if (!isj && srow >= rows) off = kPastEnd;
           load_lds(isj ? jr : mr, S + 1024 * wave, off);
         }
@@ -258,15 +264,30 @@ __device__ __forceinline__ void tile_unit(const GroupedArgs& a, const TileAt& at
 
   // ---- a stage's loads, always as many (past the last stage of nothing)
   const int mpieces = (int)(ldm / 16), jpieces = (int)(ldj / 16);
+  bool named[ML];
+  for (int i = 0; i < ML; ++i) named[i] = true;
   auto issue_m = [&](int t, char* S) {
     if (F8 && t % (512 / SI) == 0 && t < T) issue_scales(t / (512 / SI));
     const int64_t mo = MT ? (int64_t)t * SI * ldm : (int64_t)t * MR;
     const __amdgpu_buffer_rsrc_t mr = rsrc(mp + mo, t < T ? mbytes - mo : 0);
 #pragma unroll
     for (int i = 0; i < ML; ++i) {
-      bool ok = true;
+      bool ok = KIND != kDw || named[i];
       if constexpr (!MT) ok = MP * t + ((lane % MP) ^ rkey<MP>(mrow(i))) < mpieces;
       load_lds(mr, S + (wave * ML + i) * 1024, ok ? moff[i] : kPastEnd);
+    }
+  };
+  // dW: which of this lane's rows of stage t name a row of x.  dy of one that does not is left
+  // out as its x is (it may hold a NaN).  Asked for a step ahead: c2's up projection 253 us so,
+  // 257 with the look at the loads (247 without any).
+  auto look_m = [&](int t) {
+    if constexpr (KIND == kDw) {
+      if (!mapped) return;
+      const int* xi = stage_index(t);
+#pragma unroll
+      for (int i = 0; i < ML; ++i) {
+        named[i] = (uint32_t)xi[mrow(i)] < x_rows;
+      }
     }
   };
   auto issue_j = [&](int t, char* S) {
@@ -275,13 +296,13 @@ __device__ __forceinline__ void tile_unit(const GroupedArgs& a, const TileAt& at
         constexpr int kPer = kIndexRows / SI;  // stages a part of the indices
         if (t % kPer == 0 && t > 0) issue_index(t / kPer + 1);
         const __amdgpu_buffer_rsrc_t jr = rsrc(jp, t < T ? jbytes : 0);
-        const int* xi = reinterpret_cast<const int*>(extra) + t * SI % (2 * kIndexRows);
+        const int* xi = stage_index(t);
 #pragma unroll
         for (int i = 0; i < JL; ++i) {
-          const int64_t x = xi[jrow(i)];
-          const bool ok = x >= 0 && x < a.x_rows && (int64_t)t * SI + jrow(i) < at.len;
+          const uint32_t x = xi[jrow(i)];
+          const bool ok = x < x_rows && t * SI + jrow(i) < (int)at.len;
           load_lds(jr, S + kM + (wave * JL + i) * 1024,
-                   ok ? joff[i] + (uint32_t)(x * ldj) : kPastEnd);
+                   ok ? joff[i] + x * (uint32_t)ldj : kPastEnd);
         }
         return;
       }
@@ -410,9 +431,11 @@ __device__ __forceinline__ void tile_unit(const GroupedArgs& a, const TileAt& at
   issue_j(0, smem);
   __builtin_amdgcn_sched_barrier(0);
   place_m();
+  look_m(0);
   issue_m(0, smem);
 #pragma unroll
   for (int t = 1; t < STAGES; ++t) {
+    look_m(t);
     issue_m(t, smem + t * kS);
     issue_j(t, smem + t * kS);
   }
@@ -430,7 +453,10 @@ __device__ __forceinline__ void tile_unit(const GroupedArgs& a, const TileAt& at
         issue_m(t + STAGES, smem + from);
       } else {
         read(smem + from, t, ks + 1, (ks + 1) & 1);
-        if (ks == 0 && t > 0) issue_j(t - 1 + STAGES, smem + last);
+        if (ks == 0) {
+          if (t > 0) issue_j(t - 1 + STAGES, smem + last);
+          look_m(t + STAGES);
+        }
       }
       __builtin_amdgcn_sched_barrier(0);
       multiply(ks, ks & 1);

@@ -682,8 +682,8 @@ def grouped_mm_vjp(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, offsets: 
                    rows=None, dw_dtype=torch.bfloat16, need_dx=True, need_dw=True):
     """The gradients of grouped_mm for dy bf16 [R, N]: (dx, dw), dx bf16 [R, K] of each
     sorted row's x (a token's choices sum theirs: combine with weights of 1), dw
-    [E, N, K] in dw_dtype (bf16 or f32), zeros for experts without rows.  None where
-    not needed."""
+    [E, N, K] in dw_dtype (bf16 or f32), zeros for experts without rows; rows that name
+    no row of x add nothing to it.  None where not needed."""
     _dev(dy, x, w, offsets, rows)
     w = _grouped_weight("grouped_mm_vjp", w)
     _bf16("grouped_mm_vjp", "x", x)

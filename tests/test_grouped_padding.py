@@ -143,3 +143,31 @@ def test_rows_that_name_none_are_zeros_by_any_weights(pkg, dev, case):
     assert bool((y[bad] == 0).all())
     assert bool(torch.isnan(y[last, 7][ok[last]]).all())
     assert bool(torch.isfinite(y[:, 10]).all())
+
+
+@gpu
+@pytest.mark.parametrize("case", sorted(CASES))
+@pytest.mark.parametrize("long", [False, True])
+def test_rows_that_name_none_add_nothing(pkg, dev, case, long):
+    """dW of rows that name none, whatever their dy: the same bits as with zeros there."""
+    x, w, dy, offsets, rows, bad = padded(case, 12)
+    if long:  # one group, several parts of its rows and several tables of their indices
+        n = 3000
+        g = torch.Generator().manual_seed(4)
+        offsets = torch.tensor([0, n], dtype=torch.int32)
+        dy = torch.randn((n, w.shape[1]), generator=g).to(BF16)
+        rows = torch.randint(-9, 46, (n,), generator=g, dtype=torch.int32)
+        bad = (rows < 0) | (rows >= 37)
+        w = w[:1]
+    clean = torch.where(bad[:, None], 0.0, dy.float()).to(BF16)
+    dirty = dy.clone()
+    dirty[bad] = torch.tensor([torch.nan, torch.inf, -torch.inf, 3e38])[
+        torch.arange(int(bad.sum())) % 4][:, None].to(BF16)
+    c = Filled(pkg, dev)
+    a = c.vjp(*to(dev, clean, x, w, offsets, rows))[1]
+    b = c.vjp(*to(dev, dirty, x, w, offsets, rows))[1]
+    assert bool(torch.isfinite(a).all()) and torch.equal(a, b)
+    xs, g = taken(x, rows), clean.double()
+    for e in range(w.shape[0]):
+        s = slice(int(offsets[e]), int(offsets[e + 1]))
+        near(a[e], g[s].t() @ xs[s], g[s].abs().t() @ xs[s].abs(), s.stop - s.start + 1)
