@@ -423,3 +423,16 @@ def test_any_length_and_address(pkg, dev, T, d, shift, ht):
                  <= HALF[ht] * want.abs() + (1 + HALF[ht]) * rel(d) * mass).all())
     want, mass = (dd * hh * r).sum(0), (dd * hh * r).abs().sum(0)
     assert bool(((dw.cpu().double() - want).abs() <= (rel(d) + rel(T)) * mass + 1e-30).all())
+
+
+# Rows that no registers hold go by a kernel of their own, whose norm is in 64 bits, too.
+@gpu
+@pytest.mark.parametrize("ht", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T,d", [(160, 16416), (60, 20000), (3, 65536)])
+def test_codes_of_wide_rows_are_the_nearest(pkg, dev, T, d, ht):
+    x, res, w = (t.to(dev) for t in inputs(78, T, d, torch.float32, ht))
+    h, q, sc = pkg.ops.add_rms_norm(x, res, w, EPS, mode="mxfp8")
+    y = norm64(h.cpu(), w.cpu())
+    byte = scale_bytes8(y)
+    assert torch.equal(sc.cpu().long(), byte.long())
+    assert torch.equal(decode8(q.cpu(), sc.cpu()), nearest8(y, byte))
