@@ -494,6 +494,7 @@ struct RowForm {
 // 180 and 170 in f32, 127 and 125 in bf16) and needs rows enough to fill the chip; a
 // workgroup per row up to 16384.
 constexpr int64_t kWaveMost = 4096, kVjpWaveMost = 1024;
+static_assert(kWaveMost <= 8 * 64 * 8 && kVjpWaveMost <= 8 * 64 * 2, "pieces of a wave's lanes");
 RowForm row_form(int64_t T, int64_t d, bool vec, int64_t wave_most) {
   if (d > 16384 || d < 8) return {true, true, kNT, 0};
   const int tpr = d <= wave_most && T >= kNormWaveRows ? 64 : kNT;
@@ -501,24 +502,27 @@ RowForm row_form(int64_t T, int64_t d, bool vec, int64_t wave_most) {
   return {false, !vec || d % 8 != 0, tpr, need <= 1 ? 1 : need <= 2 ? 2 : need <= 4 ? 4 : 8};
 }
 
-#define MLXR_NORM_FORM(CALL, f)     \
-  do {                              \
-    if (f.tpr == 64) {              \
-      switch (f.c) {                \
-        case 1: CALL(64, 1); break; \
-        case 2: CALL(64, 2); break; \
-        case 4: CALL(64, 4); break; \
-        default: CALL(64, 8);       \
-      }                             \
-    } else {                        \
-      switch (f.c) {                \
-        case 1: CALL(256, 1); break;\
-        case 2: CALL(256, 2); break;\
-        case 4: CALL(256, 4); break;\
-        default: CALL(256, 8);      \
-      }                             \
-    }                               \
+// CALL(threads a row, pieces a thread) by f; WIDE_WAVE(CALL, f) of a wave with more than two.
+#define MLXR_NORM_FORM(CALL, f, WIDE_WAVE)          \
+  do {                                              \
+    if (f.tpr == 64) {                              \
+      if (f.c == 1)                                 \
+        CALL(64, 1);                                \
+      else if (f.c == 2)                            \
+        CALL(64, 2);                                \
+      else                                          \
+        WIDE_WAVE(CALL, f);                         \
+    } else {                                        \
+      switch (f.c) {                                \
+        case 1: CALL(256, 1); break;                \
+        case 2: CALL(256, 2); break;                \
+        case 4: CALL(256, 4); break;                \
+        default: CALL(256, 8);                      \
+      }                                             \
+    }                                               \
   } while (0)
+#define MLXR_NORM_WIDE_WAVE(CALL, f) (f.c == 4 ? CALL(64, 4) : CALL(64, 8))
+#define MLXR_NORM_NO_WIDE_WAVE(CALL, f) ((void)0)  // (kVjpWaveMost)
 
 template <bool XF32, bool HF32, bool MX>
 void run_norm(const NormArgs& a, const RowForm& f, hipStream_t s) {
@@ -531,7 +535,7 @@ void run_norm(const NormArgs& a, const RowForm& f, hipStream_t s) {
 #define MLXR_NORM_CALL(TPR, C)                                                  \
   (f.any ? add_rms_norm_kernel<XF32, HF32, MX, TPR, C, true><<<grid, kNT, 0, s>>>(a) \
          : add_rms_norm_kernel<XF32, HF32, MX, TPR, C, false><<<grid, kNT, 0, s>>>(a))
-  MLXR_NORM_FORM(MLXR_NORM_CALL, f);
+  MLXR_NORM_FORM(MLXR_NORM_CALL, f, MLXR_NORM_WIDE_WAVE);
 #undef MLXR_NORM_CALL
 }
 
@@ -567,7 +571,7 @@ void run_norm_vjp(const NormVjpArgs& a, const RowForm& f, int G, float2* coef, h
 #define MLXR_NORM_CALL(TPR, C)                                                       \
   (f.any ? add_rms_norm_vjp_kernel<YF32, HF32, TPR, C, true><<<(unsigned)G, kNT, lds, s>>>(a) \
          : add_rms_norm_vjp_kernel<YF32, HF32, TPR, C, false><<<(unsigned)G, kNT, lds, s>>>(a))
-  MLXR_NORM_FORM(MLXR_NORM_CALL, f);
+  MLXR_NORM_FORM(MLXR_NORM_CALL, f, MLXR_NORM_NO_WIDE_WAVE);
 #undef MLXR_NORM_CALL
 }
 
