@@ -536,9 +536,11 @@ int mlxr_moe_rms_norm(const void* x, int64_t T, int64_t d, const void* weight,
  * rounded once (mlxr_moe_rms_norm rounds the normalised value too), scales NULL.
  * mode "mxfp8": out uint32 [T, d/4] and scales uint8 [T, d/32] as
  * mlxr_moe_quantize makes them, but of y in f64 (32 divides d): what
- * mlxr_moe_grouped_qmm takes.  Rows holding NaN or an infinity, and without a
- * mode rows of h whose squares pass f32's range, follow the formula in f32.  Any d up to 2^20,
- * T up to 2^24 - 1; arrays aligned to their elements.  h and out must not overlap each other or the inputs. */
+ * mlxr_moe_grouped_qmm takes; a y past f32's range counts as an infinity there, and
+ * one below its normal range in steps of 2^-149.  Rows holding NaN or an infinity, and
+ * without a mode rows of h whose squares pass f32's range, follow the formula in f32.
+ * Any d up to 2^20, T up to 2^24 - 1; arrays aligned to their elements.  h and out must
+ * not overlap each other or the inputs. */
 int mlxr_moe_add_rms_norm(const void* x, int x_dtype, const void* residual,
                           int residual_dtype, int64_t T, int64_t d,
                           const void* weight, float eps, const char* mode,

@@ -436,3 +436,17 @@ def test_codes_of_wide_rows_are_the_nearest(pkg, dev, T, d, ht):
     byte = scale_bytes8(y)
     assert torch.equal(sc.cpu().long(), byte.long())
     assert torch.equal(decode8(q.cpu(), sc.cpu()), nearest8(y, byte))
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 16416])
+def test_norms_past_the_range_of_f32_are_infinities(pkg, dev, d):
+    h = torch.zeros((2, d), dtype=torch.bfloat16)
+    h[0, 3], h[1, 40] = float(d) ** 0.5, 1.0
+    w = torch.ones(d, dtype=torch.bfloat16)
+    w[3], w[40] = 3e38, -1e30
+    _, q, sc = pkg.ops.add_rms_norm(torch.zeros_like(h).to(dev), h.to(dev), w.to(dev), 0.0, "mxfp8")
+    assert sc[0, 0] == 255 and bool((q[0, :8] == 0).all()) and bool((sc[0, 1:] == 0).all())
+    y = norm64(h, w, 0.0)[1:]
+    assert torch.equal(sc[1:].cpu().long(), scale_bytes8(y).long())
+    assert torch.equal(decode8(q[1:].cpu(), sc[1:].cpu()), nearest8(y, scale_bytes8(y)))
