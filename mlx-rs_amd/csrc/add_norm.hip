@@ -238,8 +238,8 @@ __global__ __launch_bounds__(kNT) void add_rms_norm_kernel(NormArgs a) {
   }
 }
 
-// Rows that no registers hold (or no piece), a workgroup each: h is written, then read back by the
-// thread that wrote it.  mxfp8: 32 divides d, and a group is half a wave's.
+// Rows that no registers hold (or no piece), a workgroup each: h is written, then read back by
+// the thread that wrote it.  mxfp8: 32 divides d, and a group is half a wave's.
 template <bool XF32, bool HF32, bool MX>
 __global__ __launch_bounds__(kNT) void add_rms_norm_any_kernel(NormArgs a) {
   typedef norm_t<MX> sum_t;
@@ -408,8 +408,8 @@ __global__ __launch_bounds__(kNT) void add_rms_norm_vjp_kernel(NormVjpArgs a) {
   }
 }
 
-// Rows that no registers hold (or no piece), in two kernels: r and r^3 c of every row, then the columns,
-// a thread each, over a slice of the rows.
+// Rows that no registers hold (or no piece), in two kernels: r and r^2 c of every row, then the
+// columns, a thread each, over a slice of the rows.
 template <bool YF32, bool HF32>
 __global__ __launch_bounds__(kNT) void norm_vjp_rows_kernel(NormVjpArgs a, float2* coef) {
   __shared__ float red[4];

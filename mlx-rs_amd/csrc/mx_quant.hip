@@ -13,7 +13,8 @@
 // HBM-bound, one pass: a lane takes 8 values (16 bytes of bf16, 32 of f32), one
 // word of codes; the four lanes of a group find its maximum by DPP moves, as
 // integers, so that NaN compares largest.  A bank of 128 x 768 x 2048 bf16 weights: 81
-// us, 6.3 TB/s, and 71 us back, 7.2.
+// us, 6.3 TB/s, and 71 us back, 7.2.  To mxfp8 32768 rows of 2048 35 us from bf16, 59 from f32
+// (5.8 TB/s), and 8192 rows back to bf16 9.4.
 #include <algorithm>
 
 #include "mx.hpp"

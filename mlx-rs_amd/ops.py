@@ -663,8 +663,8 @@ def grouped_mm(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, rows=Non
     those), w bf16 [E, N, K].  With rows [R] x is bf16 [.., K] of any number of rows
     (a token's row taken by each of its choices), without it x's rows are the sorted
     ones.  Returns [R, N] in out_dtype (bf16 or f32); zeros in rows of no group and
-    where rows names no row of x.  K and N multiples of 8.  Not recorded by autograd: the gradients are
-    grouped_mm_vjp's."""
+    where rows names no row of x.  K and N multiples of 8.  Not recorded by autograd:
+    the gradients are grouped_mm_vjp's."""
     _dev(x, w, offsets, rows)
     w = _grouped_weight("grouped_mm", w)
     _bf16("grouped_mm", "x", x)
