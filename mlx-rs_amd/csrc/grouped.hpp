@@ -39,9 +39,10 @@ struct GroupedArgs {
                    // dW's, to be written (with dW's chunk, slices, max_parts and max_run)
 };
 
-// dW's plan, written by one workgroup of dx or of a launch of its own: where each XCD's parts start (words 0 .. 8),
-// the parts' records (expert, first row, rows, slice of a.parts or -1), and of every slice
-// the expert and how many it is the first of (0: it is not the first of an expert's).
+// dW's plan, written by one workgroup of dx or of a launch of its own: where each XCD's parts
+// start (words 0 .. 8), the parts' records (expert, first row, rows, slice of a.parts or -1),
+// and of every slice the expert and how many it is the first of (0: it is not the first of an
+// expert's).
 constexpr int kPlanHead = 16;
 inline int64_t plan_words(int64_t max_parts, int64_t slices) {
   return kPlanHead + 4 * max_parts + 2 * slices;

@@ -6,16 +6,17 @@
 // with a power-of-two scale per 32 (modes mxfp8 and mxfp4).
 //
 // One kernel body.  An output tile is TM x TJ; a stage of SI inputs of both operands goes
-// straight to LDS by 16-byte loads while the stages before are multiplied.  An operand whose inputs run along memory (x and W forward, dy
-// of dx) lies in LDS as 128-byte rows; one whose inputs run across rows (W of dx, both
-// of dW) as rows of columns, read transposed by ds_read_b64_tr_b16.
+// straight to LDS by 16-byte loads while the stages before are multiplied.  An operand whose
+// inputs run along memory (x and W forward, dy of dx) lies in LDS as rows of a stage's inputs;
+// one whose inputs run across rows (W of dx, both of dW) as rows of columns, read transposed by
+// ds_read_b64_tr_b16.
 //
 // Measured (one MI355X; c2: 128 experts, 4096 tokens of 8 choices, 768 x 2048): down 181 us,
 // its bytes at a copy's rate 122; dx 202 and 122, dW 253-261 and 98; 8 by 4 bits up 86, floor
-// 36; 256 experts of 512 x 2048, 2048 tokens of 8 choices 134, floor 117.  With 4 to 32 equal groups 770-910
-// TFLOP/s.  What bounds the ragged ones: loads and their barriers (of c2 down's 198 us by the
-// profiler's clock 195 are left without matrix instructions, 110 without loads), and the
-// workgroups' starts and ends (40 with no stage in between).
+// 36; 256 experts of 512 x 2048, 2048 tokens of 8 choices 134, floor 117.  With 4 to 32 equal
+// groups 770-910 TFLOP/s.  What bounds the ragged ones: loads and their barriers (of c2 down's
+// 198 us by the profiler's clock 195 are left without matrix instructions, 110 without loads),
+// and the workgroups' starts and ends (40 with no stage in between).
 #include <algorithm>
 #include <type_traits>
 
